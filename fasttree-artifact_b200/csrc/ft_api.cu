@@ -1157,3 +1157,5 @@ int ft_read_device_status(void* stream, int32_t* flags) {
 }
 
 }  // extern "C"
+
+#include "ft_extend_api.cuh"

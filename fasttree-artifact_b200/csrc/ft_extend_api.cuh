@@ -1,0 +1,184 @@
+// C entry points of ft_append and ft_extend (part of ft_api.cu: they use its error text, launch counter and descriptor cache).
+#pragma once
+
+#include "ft_append.cuh"
+#include "ft_extend.cuh"
+
+namespace {
+
+bool known_head_dim(int d) { return d == 16 || d == 32 || d == 64 || d == 128 || d == 256; }
+
+int check_heads(int dtype, int hq, int hkv, int d) {
+  if (dtype != FT_F16 && dtype != FT_BF16 && dtype != FT_F32)
+    return fail(FT_ERR_INVALID_ARGUMENT, "dtype %d is not one of FT_F16/FT_BF16/FT_F32", dtype);
+  if (hq <= 0 || hkv <= 0) return fail(FT_ERR_INVALID_ARGUMENT, "head counts must be positive (hq %d, hkv %d)", hq, hkv);
+  if (!known_head_dim(d)) return fail(FT_ERR_UNSUPPORTED, "head_dim %d is not one of 16, 32, 64, 128, 256", d);
+  return FT_OK;
+}
+
+// Can a tensor's rows be read and written as vectors of `elems` elements of `size` bytes?
+bool vector_rows(const void* p, int64_t s0, int64_t s1, int elems, int size) {
+  return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(elems * size - 1)) == 0 && s0 % elems == 0 && s1 % elems == 0;
+}
+
+template <typename T, int VEC>
+int launch_append(const ft::AppendParams& p, cudaStream_t st) {
+  const int units = p.head_dim / (2 * VEC), heads = (p.q != nullptr ? p.q_heads : 0) + 2 * p.kv_heads;
+  // enough threads for a token's units, two heads each, in whole warps and at most 256
+  int threads = (units * ((heads + 1) / 2) + 31) / 32 * 32;
+  threads = threads < units ? units : threads;
+  threads = threads > 256 ? 256 : threads;
+  ft::append_kernel<T, VEC><<<(unsigned)p.tokens, (unsigned)threads, 0, st>>>(p);
+  FT_CUDA_OK(cudaGetLastError());
+  count_launch();
+  return FT_OK;
+}
+
+template <typename T>
+int launch_append_for(const ft::AppendParams& p, cudaStream_t st) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const int size = (int)sizeof(T), half = p.rot / 2;
+  bool vec = p.head_dim % (2 * VEC) == 0 && half % VEC == 0 && (p.head_dim - p.rot) % (2 * VEC) == 0 &&
+             vector_rows(p.k, p.k_s0, p.k_s1, VEC, size) && vector_rows(p.v, p.v_s0, p.v_s1, VEC, size) &&
+             vector_rows(p.k_buffer, p.kb_s0, p.kb_s1, VEC, size) && vector_rows(p.v_buffer, p.vb_s0, p.vb_s1, VEC, size);
+  if (p.q != nullptr) vec = vec && vector_rows(p.q, p.q_s0, p.q_s1, VEC, size) && vector_rows(p.q_out, p.qo_s0, p.qo_s1, VEC, size);
+  return vec ? launch_append<T, VEC>(p, st) : launch_append<T, 1>(p, st);
+}
+
+const char* extend_tc_obstacle(const ft_extend_args* a) {
+  if (a->dtype == FT_F32) return "fp32 inputs";
+  if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) return "head_dim not 64, 128 or 256";
+  if (a->plan.rows_per_tile != 128) return "more than 128 query heads per KV head";
+  return "not built yet";
+}
+
+template <typename T>
+int launch_extend(const ft::ExtendParams& p, const ft_extend_args* a, bool tensor, cudaStream_t st) {
+  const int64_t ctas = (int64_t)p.num_items * p.kv_heads;
+  if (ctas > 0) {
+    if (!dry_run("extend_generic_kernel")) {
+      ft::extend_generic_kernel<T><<<(unsigned)ctas, 128, 0, st>>>(p);
+      FT_CUDA_OK(cudaGetLastError());
+      count_launch();
+    }
+  }
+  const int64_t merges = (int64_t)p.num_merged * p.heads;
+  if (merges > 0 && !dry_run("extend_merge_kernel")) {
+    // scheduled early: it reads the plan's lists, which the launch before it reads too, before it waits for that launch
+    FT_CUDA_OK(launch_early(ft::extend_merge_kernel<T>, (unsigned)((merges + 3) / 4), 128, 0, st, p));
+    count_launch();
+  }
+  return FT_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ft_append_args_size(void) { return static_cast<int>(sizeof(ft_append_args)); }
+int ft_extend_args_size(void) { return static_cast<int>(sizeof(ft_extend_args)); }
+
+int ft_append(const ft_append_args* a) {
+  if (a == nullptr) return fail(FT_ERR_INVALID_ARGUMENT, "args is NULL");
+  const int rc = check_heads(a->dtype, a->q != nullptr ? a->num_qo_heads : 1, a->num_kv_heads, a->head_dim);
+  if (rc != FT_OK) return rc;
+  if (a->tokens < 0) return fail(FT_ERR_INVALID_ARGUMENT, "tokens is negative");
+  if (a->rot_dim < 0 || a->rot_dim > a->head_dim || a->rot_dim % 2 != 0)
+    return fail(FT_ERR_INVALID_ARGUMENT, "rot_dim %d is not an even number up to head_dim %d", a->rot_dim, a->head_dim);
+  ft::AppendParams p;
+  memset(&p, 0, sizeof(p));
+  if (a->rot_dim > 0) {
+    if (a->num_axes < 1 || a->num_axes > 4) return fail(FT_ERR_INVALID_ARGUMENT, "num_axes %d is not 1 to 4", a->num_axes);
+    int64_t end = 0;
+    for (int i = 0; i < a->num_axes; ++i) {
+      if (a->sections[i] < 0) return fail(FT_ERR_INVALID_ARGUMENT, "sections[%d] is negative", i);
+      end += a->sections[i];
+      p.section_end[i] = (int32_t)(end < 0x7fffffff ? end : 0x7fffffff);
+    }
+    if (end != a->rot_dim / 2)
+      return fail(FT_ERR_INVALID_ARGUMENT, "the sections hold %lld pairs, rot_dim %d has %d", (long long)end, a->rot_dim, a->rot_dim / 2);
+    if (a->cos_sin_stride0 < 0) return fail(FT_ERR_INVALID_ARGUMENT, "cos_sin_stride0 is negative");
+  }
+  if (a->tokens == 0) return FT_OK;
+  if (a->k == nullptr || a->v == nullptr || a->k_buffer == nullptr || a->v_buffer == nullptr || a->slots == nullptr)
+    return fail(FT_ERR_INVALID_ARGUMENT, "k / v / k_buffer / v_buffer / slots is NULL");
+  if ((a->q == nullptr) != (a->q_out == nullptr)) return fail(FT_ERR_INVALID_ARGUMENT, "one of q and q_out is NULL");
+  if (a->kv_rows <= 0) return fail(FT_ERR_INVALID_ARGUMENT, "kv_rows must be positive");
+  if (a->rot_dim > 0 && (a->positions == nullptr || a->cos_sin == nullptr || a->cos_sin_rows <= 0))
+    return fail(FT_ERR_INVALID_ARGUMENT, "a rotation needs positions and a table of cosines and sines");
+  p.q = a->q, p.k = a->k, p.v = a->v, p.q_out = a->q_out, p.k_buffer = a->k_buffer, p.v_buffer = a->v_buffer;
+  p.slots = a->slots, p.positions = a->positions, p.cos_sin = a->cos_sin;
+  p.q_s0 = a->q_stride0, p.q_s1 = a->q_stride1, p.k_s0 = a->k_stride0, p.k_s1 = a->k_stride1;
+  p.v_s0 = a->v_stride0, p.v_s1 = a->v_stride1, p.qo_s0 = a->q_out_stride0, p.qo_s1 = a->q_out_stride1;
+  p.kb_s0 = a->k_buffer_stride0, p.kb_s1 = a->k_buffer_stride1, p.vb_s0 = a->v_buffer_stride0, p.vb_s1 = a->v_buffer_stride1;
+  p.kv_rows = a->kv_rows, p.positions_s0 = a->positions_stride0, p.cos_sin_rows = a->cos_sin_rows, p.cos_sin_s0 = a->cos_sin_stride0;
+  p.tokens = a->tokens, p.q_heads = a->num_qo_heads, p.kv_heads = a->num_kv_heads, p.head_dim = a->head_dim, p.rot = a->rot_dim;
+  p.axes = a->rot_dim > 0 ? a->num_axes : 0;
+  p.slots_64 = a->slots_64, p.positions_64 = a->positions_64, p.interleaved = a->interleaved != 0;
+  cudaStream_t st = static_cast<cudaStream_t>(a->stream);
+  if (a->dtype == FT_F16) return launch_append_for<__half>(p, st);
+  if (a->dtype == FT_BF16) return launch_append_for<__nv_bfloat16>(p, st);
+  return launch_append_for<float>(p, st);
+}
+
+int ft_extend(const ft_extend_args* a) {
+  if (a == nullptr) return fail(FT_ERR_INVALID_ARGUMENT, "args is NULL");
+  const int rc = check_heads(a->dtype, a->num_qo_heads, a->num_kv_heads, a->head_dim);
+  if (rc != FT_OK) return rc;
+  const ft_extend_plan_info& pl = a->plan;
+  if (pl.num_qo_heads != a->num_qo_heads || pl.num_kv_heads != a->num_kv_heads || pl.head_dim != a->head_dim ||
+      pl.elem_bytes != (a->dtype == FT_F32 ? 4 : 2))
+    return fail(FT_ERR_INVALID_ARGUMENT, "the plan was made for %d/%d heads of %d, %d bytes an element", pl.num_qo_heads, pl.num_kv_heads,
+                pl.head_dim, pl.elem_bytes);
+  if (a->path != FT_EXTEND_AUTO && a->path != FT_EXTEND_GENERIC && a->path != FT_EXTEND_TCGEN05)
+    return fail(FT_ERR_INVALID_ARGUMENT, "unknown path %d", a->path);
+  if (pl.num_items < 0 || pl.num_tokens < 0 || pl.num_merged < 0 || pl.partial_rows < 0)
+    return fail(FT_ERR_INVALID_ARGUMENT, "the plan's counts are negative");
+  if (pl.num_items == 0) return FT_OK;  // no query
+  if (a->q == nullptr || a->k_buffer == nullptr || a->v_buffer == nullptr || a->o == nullptr || a->kv_entries == nullptr || a->plan_table == nullptr)
+    return fail(FT_ERR_INVALID_ARGUMENT, "q / k_buffer / v_buffer / o / kv_entries / plan_table is NULL");
+  if (!aligned16(a->plan_table)) return fail(FT_ERR_UNSUPPORTED, "plan_table must be 16-byte aligned");
+  if (a->kv_rows <= 0) return fail(FT_ERR_INVALID_ARGUMENT, "kv_rows must be positive");
+  if (pl.kv_entries_len > a->kv_entries_len)
+    return fail(FT_ERR_INVALID_ARGUMENT, "the plan names %lld entries of kv_entries, which has %lld", (long long)pl.kv_entries_len,
+                (long long)a->kv_entries_len);
+  if (pl.q_rows > a->q_rows)
+    return fail(FT_ERR_INVALID_ARGUMENT, "the plan names %lld rows of q, which has %lld", (long long)pl.q_rows, (long long)a->q_rows);
+  if (pl.partial_rows > 0 && (a->mid_o == nullptr || a->mid_lse == nullptr || !aligned16(a->mid_o)))
+    return fail(FT_ERR_INVALID_ARGUMENT, "the plan has partial rows: mid_o (16-byte aligned) and mid_lse are needed");
+  if ((int64_t)pl.num_items * a->num_kv_heads > 0x7fffffffLL || ((int64_t)pl.num_merged * a->num_qo_heads + 3) / 4 > 0x7fffffffLL)
+    return fail(FT_ERR_TOO_LARGE, "more tasks than one launch takes");
+  const char* obstacle = extend_tc_obstacle(a);
+  if (a->path == FT_EXTEND_TCGEN05 && obstacle != nullptr) return fail(FT_ERR_UNSUPPORTED, "tcgen05 path: %s", obstacle);
+  const bool tensor = a->path != FT_EXTEND_GENERIC && obstacle == nullptr;
+
+  ft::ExtendParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = a->q, p.k = a->k_buffer, p.v = a->v_buffer, p.o = a->o, p.o_lse = a->o_lse, p.kv_entries = a->kv_entries;
+  p.items = a->plan_table + pl.items_off, p.segs = a->plan_table + pl.segments_off, p.tokens = a->plan_table + pl.tokens_off;
+  p.sm_offs = a->plan_table + pl.sm_offs_off, p.sm_tasks = a->plan_table + pl.sm_tasks_off;
+  p.merged = a->plan_table + pl.merge_off, p.merge_rows = a->plan_table + pl.merge_rows_off;
+  p.mid_o = a->mid_o, p.mid_lse = a->mid_lse;
+  p.q_s0 = a->q_stride0, p.q_s1 = a->q_stride1, p.k_s0 = a->k_stride0, p.k_s1 = a->k_stride1;
+  p.v_s0 = a->v_stride0, p.v_s1 = a->v_stride1, p.o_s0 = a->o_stride0, p.o_s1 = a->o_stride1;
+  p.kv_rows = a->kv_rows, p.q_rows = a->q_rows, p.kv_entries_len = a->kv_entries_len;
+  p.num_items = pl.num_items, p.num_merged = pl.num_merged, p.partial_rows = pl.partial_rows;
+  p.heads = a->num_qo_heads, p.kv_heads = a->num_kv_heads, p.group = a->num_qo_heads / a->num_kv_heads, p.head_dim = a->head_dim;
+  p.window = pl.window, p.tile = pl.tile_tokens;
+  p.sm_scale = a->sm_scale, p.logit_cap = a->logit_cap > 0.f ? a->logit_cap : 0.f;
+  cudaStream_t st = static_cast<cudaStream_t>(a->stream);
+  if (a->dtype == FT_F16) return launch_extend<__half>(p, a, tensor, st);
+  if (a->dtype == FT_BF16) return launch_extend<__nv_bfloat16>(p, a, tensor, st);
+  return launch_extend<float>(p, a, false, st);
+}
+
+const char* ft_extend_path_name(const ft_extend_args* args) {
+  g_kernel_names[0] = '\0';
+  g_dry_run = true;
+  const int rc = ft_extend(args);
+  g_dry_run = false;
+  if (rc != FT_OK) return nullptr;
+  return g_kernel_names;
+}
+
+}  // extern "C"

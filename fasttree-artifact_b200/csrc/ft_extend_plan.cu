@@ -1,0 +1,558 @@
+// Host-side schedule of an extend-attention step (no device code).
+//
+// The step's query tokens are laid out request by request and packed, with their GQA group, into query tiles of
+// rows_per_tile rows.  A block is one query tile, or two that read mostly the same K/V.  Its K/V is the union of what
+// its tokens may see, as a list of segments - runs of entries of the row-id table - each with the block's tokens that
+// see it: a prefix that the block's requests share stands there once.  The segments are numbered through (virtual
+// positions) and cut into tiles of tile_tokens.
+//
+// A block whose K/V is long for the machine is cut into items along the virtual positions; items leave partial rows,
+// which a second launch merges.  Every (item, KV head) is a task; tasks are dealt to the SMs longest first, each to the
+// SM that is free first by the cost model below, and of several cuts the one whose simulated schedule ends first is
+// taken.
+//
+// Layout of an item (24 ints): first segment, segments, first and last K/V tile, step, query tiles, virtual length, 0,
+// then two streams of {first token, tokens, first tile, last tile, first partial row or -1 (the output itself), query
+// tile, 0, 0}.  Two streams are two query tiles over the same K/V tiles (step 1), or one query tile whose even and odd
+// K/V tiles run as two streams with partial rows of their own (step 2).  A segment (8 ints): table offset (low, high),
+// length, position of its first token, first and last token of the block that see it, virtual position of its start, 0.
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+#include <cstring>
+#include <new>
+#include <queue>
+#include <vector>
+
+#include "fasttree_b200.h"
+
+struct ft_extend_plan {
+  std::vector<int32_t> table;
+  ft_extend_plan_info info;
+};
+
+namespace {
+
+constexpr int ITEM_INTS = 24, SEG_INTS = 8;
+
+struct Segment {
+  int64_t kv_off;
+  int32_t len, pos0, tok_lo, tok_hi, voff;
+};
+
+struct Token {
+  int32_t q_row, pos;
+};
+
+struct Block {
+  int tok0 = 0, ntok = 0, split = 0;  // its tokens; those from `split` on belong to the second query tile (split == ntok: none)
+  int seg0 = 0, nseg = 0, len = 0;    // virtual length
+  int req_lo = 0, req_hi = 0;
+};
+
+struct Item {
+  int block, t0, t1;
+  bool alternate;    // one query tile, two streams
+  int which;         // bit w: query tile w takes part
+  int lo[2], hi[2];  // tiles of the streams
+  double cost;
+};
+
+struct Costs {  // microseconds, B200: per K/V tile of two query tiles, of one in two streams or in one, and per item
+  double pair, load, alternate, single, item;
+};
+
+struct Problem {
+  const int64_t *seq, *ext, *start, *qstart, *shared;
+  int batch, group, kv_heads, rows, tile;
+  int64_t window;
+  bool two_tiles, streams;
+  int tokens_per_tile;
+  int slots;
+  Costs cost;
+};
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+class Builder {
+ public:
+  explicit Builder(const Problem& p) : p_(p) {}
+
+  void run() {
+    place_tokens();
+    pack_blocks();
+    choose_items();
+  }
+
+  std::vector<Token> tokens;
+  std::vector<Segment> segs;
+  std::vector<Block> blocks;
+  std::vector<Item> items;
+  std::vector<int> task_order;  // items x heads dealt to the slots: slot s takes sm_tasks[sm_offs[s] ..]
+  std::vector<int32_t> sm_offs, sm_tasks;
+
+ private:
+  const Problem& p_;
+  std::vector<int> req_of_, first_tok_;
+
+  int64_t prefix(int i) const { return p_.seq[i] - p_.ext[i]; }
+
+  void place_tokens() {
+    first_tok_.resize(p_.batch + 1, 0);
+    for (int i = 0; i < p_.batch; ++i) {
+      first_tok_[i] = (int)tokens.size();
+      for (int64_t t = 0; t < p_.ext[i]; ++t) {
+        tokens.push_back({(int32_t)(p_.qstart[i] + t), (int32_t)(prefix(i) + t)});
+        req_of_.push_back(i);
+      }
+    }
+    first_tok_[p_.batch] = (int)tokens.size();
+  }
+
+  // Query tiles: a request joins the tile that the one before it has not filled where that costs less K/V than a tile of
+  // its own - whole if it fits, in part if what it shares is the most of what it reads.
+  void pack_blocks() {
+    std::vector<std::pair<int, int>> tiles;  // [first, last) token
+    const int cap = p_.tokens_per_tile;
+    int cur = 0, room = 0, last = -1;  // tokens [cur, end) are in the open tile
+    int end = 0;
+    for (int i = 0; i < p_.batch; ++i) {
+      int64_t e = p_.ext[i];
+      if (e == 0) continue;
+      int at = first_tok_[i];
+      if (room > 0) {
+        int64_t common = INT64_MAX;  // with the request before it that has tokens
+        for (int k = last + 1; k <= i; ++k) common = std::min(common, p_.shared[k]);
+        const int64_t part = std::min<int64_t>(e, room), own = prefix(i) - common + part;
+        const bool join = e <= room || (common > 0 && own * cap < part * p_.seq[i]);
+        if (join) {
+          end = at + (int)part;
+          at = end;
+          e -= part;
+          room -= (int)part;
+        }
+        if (e > 0 || room == 0) {
+          tiles.push_back({cur, end});
+          room = 0;
+        }
+      }
+      while (e > 0) {
+        const int take = (int)std::min<int64_t>(e, cap);
+        cur = at;
+        end = at += take;
+        e -= take;
+        room = cap - take;
+        if (e > 0 || room == 0) {
+          tiles.push_back({cur, end});
+          room = 0;
+        }
+      }
+      last = i;
+    }
+    if (room > 0) tiles.push_back({cur, end});
+
+    for (size_t i = 0; i < tiles.size(); ++i) {
+      Block one = make_block(tiles[i].first, tiles[i].second, tiles[i].second);
+      if (p_.two_tiles && i + 1 < tiles.size()) {
+        // two tiles together where they read mostly the same
+        const size_t mark = segs.size();
+        const Block other = make_block(tiles[i + 1].first, tiles[i + 1].second, tiles[i + 1].second);
+        segs.resize(mark);
+        Block both = make_block(tiles[i].first, tiles[i + 1].second, tiles[i].second);
+        if (both.len * 100ll <= 80ll * ((int64_t)one.len + other.len)) {
+          segs.erase(segs.begin() + one.seg0, segs.begin() + both.seg0);
+          both.seg0 = one.seg0;
+          blocks.push_back(both);
+          ++i;
+          continue;
+        }
+        segs.resize(mark);
+      }
+      blocks.push_back(one);
+    }
+  }
+
+  Block make_block(int tok0, int tok1, int split) {
+    Block b;
+    b.tok0 = tok0;
+    b.ntok = tok1 - tok0;
+    b.split = split - tok0;
+    b.req_lo = req_of_[tok0];
+    b.req_hi = req_of_[tok1 - 1];
+    b.seg0 = (int)segs.size();
+    emit(b, b.req_lo, b.req_hi, 0);
+    b.nseg = (int)segs.size() - b.seg0;
+    return b;
+  }
+
+  // the tokens of requests lo .. hi that are in the block
+  std::pair<int, int> toks(const Block& b, int lo, int hi) const {
+    return {std::max(first_tok_[lo], b.tok0), std::min(first_tok_[hi + 1], b.tok0 + b.ntok)};
+  }
+
+  void emit(Block& b, int lo, int hi, int64_t depth) {
+    const std::pair<int, int> tk = toks(b, lo, hi);
+    if (tk.first >= tk.second) return;
+    int64_t first = INT64_MAX, common = INT64_MAX;
+    for (int t = tk.first; t < tk.second; ++t) first = std::min<int64_t>(first, tokens[t].pos);
+    if (lo == hi) common = tokens[tk.second - 1].pos + 1;
+    for (int k = lo + 1; k <= hi; ++k) common = std::min(common, p_.shared[k]);
+    const int64_t begin = std::max(depth, p_.window > 0 ? first - p_.window + 1 : 0);
+    if (begin < common) {
+      segs.push_back({p_.start[lo] + begin, (int32_t)(common - begin), (int32_t)begin, tk.first - b.tok0, tk.second - b.tok0, b.len});
+      b.len += (int32_t)(common - begin);
+    }
+    if (lo == hi) return;
+    const int64_t next = std::max(depth, common);
+    for (int k = lo, from = lo; k <= hi; ++k)
+      if (k == hi || p_.shared[k + 1] <= common) {
+        emit(b, from, k, next);
+        from = k + 1;
+      }
+  }
+
+  int tiles_of(const Block& b) const { return (int)ceil_div(b.len, p_.tile); }
+
+  // per K/V tile of the block: which of its query tiles see a token of it
+  std::vector<uint8_t> activity(const Block& b) const {
+    std::vector<uint8_t> act(tiles_of(b), 0);
+    for (int s = b.seg0; s < b.seg0 + b.nseg; ++s) {
+      const Segment& g = segs[s];
+      for (int w = 0; w < 2; ++w) {
+        const int lo = std::max(g.tok_lo, w == 0 ? 0 : b.split), hi = std::min(g.tok_hi, w == 0 ? b.split : b.ntok);
+        if (lo >= hi) continue;
+        int64_t from = INT64_MAX, to = 0;
+        for (int t = lo; t < hi; ++t) {
+          const int64_t pos = tokens[b.tok0 + t].pos;
+          from = std::min(from, p_.window > 0 ? pos - p_.window + 1 : 0);
+          to = std::max(to, pos + 1);
+        }
+        from = std::max<int64_t>(from - g.pos0, 0);
+        to = std::min<int64_t>(to - g.pos0, g.len);
+        if (from >= to) continue;
+        for (int64_t t = (g.voff + from) / p_.tile; t <= (g.voff + to - 1) / p_.tile; ++t) act[t] |= (uint8_t)(1 << w);
+      }
+    }
+    return act;
+  }
+
+  // tiles [t0, t1) of a block as one item; streams: whether one query tile may run as two streams
+  Item make_item(int block, const std::vector<uint8_t>& act, int t0, int t1, bool streams) const {
+    Item it;
+    it.block = block;
+    it.which = 0;
+    int n = 0;
+    for (int w = 0; w < 2; ++w) {
+      int lo = t1, hi = t0;
+      for (int t = t0; t < t1; ++t)
+        if (act[t] & (1 << w)) {
+          lo = std::min(lo, t);
+          hi = t + 1;
+        }
+      it.lo[w] = it.hi[w] = t0;
+      if (lo < hi) {
+        it.which |= 1 << w;
+        it.lo[w] = lo;
+        it.hi[w] = hi;
+        n += hi - lo;
+      }
+    }
+    it.t0 = t1;
+    it.t1 = t0;
+    for (int w = 0; w < 2; ++w)
+      if (it.which & (1 << w)) {
+        it.t0 = std::min(it.t0, it.lo[w]);
+        it.t1 = std::max(it.t1, it.hi[w]);
+      }
+    it.alternate = streams && it.which != 3 && it.t1 - it.t0 >= 2;
+    const Costs& c = p_.cost;
+    const int loaded = it.t1 - it.t0;
+    it.cost = c.item + (it.which == 3 ? c.pair * n + c.load * loaded : it.alternate ? c.alternate * loaded : c.single * loaded);
+    return it;
+  }
+
+  // Deals the tasks, longest first, to the slot that is free first; returns when the last one is done.
+  double deal(const std::vector<Item>& its, std::vector<int>* order, std::vector<int>* slot_of) const {
+    std::vector<int> by(its.size());
+    for (size_t i = 0; i < by.size(); ++i) by[i] = (int)i;
+    std::stable_sort(by.begin(), by.end(), [&](int a, int b) { return its[a].cost > its[b].cost; });
+    typedef std::pair<double, int> Free;
+    std::priority_queue<Free, std::vector<Free>, std::greater<Free>> free;
+    for (int s = 0; s < p_.slots; ++s) free.push({0.0, s});
+    double end = 0;
+    for (int i : by)
+      for (int h = 0; h < p_.kv_heads; ++h) {
+        Free f = free.top();
+        free.pop();
+        f.first += its[i].cost;
+        end = std::max(end, f.first);
+        if (order != nullptr) {
+          order->push_back(i * p_.kv_heads + h);
+          slot_of->push_back(f.second);
+        }
+        free.push(f);
+      }
+    return end;
+  }
+
+  void choose_items() {
+    const int nb = (int)blocks.size();
+    std::vector<std::vector<uint8_t>> act(nb);
+    std::vector<std::vector<int>> cuts(nb);  // section borders
+    for (int b = 0; b < nb; ++b) {
+      act[b] = activity(blocks[b]);
+      const int n = (int)act[b].size();
+      // a block of two query tiles is cut where a long run of K/V is seen by one of them alone
+      std::vector<int>& c = cuts[b];
+      c.push_back(0);
+      for (int t = 0; t < n;) {
+        int e = t;
+        while (e < n && act[b][e] == act[b][t]) ++e;
+        if (e - t >= 6 && act[b][t] != 3 && blocks[b].split < blocks[b].ntok) {
+          if (c.back() != t) c.push_back(t);
+          if (e < n) c.push_back(e);
+        }
+        t = e;
+      }
+      c.push_back(n);
+    }
+    double total = 0;
+    auto cut = [&](double limit, std::vector<Item>& out) {
+      out.clear();
+      double parts = 0;  // partial rows of the cut
+      for (int b = 0; b < nb; ++b) {
+        const size_t from = out.size();
+        for (size_t s = 0; s + 1 < cuts[b].size(); ++s) {
+          const int t0 = cuts[b][s], t1 = cuts[b][s + 1];
+          const bool whole = cuts[b].size() == 2;
+          const Item one = make_item(b, act[b], t0, t1, p_.streams && !(whole && limit <= 0));
+          if (one.which == 0) continue;
+          int n = 1;
+          if (limit > 0) {
+            const double work = one.cost - p_.cost.item;
+            n = (int)std::min<int64_t>(std::max<int64_t>((int64_t)((work + limit - 1e-9) / limit), 1), one.t1 - one.t0);
+            // a short block of one query tile stays one item that writes the output itself
+            if (whole && n == 1 && one.alternate && one.t1 - one.t0 <= 6) {
+              out.push_back(make_item(b, act[b], t0, t1, false));
+              continue;
+            }
+          }
+          for (int k = 0; k < n; ++k) {
+            const int a = one.t0 + (int)((int64_t)(one.t1 - one.t0) * k / n), e = one.t0 + (int)((int64_t)(one.t1 - one.t0) * (k + 1) / n);
+            const Item it = make_item(b, act[b], a, e, p_.streams && !(whole && limit <= 0));
+            if (it.which != 0) out.push_back(it);
+          }
+        }
+        if (out.size() - from > 1 || (out.size() > from && out[from].alternate))
+          for (size_t i = from; i < out.size(); ++i) parts += (out[i].alternate ? 2.0 : 1.0) * blocks[b].ntok;
+      }
+      return parts;
+    };
+    std::vector<Item> trial;
+    cut(0, trial);
+    for (const Item& it : trial) total += it.cost * p_.kv_heads;
+    const double even = total / p_.slots;
+    auto merge_cost = [&](double parts) {  // a launch, and the partial rows written and read back
+      return parts > 0 ? 3.0 + parts * p_.kv_heads * p_.group * 8.0 * 128 / 4e6 : 0.0;
+    };
+    double best = -1;
+    static const double pieces[] = {0, 1.0, 0.5, 0.34, 0.25, 0.12};
+    for (double f : pieces) {
+      const double parts = cut(f * even, trial);
+      const double end = deal(trial, nullptr, nullptr) + merge_cost(parts);
+      if (best < 0 || end < best * 0.98) {
+        best = end;
+        items = trial;
+      }
+      if (f == 0 && end <= 1.04 * even + 1.0) break;  // nothing to gain
+    }
+    std::vector<int> order, slot;
+    deal(items, &order, &slot);
+    sm_offs.assign(p_.slots + 1, 0);
+    for (int s : slot) ++sm_offs[s + 1];
+    for (int s = 0; s < p_.slots; ++s) sm_offs[s + 1] += sm_offs[s];
+    sm_tasks.resize(order.size());
+    std::vector<int32_t> at(sm_offs.begin(), sm_offs.end() - 1);
+    for (size_t i = 0; i < order.size(); ++i) sm_tasks[at[slot[i]]++] = order[i];
+  }
+};
+
+void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
+  ft_extend_plan_info& info = out->info;
+  std::vector<int32_t>& t = out->table;
+  auto align = [&] { t.resize((t.size() + 3) / 4 * 4, 0); };
+  // partial rows: every stream of an item of a block with more than one of them has its tokens' rows
+  std::vector<int> streams(b.blocks.size(), 0);
+  for (const Item& it : b.items) streams[it.block] += it.alternate ? 2 : 1;
+  std::vector<char> partial(b.blocks.size(), 0);
+  {
+    std::vector<int> n_items(b.blocks.size(), 0);
+    for (const Item& it : b.items) ++n_items[it.block];
+    for (const Item& it : b.items) partial[it.block] |= (char)(n_items[it.block] > 1 || it.alternate);
+  }
+  std::vector<std::vector<std::pair<int, int>>> runs(b.blocks.size());  // per block: {first partial row, first token | tokens << 16}
+  int64_t rows = 0;
+  info.items_off = 0;
+  for (const Item& it : b.items) {
+    const Block& blk = b.blocks[it.block];
+    int32_t x[ITEM_INTS] = {blk.seg0, blk.nseg, it.t0, it.t1, it.alternate ? 2 : 1, it.which == 3 ? 2 : 1, blk.len, 0};
+    int q_tile = 0;
+    for (int w = 0; w < 2; ++w) {
+      const int of = it.alternate ? (it.which == 1 ? 0 : 1) : w;  // the query tile of this stream
+      if (!(it.which & (1 << of))) continue;
+      const int first = of == 0 ? 0 : blk.split, n = of == 0 ? blk.split : blk.ntok - blk.split;
+      // one query tile is always tile 0 of its item, and one stream stream 0
+      int32_t* s = x + 8 + 8 * (it.alternate ? w : q_tile);
+      s[0] = blk.tok0 + first;
+      s[1] = n;
+      s[2] = it.alternate ? it.t0 + w : it.lo[of];
+      s[3] = it.alternate ? it.t1 : it.hi[of];
+      s[4] = -1;
+      s[5] = it.alternate ? 0 : q_tile;
+      s[6] = first;
+      if (partial[it.block]) {
+        s[4] = (int32_t)rows;
+        runs[it.block].push_back({(int)rows, first | n << 16});
+        rows += n;
+      }
+      ++q_tile;
+    }
+    t.insert(t.end(), x, x + ITEM_INTS);
+  }
+  info.segments_off = (int64_t)t.size();
+  info.kv_entries_len = 0;
+  for (const Segment& g : b.segs) {
+    const int32_t x[SEG_INTS] = {(int32_t)(uint32_t)(g.kv_off & 0xffffffffll), (int32_t)(g.kv_off >> 32), g.len, g.pos0, g.tok_lo, g.tok_hi, g.voff, 0};
+    t.insert(t.end(), x, x + SEG_INTS);
+    info.kv_entries_len = std::max(info.kv_entries_len, g.kv_off + g.len);
+  }
+  align();
+  info.tokens_off = (int64_t)t.size();
+  info.q_rows = 0;
+  for (const Token& k : b.tokens) {
+    t.push_back(k.q_row);
+    t.push_back(k.pos);
+    info.q_rows = std::max<int64_t>(info.q_rows, (int64_t)k.q_row + 1);
+  }
+  align();
+  info.sm_offs_off = (int64_t)t.size();
+  t.insert(t.end(), b.sm_offs.begin(), b.sm_offs.end());
+  align();
+  info.sm_tasks_off = (int64_t)t.size();
+  t.insert(t.end(), b.sm_tasks.begin(), b.sm_tasks.end());
+  align();
+  // merged tokens: {row of q, first entry of its list of partial rows, entries, 0}, then the lists
+  std::vector<int32_t> merged, lists;
+  for (size_t k = 0; k < b.blocks.size(); ++k) {
+    if (!partial[k]) continue;
+    for (int i = 0; i < b.blocks[k].ntok; ++i) {
+      const int32_t from = (int32_t)lists.size();
+      for (const auto& r : runs[k]) {
+        const int first = r.second & 0xffff, n = r.second >> 16;
+        if (i >= first && i < first + n) lists.push_back(r.first + i - first);
+      }
+      const int32_t x[4] = {b.tokens[b.blocks[k].tok0 + i].q_row, from, (int32_t)lists.size() - from, 0};
+      merged.insert(merged.end(), x, x + 4);
+    }
+  }
+  info.merge_off = (int64_t)t.size();
+  t.insert(t.end(), merged.begin(), merged.end());
+  info.merge_rows_off = (int64_t)t.size();
+  t.insert(t.end(), lists.begin(), lists.end());
+  align();
+  info.table_ints = (int64_t)t.size();
+  info.pieces = (int64_t)b.items.size();
+  info.num_items = (int32_t)b.items.size();
+  info.num_segments = (int32_t)b.segs.size();
+  info.num_tokens = (int32_t)b.tokens.size();
+  info.num_merged = (int32_t)(merged.size() / 4);
+  info.partial_rows = (int32_t)rows;
+  info.num_sms = p.slots;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ft_extend_plan_build(const int64_t* seq_lens, const int64_t* extend_lens, const int64_t* kv_starts, const int64_t* q_starts,
+                         const int64_t* shared_with_previous, int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
+                         int32_t head_dim, int32_t elem_bytes, int64_t window, int32_t num_sms, ft_extend_plan** out) {
+  if (out == nullptr) return FT_ERR_INVALID_ARGUMENT;
+  *out = nullptr;
+  if (batch < 0 || num_qo_heads <= 0 || num_kv_heads <= 0 || num_qo_heads % num_kv_heads != 0 || num_sms <= 0 || window < 0 ||
+      (elem_bytes != 2 && elem_bytes != 4))
+    return FT_ERR_INVALID_ARGUMENT;
+  if (batch > 0 && (!seq_lens || !extend_lens || !kv_starts || !q_starts || !shared_with_previous)) return FT_ERR_INVALID_ARGUMENT;
+  if (!(head_dim == 16 || head_dim == 32 || head_dim == 64 || head_dim == 128 || head_dim == 256)) return FT_ERR_UNSUPPORTED;
+  int64_t total = 0, most = 0;
+  for (int i = 0; i < batch; ++i) {
+    const int64_t cached = seq_lens[i] - extend_lens[i];
+    if (extend_lens[i] < 0 || cached < 0 || kv_starts[i] < 0 || q_starts[i] < 0 || shared_with_previous[i] < 0)
+      return FT_ERR_INVALID_ARGUMENT;
+    if (shared_with_previous[i] > cached || (shared_with_previous[i] > 0 && (i == 0 || shared_with_previous[i] > seq_lens[i - 1] - extend_lens[i - 1])))
+      return FT_ERR_INVALID_ARGUMENT;
+    if (seq_lens[i] > INT32_MAX / 2 || q_starts[i] + extend_lens[i] > INT32_MAX / 2) return FT_ERR_TOO_LARGE;
+    total += extend_lens[i];
+    most = std::max(most, seq_lens[i]);
+  }
+  if (total > INT32_MAX / 64 || window > INT32_MAX) return FT_ERR_TOO_LARGE;
+  try {
+    Problem p;
+    p.seq = seq_lens, p.ext = extend_lens, p.start = kv_starts, p.qstart = q_starts, p.shared = shared_with_previous;
+    p.batch = batch;
+    p.group = num_qo_heads / num_kv_heads;
+    p.kv_heads = num_kv_heads;
+    p.window = window > most ? 0 : window;  // a window that hides nothing is none
+    const bool tensor = elem_bytes == 2 && head_dim >= 64 && p.group <= 128;
+    p.rows = tensor ? 128 : 16;
+    p.tile = tensor ? (head_dim == 256 ? 64 : 128) : 32;
+    p.two_tiles = p.streams = tensor && head_dim <= 128;
+    p.tokens_per_tile = std::max(1, p.rows / p.group);
+    p.slots = tensor ? num_sms : 4 * num_sms;
+    p.cost = tensor ? (head_dim == 256 ? Costs{1.0, 0, 1.0, 1.0, 3.0} : Costs{0.6, 0.15, 0.75, 1.1, 2.5}) : Costs{2.0, 0, 2.0, 2.0, 3.0};
+    Builder b(p);
+    b.run();
+    // what the tables' 32-bit fields hold
+    int64_t virt = 0, rows = 0;
+    for (const Block& blk : b.blocks) virt = std::max<int64_t>(virt, blk.len);
+    for (const Item& it : b.items) rows += 2 * (int64_t)b.blocks[it.block].ntok;
+    if (virt > INT32_MAX / 2 || rows > INT32_MAX || (int64_t)b.items.size() * num_kv_heads > INT32_MAX / 2) return FT_ERR_TOO_LARGE;
+    ft_extend_plan* plan = new ft_extend_plan();
+    std::memset(&plan->info, 0, sizeof(plan->info));
+    plan->info.num_qo_heads = num_qo_heads;
+    plan->info.num_kv_heads = num_kv_heads;
+    plan->info.head_dim = head_dim;
+    plan->info.window = (int32_t)p.window;
+    plan->info.elem_bytes = elem_bytes;
+    plan->info.rows_per_tile = p.rows;
+    plan->info.tile_tokens = p.tile;
+    try {
+      pack(p, b, plan);
+    } catch (...) {
+      delete plan;
+      throw;
+    }
+    *out = plan;
+  } catch (const std::bad_alloc&) {
+    return FT_ERR_TOO_LARGE;
+  } catch (...) {
+    return FT_ERR_INVALID_ARGUMENT;
+  }
+  return FT_OK;
+}
+
+int ft_extend_plan_get_info(const ft_extend_plan* plan, ft_extend_plan_info* info) {
+  if (plan == nullptr || info == nullptr) return FT_ERR_INVALID_ARGUMENT;
+  *info = plan->info;
+  return FT_OK;
+}
+
+int ft_extend_plan_copy(const ft_extend_plan* plan, int32_t* table) {
+  if (plan == nullptr || table == nullptr) return FT_ERR_INVALID_ARGUMENT;
+  if (!plan->table.empty()) std::memcpy(table, plan->table.data(), plan->table.size() * sizeof(int32_t));
+  return FT_OK;
+}
+
+void ft_extend_plan_free(ft_extend_plan* plan) { delete plan; }
+
+}  // extern "C"

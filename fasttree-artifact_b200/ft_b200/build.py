@@ -13,7 +13,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB_PATH = os.path.join(PKG_DIR, "libfasttree_b200.so")
 
-SOURCES = ["ft_api.cu", "ft_planner.cu"]
+SOURCES = ["ft_api.cu", "ft_planner.cu", "ft_extend_plan.cu"]
 
 CALL_PATH = os.path.join(PKG_DIR, "ft_call.so")     # Python extension: checks, argument block and call of a decode step
 CALL_SOURCE = os.path.join(CSRC, "ft_call.cpp")

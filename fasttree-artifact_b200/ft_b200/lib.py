@@ -17,7 +17,7 @@ PATHS = {"auto": FT_PATH_AUTO, "generic": FT_PATH_GENERIC, "mma": FT_PATH_MMA, "
 
 FT_STATIC_SCRATCH_BYTES = 16 << 20      # capacity of the array behind ft_decode_static_scratch
 
-FT_DEV_BAD_KV_INDEX, FT_DEV_BAD_Q_INDEX, FT_DEV_BAD_ROW_INDEX, FT_DEV_WAIT_TIMEOUT = 1, 2, 4, 8
+FT_DEV_BAD_KV_INDEX, FT_DEV_BAD_Q_INDEX, FT_DEV_BAD_ROW_INDEX, FT_DEV_WAIT_TIMEOUT, FT_DEV_BAD_POSITION = 1, 2, 4, 8, 16
 
 EXPORTS = ["ft_version", "ft_decode_args_size", "ft_last_error", "ft_decode", "ft_stage1", "ft_stage2",
            "ft_decode_static_scratch", "ft_decode_host_io", "ft_selftest_bounded_wait", "ft_read_wait_diagnostics", "ft_bump_kv_lens",
@@ -25,7 +25,11 @@ EXPORTS = ["ft_version", "ft_decode_args_size", "ft_last_error", "ft_decode", "f
            "ft_read_device_status", "ft_launch_count", "ft_stage1_path_name",
            "ft_plan_b200_build", "ft_plan_b200_build_direct", "ft_plan_get_info", "ft_plan_copy_tables", "ft_plan_copy_row_ranges",
            "ft_plan_copy_aux_segments",
-           "ft_plan_free"]
+           "ft_plan_free",
+           "ft_append_args_size", "ft_append", "ft_extend_plan_build", "ft_extend_plan_get_info", "ft_extend_plan_copy",
+           "ft_extend_plan_free", "ft_extend_args_size", "ft_extend", "ft_extend_path_name"]
+
+EXTEND_PATHS = {"auto": 0, "generic": 1, "tcgen05": 2}
 
 
 class FastTreeError(RuntimeError):
@@ -90,6 +94,37 @@ class DecodeArgs(ctypes.Structure):
         ("few_tokens", ctypes.c_int64), ("few_longest", ctypes.c_int32), ("few_over_8_rows", ctypes.c_int32),
         ("many_longest", ctypes.c_int32), ("plan_rows", ctypes.c_int32),
     ]
+
+
+class AppendArgs(ctypes.Structure):
+    """Mirror of ``struct ft_append_args``."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out", "k_buffer", "v_buffer", "slots", "positions", "cos_sin")] + [
+        (n, ctypes.c_int32) for n in ("dtype", "tokens", "num_qo_heads", "num_kv_heads", "head_dim", "rot_dim", "num_axes")] + [
+        ("sections", ctypes.c_int32 * 4)] + [(n, ctypes.c_int32) for n in ("interleaved", "slots_64", "positions_64")] + [
+        (n, ctypes.c_int64) for n in (
+            "kv_rows", "cos_sin_rows", "cos_sin_stride0", "positions_stride0", "q_stride0", "q_stride1", "k_stride0", "k_stride1",
+            "v_stride0", "v_stride1", "q_out_stride0", "q_out_stride1", "k_buffer_stride0", "k_buffer_stride1",
+            "v_buffer_stride0", "v_buffer_stride1")] + [("stream", ctypes.c_void_p)]
+
+
+class ExtendPlanInfo(ctypes.Structure):
+    """Mirror of ``struct ft_extend_plan_info``."""
+    _fields_ = [(n, ctypes.c_int64) for n in ("table_ints", "items_off", "segments_off", "tokens_off", "sm_offs_off", "sm_tasks_off",
+                                              "merge_off", "merge_rows_off", "kv_entries_len", "q_rows", "pieces")] + [
+        (n, ctypes.c_int32) for n in ("num_items", "num_segments", "num_tokens", "num_merged", "partial_rows", "num_sms",
+                                      "num_qo_heads", "num_kv_heads", "head_dim", "window", "elem_bytes", "rows_per_tile",
+                                      "tile_tokens", "reserved")]
+
+
+class ExtendArgs(ctypes.Structure):
+    """Mirror of ``struct ft_extend_args``."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k_buffer", "v_buffer", "o", "o_lse")] + [
+        (n, ctypes.c_int32) for n in ("dtype", "num_qo_heads", "num_kv_heads", "head_dim", "path")] + [
+        ("sm_scale", ctypes.c_float), ("logit_cap", ctypes.c_float), ("reserved", ctypes.c_int32)] + [
+        (n, ctypes.c_int64) for n in ("q_rows", "kv_rows", "q_stride0", "q_stride1", "k_stride0", "k_stride1", "v_stride0",
+                                      "v_stride1", "o_stride0", "o_stride1")] + [
+        ("kv_entries", ctypes.c_void_p), ("kv_entries_len", ctypes.c_int64), ("plan_table", ctypes.c_void_p),
+        ("plan", ExtendPlanInfo), ("mid_o", ctypes.c_void_p), ("mid_lse", ctypes.c_void_p), ("stream", ctypes.c_void_p)]
 
 
 _lock = threading.Lock()
@@ -171,6 +206,24 @@ def load():
         lib.ft_plan_copy_aux_segments.restype = ctypes.c_int
         lib.ft_plan_free.argtypes = [ctypes.c_void_p]
         lib.ft_plan_free.restype = None
+        for size, struct in ((lib.ft_append_args_size, AppendArgs), (lib.ft_extend_args_size, ExtendArgs)):
+            if size() != ctypes.sizeof(struct):
+                raise FastTreeError(-1, "%s of the library (%d bytes) differs from the binding (%d)"
+                                    % (struct.__name__, size(), ctypes.sizeof(struct)))
+        lib.ft_append.argtypes = [ctypes.POINTER(AppendArgs)]
+        lib.ft_append.restype = ctypes.c_int
+        lib.ft_extend.argtypes = [ctypes.POINTER(ExtendArgs)]
+        lib.ft_extend.restype = ctypes.c_int
+        lib.ft_extend_path_name.argtypes = [ctypes.POINTER(ExtendArgs)]
+        lib.ft_extend_path_name.restype = ctypes.c_char_p
+        lib.ft_extend_plan_build.argtypes = [i64p] * 5 + [i32] * 5 + [i64, i32, ctypes.POINTER(ctypes.c_void_p)]
+        lib.ft_extend_plan_build.restype = ctypes.c_int
+        lib.ft_extend_plan_get_info.argtypes = [ctypes.c_void_p, ctypes.POINTER(ExtendPlanInfo)]
+        lib.ft_extend_plan_get_info.restype = ctypes.c_int
+        lib.ft_extend_plan_copy.argtypes = [ctypes.c_void_p, i32p]
+        lib.ft_extend_plan_copy.restype = ctypes.c_int
+        lib.ft_extend_plan_free.argtypes = [ctypes.c_void_p]
+        lib.ft_extend_plan_free.restype = None
         _lib = lib
     return _lib
 
@@ -195,8 +248,9 @@ def call_module():
             loader = importlib.machinery.ExtensionFileLoader("ft_call", _build.CALL_PATH)
             mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("ft_call", loader))
             loader.exec_module(mod)
-            mod.bind(*(ctypes.cast(getattr(handle, n), ctypes.c_void_p).value for n in ("ft_decode", "ft_stage1", "ft_stage2")),
-                     handle.ft_decode_args_size())
+            mod.bind(*(ctypes.cast(getattr(handle, n), ctypes.c_void_p).value
+                       for n in ("ft_decode", "ft_stage1", "ft_stage2", "ft_append", "ft_extend")),
+                     handle.ft_decode_args_size(), handle.ft_append_args_size(), handle.ft_extend_args_size())
             _call = mod
     return _call
 

@@ -19,6 +19,7 @@ if _PKG not in sys.path:
     sys.path.insert(0, _PKG)
 
 from ft_b200 import engine as _engine      # noqa: E402
+from ft_b200 import extend as _extend      # noqa: E402
 from ft_b200 import planner as _planner    # noqa: E402
 
 
@@ -163,3 +164,24 @@ def fasttree_decode_host_io(q, k_buffer, v_buffer, o, *aux_and_tiles, logit_cap=
             _HOST_IO_CALLS.clear()
         _HOST_IO_CALLS[key] = call
     call()
+
+
+def fasttree_append(q, k, v, k_buffer, v_buffer, slots, q_out=None, positions=None, cos_sin=None, sections=None,
+                    interleaved=False):
+    """A step's new tokens enter the paged cache: ``q`` and ``k`` are turned by their positions, ``k`` and ``v`` go to the
+    pool rows ``slots`` (:func:`ft_b200.extend.append`).  No counterpart in the reference, whose host does this."""
+    _extend.append(q, k, v, k_buffer, v_buffer, slots, q_out=q_out, positions=positions, cos_sin=cos_sin, sections=sections,
+                   interleaved=interleaved)
+
+
+def fasttree_extend_preparation(seq_lens, extend_lens, kv_starts, num_qo_heads, num_kv_heads, head_dim, dtype,
+                                shared_prefixes=None, window=0, device="cuda"):
+    """Plan for :func:`fasttree_extend`, one per step, for every layer (:func:`ft_b200.extend.prepare`)."""
+    return _extend.prepare(seq_lens, extend_lens, kv_starts, num_qo_heads, num_kv_heads, head_dim, dtype,
+                           shared_prefixes=shared_prefixes, window=window, device=device)
+
+
+def fasttree_extend(q, k_buffer, v_buffer, o, kv_entries, plan, sm_scale, logit_cap=-1, o_lse=None):
+    """Causal attention of a step's new tokens - one per request, a question, a whole prompt - over the paged cache; writes
+    ``o`` on the current CUDA stream (:func:`ft_b200.extend.extend`).  Here ``logit_cap`` is applied."""
+    _extend.extend(q, k_buffer, v_buffer, o, kv_entries, plan, sm_scale, logit_cap=logit_cap, o_lse=o_lse)

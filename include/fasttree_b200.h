@@ -56,7 +56,8 @@ enum ft_device_flag {
   FT_DEV_BAD_KV_INDEX = 1,  /* a gathered K/V row index was outside [0, kv_rows) */
   FT_DEV_BAD_Q_INDEX = 2,   /* a request id was outside [0, batch) */
   FT_DEV_BAD_ROW_INDEX = 4, /* a partial-row id was outside [0, num_partial_rows) */
-  FT_DEV_WAIT_TIMEOUT = 8   /* a bounded barrier wait gave up */
+  FT_DEV_WAIT_TIMEOUT = 8,  /* a bounded barrier wait gave up */
+  FT_DEV_BAD_POSITION = 16  /* ft_append: a position was outside the cosine / sine table */
 };
 
 /*
@@ -354,6 +355,125 @@ int ft_plan_copy_tables(const ft_plan* plan, int32_t* vnode_to_kv_entries, int32
  * when short nodes were packed into groups); FT_ERR_INVALID_ARGUMENT otherwise. */
 int ft_plan_copy_row_ranges(const ft_plan* plan, int32_t* vnode_q_kv_ranges);
 void ft_plan_free(ft_plan* plan);
+
+/* ---- new tokens: into the paged cache, and their attention -----------------------------------------------
+ * The reference leaves both to its host (SGLang's rotary embedding, store_kv_cache and extend attention kernels);
+ * they have no counterpart in it. */
+
+/* A step's new tokens enter the paged cache: q and k are turned by the tokens' positions, k and v are written to the
+ * tokens' pool rows.  Pair i < rot_dim / 2 of a head - its elements (i, i + rot_dim / 2), or (2 i, 2 i + 1) if
+ * interleaved - becomes (x1 c - x2 s, x2 c + x1 s), with c = cos_sin[pos][i], s = cos_sin[pos][rot_dim / 2 + i] and pos
+ * the token's position along the axis whose section the pair falls into; the elements from rot_dim on stay as they are.
+ * All pointers are device pointers, strides are in elements, the innermost stride is 1. */
+typedef struct ft_append_args {
+  const void* q;       /* [tokens, num_qo_heads, head_dim], or NULL: keys and values only */
+  const void* k;       /* [tokens, num_kv_heads, head_dim]                                 */
+  const void* v;       /* same shape as k                                                  */
+  void* q_out;         /* shape of q; may be q itself, must not overlap it otherwise       */
+  void* k_buffer;      /* [kv_rows, num_kv_heads, head_dim], written at the slots          */
+  void* v_buffer;
+  const void* slots;   /* [tokens] pool rows, int32 or int64; -1: a padding token, which is not stored.  A row named twice
+                          holds either token's values, or parts of both */
+  const void* positions; /* [num_axes][tokens] int32 or int64 */
+  const float* cos_sin;  /* [cos_sin_rows, rot_dim] fp32: cosines, then sines */
+  int32_t dtype;       /* enum ft_dtype, of every tensor but the tables */
+  int32_t tokens;
+  int32_t num_qo_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t rot_dim;     /* 0: no rotation (positions, cos_sin unused); else even and at most head_dim */
+  int32_t num_axes;    /* 1 to 4 */
+  int32_t sections[4]; /* pairs of each axis, in order; together rot_dim / 2 */
+  int32_t interleaved;
+  int32_t slots_64;
+  int32_t positions_64;
+  int64_t kv_rows;
+  int64_t cos_sin_rows, cos_sin_stride0, positions_stride0;
+  int64_t q_stride0, q_stride1;
+  int64_t k_stride0, k_stride1;
+  int64_t v_stride0, v_stride1;
+  int64_t q_out_stride0, q_out_stride1;
+  int64_t k_buffer_stride0, k_buffer_stride1;
+  int64_t v_buffer_stride0, v_buffer_stride1;
+  void* stream;        /* cudaStream_t */
+} ft_append_args;
+
+int ft_append_args_size(void);
+
+/* One launch on args->stream; no host synchronisation, nothing is allocated.  A slot that is neither -1 nor a pool row is
+ * skipped and flagged (FT_DEV_BAD_KV_INDEX); a token with a position outside the table is left out whole and flagged
+ * (FT_DEV_BAD_POSITION). */
+int ft_append(const ft_append_args* args);
+
+/* The schedule of one extend-attention step: which query rows run together, over which K/V, on which SM.  Pure host code,
+ * like ft_plan.  `batch` requests; request i has seq_lens[i] tokens in the cache, of which the last extend_lens[i] are the
+ * step's queries (rows q_starts[i] .. of q); its tokens' pool rows are kv_entries[kv_starts[i] ..].  Requests that share a
+ * prefix stand next to one another: the first shared_with_previous[i] entries of request i are those of request i - 1
+ * (0: nothing is known; at most the cached part seq_len - extend_len of either), and such a prefix is read once for all of
+ * them.  window > 0: a query sees the newest `window` positions up to its own.  elem_bytes: 2 or 4. */
+typedef struct ft_extend_plan ft_extend_plan;
+
+typedef struct ft_extend_plan_info {
+  int64_t table_ints;     /* length of the table that ft_extend_plan_copy fills */
+  int64_t items_off, segments_off, tokens_off, sm_offs_off, sm_tasks_off, merge_off, merge_rows_off; /* its parts */
+  int64_t kv_entries_len; /* entries of kv_entries that the plan names: at least as many have to be there */
+  int64_t q_rows;         /* one more than the largest row of q that it names */
+  int64_t pieces;         /* work items */
+  int32_t num_items, num_segments, num_tokens, num_merged; /* num_merged: query tokens whose K/V is split over items */
+  int32_t partial_rows;   /* rows of mid_o / mid_lse */
+  int32_t num_sms;        /* CTAs of the scheduled form */
+  int32_t num_qo_heads, num_kv_heads, head_dim, window, elem_bytes;
+  int32_t rows_per_tile, tile_tokens; /* query rows (tokens x GQA group) of a query tile, tokens of a K/V tile */
+  int32_t reserved;
+} ft_extend_plan_info;
+
+int ft_extend_plan_build(const int64_t* seq_lens, const int64_t* extend_lens, const int64_t* kv_starts, const int64_t* q_starts,
+                         const int64_t* shared_with_previous, int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
+                         int32_t head_dim, int32_t elem_bytes, int64_t window, int32_t num_sms, ft_extend_plan** out);
+int ft_extend_plan_get_info(const ft_extend_plan* plan, ft_extend_plan_info* info);
+int ft_extend_plan_copy(const ft_extend_plan* plan, int32_t* table);
+void ft_extend_plan_free(ft_extend_plan* plan);
+
+enum ft_extend_path {
+  FT_EXTEND_AUTO = 0,
+  FT_EXTEND_GENERIC = 1, /* scalar fp32 kernel, a warp per query row: any dtype, head_dim <= 256 */
+  FT_EXTEND_TCGEN05 = 2  /* tcgen05/TMEM kernel: 16-bit types, head_dim 64, 128, 256, at most 128 query heads per KV head */
+};
+
+/* Causal attention of a step's new tokens over the paged cache that holds their prefixes and themselves:
+ * o[t] = softmax_j(cap(sm_scale q[t] . k_j)) v_j over the positions j <= pos(t) of t's request, or the newest `window` of
+ * them; cap(s) = logit_cap tanh(s / logit_cap) if logit_cap > 0, else s.  Rows of o that no query of the plan names are left
+ * as they are. */
+typedef struct ft_extend_args {
+  const void* q;         /* [q_rows, num_qo_heads, head_dim] */
+  const void* k_buffer;  /* [kv_rows, num_kv_heads, head_dim] */
+  const void* v_buffer;
+  void* o;               /* shape of q, written */
+  float* o_lse;          /* optional [q_rows, num_qo_heads] log(sum)+max, or NULL */
+  int32_t dtype;
+  int32_t num_qo_heads, num_kv_heads, head_dim;
+  int32_t path;          /* enum ft_extend_path */
+  float sm_scale;
+  float logit_cap;       /* <= 0: no cap */
+  int32_t reserved;
+  int64_t q_rows, kv_rows;
+  int64_t q_stride0, q_stride1;
+  int64_t k_stride0, k_stride1;
+  int64_t v_stride0, v_stride1;
+  int64_t o_stride0, o_stride1;
+  const int32_t* kv_entries; /* pool rows, the table that the plan's kv_starts index */
+  int64_t kv_entries_len;
+  const int32_t* plan_table; /* device copy of the table of ft_extend_plan_copy, 16-byte aligned */
+  ft_extend_plan_info plan;
+  float* mid_o;          /* [partial_rows, num_qo_heads, head_dim] and [partial_rows, num_qo_heads], packed; the call's */
+  float* mid_lse;        /* own scratch, may be NULL if the plan has no partial rows.  Calls that may overlap need their own */
+  void* stream;
+} ft_extend_args;
+
+int ft_extend_args_size(void);
+int ft_extend(const ft_extend_args* args);
+/* names of the kernels that ft_extend would launch, as ft_stage1_path_name gives them */
+const char* ft_extend_path_name(const ft_extend_args* args);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,167 @@
+"""The schedule of extend attention, checked on the host: what every query token is shown, exactly once, and nothing else."""
+import random
+
+import numpy as np
+import pytest
+import torch
+
+import extend_cases
+from ft_b200 import extend, lib
+
+ITEM, SEG = 24, 8
+
+
+def shown(info, table, entries):
+    """Per q row: the pool rows it is shown, in the order of the items (with repetitions, were there any), its writers and the
+    partial rows of its merge list."""
+    t = table.tolist()
+    items = [t[info.items_off + ITEM * i:info.items_off + ITEM * (i + 1)] for i in range(info.num_items)]
+    seen, writers, parts = {}, {}, {}
+    for it in items:
+        seg0, nseg, t0, t1, step, q_tiles, length = it[:7]
+        for w in range(2):
+            tok0, ntok, lo, hi, part, q_tile, first = it[8 + 8 * w:15 + 8 * w]
+            assert 0 <= q_tile < q_tiles
+            if ntok:
+                assert t0 <= lo < hi <= t1 and ntok * (info.num_qo_heads // info.num_kv_heads) <= max(
+                    info.rows_per_tile, info.num_qo_heads // info.num_kv_heads)
+            for tok in range(ntok):
+                q_row, pos = t[info.tokens_off + 2 * (tok0 + tok):info.tokens_off + 2 * (tok0 + tok) + 2]
+                got = []
+                for s in range(seg0, seg0 + nseg):
+                    lo32, hi32, slen, pos0, tlo, thi, voff, _ = t[info.segments_off + SEG * s:info.segments_off + SEG * (s + 1)]
+                    off = (hi32 << 32) | (lo32 & 0xffffffff)
+                    assert 0 <= voff and voff + slen <= length
+                    if not tlo <= first + tok < thi:
+                        continue
+                    a = max(pos - info.window + 1 - pos0, 0) if info.window else 0
+                    for j in range(a, min(slen, pos + 1 - pos0)):
+                        tile = (voff + j) // info.tile_tokens
+                        if lo <= tile < hi and (step == 1 or (tile - lo) % 2 == 0):
+                            got.append(int(entries[off + j]))
+                seen.setdefault(q_row, []).extend(got)
+                if part >= 0:
+                    parts.setdefault(q_row, []).append(part + tok)
+                else:
+                    writers[q_row] = writers.get(q_row, 0) + 1
+    merged = {}
+    for i in range(info.num_merged):
+        q_row, off, n, _ = t[info.merge_off + 4 * i:info.merge_off + 4 * i + 4]
+        merged[q_row] = t[info.merge_rows_off + off:info.merge_rows_off + off + n]
+        writers[q_row] = writers.get(q_row, 0) + 1
+    return seen, writers, parts, merged
+
+
+def check(seq, ext, shared, hq, hkv, d, dtype=torch.float16, window=0, sms=148):
+    table, _ = extend_cases.pool(seq, ext, shared)
+    width = table.shape[1]
+    info, plan, _, _ = extend.host_plan(seq, ext, [r * width for r in range(len(seq))], hq, hkv, d, dtype,
+                                        shared_prefixes=shared, window=window, num_sms=sms)
+    entries = table.reshape(-1).numpy()
+    seen, writers, parts, merged = shown(info, plan, entries)
+    row = 0
+    for r, (n, e) in enumerate(zip(seq, ext)):
+        for i in range(e):
+            pos = n - e + i
+            want = entries[r * width + (max(0, pos - window + 1) if window else 0):r * width + pos + 1]
+            assert sorted(seen[row]) == sorted(want.tolist()), (r, i)
+            assert writers[row] == 1
+            assert sorted(merged.get(row, [])) == sorted(parts.get(row, []))
+            row += 1
+    assert row == info.num_tokens == sum(ext) and set(seen) == set(range(row))
+    used = sorted(x for p in parts.values() for x in p)
+    assert used == list(range(info.partial_rows))                  # no partial row has two writers
+    # every task is dealt once
+    offs = plan[info.sm_offs_off:info.sm_offs_off + info.num_sms + 1]
+    tasks = plan[info.sm_tasks_off:info.sm_tasks_off + info.num_items * hkv]
+    assert offs[0] == 0 and (np.diff(offs) >= 0).all() and offs[-1] == info.num_items * hkv
+    assert sorted(tasks.tolist()) == list(range(info.num_items * hkv))
+    return info
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.float16, 64), (torch.bfloat16, 128), (torch.bfloat16, 256), (torch.float32, 128),
+                                     (torch.float16, 16)])
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (16, 16), (28, 4), (16, 1), (5, 1)])
+def test_every_token_is_shown_its_positions_once(dtype, d, hq, hkv):
+    check([1, 130, 257, 40], [1, 130, 7, 40], [], hq, hkv, d, dtype)
+    check([700] * 6, [1, 0, 3, 1, 60, 2], [(list(range(6)), 500)], hq, hkv, d, dtype)
+    check([300, 310, 500, 520, 90], [9, 17, 1, 33, 90], [([0, 1], 200), ([2, 3], 470), ([0, 1, 2, 3], 128)], hq, hkv, d, dtype)
+
+
+@pytest.mark.parametrize("window", [1, 2, 100, 128, 1000, 5000])
+def test_windows(window):
+    check([900, 300, 1500], [40, 300, 1], [], 8, 2, 128, window=window)
+    check([700] * 5, [3, 1, 20, 1, 1], [(list(range(5)), 640)], 8, 2, 128, window=window)
+    check([700] * 5, [3, 1, 20, 1, 1], [(list(range(5)), 640)], 8, 2, 256, torch.bfloat16, window=window)
+
+
+def test_no_requests_and_requests_without_new_tokens():
+    assert check([], [], [], 8, 2, 128).num_items == 0
+    assert check([50, 60], [0, 0], [([0, 1], 50)], 8, 2, 128).num_items == 0
+    check([50, 60, 70], [0, 1, 0], [([0, 1, 2], 50)], 8, 2, 128)
+
+
+def test_long_context_is_cut_into_items():
+    info = check([20000], [1], [], 8, 1, 128)
+    assert info.num_items > 20 and info.num_merged == 1
+    info = check([20000] * 2, [1, 1], [([0, 1], 19990)], 8, 1, 128)
+    assert info.num_items > 20
+
+
+def test_a_shared_prefix_stands_once():
+    n = 16
+    alone = check([4100] * n, [2] * n, [], 8, 2, 128)
+    together = check([4100] * n, [2] * n, [(list(range(n)), 4098)], 8, 2, 128)
+    assert together.num_segments < alone.num_segments * 2 + n
+    def tokens(info, plan):
+        return sum(plan[info.segments_off + SEG * s + 2] for s in range(info.num_segments))
+
+    table, _ = extend_cases.pool([4100] * n, [2] * n, [(list(range(n)), 4098)])
+    starts = [r * table.shape[1] for r in range(n)]
+    a = extend.host_plan([4100] * n, [2] * n, starts, 8, 2, 128, torch.float16)
+    b = extend.host_plan([4100] * n, [2] * n, starts, 8, 2, 128, torch.float16, shared_prefixes=[(list(range(n)), 4098)])
+    assert tokens(b[0], b[1]) == 4098 + 2 * n and tokens(a[0], a[1]) == 4100 * n
+
+
+def test_random_steps():
+    rng = random.Random(5)
+    for _ in range(60):
+        n = rng.randint(1, 12)
+        shared_len = rng.choice((0, rng.randint(1, 600)))
+        cached = [shared_len + rng.choice((0, rng.randint(0, 500))) for _ in range(n)]
+        ext = [rng.choice((0, 1, rng.randint(1, 90))) for _ in range(n)]
+        seq = [c + e for c, e in zip(cached, ext)]
+        groups = []
+        if shared_len and n > 1:
+            groups.append((list(range(n)), shared_len))
+            half = list(range(0, n, 2))
+            if len(half) > 1:
+                groups.append((half, min(cached[m] for m in half)))
+        hq, hkv = rng.choice(((8, 2), (4, 4), (7, 1), (16, 2)))
+        check(seq, ext, groups, hq, hkv, rng.choice((64, 128, 256)), rng.choice((torch.float16, torch.float32)),
+              window=rng.choice((0, 0, rng.randint(1, 700))), sms=rng.choice((4, 148)))
+
+
+def test_offsets_beyond_32_bits():
+    start = [3 << 32, (3 << 32) + 1000]
+    info, plan, _, _ = extend.host_plan([300, 200], [5, 6], start, 8, 2, 128, torch.float16)
+    offs = {int((int(plan[info.segments_off + SEG * s + 1]) << 32) | (int(plan[info.segments_off + SEG * s]) & 0xffffffff))
+            for s in range(info.num_segments)}
+    assert offs == set(start) and info.kv_entries_len == (3 << 32) + 1200
+
+
+def test_refusals():
+    ok = dict(seq_lens=[5, 6], extend_lens=[1, 2], kv_starts=[0, 10], num_qo_heads=8, num_kv_heads=2, head_dim=128,
+              dtype=torch.float16)
+    extend.host_plan(**ok)
+    for bad in (dict(extend_lens=[1]), dict(extend_lens=[6, 1]), dict(extend_lens=[-1, 1]), dict(kv_starts=[-1, 0]),
+                dict(num_qo_heads=7), dict(num_kv_heads=0), dict(dtype=torch.int8), dict(window=-1), dict(seq_lens=[5.5, 6.5]),
+                dict(shared_prefixes=[([0, 1], 5)]), dict(shared_prefixes=[([0, 2], 1)]), dict(shared_prefixes=[([0, 1], -1)])):
+        with pytest.raises(ValueError):
+            extend.host_plan(**{**ok, **bad})
+    with pytest.raises(lib.FastTreeError):
+        extend.host_plan(**{**ok, "head_dim": 96})
+    with pytest.raises(lib.FastTreeError):
+        extend.host_plan(**{**ok, "seq_lens": [2 ** 31, 6]})
+    with pytest.raises(ValueError):
+        extend.prepare(**ok, device="cpu")
