@@ -292,7 +292,24 @@ struct MapKey {
 
 // Descriptor of a [rows, heads, head_dim] 16-bit tensor (element strides s0, s1), box 64 (head_dim) x box_heads x
 // box_rows, 128-byte swizzle; with box_heads 0 the same tensor as [rows, all elements of a row] with a box of 64 x 1,
-// the form that gathers rows.  Descriptors are cached by buffer identity (encoding one costs about a microsecond)
+// the form that gathers rows.
+bool encode_map(CUtensorMap* out, const void* base, int dtype, int head_dim, int64_t rows, int heads, int64_t s0, int64_t s1,
+                int box_heads, int box_rows) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (enc == nullptr || rows <= 0 || rows > 0x7fffffffLL || heads <= 0) return false;
+  const bool flat = box_heads == 0;
+  const int64_t row_elems = (int64_t)(heads - 1) * s1 + head_dim;
+  if (flat && (s1 < 0 || row_elems > s0 || row_elems > 0x7fffffffLL)) return false;  // rows that overlap: no 2-D tensor
+  const cuuint64_t dims[3] = {(cuuint64_t)(flat ? row_elems : head_dim), (cuuint64_t)(flat ? rows : heads), (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)(flat ? s0 : s1) * 2, (cuuint64_t)s0 * 2};  // bytes, for dimensions 1 and 2
+  const cuuint32_t box[3] = {64, (cuuint32_t)(flat ? 1 : box_heads), (cuuint32_t)box_rows};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return enc(out, dtype == FT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, flat ? 2 : 3,
+             const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// encode_map for the decode kernels.  Descriptors are cached by buffer identity (encoding one costs about a microsecond)
 // in a hash table of 1024 slots, probed linearly over 8 slots; a full neighbourhood evicts its first slot.  A
 // serving process holds four descriptors per layer's K/V buffers (six at head_dim 256) plus two per query shape - a few
 // hundred at most.
@@ -321,21 +338,8 @@ bool tensor_map(CUtensorMap* out, const void* base, int dtype, int head_dim, int
     if (!used[j] && slot < 0) slot = j;
   }
   if (slot < 0) slot = home;
-  EncodeTiledFn enc = encode_tiled_fn();
-  if (enc == nullptr || rows <= 0 || rows > 0x7fffffffLL || heads <= 0) return false;
-  const bool flat = box_heads == 0;
-  const int64_t row_elems = (int64_t)(heads - 1) * s1 + head_dim;
-  if (flat && (s1 < 0 || row_elems > s0 || row_elems > 0x7fffffffLL)) return false;  // rows that overlap: no 2-D tensor
-  const cuuint64_t dims[3] = {(cuuint64_t)(flat ? row_elems : head_dim), (cuuint64_t)(flat ? rows : heads), (cuuint64_t)rows};
-  const cuuint64_t strides[2] = {(cuuint64_t)(flat ? s0 : s1) * 2, (cuuint64_t)s0 * 2};  // bytes, for dimensions 1 and 2
-  const cuuint32_t box[3] = {64, (cuuint32_t)(flat ? 1 : box_heads), (cuuint32_t)box_rows};
-  const cuuint32_t estr[3] = {1, 1, 1};
   CUtensorMap m;
-  const CUresult rc = enc(&m, dtype == FT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, flat ? 2 : 3,
-                          const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (rc != CUDA_SUCCESS) return false;
+  if (!encode_map(&m, base, dtype, head_dim, rows, heads, s0, s1, box_heads, box_rows)) return false;
   keys[slot] = key;
   maps[slot] = m;
   used[slot] = true;

@@ -3,6 +3,7 @@
 
 #include "ft_append.cuh"
 #include "ft_extend.cuh"
+#include "ft_extend_tc.cuh"
 
 namespace {
 
@@ -45,22 +46,80 @@ int launch_append_for(const ft::AppendParams& p, cudaStream_t st) {
   return vec ? launch_append<T, VEC>(p, st) : launch_append<T, 1>(p, st);
 }
 
+// Can the tensor-core kernel take these arguments?  A reason, or NULL.
 const char* extend_tc_obstacle(const ft_extend_args* a) {
   if (a->dtype == FT_F32) return "fp32 inputs";
   if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) return "head_dim not 64, 128 or 256";
   if (a->plan.rows_per_tile != 128) return "more than 128 query heads per KV head";
-  return "not built yet";
+  // (a stride along one head is never used)
+  const int64_t q1 = a->num_qo_heads > 1 ? a->q_stride1 : 0, o1 = a->num_qo_heads > 1 ? a->o_stride1 : 0;
+  const int64_t k1 = a->num_kv_heads > 1 ? a->k_stride1 : 0, v1 = a->num_kv_heads > 1 ? a->v_stride1 : 0;
+  if (!vector_rows(a->q, a->q_stride0, q1, 8, 2) || !vector_rows(a->k_buffer, a->k_stride0, k1, 8, 2) ||
+      !vector_rows(a->v_buffer, a->v_stride0, v1, 8, 2) || !vector_rows(a->o, a->o_stride0, o1, 8, 2))
+    return "q, k_buffer, v_buffer and o need 16-byte aligned rows";
+  return nullptr;
+}
+
+// The descriptors of a call.  They are made anew for each: a step's queries are new tensors every time.  false: the queries'
+// layout has none, and the scalar kernel takes the call.
+template <int D>
+bool extend_maps(ft::ExtendTcParams& tp, const ft_extend_args* a) {
+  const int G = a->num_qo_heads / a->num_kv_heads, tile = ft::ExtCfg<D>::TILE, dt = a->dtype;
+  const int64_t q1 = a->num_qo_heads > 1 ? a->q_stride1 : D, k1 = a->num_kv_heads > 1 ? a->k_stride1 : D, v1 = a->num_kv_heads > 1 ? a->v_stride1 : D;
+  tp.q_box_heads = G % 8 == 0 ? 8 : G;
+  if (!encode_map(&tp.q_map, a->q, dt, D, a->q_rows, a->num_qo_heads, a->q_stride0, q1, tp.q_box_heads, 1) ||
+      !encode_map(&tp.q_map_tile, a->q, dt, D, a->q_rows, a->num_qo_heads, a->q_stride0, q1, G, 128 / G))
+    return false;
+  tp.has_tma = encode_map(&tp.k_map, a->k_buffer, dt, D, a->kv_rows, a->num_kv_heads, a->k_stride0, k1, 1, tile) &&
+               encode_map(&tp.v_map, a->v_buffer, dt, D, a->kv_rows, a->num_kv_heads, a->v_stride0, v1, 1, tile);
+  tp.has_gather4 = encode_map(&tp.k_rows_map, a->k_buffer, dt, D, a->kv_rows, a->num_kv_heads, a->k_stride0, k1, 0, 1) &&
+                   encode_map(&tp.v_rows_map, a->v_buffer, dt, D, a->kv_rows, a->num_kv_heads, a->v_stride0, v1, 0, 1);
+  return true;
+}
+
+template <typename T, int D, bool CAP>
+int launch_extend_tc(const ft::ExtendTcParams& tp, int ctas, cudaStream_t st) {
+  using C = ft::ExtCfg<D>;
+  auto kernel = ft::extend_tc_kernel<T, D, CAP>;
+  static OncePerDevice once;
+  FT_CUDA_OK(raise_smem_limit(once, kernel, C::SMEM_BYTES));
+  if (C::NW == 2) {  // the warpgroups trade the registers that the block is launched with: it has to have them
+    static const int regs = [&] {
+      cudaFuncAttributes at;
+      return cudaFuncGetAttributes(&at, kernel) == cudaSuccess ? at.numRegs : 0;
+    }();
+    if (regs != C::REGS_LAUNCH) return fail(FT_ERR_UNSUPPORTED, "the kernel was built with %d registers a thread, not %d", regs, C::REGS_LAUNCH);
+  }
+  kernel<<<(unsigned)ctas, C::THREADS, C::SMEM_BYTES, st>>>(tp);
+  FT_CUDA_OK(cudaGetLastError());
+  count_launch();
+  return FT_OK;
+}
+
+// 1: launched (or named), 0: this call's layout has no descriptors, < 0: an error
+template <typename T, int D>
+int try_extend_tc(const ft::ExtendParams& p, const ft_extend_args* a, cudaStream_t st) {
+  ft::ExtendTcParams tp;
+  memset(&tp, 0, sizeof(tp));
+  tp.p = p;
+  if (!extend_maps<D>(tp, a)) return 0;
+  if (dry_run("extend_tc_kernel")) return 1;
+  const int rc = p.logit_cap > 0.f ? launch_extend_tc<T, D, true>(tp, a->plan.num_sms, st) : launch_extend_tc<T, D, false>(tp, a->plan.num_sms, st);
+  return rc == FT_OK ? 1 : rc;
 }
 
 template <typename T>
 int launch_extend(const ft::ExtendParams& p, const ft_extend_args* a, bool tensor, cudaStream_t st) {
-  const int64_t ctas = (int64_t)p.num_items * p.kv_heads;
-  if (ctas > 0) {
-    if (!dry_run("extend_generic_kernel")) {
-      ft::extend_generic_kernel<T><<<(unsigned)ctas, 128, 0, st>>>(p);
-      FT_CUDA_OK(cudaGetLastError());
-      count_launch();
-    }
+  int done = 0;
+  if constexpr (sizeof(T) == 2) {
+    if (tensor) done = p.head_dim == 64 ? try_extend_tc<T, 64>(p, a, st) : p.head_dim == 128 ? try_extend_tc<T, 128>(p, a, st) : try_extend_tc<T, 256>(p, a, st);
+    if (done < 0) return done;
+    if (tensor && done == 0 && a->path == FT_EXTEND_TCGEN05) return fail(FT_ERR_UNSUPPORTED, "tcgen05 path: no TMA descriptor for the layout of q");
+  }
+  if (done == 0 && !dry_run("extend_generic_kernel")) {
+    ft::extend_generic_kernel<T><<<(unsigned)(p.num_items * p.kv_heads), 128, 0, st>>>(p);
+    FT_CUDA_OK(cudaGetLastError());
+    count_launch();
   }
   const int64_t merges = (int64_t)p.num_merged * p.heads;
   if (merges > 0 && !dry_run("extend_merge_kernel")) {
@@ -159,8 +218,8 @@ int ft_extend(const ft_extend_args* a) {
   p.sm_offs = a->plan_table + pl.sm_offs_off, p.sm_tasks = a->plan_table + pl.sm_tasks_off;
   p.merged = a->plan_table + pl.merge_off, p.merge_rows = a->plan_table + pl.merge_rows_off;
   p.mid_o = a->mid_o, p.mid_lse = a->mid_lse;
-  p.q_s0 = a->q_stride0, p.q_s1 = a->q_stride1, p.k_s0 = a->k_stride0, p.k_s1 = a->k_stride1;
-  p.v_s0 = a->v_stride0, p.v_s1 = a->v_stride1, p.o_s0 = a->o_stride0, p.o_s1 = a->o_stride1;
+  p.q_s0 = a->q_stride0, p.q_s1 = a->q_stride1, p.k_s0 = a->k_stride0, p.k_s1 = a->num_kv_heads > 1 ? a->k_stride1 : 0;
+  p.v_s0 = a->v_stride0, p.v_s1 = a->num_kv_heads > 1 ? a->v_stride1 : 0, p.o_s0 = a->o_stride0, p.o_s1 = a->o_stride1;
   p.kv_rows = a->kv_rows, p.q_rows = a->q_rows, p.kv_entries_len = a->kv_entries_len;
   p.num_items = pl.num_items, p.num_merged = pl.num_merged, p.partial_rows = pl.partial_rows;
   p.heads = a->num_qo_heads, p.kv_heads = a->num_kv_heads, p.group = a->num_qo_heads / a->num_kv_heads, p.head_dim = a->head_dim;

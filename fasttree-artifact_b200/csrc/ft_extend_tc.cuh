@@ -1,0 +1,642 @@
+// Extend attention on the 5th-generation tensor cores: a CTA per SM walks its share of the plan's (item, KV head) tasks.
+//
+//   S_w[128 x TILE] = Q_w[128 x D] . K_tile^T      tcgen05.mma, A and B K-major
+//   O_w[128 x D]   += P_w[128 x TILE] . V_tile     tcgen05.mma, A = P in tensor memory, B MN-major
+//
+// At head_dim 64 and 128 two streams w = 0, 1 run through the K/V tiles: two query tiles (128 packed rows of tokens x GQA
+// group each) that share every K/V tile in shared memory, or one query tile whose even and odd K/V tiles are streams of
+// their own, so that either way one stream's softmax runs beside the other's products.  At head_dim 256, where O alone is
+// half of tensor memory, there is one stream, and the scores of a tile are computed beside the softmax of the one before.
+//
+// Roles (warps): one softmax warpgroup per stream (thread = query row = TMEM lane), then one warp each for the MMA issue,
+// K loads, V loads and Q loads.  All of them walk the same task list on their own; mbarriers (full / empty per buffer) are
+// the only hand-offs, and the counters behind their phases run on from task to task, so the next task's Q and K are loaded
+// and its first scores computed while the last rows of the task before are normalised and stored.  Every wait is bounded
+// and unwinds the CTA through an abort flag.
+//
+// A K/V tile whose rows are consecutive in the pool is one TMA box per 64 columns; any other is gathered four rows at a
+// time through the TMA unit, its last rows with 16-byte copies.  Rows of V behind the last token are zeroed up to the next
+// 16, where the product ends; rows of K are not: their scores are masked.
+//
+// Softmax: a thread reads its row of S, masks what the row does not see (bits from the tile's segments; tiles inside one
+// segment and inside the row's range skip that), keeps a running maximum that may lag by 2^8 before O is rescaled in
+// tensor memory, and writes P in the storage type; the row's sum is of the unrounded probabilities in fp32.  P takes the
+// place of S, except at head_dim 64, where the products have different shapes and their order is not the order of issue:
+// there P has columns of its own.  When a stream's scores are ready all its earlier products are done (tcgen05.commit covers
+// every MMA issued before it), so no wait is needed before O is rescaled with two streams; with one there is a barrier for it.
+//
+// Capped scores: cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap)).
+//
+// Rows of V that a query does not see are multiplied by P = 0, and 0 x Inf is NaN: a row that is not shown everything and did
+// not come out finite is computed again from its own tokens (extend_row).
+#pragma once
+
+#include "ft_extend.cuh"
+#include "ft_stage1_tc.cuh"
+
+namespace ft {
+
+struct alignas(64) ExtendTcParams {
+  CUtensorMap k_map;       // [rows, kv heads, head_dim], box 64 x 1 x TILE
+  CUtensorMap v_map;
+  CUtensorMap k_rows_map;  // [rows, all heads' elements], box 64 x 1, for gathers
+  CUtensorMap v_rows_map;
+  CUtensorMap q_map;       // [q rows, heads, head_dim], box 64 x G x 1 (at most 8 heads where G is a multiple of 8)
+  CUtensorMap q_map_tile;  // box 64 x G x 128 / G
+  ExtendParams p;
+  int has_tma, has_gather4, q_box_heads;
+};
+
+template <int D_>
+struct ExtCfg {
+  static constexpr int D = D_;
+  static constexpr int NW = D <= 128 ? 2 : 1;       // streams
+  static constexpr int TILE = D <= 128 ? 128 : 64;  // tokens of a K/V tile
+  static constexpr int NB = D / 64;                 // 64-element column blocks of an operand row
+  static constexpr int THREADS = 128 * NW + 128;
+  static constexpr int Q_BYTES = NB * 16384;        // one query tile
+  static constexpr int KV_BLOCK = TILE * 128;       // one column block of a K/V tile
+  static constexpr int KV_BYTES = NB * KV_BLOCK;
+  static constexpr int NSK = D == 64 ? 5 : 3, NSV = D == 64 ? 5 : 2;
+  static constexpr int Q_OFF = 0, K_OFF = NW * Q_BYTES, V_OFF = K_OFF + NSK * KV_BYTES;
+  static constexpr int IDS_OFF = V_OFF + NSV * KV_BYTES;  // row ids of the tile being gathered, K's and V's
+  static constexpr int BAR_OFF = IDS_OFF + 2 * TILE * 4;
+  static constexpr int K_FULL = 0, K_EMPTY = K_FULL + NSK, V_FULL = K_EMPTY + NSK, V_EMPTY = V_FULL + NSV, S_FULL = V_EMPTY + NSV,
+                       P_FULL = S_FULL + 2, O_FULL = P_FULL + 2, PV_DONE = O_FULL + 2, Q_FULL = PV_DONE + 2, Q_EMPTY = Q_FULL + 1,
+                       NBARS = Q_EMPTY + 1;
+  static constexpr int ABORT_OFF = BAR_OFF + NBARS * 8, TMEM_SLOT_OFF = ABORT_OFF + 4, SMEM_BYTES = TMEM_SLOT_OFF + 4;
+  // tensor memory columns.  Two streams: S_w, then O_w, then (head_dim 64) P_w.  One: two S buffers, O.
+  static constexpr int S_COL = 0, O_COL = 256, P_COL = D == 64 ? 384 : S_COL;
+  static constexpr int S_STEP = NW == 2 ? 128 : 64, P_STEP = D == 64 ? 64 : S_STEP;
+  static constexpr int PV_N = D == 128 ? 128 : 64;  // columns of O per product
+  static constexpr int CPR = D / 8;                 // 16-byte chunks of a row
+  static constexpr int REGS_SOFTMAX = 208, REGS_OTHER = 88, REGS_LAUNCH = 168;
+  static constexpr int WAIT_LIMIT = 1 << 22;
+  static_assert(SMEM_BYTES <= 232448, "one CTA must fit in one SM's shared memory");
+  static_assert(NW != 2 || (2 * REGS_SOFTMAX + REGS_OTHER) * 128 <= REGS_LAUNCH * THREADS, "register trade must balance");
+};
+
+template <int D>
+__device__ __forceinline__ bool ext_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  for (int it = 0; it < ExtCfg<D>::WAIT_LIMIT; ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((it & 15) == 15 && *abort_flag != 0) return false;
+  }
+  return false;
+}
+
+// Walks the segments of a block forward, tile by tile.
+struct SegmentCursor {
+  const int32_t* segs;
+  int at, end;
+  ExtendSegment g;
+  __device__ __forceinline__ void open(const int32_t* table, int seg0, int nseg) {
+    segs = table;
+    at = seg0;
+    end = seg0 + nseg;
+    g = extend_segment(segs, at);
+  }
+  // the segment that holds virtual position v, or the last one
+  __device__ __forceinline__ void forward(int v) {
+    while (v >= g.voff + g.len && at + 1 < end) g = extend_segment(segs, ++at);
+  }
+};
+
+template <typename T, int D, bool CAP>
+__global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const __grid_constant__ ExtendTcParams tp) {
+  using C = ExtCfg<D>;
+  constexpr int TILE = C::TILE, NB = C::NB, NW = C::NW;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const ExtendParams& p = tp.p;
+  const uint32_t sm = smem_u32(smem), bars = sm + C::BAR_OFF;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::ABORT_OFF);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::TMEM_SLOT_OFF);
+  auto bar = [&](int i) { return bars + 8u * i; };
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  allow_dependent_launch();
+  wait_for_prior_grid();
+  const int task_lo = p.sm_offs[blockIdx.x], task_hi = p.sm_offs[blockIdx.x + 1];
+  if (task_lo >= task_hi) return;
+  if ((sm & 1023u) != 0u) {  // the swizzled operand layout needs a 1024-byte aligned window
+    if (tid == 0) flag_error(FT_DEV_WAIT_TIMEOUT);
+    return;
+  }
+  if (tid == 0) {
+    for (int b = 0; b < C::NSK; ++b) {
+      mbar_init(bar(C::K_FULL + b), 32);
+      mbar_init(bar(C::K_EMPTY + b), 1);
+    }
+    for (int b = 0; b < C::NSV; ++b) {
+      mbar_init(bar(C::V_FULL + b), 32);
+      mbar_init(bar(C::V_EMPTY + b), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar(C::S_FULL + b), 1);
+      mbar_init(bar(C::P_FULL + b), 128);
+      mbar_init(bar(C::O_FULL + b), 1);
+      mbar_init(bar(C::PV_DONE + b), 1);
+    }
+    mbar_init(bar(C::Q_FULL), 1);
+    mbar_init(bar(C::Q_EMPTY), 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(sm + C::TMEM_SLOT_OFF), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int G = p.group;
+  bool dead = false;
+  auto give_up = [&]() {
+    *abort_flag = 1;
+    flag_error(FT_DEV_WAIT_TIMEOUT);
+    dead = true;
+  };
+  auto item_of = [&](int n, int& kvh) {
+    const int task = __ldg(p.sm_tasks + n);
+    kvh = task % p.kv_heads;
+    return p.items + (int64_t)EXT_ITEM_INTS * (task / p.kv_heads);
+  };
+
+  if (warp < 4 * NW) {
+    // ====================================================================== softmax, one query row per thread
+    if constexpr (NW == 2) reg_grow<C::REGS_SOFTMAX>();
+    const int w = warp >> 2, row = tid & 127;
+    const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t o_col = t_lane + C::O_COL + w * D;
+    const float scale = p.sm_scale == 0.f ? 1.17549435e-38f : fabsf(p.sm_scale);
+    constexpr float LOG2E = 1.4426950408889634f;
+    // scores in powers of two: S x scale2; capped ones c2 - 2 c2 / (1 + 2^(S x k2))
+    const float scale2 = CAP ? 1.f : scale * LOG2E;
+    const float c2 = CAP ? p.logit_cap * LOG2E : 0.f, k2 = CAP ? 2.f * LOG2E * scale / p.logit_cap : 0.f;
+    int tiles_done = 0, items_done = 0;
+    for (int n = task_lo; n < task_hi && !dead; ++n) {
+      int kvh;
+      const int32_t* item = item_of(n, kvh);
+      const ExtendStream st = extend_stream(item, w);
+      if (st.ntok == 0) continue;
+      const int step = __ldg(item + 4);
+      const int rows = st.ntok * G;
+      const bool live = row < rows, warp_live = (row & ~31) < rows;
+      const int tok = live ? row / G : 0, head = kvh * G + (live ? row - tok * G : 0);
+      const int2 tk = __ldg(reinterpret_cast<const int2*>(p.tokens) + st.tok0 + tok);
+      const int pos = tk.y, btok = st.first + tok;
+      SegmentCursor cur;
+      cur.open(p.segs, __ldg(item), __ldg(item + 1));
+      float m_used = -INFINITY, l_run = 0.f;
+      bool hidden = false;  // this row was shown less than all of its tiles
+      for (int t = st.lo; t < st.hi; t += step) {
+        const int v0 = t * TILE;
+        // which of the tile's tokens this row sees
+        uint32_t see[TILE / 32];
+        cur.forward(v0);
+        bool all = false;
+        if (live) {
+          int lo, hi;
+          extend_in_sight(cur.g, btok, pos, p.window, lo, hi);
+          all = lo <= v0 && hi >= v0 + TILE;
+        }
+        bool any = all;
+        if (!__all_sync(0xffffffffu, all || !live)) {
+#pragma unroll
+          for (int k = 0; k < TILE / 32; ++k) see[k] = 0;
+          SegmentCursor c2r = cur;
+          while (true) {  // (the same segments for the whole warp)
+            if (live) {
+              int lo, hi;
+              extend_in_sight(c2r.g, btok, pos, p.window, lo, hi);
+              lo -= v0;
+              hi -= v0;
+#pragma unroll
+              for (int k = 0; k < TILE / 32; ++k) see[k] |= bits_below(hi - 32 * k) & ~bits_below(lo - 32 * k);
+            }
+            if (c2r.g.voff + c2r.g.len >= v0 + TILE || c2r.at + 1 >= c2r.end) break;
+            c2r.g = extend_segment(c2r.segs, ++c2r.at);
+          }
+          uint32_t some = 0;
+#pragma unroll
+          for (int k = 0; k < TILE / 32; ++k) some |= see[k];
+          any = some != 0;
+          hidden |= !all;
+        }
+        const int buf = NW == 2 ? w : tiles_done & 1;
+        const uint32_t phase = NW == 2 ? (uint32_t)tiles_done & 1u : (uint32_t)(tiles_done >> 1) & 1u;
+        ++tiles_done;
+        const uint32_t s_col = t_lane + C::S_COL + buf * C::S_STEP, p_col = t_lane + C::P_COL + buf * C::P_STEP;
+        if (!ext_wait<D>(bar(C::S_FULL + buf), phase, abort_flag)) {
+          give_up();
+          break;
+        }
+        tc_fence_after();
+        if (!__any_sync(0xffffffffu, any)) {  // nothing in sight of the warp's rows
+          if (warp_live) {
+            float zero[32];
+#pragma unroll
+            for (int c = 0; c < 32; ++c) zero[c] = 0.f;
+#pragma unroll
+            for (int c = 0; c < TILE / 64; ++c) tmem_st32(p_col + 32 * c, zero);
+            tmem_wait_st();
+          }
+          tc_fence_before();
+          mbar_arrive(bar(C::P_FULL + buf));
+          continue;
+        }
+        float s[TILE];
+#pragma unroll
+        for (int c = 0; c < TILE / 32; ++c) tmem_ld32_nowait(s_col + 32 * c, *reinterpret_cast<float(*)[32]>(&s[32 * c]));
+        tmem_wait_ld();
+        if constexpr (CAP) {
+#pragma unroll
+          for (int c = 0; c < TILE; ++c) {
+            float y, r;
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(s[c] * k2));
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y + 1.f));
+            s[c] = fmaf(-2.f * c2, r, c2);
+          }
+        }
+        if (!__all_sync(0xffffffffu, all || !live)) {
+#pragma unroll
+          for (int k = 0; k < TILE / 32; ++k)
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if ((see[k] & (1u << c)) == 0) s[32 * k + c] = -INFINITY;
+        }
+        float mx4[4] = {fmaxf(s[0], s[1]), fmaxf(s[2], s[3]), fmaxf(s[4], s[5]), fmaxf(s[6], s[7])};
+#pragma unroll
+        for (int c = 8; c < TILE; c += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) asm("max.f32 %0, %0, %1, %2;" : "+f"(mx4[k]) : "f"(s[c + 2 * k]), "f"(s[c + 2 * k + 1]));
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale2;
+        float corr = 1.f;
+        bool grow = false;
+        if (mx > m_used + 8.f || m_used == -INFINITY) {  // the offset may lag the true maximum by up to 2^8
+          if (mx > -INFINITY) {
+            grow = m_used > -INFINITY;
+            corr = fast_exp2(m_used - mx);  // 0 at the row's first tokens
+            m_used = mx;
+          }
+        }
+        l_run *= corr;
+        if (t > st.lo && __any_sync(0xffffffffu, grow)) {
+          if constexpr (NW == 1) {  // P.V of the tile before has to be done
+            if (!ext_wait<D>(bar(C::PV_DONE + (buf ^ 1)), (uint32_t)((tiles_done - 2) >> 1) & 1u, abort_flag)) {
+              give_up();
+              break;
+            }
+            tc_fence_after();
+          }
+#pragma unroll
+          for (int cb = 0; cb < D / 32; ++cb) {
+            float o[32];
+            tmem_ld32(o_col + cb * 32, o);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) o[c] *= corr;
+            tmem_st32(o_col + cb * 32, o);
+          }
+        }
+        const float neg_off = m_used == -INFINITY ? 0.f : -m_used;
+        const float2 sc2 = make_float2(scale2, scale2), no2 = make_float2(neg_off, neg_off);
+        float2 sum4[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int h = 0; h < TILE / 64; ++h) {
+          uint32_t wds[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            float2 x = __ffma2_rn(make_float2(s[64 * h + 2 * i], s[64 * h + 2 * i + 1]), sc2, no2);
+            x.x = fast_exp2(x.x);
+            x.y = fast_exp2(x.y);
+            sum4[i & 3] = __fadd2_rn(sum4[i & 3], x);
+            wds[i] = pack2<T>(x.x, x.y);
+          }
+          tmem_st32(p_col + 32 * h, *reinterpret_cast<float(*)[32]>(&wds[0]));
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar(C::P_FULL + buf));
+        const float2 sum2 = __fadd2_rn(__fadd2_rn(sum4[0], sum4[1]), __fadd2_rn(sum4[2], sum4[3]));
+        l_run += sum2.x + sum2.y;
+      }
+      if (dead) break;
+      // ---- the row's result: normalised, to o or to its partial row
+      if (!ext_wait<D>(bar(C::O_FULL + w), (uint32_t)items_done & 1u, abort_flag)) {
+        give_up();
+        break;
+      }
+      ++items_done;
+      tc_fence_after();
+      if (!warp_live) continue;
+      const bool store = live && tk.x >= 0 && tk.x < p.q_rows;
+      if (live && !store) flag_error(FT_DEV_BAD_Q_INDEX);
+      const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+      float2 finite = make_float2(0.f, 0.f);  // 0 x every element: 0, or NaN
+      float* mid = st.part >= 0 ? p.mid_o + ((int64_t)(st.part + tok) * p.heads + head) * D : nullptr;
+      T* out = reinterpret_cast<T*>(p.o) + (int64_t)(store ? tk.x : 0) * p.o_s0 + (int64_t)head * p.o_s1;
+#pragma unroll
+      for (int cb = 0; cb < D / 32; ++cb) {
+        float o[32];
+        tmem_ld32(o_col + cb * 32, o);
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          const float2 x = __fmul2_rn(make_float2(o[2 * c], o[2 * c + 1]), make_float2(inv, inv));
+          finite = __ffma2_rn(x, make_float2(0.f, 0.f), finite);
+          o[2 * c] = x.x;
+          o[2 * c + 1] = x.y;
+        }
+        if (store) {
+          if (mid != nullptr) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              reinterpret_cast<float4*>(mid + cb * 32)[c] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              reinterpret_cast<uint4*>(out + cb * 32)[c] = make_uint4(pack2<T>(o[8 * c], o[8 * c + 1]), pack2<T>(o[8 * c + 2], o[8 * c + 3]),
+                                                                     pack2<T>(o[8 * c + 4], o[8 * c + 5]), pack2<T>(o[8 * c + 6], o[8 * c + 7]));
+          }
+        }
+      }
+      if (store)
+        extend_store_lse(p, st.part, tok, tk.x, head, l_run == 0.f ? -INFINITY : (m_used + log2f(l_run)) * 0.6931471805599453f);
+      const bool spoiled = store && hidden && !(finite.x + finite.y == 0.f);
+      for (uint32_t todo = __ballot_sync(0xffffffffu, spoiled); todo != 0; todo &= todo - 1) {
+        const int r = (row & ~31) + __ffs(todo) - 1;
+        __syncwarp();
+        extend_row<T>(p, item, st, r / G, kvh * G + r % G);
+      }
+    }
+  } else {
+    if constexpr (NW == 2) reg_shrink<C::REGS_OTHER>();
+    const int role = warp - 4 * NW;
+    if (role == 0) {
+      // ==================================================================== MMA issue
+      if (lane == 0) {
+        const uint32_t idesc_s = tc_idesc<T>(128, TILE, false, p.sm_scale < 0.f), idesc_o = tc_idesc<T>(128, C::PV_N, true);
+        int kt = 0, vt = 0;  // K and V tiles taken
+        int tiles_done[2] = {0, 0}, items = 0;
+        for (int n = task_lo; n < task_hi && !dead; ++n, ++items) {
+          int kvh;
+          const int32_t* item = item_of(n, kvh);
+          const int t0 = __ldg(item + 2), t1 = __ldg(item + 3), step = __ldg(item + 4), len = __ldg(item + 6);
+          const ExtendStream s0 = extend_stream(item, 0), s1 = NW == 2 ? extend_stream(item, 1) : s0;
+          auto active = [&](int w, int t) {
+            const int lo = w == 0 ? s0.lo : s1.lo, hi = w == 0 ? s0.hi : s1.hi;
+            return t >= lo && t < hi && (step == 1 || ((t - lo) & 1) == 0);
+          };
+          if (!ext_wait<D>(bar(C::Q_FULL), (uint32_t)items & 1u, abort_flag)) {
+            give_up();
+            break;
+          }
+          bool k_here = false, v_here = false;
+          auto wait_k = [&]() {
+            if (!k_here && !ext_wait<D>(bar(C::K_FULL + kt % C::NSK), (uint32_t)(kt / C::NSK) & 1u, abort_flag)) give_up();
+            k_here = true;
+          };
+          auto wait_v = [&]() {
+            if (!v_here && !ext_wait<D>(bar(C::V_FULL + vt % C::NSV), (uint32_t)(vt / C::NSV) & 1u, abort_flag)) give_up();
+            v_here = true;
+          };
+          auto issue_qk = [&](int w, int buf, int q_tile) {
+            wait_k();
+            if (dead) return;
+            proxy_fence();
+            tc_fence_after();
+            const uint64_t q_desc = tc_desc(sm + C::Q_OFF + q_tile * C::Q_BYTES, 16, 1024);
+            const uint64_t k_desc = tc_desc(sm + C::K_OFF + (kt % C::NSK) * C::KV_BYTES, 16, 1024);
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks)  // k-steps of 16 along head_dim: +32 B inside a block, +1 block after 4
+              tc_mma(tmem + C::S_COL + buf * C::S_STEP, q_desc + (uint64_t)((ks >> 2) * (16384 >> 4) + (ks & 3) * 2),
+                     k_desc + (uint64_t)((ks >> 2) * (C::KV_BLOCK >> 4) + (ks & 3) * 2), idesc_s, ks > 0);
+            tc_commit(bar(C::S_FULL + buf));
+          };
+          auto issue_pv = [&](int w, int t, bool first, bool last) {
+            const int g = tiles_done[w]++, buf = NW == 2 ? w : g & 1;
+            const uint32_t phase = NW == 2 ? (uint32_t)g & 1u : (uint32_t)(g >> 1) & 1u;
+            if (!ext_wait<D>(bar(C::P_FULL + buf), phase, abort_flag)) give_up();
+            if (!dead) wait_v();
+            if (dead) return;
+            proxy_fence();
+            tc_fence_after();
+            const uint32_t a = tmem + C::P_COL + buf * C::P_STEP, v_buf = sm + C::V_OFF + (vt % C::NSV) * C::KV_BYTES;
+            const int ksteps = min(TILE, len - t * TILE + 15) >> 4;  // the rows of V behind the next 16 are not defined
+#pragma unroll
+            for (int h = 0; h < D / C::PV_N; ++h) {
+              const uint64_t v_desc = tc_desc(v_buf + h * C::KV_BLOCK, C::KV_BLOCK, 1024);
+              for (int ks = 0; ks < ksteps; ++ks)
+                tc_mma_ts(tmem + C::O_COL + w * D + h * C::PV_N, a + (uint32_t)(ks * 8), v_desc + (uint64_t)(ks * 128), idesc_o,
+                          (!first || ks > 0) ? 1u : 0u);
+            }
+            if (NW == 1) tc_commit(bar(C::PV_DONE + buf));
+            if (last) tc_commit(bar(C::O_FULL + w));
+          };
+          auto release_k = [&]() {
+            wait_k();
+            if (!dead) tc_commit(bar(C::K_EMPTY + kt % C::NSK));
+            ++kt;
+            k_here = false;
+          };
+          auto release_v = [&]() {
+            wait_v();
+            if (!dead) tc_commit(bar(C::V_EMPTY + vt % C::NSV));
+            ++vt;
+            v_here = false;
+          };
+          if constexpr (NW == 2) {
+            // iteration t: the products with V of tile t - step, then the scores of tile t, stream by stream
+            for (int t = t0; t < t1 + step && !dead; ++t) {
+              const int tp_ = t - step;
+#pragma unroll
+              for (int w = 0; w < 2; ++w) {
+                const int lo = w == 0 ? s0.lo : s1.lo, hi = w == 0 ? s0.hi : s1.hi;
+                if (tp_ >= t0 && active(w, tp_)) issue_pv(w, tp_, tp_ == lo, tp_ + step >= hi);
+                if (!dead && t < t1 && active(w, t)) issue_qk(w, w, w == 0 ? s0.q_tile : s1.q_tile);
+                if (dead) break;
+              }
+              if (t < t1 && !dead) release_k();
+              if (t == t1 - 1 && !dead) tc_commit(bar(C::Q_EMPTY));
+              if (tp_ >= t0 && tp_ < t1 && !dead) release_v();
+            }
+          } else {
+            for (int t = t0; t <= t1 && !dead; ++t) {
+              if (t < t1) {
+                issue_qk(0, (tiles_done[0] + (t > t0 ? 1 : 0)) & 1, 0);
+                if (!dead) release_k();
+                if (t == t1 - 1 && !dead) tc_commit(bar(C::Q_EMPTY));
+              }
+              if (t > t0 && !dead) {
+                issue_pv(0, t - 1, t - 1 == t0, t == t1);
+                if (!dead) release_v();
+              }
+            }
+          }
+        }
+      }
+      __syncwarp();
+    } else if (role <= 2) {
+      // ==================================================================== K loads (role 1), V loads (role 2)
+      const bool is_k = role == 1;
+      const CUtensorMap* map = is_k ? &tp.k_map : &tp.v_map;
+      const CUtensorMap* rows_map = is_k ? &tp.k_rows_map : &tp.v_rows_map;
+      const int64_t s0 = is_k ? p.k_s0 : p.v_s0, s1 = is_k ? p.k_s1 : p.v_s1;
+      const T* base0 = reinterpret_cast<const T*>(is_k ? p.k : p.v);
+      const int full0 = is_k ? C::K_FULL : C::V_FULL, empty0 = is_k ? C::K_EMPTY : C::V_EMPTY, stages = is_k ? C::NSK : C::NSV;
+      const uint32_t ring = sm + (is_k ? C::K_OFF : C::V_OFF);
+      const uint32_t ids_sm = sm + C::IDS_OFF + (is_k ? 0 : TILE * 4);
+      const uint32_t row_lim = (uint32_t)(p.kv_rows < 0x7fffffffLL ? p.kv_rows : 0x7fffffffLL);
+      int count = 0;
+      for (int n = task_lo; n < task_hi && !dead; ++n) {
+        int kvh;
+        const int32_t* item = item_of(n, kvh);
+        const int t0 = __ldg(item + 2), t1 = __ldg(item + 3), len = __ldg(item + 6);
+        SegmentCursor cur;
+        cur.open(p.segs, __ldg(item), __ldg(item + 1));
+        const T* base = base0 + (int64_t)kvh * s1;
+        auto fetch_ids = [&](int t, int (&dst)[TILE / 32]) {
+          cur.forward(t * TILE);
+          SegmentCursor c = cur;
+#pragma unroll
+          for (int h = 0; h < TILE / 32; ++h) {
+            const int v = t * TILE + lane + 32 * h;
+            dst[h] = -1;
+            if (v < len) {
+              c.forward(v);
+              dst[h] = __ldg(p.kv_entries + c.g.kv_off + (v - c.g.voff));
+            }
+          }
+        };
+        int id[TILE / 32], nxt[TILE / 32];
+        fetch_ids(t0, id);
+        for (int t = t0; t < t1; ++t, ++count) {
+          if (t + 1 < t1) fetch_ids(t + 1, nxt);
+          const int valid = min(TILE, len - t * TILE);
+          const int first = __shfl_sync(0xffffffffu, id[0], 0);
+          bool dense = true, in_pool = true;
+#pragma unroll
+          for (int h = 0; h < TILE / 32; ++h) {
+            dense &= id[h] == first + lane + 32 * h;
+            in_pool &= lane + 32 * h >= valid || (uint32_t)id[h] < row_lim;
+          }
+          in_pool = __all_sync(0xffffffffu, in_pool);
+          dense = tp.has_tma && valid == TILE && in_pool && __all_sync(0xffffffffu, dense);
+          const int b = count % stages;
+          if (!ext_wait<D>(bar(empty0 + b), ((uint32_t)(count / stages) & 1u) ^ 1u, abort_flag)) {
+            give_up();
+            break;
+          }
+          const uint32_t buf = ring + b * C::KV_BYTES, full = bar(full0 + b);
+          if (dense) {
+            if (lane == 0) {
+              mbar_arrive_expect_tx(full, C::KV_BYTES);
+#pragma unroll
+              for (int h = 0; h < NB; ++h) tma_load_3d(buf + h * C::KV_BLOCK, map, 64 * h, kvh, first, full);
+            } else {
+              mbar_arrive(full);
+            }
+          } else {
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < TILE / 32; ++h)
+              asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(ids_sm + (lane + 32 * h) * 4), "r"(id[h]) : "memory");
+            int done = 0;
+            if (tp.has_gather4 && in_pool) {
+              done = valid & ~3;
+              if (lane == 0 && done > 0) mbar_expect_tx(full, (uint32_t)done * (2u * D));
+              __syncwarp();
+              for (int i = lane; i < done / 4 * NB; i += 32) {
+                const int blk = i % NB, r = i / NB * 4;
+                int r0, r1, r2, r3;
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(ids_sm + r * 4));
+                tma_gather4(buf + blk * C::KV_BLOCK + r * 128, rows_map, kvh * (int)s1 + 64 * blk, r0, r1, r2, r3, full);
+              }
+            } else {
+              __syncwarp();
+            }
+            // what is left, 16 bytes at a time; of V zeros up to the next 16 rows
+            const int end = is_k ? valid : (valid + 15) & ~15, c16 = lane % C::CPR;
+            for (int r = done + lane / C::CPR; r < end; r += 32 / C::CPR) {
+              int row_id;
+              asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(row_id) : "r"(ids_sm + r * 4));
+              const bool ok = (uint32_t)row_id < row_lim;  // (behind the last token -1)
+              cp_async16_zfill(buf + (uint32_t)((c16 >> 3) * C::KV_BLOCK) + tc_swz(r, c16 & 7, 0), base + (int64_t)(ok ? row_id : 0) * s0 + c16 * 8, ok);
+            }
+            if (!in_pool && lane == 0) flag_error(FT_DEV_BAD_KV_INDEX);
+            mbar_arrive_on_cp_async(full);
+          }
+#pragma unroll
+          for (int h = 0; h < TILE / 32; ++h) id[h] = nxt[h];
+        }
+      }
+      cp_async_wait<0>();
+    } else {
+      // ==================================================================== Q loads
+      int items = 0;
+      for (int n = task_lo; n < task_hi && !dead; ++n, ++items) {
+        int kvh;
+        const int32_t* item = item_of(n, kvh);
+        const int q_tiles = __ldg(item + 5);
+        if (!ext_wait<D>(bar(C::Q_EMPTY), ((uint32_t)items & 1u) ^ 1u, abort_flag)) {
+          give_up();
+          break;
+        }
+        // bytes first: a whole tile if its tokens' rows are consecutive, else a box per token
+        uint32_t bytes = 0;
+        bool in_order[2] = {false, false};
+        int first[2] = {0, 0};
+        for (int w = 0; w < q_tiles; ++w) {
+          const ExtendStream st = extend_stream(item, w);
+          first[w] = __ldg(p.tokens + 2 * st.tok0);
+          bool mine = true, valid = true;
+          int rows = 0;
+          for (int i = lane; i < st.ntok; i += 32) {
+            const int r = __ldg(p.tokens + 2 * (st.tok0 + i));
+            mine &= r == first[w] + i;
+            if (r >= 0 && r < p.q_rows) ++rows;
+            else valid = false;
+          }
+          in_order[w] = __all_sync(0xffffffffu, mine && valid);
+          rows = __reduce_add_sync(0xffffffffu, rows);
+          bytes += in_order[w] ? (uint32_t)(128 / G * G) * (2u * D) : (uint32_t)rows * G * (2u * D);
+        }
+        if (lane == 0) mbar_arrive_expect_tx(bar(C::Q_FULL), bytes);
+        __syncwarp();
+        for (int w = 0; w < q_tiles; ++w) {
+          const ExtendStream st = extend_stream(item, w);
+          const uint32_t dst = sm + C::Q_OFF + w * C::Q_BYTES;
+          if (in_order[w]) {
+            if (lane < NB) tma_load_3d(dst + lane * 16384, &tp.q_map_tile, 64 * lane, kvh * G, first[w], bar(C::Q_FULL));
+          } else {
+            for (int i = lane; i < st.ntok; i += 32) {
+              const int r = __ldg(p.tokens + 2 * (st.tok0 + i));
+              if (r < 0 || r >= p.q_rows) continue;
+              for (int sub = 0; sub < G; sub += tp.q_box_heads)
+#pragma unroll
+                for (int h = 0; h < NB; ++h)
+                  tma_load_3d(dst + (uint32_t)(i * G + sub) * 128 + h * 16384, &tp.q_map, 64 * h, kvh * G + sub, r, bar(C::Q_FULL));
+            }
+          }
+        }
+      }
+    }
+  }
+
+  // ---- release tensor memory
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag != 0)  // copies that nobody waits for any more land before the CTA ends
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+}  // namespace ft
