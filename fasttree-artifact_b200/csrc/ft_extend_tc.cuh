@@ -62,7 +62,7 @@ struct ExtCfg {
   static constexpr int IDS_OFF = V_OFF + NSV * KV_BYTES;  // row ids of the tile being gathered, K's and V's
   static constexpr int BAR_OFF = IDS_OFF + 2 * TILE * 4;
   static constexpr int K_FULL = 0, K_EMPTY = K_FULL + NSK, V_FULL = K_EMPTY + NSK, V_EMPTY = V_FULL + NSV, S_FULL = V_EMPTY + NSV,
-                       P_FULL = S_FULL + 2, O_FULL = P_FULL + 2, PV_DONE = O_FULL + 2, Q_FULL = PV_DONE + 2, Q_EMPTY = Q_FULL + 1,
+                       P_HALF = S_FULL + 2, P_FULL = P_HALF + 2, O_FULL = P_FULL + 2, PV_DONE = O_FULL + 2, Q_FULL = PV_DONE + 2, Q_EMPTY = Q_FULL + 1,
                        NBARS = Q_EMPTY + 1;
   static constexpr int ABORT_OFF = BAR_OFF + NBARS * 8, TMEM_SLOT_OFF = ABORT_OFF + 4, SMEM_BYTES = TMEM_SLOT_OFF + 4;
   // tensor memory columns.  Two streams: S_w, then O_w, then (head_dim 64) P_w.  One: two S buffers, O.
@@ -75,6 +75,41 @@ struct ExtCfg {
   static_assert(SMEM_BYTES <= 232448, "one CTA must fit in one SM's shared memory");
   static_assert(NW != 2 || (2 * REGS_SOFTMAX + REGS_OTHER) * 128 <= REGS_LAUNCH * THREADS, "register trade must balance");
 };
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// One lane of the (whole) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(one));
+  return one != 0;
+}
+
+// Operand descriptors as two words: the low one holds the address and the leading offset, the high one the stride of 8 rows (1024
+// bytes), the version and the 128-byte swizzle, which are the same for every operand here.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo_bytes) { return ((addr >> 4) & 0x3fffu) | ((lbo_bytes >> 4) << 16); }
+constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(acc), "r"(DESC_HI)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(acc), "r"(DESC_HI)
+      : "memory");
+}
 
 template <int D>
 __device__ __forceinline__ bool ext_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
@@ -89,6 +124,38 @@ __device__ __forceinline__ bool ext_wait(uint32_t bar, uint32_t parity, volatile
     if ((it & 15) == 15 && *abort_flag != 0) return false;
   }
   return false;
+}
+
+// What the row `row` of stream w of task n sees of the tile that starts at virtual position v0, as bits; false: nothing.  `seg`
+// is the item's segment that held the tile before (-1: none yet) and becomes the one that holds v0; [all_lo, all_hi) becomes the
+// part of it that the row sees whole, seg_end its end.
+template <int TILE>
+__device__ __noinline__ bool see_tile(const ExtendParams& p, int n, int w, int row, int v0, int& seg, int& seg_end, int& all_lo, int& all_hi,
+                                      uint32_t (&see)[TILE / 32]) {
+  const int32_t* item = p.items + (int64_t)EXT_ITEM_INTS * (__ldg(p.sm_tasks + n) / p.kv_heads);
+  const ExtendStream st = extend_stream(item, w);
+  const bool live = row < st.ntok * p.group;
+  const int tok = live ? row / p.group : 0, pos = __ldg(p.tokens + 2 * (st.tok0 + tok) + 1);
+  const int end = __ldg(item) + __ldg(item + 1);
+  if (seg < 0) seg = __ldg(item);
+  ExtendSegment g = extend_segment(p.segs, seg);
+  while (v0 >= g.voff + g.len && seg + 1 < end) g = extend_segment(p.segs, ++seg);
+  seg_end = g.voff + g.len;
+  extend_in_sight(g, st.first + tok, pos, p.window, all_lo, all_hi);
+#pragma unroll
+  for (int k = 0; k < TILE / 32; ++k) see[k] = 0;
+  for (int sg = seg;;) {  // (the same segments for the whole warp)
+    int lo, hi;
+    extend_in_sight(g, st.first + tok, pos, p.window, lo, hi);
+#pragma unroll
+    for (int k = 0; k < TILE / 32; ++k) see[k] |= live ? bits_below(hi - v0 - 32 * k) & ~bits_below(lo - v0 - 32 * k) : 0u;
+    if (g.voff + g.len >= v0 + TILE || sg + 1 >= end) break;
+    g = extend_segment(p.segs, ++sg);
+  }
+  uint32_t some = 0;
+#pragma unroll
+  for (int k = 0; k < TILE / 32; ++k) some |= see[k];
+  return some != 0;
 }
 
 // Walks the segments of a block forward, tile by tile.
@@ -118,7 +185,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::ABORT_OFF);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::TMEM_SLOT_OFF);
   auto bar = [&](int i) { return bars + 8u * i; };
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   allow_dependent_launch();
   wait_for_prior_grid();
   const int task_lo = p.sm_offs[blockIdx.x], task_hi = p.sm_offs[blockIdx.x + 1];
@@ -138,6 +205,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar(C::S_FULL + b), 1);
+      mbar_init(bar(C::P_HALF + b), 128);
       mbar_init(bar(C::P_FULL + b), 128);
       mbar_init(bar(C::O_FULL + b), 1);
       mbar_init(bar(C::PV_DONE + b), 1);
@@ -179,55 +247,42 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
     // scores in powers of two: S x scale2; capped ones c2 - 2 c2 / (1 + 2^(S x k2))
     const float scale2 = CAP ? 1.f : scale * LOG2E;
     const float c2 = CAP ? p.logit_cap * LOG2E : 0.f, k2 = CAP ? 2.f * LOG2E * scale / p.logit_cap : 0.f;
+    auto capped = [&](float x) {
+      float y, r;
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * k2));
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y + 1.f));
+      return fmaf(-2.f * c2, r, c2);
+    };
     int tiles_done = 0, items_done = 0;
     for (int n = task_lo; n < task_hi && !dead; ++n) {
-      int kvh;
-      const int32_t* item = item_of(n, kvh);
-      const ExtendStream st = extend_stream(item, w);
-      if (st.ntok == 0) continue;
-      const int step = __ldg(item + 4);
-      const int rows = st.ntok * G;
-      const bool live = row < rows, warp_live = (row & ~31) < rows;
-      const int tok = live ? row / G : 0, head = kvh * G + (live ? row - tok * G : 0);
-      const int2 tk = __ldg(reinterpret_cast<const int2*>(p.tokens) + st.tok0 + tok);
-      const int pos = tk.y, btok = st.first + tok;
-      SegmentCursor cur;
-      cur.open(p.segs, __ldg(item), __ldg(item + 1));
+      int lo, hi, step, rows;  // of the stream: K/V tiles lo, lo + step, ... below hi, rows of the query tile
+      {
+        int kvh;
+        const int32_t* item = item_of(n, kvh);
+        const ExtendStream st = extend_stream(item, w);
+        lo = st.lo;
+        hi = st.hi;
+        rows = st.ntok * G;
+        step = __ldg(item + 4);
+      }
+      if (rows == 0) continue;
+      const bool warp_live = (row & ~31) < rows;
       float m_used = -INFINITY, l_run = 0.f;
       bool hidden = false;  // this row was shown less than all of its tiles
-      for (int t = st.lo; t < st.hi; t += step) {
+      // Virtual positions [all_lo, all_hi) of segment `seg`, every one of which the row sees: a tile inside them needs no mask.
+      // (What only the other tiles and the end need is read again there: the registers go to the scores.)
+      int seg = -1, seg_end = 0, all_lo = 0, all_hi = 0;
+      for (int t = lo; t < hi; t += step) {
         const int v0 = t * TILE;
-        // which of the tile's tokens this row sees
         uint32_t see[TILE / 32];
-        cur.forward(v0);
-        bool all = false;
-        if (live) {
-          int lo, hi;
-          extend_in_sight(cur.g, btok, pos, p.window, lo, hi);
-          all = lo <= v0 && hi >= v0 + TILE;
-        }
-        bool any = all;
-        if (!__all_sync(0xffffffffu, all || !live)) {
+        bool any = row < rows, full = true;
+        if (v0 >= seg_end || !__all_sync(0xffffffffu, row >= rows || (v0 >= all_lo && v0 + TILE <= all_hi))) {
+          any = see_tile<TILE>(p, n, w, row, v0, seg, seg_end, all_lo, all_hi, see);
+          bool everything = true;
 #pragma unroll
-          for (int k = 0; k < TILE / 32; ++k) see[k] = 0;
-          SegmentCursor c2r = cur;
-          while (true) {  // (the same segments for the whole warp)
-            if (live) {
-              int lo, hi;
-              extend_in_sight(c2r.g, btok, pos, p.window, lo, hi);
-              lo -= v0;
-              hi -= v0;
-#pragma unroll
-              for (int k = 0; k < TILE / 32; ++k) see[k] |= bits_below(hi - 32 * k) & ~bits_below(lo - 32 * k);
-            }
-            if (c2r.g.voff + c2r.g.len >= v0 + TILE || c2r.at + 1 >= c2r.end) break;
-            c2r.g = extend_segment(c2r.segs, ++c2r.at);
-          }
-          uint32_t some = 0;
-#pragma unroll
-          for (int k = 0; k < TILE / 32; ++k) some |= see[k];
-          any = some != 0;
-          hidden |= !all;
+          for (int k = 0; k < TILE / 32; ++k) everything &= see[k] == 0xffffffffu;
+          hidden |= !everything;
+          full = __all_sync(0xffffffffu, everything || row >= rows);
         }
         const int buf = NW == 2 ? w : tiles_done & 1;
         const uint32_t phase = NW == 2 ? (uint32_t)tiles_done & 1u : (uint32_t)(tiles_done >> 1) & 1u;
@@ -248,6 +303,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
             tmem_wait_st();
           }
           tc_fence_before();
+          mbar_arrive(bar(C::P_HALF + buf));
           mbar_arrive(bar(C::P_FULL + buf));
           continue;
         }
@@ -255,16 +311,8 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
 #pragma unroll
         for (int c = 0; c < TILE / 32; ++c) tmem_ld32_nowait(s_col + 32 * c, *reinterpret_cast<float(*)[32]>(&s[32 * c]));
         tmem_wait_ld();
-        if constexpr (CAP) {
-#pragma unroll
-          for (int c = 0; c < TILE; ++c) {
-            float y, r;
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(s[c] * k2));
-            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y + 1.f));
-            s[c] = fmaf(-2.f * c2, r, c2);
-          }
-        }
-        if (!__all_sync(0xffffffffu, all || !live)) {
+        if (!full) {
+          __syncwarp();  // (a branch: as predicated code this would run for every tile)
 #pragma unroll
           for (int k = 0; k < TILE / 32; ++k)
 #pragma unroll
@@ -276,7 +324,11 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
         for (int c = 8; c < TILE; c += 8)
 #pragma unroll
           for (int k = 0; k < 4; ++k) asm("max.f32 %0, %0, %1, %2;" : "+f"(mx4[k]) : "f"(s[c + 2 * k]), "f"(s[c + 2 * k + 1]));
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale2;
+        float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+        if constexpr (CAP)
+          mx = any ? capped(mx) : -INFINITY;
+        else
+          mx *= scale2;
         float corr = 1.f;
         bool grow = false;
         if (mx > m_used + 8.f || m_used == -INFINITY) {  // the offset may lag the true maximum by up to 2^8
@@ -287,44 +339,51 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
           }
         }
         l_run *= corr;
-        if (t > st.lo && __any_sync(0xffffffffu, grow)) {
-          if constexpr (NW == 1) {  // P.V of the tile before has to be done
-            if (!ext_wait<D>(bar(C::PV_DONE + (buf ^ 1)), (uint32_t)((tiles_done - 2) >> 1) & 1u, abort_flag)) {
-              give_up();
-              break;
-            }
-            tc_fence_after();
-          }
-#pragma unroll
-          for (int cb = 0; cb < D / 32; ++cb) {
-            float o[32];
-            tmem_ld32(o_col + cb * 32, o);
-#pragma unroll
-            for (int c = 0; c < 32; ++c) o[c] *= corr;
-            tmem_st32(o_col + cb * 32, o);
-          }
-        }
         const float neg_off = m_used == -INFINITY ? 0.f : -m_used;
         const float2 sc2 = make_float2(scale2, scale2), no2 = make_float2(neg_off, neg_off);
-        float2 sum4[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        // P, in halves: the first is handed over while the second is made
 #pragma unroll
-        for (int h = 0; h < TILE / 64; ++h) {
-          uint32_t wds[32];
+        for (int h = 0; h < 2; ++h) {
+          uint32_t wds[TILE / 4];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float2 x = __ffma2_rn(make_float2(s[64 * h + 2 * i], s[64 * h + 2 * i + 1]), sc2, no2);
+          for (int i = 0; i < TILE / 4; ++i) {
+            float2 x = make_float2(s[h * (TILE / 2) + 2 * i], s[h * (TILE / 2) + 2 * i + 1]);
+            if constexpr (CAP) {
+              // (a masked score, -inf, stays one)
+              x.x = x.x == -INFINITY ? x.x : capped(x.x);
+              x.y = x.y == -INFINITY ? x.y : capped(x.y);
+            }
+            x = __ffma2_rn(x, sc2, no2);
             x.x = fast_exp2(x.x);
             x.y = fast_exp2(x.y);
-            sum4[i & 3] = __fadd2_rn(sum4[i & 3], x);
+            sum2[i & 1] = __fadd2_rn(sum2[i & 1], x);
             wds[i] = pack2<T>(x.x, x.y);
           }
-          tmem_st32(p_col + 32 * h, *reinterpret_cast<float(*)[32]>(&wds[0]));
+          if constexpr (TILE == 128)
+            tmem_st32(p_col + 32 * h, *reinterpret_cast<float(*)[32]>(&wds[0]));
+          else
+            tmem_st16(p_col + 16 * h, *reinterpret_cast<uint32_t(*)[16]>(&wds[0]));
+          if (h == 0 && t > lo && __any_sync(0xffffffffu, grow)) {
+            if constexpr (NW == 1) {  // P.V of the tile before has to be done
+              if (!ext_wait<D>(bar(C::PV_DONE + (buf ^ 1)), (uint32_t)((tiles_done - 2) >> 1) & 1u, abort_flag)) give_up();
+              tc_fence_after();
+            }
+#pragma unroll
+            for (int cb = 0; cb < D / 32; ++cb) {
+              float o[32];
+              tmem_ld32(o_col + cb * 32, o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] *= corr;
+              tmem_st32(o_col + cb * 32, o);
+            }
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(bar((h == 1 ? C::P_FULL : C::P_HALF) + buf));
         }
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(bar(C::P_FULL + buf));
-        const float2 sum2 = __fadd2_rn(__fadd2_rn(sum4[0], sum4[1]), __fadd2_rn(sum4[2], sum4[3]));
-        l_run += sum2.x + sum2.y;
+        l_run += (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
+        if (dead) break;
       }
       if (dead) break;
       // ---- the row's result: normalised, to o or to its partial row
@@ -335,6 +394,12 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       ++items_done;
       tc_fence_after();
       if (!warp_live) continue;
+      int kvh;
+      const int32_t* item = item_of(n, kvh);
+      const ExtendStream st = extend_stream(item, w);
+      const bool live = row < rows;
+      const int tok = live ? row / G : 0, head = kvh * G + (live ? row - tok * G : 0);
+      const int2 tk = __ldg(reinterpret_cast<const int2*>(p.tokens) + st.tok0 + tok);
       const bool store = live && tk.x >= 0 && tk.x < p.q_rows;
       if (live && !store) flag_error(FT_DEV_BAD_Q_INDEX);
       const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
@@ -379,103 +444,142 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
     const int role = warp - 4 * NW;
     if (role == 0) {
       // ==================================================================== MMA issue
-      if (lane == 0) {
-        const uint32_t idesc_s = tc_idesc<T>(128, TILE, false, p.sm_scale < 0.f), idesc_o = tc_idesc<T>(128, C::PV_N, true);
-        int kt = 0, vt = 0;  // K and V tiles taken
-        int tiles_done[2] = {0, 0}, items = 0;
-        for (int n = task_lo; n < task_hi && !dead; ++n, ++items) {
+      // The whole warp walks the loop, on values that are the same in every lane (broadcast where they come from memory), so that
+      // the operands of an MMA stand in uniform registers; one lane issues.  With a loop for one lane alone, every MMA waits
+      // for its operands' way into uniform registers: 120 cycles an MMA that takes 64 (4096 tokens behind 12288, 64/8 heads:
+      // 1980 -> 1590 us).
+      const uint32_t idesc_s = tc_idesc<T>(128, TILE, false, p.sm_scale < 0.f), idesc_o = tc_idesc<T>(128, C::PV_N, true);
+      const uint32_t bars_u = __shfl_sync(0xffffffffu, bars, 0), sm_u = __shfl_sync(0xffffffffu, sm, 0), tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+      const bool issuer = elect_one();
+      auto ubar = [&](int i) { return bars_u + 8u * (uint32_t)i; };
+      auto wait = [&](uint32_t b, uint32_t phase) {
+        if (!__all_sync(0xffffffffu, ext_wait<D>(b, phase, abort_flag))) give_up();
+      };
+      int k_stage = 0, v_stage = 0;
+      uint32_t k_phase = 0, v_phase = 0;
+      int tiles_done[2] = {0, 0};
+      uint32_t q_phase = 0;
+      const int tasks_u = __shfl_sync(0xffffffffu, task_hi - task_lo, 0);
+      for (int n = 0; n < tasks_u && !dead; ++n) {
+        int t0, t1, step, len, lo[2], hi[2], q_tile[2];
+        {
           int kvh;
-          const int32_t* item = item_of(n, kvh);
-          const int t0 = __ldg(item + 2), t1 = __ldg(item + 3), step = __ldg(item + 4), len = __ldg(item + 6);
-          const ExtendStream s0 = extend_stream(item, 0), s1 = NW == 2 ? extend_stream(item, 1) : s0;
-          auto active = [&](int w, int t) {
-            const int lo = w == 0 ? s0.lo : s1.lo, hi = w == 0 ? s0.hi : s1.hi;
-            return t >= lo && t < hi && (step == 1 || ((t - lo) & 1) == 0);
-          };
-          if (!ext_wait<D>(bar(C::Q_FULL), (uint32_t)items & 1u, abort_flag)) {
-            give_up();
-            break;
+          const int32_t* item = item_of(task_lo + n, kvh);
+          t0 = __shfl_sync(0xffffffffu, __ldg(item + 2), 0);
+          t1 = __shfl_sync(0xffffffffu, __ldg(item + 3), 0);
+          step = __shfl_sync(0xffffffffu, __ldg(item + 4), 0);
+          len = __shfl_sync(0xffffffffu, __ldg(item + 6), 0);
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const ExtendStream st = extend_stream(item, w);
+            lo[w] = __shfl_sync(0xffffffffu, st.lo, 0);
+            hi[w] = __shfl_sync(0xffffffffu, st.hi, 0);
+            q_tile[w] = __shfl_sync(0xffffffffu, st.q_tile, 0);
           }
-          bool k_here = false, v_here = false;
-          auto wait_k = [&]() {
-            if (!k_here && !ext_wait<D>(bar(C::K_FULL + kt % C::NSK), (uint32_t)(kt / C::NSK) & 1u, abort_flag)) give_up();
-            k_here = true;
-          };
-          auto wait_v = [&]() {
-            if (!v_here && !ext_wait<D>(bar(C::V_FULL + vt % C::NSV), (uint32_t)(vt / C::NSV) & 1u, abort_flag)) give_up();
-            v_here = true;
-          };
-          auto issue_qk = [&](int w, int buf, int q_tile) {
-            wait_k();
-            if (dead) return;
-            proxy_fence();
-            tc_fence_after();
-            const uint64_t q_desc = tc_desc(sm + C::Q_OFF + q_tile * C::Q_BYTES, 16, 1024);
-            const uint64_t k_desc = tc_desc(sm + C::K_OFF + (kt % C::NSK) * C::KV_BYTES, 16, 1024);
+        }
+        auto active = [&](int w, int t) { return t >= lo[w] && t < hi[w] && (step == 1 || ((t - lo[w]) & 1) == 0); };
+        wait(ubar(C::Q_FULL), q_phase);
+        q_phase ^= 1u;
+        if (dead) break;
+        bool k_here = false, v_here = false;
+        auto wait_k = [&]() {
+          if (!k_here) wait(ubar(C::K_FULL + k_stage), k_phase);
+          k_here = true;
+        };
+        auto wait_v = [&]() {
+          if (!v_here) wait(ubar(C::V_FULL + v_stage), v_phase);
+          v_here = true;
+        };
+        auto issue_qk = [&](int buf, int tile) {
+          wait_k();
+          if (dead) return;
+          proxy_fence();
+          tc_fence_after();
+          const uint32_t a = desc_lo(sm_u + C::Q_OFF + tile * C::Q_BYTES, 16), b = desc_lo(sm_u + C::K_OFF + k_stage * C::KV_BYTES, 16);
+          const uint32_t d = tmem_u + C::S_COL + buf * C::S_STEP, done = ubar(C::S_FULL + buf);
+          if (issuer) {
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks)  // k-steps of 16 along head_dim: +32 B inside a block, +1 block after 4
-              tc_mma(tmem + C::S_COL + buf * C::S_STEP, q_desc + (uint64_t)((ks >> 2) * (16384 >> 4) + (ks & 3) * 2),
-                     k_desc + (uint64_t)((ks >> 2) * (C::KV_BLOCK >> 4) + (ks & 3) * 2), idesc_s, ks > 0);
-            tc_commit(bar(C::S_FULL + buf));
-          };
-          auto issue_pv = [&](int w, int t, bool first, bool last) {
-            const int g = tiles_done[w]++, buf = NW == 2 ? w : g & 1;
-            const uint32_t phase = NW == 2 ? (uint32_t)g & 1u : (uint32_t)(g >> 1) & 1u;
-            if (!ext_wait<D>(bar(C::P_FULL + buf), phase, abort_flag)) give_up();
-            if (!dead) wait_v();
+              mma_ss(d, a + (uint32_t)((ks >> 2) * (16384 >> 4) + (ks & 3) * 2), b + (uint32_t)((ks >> 2) * (C::KV_BLOCK >> 4) + (ks & 3) * 2),
+                     idesc_s, ks > 0);
+            tc_commit(done);
+          }
+          __syncwarp();
+        };
+        auto issue_pv = [&](int w, int t, bool first, bool last) {
+          const int g = tiles_done[w]++, buf = NW == 2 ? w : g & 1;
+          const uint32_t phase = NW == 2 ? (uint32_t)g & 1u : (uint32_t)(g >> 1) & 1u;
+          const uint32_t a = tmem_u + C::P_COL + buf * C::P_STEP, b = desc_lo(sm_u + C::V_OFF + v_stage * C::KV_BYTES, C::KV_BLOCK);
+          const uint32_t d = tmem_u + C::O_COL + w * D, pv_done = ubar(C::PV_DONE + buf), o_full = ubar(C::O_FULL + w);
+          const int ksteps = min(TILE, len - t * TILE + 15) >> 4;  // the rows of V behind the next 16 are not defined
+          const bool whole = ksteps == TILE / 16;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            wait(ubar((half == 0 ? C::P_HALF : C::P_FULL) + buf), phase);
+            if (half == 0 && !dead) wait_v();
             if (dead) return;
             proxy_fence();
             tc_fence_after();
-            const uint32_t a = tmem + C::P_COL + buf * C::P_STEP, v_buf = sm + C::V_OFF + (vt % C::NSV) * C::KV_BYTES;
-            const int ksteps = min(TILE, len - t * TILE + 15) >> 4;  // the rows of V behind the next 16 are not defined
+            if (issuer) {
 #pragma unroll
-            for (int h = 0; h < D / C::PV_N; ++h) {
-              const uint64_t v_desc = tc_desc(v_buf + h * C::KV_BLOCK, C::KV_BLOCK, 1024);
-              for (int ks = 0; ks < ksteps; ++ks)
-                tc_mma_ts(tmem + C::O_COL + w * D + h * C::PV_N, a + (uint32_t)(ks * 8), v_desc + (uint64_t)(ks * 128), idesc_o,
-                          (!first || ks > 0) ? 1u : 0u);
-            }
-            if (NW == 1) tc_commit(bar(C::PV_DONE + buf));
-            if (last) tc_commit(bar(C::O_FULL + w));
-          };
-          auto release_k = [&]() {
-            wait_k();
-            if (!dead) tc_commit(bar(C::K_EMPTY + kt % C::NSK));
-            ++kt;
-            k_here = false;
-          };
-          auto release_v = [&]() {
-            wait_v();
-            if (!dead) tc_commit(bar(C::V_EMPTY + vt % C::NSV));
-            ++vt;
-            v_here = false;
-          };
-          if constexpr (NW == 2) {
-            // iteration t: the products with V of tile t - step, then the scores of tile t, stream by stream
-            for (int t = t0; t < t1 + step && !dead; ++t) {
-              const int tp_ = t - step;
+              for (int h = 0; h < D / C::PV_N; ++h)
 #pragma unroll
-              for (int w = 0; w < 2; ++w) {
-                const int lo = w == 0 ? s0.lo : s1.lo, hi = w == 0 ? s0.hi : s1.hi;
-                if (tp_ >= t0 && active(w, tp_)) issue_pv(w, tp_, tp_ == lo, tp_ + step >= hi);
-                if (!dead && t < t1 && active(w, t)) issue_qk(w, w, w == 0 ? s0.q_tile : s1.q_tile);
-                if (dead) break;
+                for (int ks = half * TILE / 32; ks < (half + 1) * TILE / 32; ++ks)
+                  if (whole || ks < ksteps)
+                    mma_ts(d + h * C::PV_N, a + (uint32_t)(ks * 8), b + (uint32_t)(h * (C::KV_BLOCK >> 4) + ks * 128), idesc_o,
+                           ks > 0 ? 1u : (first ? 0u : 1u));
+              if (half == 1) {
+                if (NW == 1) tc_commit(pv_done);
+                if (last) tc_commit(o_full);
               }
-              if (t < t1 && !dead) release_k();
-              if (t == t1 - 1 && !dead) tc_commit(bar(C::Q_EMPTY));
-              if (tp_ >= t0 && tp_ < t1 && !dead) release_v();
             }
-          } else {
-            for (int t = t0; t <= t1 && !dead; ++t) {
-              if (t < t1) {
-                issue_qk(0, (tiles_done[0] + (t > t0 ? 1 : 0)) & 1, 0);
-                if (!dead) release_k();
-                if (t == t1 - 1 && !dead) tc_commit(bar(C::Q_EMPTY));
-              }
-              if (t > t0 && !dead) {
-                issue_pv(0, t - 1, t - 1 == t0, t == t1);
-                if (!dead) release_v();
-              }
+            __syncwarp();
+          }
+        };
+        auto release_k = [&]() {
+          wait_k();
+          if (dead) return;
+          if (issuer) tc_commit(ubar(C::K_EMPTY + k_stage));
+          if (++k_stage == C::NSK) {
+            k_stage = 0;
+            k_phase ^= 1u;
+          }
+          k_here = false;
+        };
+        auto release_v = [&]() {
+          wait_v();
+          if (dead) return;
+          if (issuer) tc_commit(ubar(C::V_EMPTY + v_stage));
+          if (++v_stage == C::NSV) {
+            v_stage = 0;
+            v_phase ^= 1u;
+          }
+          v_here = false;
+        };
+        if constexpr (NW == 2) {
+          // iteration t: the products with V of tile t - step, then the scores of tile t, stream by stream
+          for (int t = t0; t < t1 + step && !dead; ++t) {
+            const int before = t - step;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              if (before >= t0 && active(w, before)) issue_pv(w, before, before == lo[w], before + step >= hi[w]);
+              if (!dead && t < t1 && active(w, t)) issue_qk(w, q_tile[w]);
+            }
+            if (dead) break;
+            if (t < t1) release_k();
+            if (t == t1 - 1 && !dead && issuer) tc_commit(ubar(C::Q_EMPTY));
+            if (before >= t0 && before < t1 && !dead) release_v();
+          }
+        } else {
+          for (int t = t0; t <= t1 && !dead; ++t) {
+            if (t < t1) {
+              issue_qk((tiles_done[0] + (t > t0 ? 1 : 0)) & 1, 0);
+              if (!dead) release_k();
+              if (t == t1 - 1 && !dead && issuer) tc_commit(ubar(C::Q_EMPTY));
+            }
+            if (t > t0 && !dead) {
+              issue_pv(0, t - 1, t - 1 == t0, t == t1);
+              if (!dead) release_v();
             }
           }
         }
