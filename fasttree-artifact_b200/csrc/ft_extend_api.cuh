@@ -108,6 +108,19 @@ int try_extend_tc(const ft::ExtendParams& p, const ft_extend_args* a, cudaStream
   return rc == FT_OK ? 1 : rc;
 }
 
+// scheduled early: it reads the plan's lists, which the launch before it reads too, before it waits for that launch
+template <typename T, int D>
+int launch_extend_merge(const ft::ExtendParams& p, cudaStream_t st) {
+  const int64_t pairs = (int64_t)p.num_merged * p.heads;
+  const bool split = p.partial_rows > 8LL * p.num_merged;  // more than eight rows a token
+  if (split)
+    FT_CUDA_OK(launch_early(ft::extend_merge_kernel<T, D, 4>, (unsigned)pairs, 128, 0, st, p));
+  else
+    FT_CUDA_OK(launch_early(ft::extend_merge_kernel<T, D, 1>, (unsigned)((pairs + 3) / 4), 128, 0, st, p));
+  count_launch();
+  return FT_OK;
+}
+
 template <typename T>
 int launch_extend(const ft::ExtendParams& p, const ft_extend_args* a, bool tensor, cudaStream_t st) {
   int done = 0;
@@ -121,11 +134,14 @@ int launch_extend(const ft::ExtendParams& p, const ft_extend_args* a, bool tenso
     FT_CUDA_OK(cudaGetLastError());
     count_launch();
   }
-  const int64_t merges = (int64_t)p.num_merged * p.heads;
-  if (merges > 0 && !dry_run("extend_merge_kernel")) {
-    // scheduled early: it reads the plan's lists, which the launch before it reads too, before it waits for that launch
-    FT_CUDA_OK(launch_early(ft::extend_merge_kernel<T>, (unsigned)((merges + 3) / 4), 128, 0, st, p));
-    count_launch();
+  if (p.num_merged > 0 && !dry_run("extend_merge_kernel")) {
+    switch (p.head_dim) {
+      case 16: return launch_extend_merge<T, 16>(p, st);
+      case 32: return launch_extend_merge<T, 32>(p, st);
+      case 64: return launch_extend_merge<T, 64>(p, st);
+      case 128: return launch_extend_merge<T, 128>(p, st);
+      default: return launch_extend_merge<T, 256>(p, st);
+    }
   }
   return FT_OK;
 }
@@ -205,7 +221,7 @@ int ft_extend(const ft_extend_args* a) {
     return fail(FT_ERR_INVALID_ARGUMENT, "the plan names %lld rows of q, which has %lld", (long long)pl.q_rows, (long long)a->q_rows);
   if (pl.partial_rows > 0 && (a->mid_o == nullptr || a->mid_lse == nullptr || !aligned16(a->mid_o)))
     return fail(FT_ERR_INVALID_ARGUMENT, "the plan has partial rows: mid_o (16-byte aligned) and mid_lse are needed");
-  if ((int64_t)pl.num_items * a->num_kv_heads > 0x7fffffffLL || ((int64_t)pl.num_merged * a->num_qo_heads + 3) / 4 > 0x7fffffffLL)
+  if ((int64_t)pl.num_items * a->num_kv_heads > 0x7fffffffLL || (int64_t)pl.num_merged * a->num_qo_heads > 0x7fffffffLL)
     return fail(FT_ERR_TOO_LARGE, "more tasks than one launch takes");
   const char* obstacle = extend_tc_obstacle(a);
   if (a->path == FT_EXTEND_TCGEN05 && obstacle != nullptr) return fail(FT_ERR_UNSUPPORTED, "tcgen05 path: %s", obstacle);
@@ -214,8 +230,8 @@ int ft_extend(const ft_extend_args* a) {
   ft::ExtendParams p;
   memset(&p, 0, sizeof(p));
   p.q = a->q, p.k = a->k_buffer, p.v = a->v_buffer, p.o = a->o, p.o_lse = a->o_lse, p.kv_entries = a->kv_entries;
-  p.items = a->plan_table + pl.items_off, p.segs = a->plan_table + pl.segments_off, p.tokens = a->plan_table + pl.tokens_off;
-  p.sm_offs = a->plan_table + pl.sm_offs_off, p.sm_tasks = a->plan_table + pl.sm_tasks_off;
+  p.items = a->plan_table + pl.items_off, p.tokens = a->plan_table + pl.tokens_off;
+  p.tiles = a->plan_table + pl.tiles_off, p.extra = a->plan_table + pl.extra_off, p.sms = a->plan_table + pl.sms_off, p.sm_tasks = a->plan_table + pl.sm_tasks_off;
   p.merged = a->plan_table + pl.merge_off, p.merge_rows = a->plan_table + pl.merge_rows_off;
   p.mid_o = a->mid_o, p.mid_lse = a->mid_lse;
   p.q_s0 = a->q_stride0, p.q_s1 = a->q_stride1, p.k_s0 = a->k_stride0, p.k_s1 = a->num_kv_heads > 1 ? a->k_stride1 : 0;
@@ -223,7 +239,7 @@ int ft_extend(const ft_extend_args* a) {
   p.kv_rows = a->kv_rows, p.q_rows = a->q_rows, p.kv_entries_len = a->kv_entries_len;
   p.num_items = pl.num_items, p.num_merged = pl.num_merged, p.partial_rows = pl.partial_rows;
   p.heads = a->num_qo_heads, p.kv_heads = a->num_kv_heads, p.group = a->num_qo_heads / a->num_kv_heads, p.head_dim = a->head_dim;
-  p.window = pl.window, p.tile = pl.tile_tokens;
+  p.tile = pl.tile_tokens;
   p.sm_scale = a->sm_scale, p.logit_cap = a->logit_cap > 0.f ? a->logit_cap : 0.f;
   cudaStream_t st = static_cast<cudaStream_t>(a->stream);
   if (a->dtype == FT_F16) return launch_extend<__half>(p, a, tensor, st);

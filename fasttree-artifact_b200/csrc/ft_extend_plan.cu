@@ -11,11 +11,17 @@
 // SM that is free first by the cost model below, and of several cuts the one whose simulated schedule ends first is
 // taken.
 //
-// Layout of an item (24 ints): first segment, segments, first and last K/V tile, step, query tiles, virtual length, 0,
-// then two streams of {first token, tokens, first tile, last tile, first partial row or -1 (the output itself), query
-// tile, 0, 0}.  Two streams are two query tiles over the same K/V tiles (step 1), or one query tile whose even and odd
-// K/V tiles run as two streams with partial rows of their own (step 2).  A segment (8 ints): table offset (low, high),
-// length, position of its first token, first and last token of the block that see it, virtual position of its start, 0.
+// Layout of the table, in ints.
+// CTA (4): its first task in sm_tasks, one past its last, the first task itself, 0.
+// Item (32): first and last K/V tile, step, query tiles, virtual length, the block's first record in the tile table, 0, 0, then two
+//   streams of {first token, tokens, first tile, last tile, first partial row or -1 (the output itself), query tile of the item,
+//   first token within the block, query tile of the block}, then the record of its first tile.  Two streams are two query tiles
+//   over the same K/V tiles (step 1), or one query tile whose even and odd K/V tiles run as two streams with partial rows of
+//   their own (step 2).
+// Tile (8): table offset of its first token (low, high), tokens, -1 if the tokens' offsets are consecutive, else the place of
+//   their offsets (low, high each) in the extra table; per query tile of the block -1 if each of its tokens sees the whole tile of
+//   tile_tokens, else the place of the bits of those that the block's tokens see, a word per 32 and token; 0, 0.
+// Token (2): row of q, position.  Merged token (4): row of q, first entry of its list of partial rows, entries, 0.
 #include <algorithm>
 #include <climits>
 #include <cstdint>
@@ -33,7 +39,7 @@ struct ft_extend_plan {
 
 namespace {
 
-constexpr int ITEM_INTS = 24, SEG_INTS = 8;
+constexpr int ITEM_INTS = 32;
 
 struct Segment {
   int64_t kv_off;
@@ -392,10 +398,77 @@ void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
   }
   std::vector<std::vector<std::pair<int, int>>> runs(b.blocks.size());  // per block: {first partial row, first token | tokens << 16}
   int64_t rows = 0;
+  // records of the blocks' tiles
+  std::vector<int32_t> tiles, extra, tile0(b.blocks.size(), 0);
+  const int words = p.tile / 32;
+  info.kv_entries_len = 0;
+  for (size_t k = 0; k < b.blocks.size(); ++k) {
+    const Block& blk = b.blocks[k];
+    tile0[k] = (int32_t)(tiles.size() / 8);
+    // what token t of the block sees of segment g, as virtual positions
+    auto sight = [&](const Segment& g, int t, int64_t& from, int64_t& to) {
+      const int64_t pos = b.tokens[blk.tok0 + t].pos;
+      from = g.voff + std::max<int64_t>(p.window > 0 ? pos - p.window + 1 - g.pos0 : 0, 0);
+      to = g.voff + std::min<int64_t>(g.len, pos + 1 - g.pos0);
+    };
+    int sg = blk.seg0, sg_known = -1;
+    int64_t all_lo[2] = {0, 0}, all_hi[2] = {0, 0};  // what all tokens of query tile w see of segment sg
+    for (int v0 = 0; v0 < blk.len; v0 += p.tile) {
+      while (b.segs[sg].voff + b.segs[sg].len <= v0) ++sg;
+      const int v1 = std::min(v0 + p.tile, blk.len);
+      const Segment& g = b.segs[sg];
+      const int64_t off = g.kv_off + (v0 - g.voff);
+      const bool single = g.voff + g.len >= v1;
+      int32_t x[8] = {(int32_t)(uint32_t)(off & 0xffffffffll), (int32_t)(off >> 32), v1 - v0, -1, -1, -1, 0, 0};
+      if (!single) {
+        x[3] = (int32_t)extra.size();
+        extra.resize(extra.size() + 2 * p.tile, 0);
+        for (int s = sg; s < blk.seg0 + blk.nseg && b.segs[s].voff < v1; ++s)
+          for (int v = std::max(v0, (int)b.segs[s].voff); v < std::min(v1, b.segs[s].voff + b.segs[s].len); ++v) {
+            const int64_t e = b.segs[s].kv_off + (v - b.segs[s].voff);
+            extra[x[3] + 2 * (v - v0)] = (int32_t)(uint32_t)(e & 0xffffffffll);
+            extra[x[3] + 2 * (v - v0) + 1] = (int32_t)(e >> 32);
+          }
+      } else if (sg != sg_known) {
+        sg_known = sg;
+        for (int w = 0; w < 2; ++w) {
+          const int lo = w == 0 ? 0 : blk.split, hi = w == 0 ? blk.split : blk.ntok;
+          all_lo[w] = 0;
+          all_hi[w] = g.tok_lo <= lo && g.tok_hi >= hi ? INT64_MAX : 0;
+          for (int t = lo; t < hi && all_hi[w] > 0; ++t) {
+            int64_t from, to;
+            sight(g, t, from, to);
+            all_lo[w] = std::max(all_lo[w], from);
+            all_hi[w] = std::min(all_hi[w], to);
+          }
+        }
+      }
+      int32_t bits_at = -1;
+      for (int w = 0; w < 2; ++w) {
+        if (single && v1 - v0 == p.tile && v0 >= all_lo[w] && v1 <= all_hi[w]) continue;
+        if (bits_at < 0) {
+          bits_at = (int32_t)extra.size();
+          extra.resize(extra.size() + (size_t)(blk.ntok * words + 3) / 4 * 4, 0);
+          for (int s = sg; s < blk.seg0 + blk.nseg && b.segs[s].voff < v1; ++s)
+            for (int t = b.segs[s].tok_lo; t < b.segs[s].tok_hi; ++t) {
+              int64_t from, to;
+              sight(b.segs[s], t, from, to);
+              for (int64_t v = std::max<int64_t>(from, v0); v < std::min<int64_t>(to, v1); ++v)
+                extra[bits_at + t * words + (v - v0) / 32] |= (int32_t)(1u << ((v - v0) & 31));
+            }
+        }
+        x[4 + w] = bits_at;
+      }
+      tiles.insert(tiles.end(), x, x + 8);
+      if (extra.size() > (size_t)INT32_MAX / 2) throw std::bad_alloc();
+    }
+  }
+  for (const Segment& g : b.segs) info.kv_entries_len = std::max(info.kv_entries_len, g.kv_off + g.len);
   info.items_off = 0;
   for (const Item& it : b.items) {
     const Block& blk = b.blocks[it.block];
-    int32_t x[ITEM_INTS] = {blk.seg0, blk.nseg, it.t0, it.t1, it.alternate ? 2 : 1, it.which == 3 ? 2 : 1, blk.len, 0};
+    int32_t x[ITEM_INTS] = {it.t0, it.t1, it.alternate ? 2 : 1, it.which == 3 ? 2 : 1, blk.len, tile0[it.block], 0, 0};
+    std::memcpy(x + 24, tiles.data() + 8 * ((size_t)tile0[it.block] + it.t0), 8 * sizeof(int32_t));
     int q_tile = 0;
     for (int w = 0; w < 2; ++w) {
       const int of = it.alternate ? (it.which == 1 ? 0 : 1) : w;  // the query tile of this stream
@@ -410,6 +483,7 @@ void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
       s[4] = -1;
       s[5] = it.alternate ? 0 : q_tile;
       s[6] = first;
+      s[7] = of;
       if (partial[it.block]) {
         s[4] = (int32_t)rows;
         runs[it.block].push_back({(int)rows, first | n << 16});
@@ -418,13 +492,6 @@ void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
       ++q_tile;
     }
     t.insert(t.end(), x, x + ITEM_INTS);
-  }
-  info.segments_off = (int64_t)t.size();
-  info.kv_entries_len = 0;
-  for (const Segment& g : b.segs) {
-    const int32_t x[SEG_INTS] = {(int32_t)(uint32_t)(g.kv_off & 0xffffffffll), (int32_t)(g.kv_off >> 32), g.len, g.pos0, g.tok_lo, g.tok_hi, g.voff, 0};
-    t.insert(t.end(), x, x + SEG_INTS);
-    info.kv_entries_len = std::max(info.kv_entries_len, g.kv_off + g.len);
   }
   align();
   info.tokens_off = (int64_t)t.size();
@@ -435,9 +502,16 @@ void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
     info.q_rows = std::max<int64_t>(info.q_rows, (int64_t)k.q_row + 1);
   }
   align();
-  info.sm_offs_off = (int64_t)t.size();
-  t.insert(t.end(), b.sm_offs.begin(), b.sm_offs.end());
+  info.tiles_off = (int64_t)t.size();
+  t.insert(t.end(), tiles.begin(), tiles.end());
+  info.extra_off = (int64_t)t.size();
+  t.insert(t.end(), extra.begin(), extra.end());
   align();
+  info.sms_off = (int64_t)t.size();
+  for (int c = 0; c < p.slots; ++c) {
+    const int32_t x[4] = {b.sm_offs[c], b.sm_offs[c + 1], b.sm_offs[c] < b.sm_offs[c + 1] ? b.sm_tasks[b.sm_offs[c]] : -1, 0};
+    t.insert(t.end(), x, x + 4);
+  }
   info.sm_tasks_off = (int64_t)t.size();
   t.insert(t.end(), b.sm_tasks.begin(), b.sm_tasks.end());
   align();
@@ -461,9 +535,8 @@ void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
   t.insert(t.end(), lists.begin(), lists.end());
   align();
   info.table_ints = (int64_t)t.size();
-  info.pieces = (int64_t)b.items.size();
   info.num_items = (int32_t)b.items.size();
-  info.num_segments = (int32_t)b.segs.size();
+  info.num_tiles = (int32_t)(tiles.size() / 8);
   info.num_tokens = (int32_t)b.tokens.size();
   info.num_merged = (int32_t)(merged.size() / 4);
   info.partial_rows = (int32_t)rows;

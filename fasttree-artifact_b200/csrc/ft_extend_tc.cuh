@@ -18,8 +18,8 @@
 // time through the TMA unit, its last rows with 16-byte copies.  Rows of V behind the last token are zeroed up to the next
 // 16, where the product ends; rows of K are not: their scores are masked.
 //
-// Softmax: a thread reads its row of S, masks what the row does not see (bits from the tile's segments; tiles inside one
-// segment and inside the row's range skip that), keeps a running maximum that may lag by 2^8 before O is rescaled in
+// Softmax: a thread reads its row of S, masks what the row does not see (bits from the plan; a tile that all of the query tile's
+// rows see whole has none), keeps a running maximum that may lag by 2^8 before O is rescaled in
 // tensor memory, and writes P in the storage type; the row's sum is of the unrounded probabilities in fp32.  P takes the
 // place of S, except at head_dim 64, where the products have different shapes and their order is not the order of issue:
 // there P has columns of its own.  When a stream's scores are ready all its earlier products are done (tcgen05.commit covers
@@ -111,8 +111,14 @@ __device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_
       : "memory");
 }
 
+__device__ __forceinline__ int ext_aborted(uint32_t flag) {
+  int x;
+  asm volatile("ld.volatile.shared.b32 %0, [%1];\n" : "=r"(x) : "r"(flag) : "memory");
+  return x;
+}
+
 template <int D>
-__device__ __forceinline__ bool ext_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool ext_wait(uint32_t bar, uint32_t parity, uint32_t abort_flag) {
   for (int it = 0; it < ExtCfg<D>::WAIT_LIMIT; ++it) {
     uint32_t ok;
     asm volatile(
@@ -121,59 +127,10 @@ __device__ __forceinline__ bool ext_wait(uint32_t bar, uint32_t parity, volatile
         : "r"(bar), "r"(parity)
         : "memory");
     if (ok) return true;
-    if ((it & 15) == 15 && *abort_flag != 0) return false;
+    if ((it & 15) == 15 && ext_aborted(abort_flag) != 0) return false;
   }
   return false;
 }
-
-// What the row `row` of stream w of task n sees of the tile that starts at virtual position v0, as bits; false: nothing.  `seg`
-// is the item's segment that held the tile before (-1: none yet) and becomes the one that holds v0; [all_lo, all_hi) becomes the
-// part of it that the row sees whole, seg_end its end.
-template <int TILE>
-__device__ __noinline__ bool see_tile(const ExtendParams& p, int n, int w, int row, int v0, int& seg, int& seg_end, int& all_lo, int& all_hi,
-                                      uint32_t (&see)[TILE / 32]) {
-  const int32_t* item = p.items + (int64_t)EXT_ITEM_INTS * (__ldg(p.sm_tasks + n) / p.kv_heads);
-  const ExtendStream st = extend_stream(item, w);
-  const bool live = row < st.ntok * p.group;
-  const int tok = live ? row / p.group : 0, pos = __ldg(p.tokens + 2 * (st.tok0 + tok) + 1);
-  const int end = __ldg(item) + __ldg(item + 1);
-  if (seg < 0) seg = __ldg(item);
-  ExtendSegment g = extend_segment(p.segs, seg);
-  while (v0 >= g.voff + g.len && seg + 1 < end) g = extend_segment(p.segs, ++seg);
-  seg_end = g.voff + g.len;
-  extend_in_sight(g, st.first + tok, pos, p.window, all_lo, all_hi);
-#pragma unroll
-  for (int k = 0; k < TILE / 32; ++k) see[k] = 0;
-  for (int sg = seg;;) {  // (the same segments for the whole warp)
-    int lo, hi;
-    extend_in_sight(g, st.first + tok, pos, p.window, lo, hi);
-#pragma unroll
-    for (int k = 0; k < TILE / 32; ++k) see[k] |= live ? bits_below(hi - v0 - 32 * k) & ~bits_below(lo - v0 - 32 * k) : 0u;
-    if (g.voff + g.len >= v0 + TILE || sg + 1 >= end) break;
-    g = extend_segment(p.segs, ++sg);
-  }
-  uint32_t some = 0;
-#pragma unroll
-  for (int k = 0; k < TILE / 32; ++k) some |= see[k];
-  return some != 0;
-}
-
-// Walks the segments of a block forward, tile by tile.
-struct SegmentCursor {
-  const int32_t* segs;
-  int at, end;
-  ExtendSegment g;
-  __device__ __forceinline__ void open(const int32_t* table, int seg0, int nseg) {
-    segs = table;
-    at = seg0;
-    end = seg0 + nseg;
-    g = extend_segment(segs, at);
-  }
-  // the segment that holds virtual position v, or the last one
-  __device__ __forceinline__ void forward(int v) {
-    while (v >= g.voff + g.len && at + 1 < end) g = extend_segment(segs, ++at);
-  }
-};
 
 template <typename T, int D, bool CAP>
 __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const __grid_constant__ ExtendTcParams tp) {
@@ -182,13 +139,15 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
   extern __shared__ __align__(1024) uint8_t smem[];
   const ExtendParams& p = tp.p;
   const uint32_t sm = smem_u32(smem), bars = sm + C::BAR_OFF;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::ABORT_OFF);
+  const uint32_t abort_flag = sm + C::ABORT_OFF;
+  auto set_abort = [&](int x) { asm volatile("st.volatile.shared.b32 [%0], %1;\n" ::"r"(abort_flag), "r"(x) : "memory"); };
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::TMEM_SLOT_OFF);
   auto bar = [&](int i) { return bars + 8u * i; };
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   allow_dependent_launch();
   wait_for_prior_grid();
-  const int task_lo = p.sm_offs[blockIdx.x], task_hi = p.sm_offs[blockIdx.x + 1];
+  const int4 share = __ldg(reinterpret_cast<const int4*>(p.sms) + blockIdx.x);
+  const int task_lo = share.x, task_hi = share.y;
   if (task_lo >= task_hi) return;
   if ((sm & 1023u) != 0u) {  // the swizzled operand layout needs a 1024-byte aligned window
     if (tid == 0) flag_error(FT_DEV_WAIT_TIMEOUT);
@@ -212,7 +171,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
     }
     mbar_init(bar(C::Q_FULL), 1);
     mbar_init(bar(C::Q_EMPTY), 1);
-    *abort_flag = 0;
+    set_abort(0);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 0) {
@@ -226,12 +185,12 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
   const int G = p.group;
   bool dead = false;
   auto give_up = [&]() {
-    *abort_flag = 1;
+    set_abort(1);
     flag_error(FT_DEV_WAIT_TIMEOUT);
     dead = true;
   };
   auto item_of = [&](int n, int& kvh) {
-    const int task = __ldg(p.sm_tasks + n);
+    const int task = n == task_lo ? share.z : __ldg(p.sm_tasks + n);
     kvh = task % p.kv_heads;
     return p.items + (int64_t)EXT_ITEM_INTS * (task / p.kv_heads);
   };
@@ -255,7 +214,9 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
     };
     int tiles_done = 0, items_done = 0;
     for (int n = task_lo; n < task_hi && !dead; ++n) {
-      int lo, hi, step, rows;  // of the stream: K/V tiles lo, lo + step, ... below hi, rows of the query tile
+      int lo, hi, step, rows;    // of the stream: K/V tiles lo, lo + step, ... below hi, rows of the query tile
+      const int32_t* mask_of;    // per K/V tile, every eighth int: where its bits are, or -1
+      const int32_t* bits = nullptr;  // of this row's token
       {
         int kvh;
         const int32_t* item = item_of(n, kvh);
@@ -263,37 +224,28 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
         lo = st.lo;
         hi = st.hi;
         rows = st.ntok * G;
-        step = __ldg(item + 4);
+        step = __ldg(item + 2);
+        mask_of = p.tiles + 8 * (int64_t)__ldg(item + 5) + 4 + st.block_tile;
+        bits = p.extra + (st.first + (row < rows ? row / G : 0)) * (TILE / 32);
       }
       if (rows == 0) continue;
       const bool warp_live = (row & ~31) < rows;
       float m_used = -INFINITY, l_run = 0.f;
       bool hidden = false;  // this row was shown less than all of its tiles
-      // Virtual positions [all_lo, all_hi) of segment `seg`, every one of which the row sees: a tile inside them needs no mask.
-      // (What only the other tiles and the end need is read again there: the registers go to the scores.)
-      int seg = -1, seg_end = 0, all_lo = 0, all_hi = 0;
-      for (int t = lo; t < hi; t += step) {
-        const int v0 = t * TILE;
-        uint32_t see[TILE / 32];
-        bool any = row < rows, full = true;
-        if (v0 >= seg_end || !__all_sync(0xffffffffu, row >= rows || (v0 >= all_lo && v0 + TILE <= all_hi))) {
-          any = see_tile<TILE>(p, n, w, row, v0, seg, seg_end, all_lo, all_hi, see);
-          bool everything = true;
-#pragma unroll
-          for (int k = 0; k < TILE / 32; ++k) everything &= see[k] == 0xffffffffu;
-          hidden |= !everything;
-          full = __all_sync(0xffffffffu, everything || row >= rows);
-        }
+      uint32_t see[TILE / 32];
+      bool any = true;
+      auto tile = [&](auto masked, const int t) {
+        constexpr bool MASKED = decltype(masked)::value;
         const int buf = NW == 2 ? w : tiles_done & 1;
         const uint32_t phase = NW == 2 ? (uint32_t)tiles_done & 1u : (uint32_t)(tiles_done >> 1) & 1u;
         ++tiles_done;
         const uint32_t s_col = t_lane + C::S_COL + buf * C::S_STEP, p_col = t_lane + C::P_COL + buf * C::P_STEP;
         if (!ext_wait<D>(bar(C::S_FULL + buf), phase, abort_flag)) {
           give_up();
-          break;
+          return;
         }
         tc_fence_after();
-        if (!__any_sync(0xffffffffu, any)) {  // nothing in sight of the warp's rows
+        if (MASKED && !__any_sync(0xffffffffu, any)) {  // nothing in sight of the warp's rows
           if (warp_live) {
             float zero[32];
 #pragma unroll
@@ -305,14 +257,13 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
           tc_fence_before();
           mbar_arrive(bar(C::P_HALF + buf));
           mbar_arrive(bar(C::P_FULL + buf));
-          continue;
+          return;
         }
         float s[TILE];
 #pragma unroll
         for (int c = 0; c < TILE / 32; ++c) tmem_ld32_nowait(s_col + 32 * c, *reinterpret_cast<float(*)[32]>(&s[32 * c]));
         tmem_wait_ld();
-        if (!full) {
-          __syncwarp();  // (a branch: as predicated code this would run for every tile)
+        if constexpr (MASKED) {
 #pragma unroll
           for (int k = 0; k < TILE / 32; ++k)
 #pragma unroll
@@ -326,7 +277,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
           for (int k = 0; k < 4; ++k) asm("max.f32 %0, %0, %1, %2;" : "+f"(mx4[k]) : "f"(s[c + 2 * k]), "f"(s[c + 2 * k + 1]));
         float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
         if constexpr (CAP)
-          mx = any ? capped(mx) : -INFINITY;
+          mx = !MASKED || any ? capped(mx) : -INFINITY;
         else
           mx *= scale2;
         float corr = 1.f;
@@ -351,8 +302,8 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
             float2 x = make_float2(s[h * (TILE / 2) + 2 * i], s[h * (TILE / 2) + 2 * i + 1]);
             if constexpr (CAP) {
               // (a masked score, -inf, stays one)
-              x.x = x.x == -INFINITY ? x.x : capped(x.x);
-              x.y = x.y == -INFINITY ? x.y : capped(x.y);
+              x.x = MASKED && x.x == -INFINITY ? x.x : capped(x.x);
+              x.y = MASKED && x.y == -INFINITY ? x.y : capped(x.y);
             }
             x = __ffma2_rn(x, sc2, no2);
             x.x = fast_exp2(x.x);
@@ -383,7 +334,31 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
           mbar_arrive(bar((h == 1 ? C::P_FULL : C::P_HALF) + buf));
         }
         l_run += (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
-        if (dead) break;
+      };
+      // Two loops, so that the one over tiles that every row sees whole has no masks in it: with one loop the scores do not all fit
+      // the registers (4096 tokens behind 12288, 64/8 heads: 1910 us, with two NNN).  Where the next tile's bits are is read a
+      // tile ahead.
+      auto mask_at = [&](int t) { return t < hi ? __ldg(mask_of + 8 * t) : -1; };
+      int mask = mask_at(lo);
+      for (int t = lo; t < hi && !dead;) {
+        while (mask < 0 && t < hi && !dead) {
+          mask = mask_at(t + step);
+          tile(std::false_type{}, t);
+          t += step;
+        }
+        if (t >= hi || dead) break;
+        uint32_t some = 0, every = 0xffffffffu;
+#pragma unroll
+        for (int k = 0; k < TILE / 32; ++k) {
+          see[k] = row < rows ? (uint32_t)__ldg(bits + mask + k) : 0u;
+          some |= see[k];
+          every &= see[k];
+        }
+        any = some != 0;
+        hidden |= every != 0xffffffffu;
+        mask = mask_at(t + step);
+        tile(std::true_type{}, t);
+        t += step;
       }
       if (dead) break;
       // ---- the row's result: normalised, to o or to its partial row
@@ -465,10 +440,10 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
         {
           int kvh;
           const int32_t* item = item_of(task_lo + n, kvh);
-          t0 = __shfl_sync(0xffffffffu, __ldg(item + 2), 0);
-          t1 = __shfl_sync(0xffffffffu, __ldg(item + 3), 0);
-          step = __shfl_sync(0xffffffffu, __ldg(item + 4), 0);
-          len = __shfl_sync(0xffffffffu, __ldg(item + 6), 0);
+          t0 = __shfl_sync(0xffffffffu, __ldg(item), 0);
+          t1 = __shfl_sync(0xffffffffu, __ldg(item + 1), 0);
+          step = __shfl_sync(0xffffffffu, __ldg(item + 2), 0);
+          len = __shfl_sync(0xffffffffu, __ldg(item + 4), 0);
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             const ExtendStream st = extend_stream(item, w);
@@ -587,106 +562,168 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       __syncwarp();
     } else if (role <= 2) {
       // ==================================================================== K loads (role 1), V loads (role 2)
-      const bool is_k = role == 1;
+      auto load_all = [&](auto which) {
+      constexpr bool is_k = decltype(which)::value;
       const CUtensorMap* map = is_k ? &tp.k_map : &tp.v_map;
       const CUtensorMap* rows_map = is_k ? &tp.k_rows_map : &tp.v_rows_map;
       const int64_t s0 = is_k ? p.k_s0 : p.v_s0, s1 = is_k ? p.k_s1 : p.v_s1;
       const T* base0 = reinterpret_cast<const T*>(is_k ? p.k : p.v);
-      const int full0 = is_k ? C::K_FULL : C::V_FULL, empty0 = is_k ? C::K_EMPTY : C::V_EMPTY, stages = is_k ? C::NSK : C::NSV;
+      constexpr int full0 = is_k ? C::K_FULL : C::V_FULL, empty0 = is_k ? C::K_EMPTY : C::V_EMPTY, stages = is_k ? C::NSK : C::NSV;
       const uint32_t ring = sm + (is_k ? C::K_OFF : C::V_OFF);
       const uint32_t ids_sm = sm + C::IDS_OFF + (is_k ? 0 : TILE * 4);
       const uint32_t row_lim = (uint32_t)(p.kv_rows < 0x7fffffffLL ? p.kv_rows : 0x7fffffffLL);
-      int count = 0;
-      for (int n = task_lo; n < task_hi && !dead; ++n) {
-        int kvh;
-        const int32_t* item = item_of(n, kvh);
-        const int t0 = __ldg(item + 2), t1 = __ldg(item + 3), len = __ldg(item + 6);
-        SegmentCursor cur;
-        cur.open(p.segs, __ldg(item), __ldg(item + 1));
-        const T* base = base0 + (int64_t)kvh * s1;
-        auto fetch_ids = [&](int t, int (&dst)[TILE / 32]) {
-          cur.forward(t * TILE);
-          SegmentCursor c = cur;
+      // The tiles of the CTA's tasks, one after the other, on a conveyor: the record of the tile after next but two is read, the
+      // table entries of the next but two are known, the row ids of three tiles are under way.  (A plain load that is sent off
+      // beside a hundred kilobytes of tile copies comes back after them; and a mixed tile's ids are two loads deep.)
+      struct Head {  // of a task: its tiles and where their records are
+        int t0, t1, tile0, kvh;
+        int4 rec;
+      };
+      struct Ids {  // row ids of a tile in flight; valid 0: there is no such tile
+        int id[TILE / 32], valid, kvh;
+      };
+      auto head_of = [&](int n) {
+        Head h;
+        const int32_t* item = item_of(n, h.kvh);
+        const int4 x = __ldg(reinterpret_cast<const int4*>(item)), y = __ldg(reinterpret_cast<const int4*>(item + 4));
+        h.t0 = x.x;
+        h.t1 = x.y;
+        h.tile0 = y.y;
+        h.rec = __ldg(reinterpret_cast<const int4*>(item + 24));
+        return h;
+      };
+      int n_next = task_lo;                 // the task whose head is in `next`
+      Head cur = head_of(task_lo), next = cur;
+      int t_rec = cur.t0;                   // tile of `rec`
+      int4 rec = cur.rec;
+      bool rec_here = true;
+      ++n_next;
+      if (n_next < task_hi) next = head_of(n_next);
+      int rec_kvh = cur.kvh;
+      auto advance_rec = [&]() {            // rec becomes the record of the following tile
+        if (++t_rec < cur.t1) {
+          rec = __ldg(reinterpret_cast<const int4*>(p.tiles) + 2 * ((int64_t)cur.tile0 + t_rec));
+        } else if (n_next < task_hi) {
+          cur = next;
+          t_rec = cur.t0;
+          rec = cur.rec;
+          rec_kvh = cur.kvh;
+          ++n_next;
+          if (n_next < task_hi) next = head_of(n_next);
+        } else {
+          rec_here = false;
+        }
+      };
+      int64_t entry[TILE / 32];
+      int entry_valid = 0, entry_kvh = 0;
+      auto advance_entries = [&]() {        // the entries become those of rec's tile
+        entry_valid = rec_here ? rec.z : 0;
+        entry_kvh = rec_kvh;
+        if (rec_here) {
 #pragma unroll
-          for (int h = 0; h < TILE / 32; ++h) {
-            const int v = t * TILE + lane + 32 * h;
-            dst[h] = -1;
-            if (v < len) {
-              c.forward(v);
-              dst[h] = __ldg(p.kv_entries + c.g.kv_off + (v - c.g.voff));
-            }
-          }
-        };
-        int id[TILE / 32], nxt[TILE / 32];
-        fetch_ids(t0, id);
-        for (int t = t0; t < t1; ++t, ++count) {
-          if (t + 1 < t1) fetch_ids(t + 1, nxt);
-          const int valid = min(TILE, len - t * TILE);
-          const int first = __shfl_sync(0xffffffffu, id[0], 0);
-          bool dense = true, in_pool = true;
+          for (int h = 0; h < TILE / 32; ++h) entry[h] = lane + 32 * h < rec.z ? extend_entry(p, rec, lane + 32 * h) : 0;
+          advance_rec();
+        }
+      };
+      auto refill = [&](Ids& x) {
+        x.valid = entry_valid;
+        x.kvh = entry_kvh;
 #pragma unroll
-          for (int h = 0; h < TILE / 32; ++h) {
-            dense &= id[h] == first + lane + 32 * h;
-            in_pool &= lane + 32 * h >= valid || (uint32_t)id[h] < row_lim;
-          }
-          in_pool = __all_sync(0xffffffffu, in_pool);
-          dense = tp.has_tma && valid == TILE && in_pool && __all_sync(0xffffffffu, dense);
-          const int b = count % stages;
-          if (!ext_wait<D>(bar(empty0 + b), ((uint32_t)(count / stages) & 1u) ^ 1u, abort_flag)) {
-            give_up();
-            break;
-          }
-          const uint32_t buf = ring + b * C::KV_BYTES, full = bar(full0 + b);
-          if (dense) {
-            if (lane == 0) {
-              mbar_arrive_expect_tx(full, C::KV_BYTES);
+        for (int h = 0; h < TILE / 32; ++h) {
+          x.id[h] = -1;
+          if (lane + 32 * h < entry_valid) x.id[h] = __ldg(p.kv_entries + entry[h]);
+        }
+        advance_entries();
+      };
+      int stage = 0;
+      uint32_t phase = 1;
+      auto load_tile = [&](const Ids& x) {
+        const int valid = x.valid, first = __shfl_sync(0xffffffffu, x.id[0], 0);
+        bool dense = true, in_pool = true;
 #pragma unroll
-              for (int h = 0; h < NB; ++h) tma_load_3d(buf + h * C::KV_BLOCK, map, 64 * h, kvh, first, full);
-            } else {
-              mbar_arrive(full);
+        for (int h = 0; h < TILE / 32; ++h) {
+          dense &= x.id[h] == first + lane + 32 * h;
+          in_pool &= lane + 32 * h >= valid || (uint32_t)x.id[h] < row_lim;
+        }
+        in_pool = __all_sync(0xffffffffu, in_pool);
+        dense = tp.has_tma && valid == TILE && in_pool && __all_sync(0xffffffffu, dense);
+        if (!__all_sync(0xffffffffu, ext_wait<D>(bar(empty0 + stage), phase, abort_flag))) {
+          give_up();
+          return;
+        }
+        const uint32_t buf = ring + stage * C::KV_BYTES, full = bar(full0 + stage);
+        if (dense) {
+          if (lane == 0) {
+            mbar_arrive_expect_tx(full, C::KV_BYTES);
+#pragma unroll
+            for (int h = 0; h < NB; ++h) tma_load_3d(buf + h * C::KV_BLOCK, map, 64 * h, x.kvh, first, full);
+          } else {
+            mbar_arrive(full);
+          }
+        } else {
+          __syncwarp();
+#pragma unroll
+          for (int h = 0; h < TILE / 32; ++h)
+            asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(ids_sm + (lane + 32 * h) * 4), "r"(x.id[h]) : "memory");
+          int done = 0;
+          if (tp.has_gather4 && in_pool) {
+            done = valid & ~3;
+            if (lane == 0 && done > 0) mbar_expect_tx(full, (uint32_t)done * (2u * D));
+            __syncwarp();
+            for (int i = lane; i < done / 4 * NB; i += 32) {
+              const int blk = i % NB, r = i / NB * 4;
+              int r0, r1, r2, r3;
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(ids_sm + r * 4));
+              tma_gather4(buf + blk * C::KV_BLOCK + r * 128, rows_map, x.kvh * (int)s1 + 64 * blk, r0, r1, r2, r3, full);
             }
           } else {
             __syncwarp();
-#pragma unroll
-            for (int h = 0; h < TILE / 32; ++h)
-              asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(ids_sm + (lane + 32 * h) * 4), "r"(id[h]) : "memory");
-            int done = 0;
-            if (tp.has_gather4 && in_pool) {
-              done = valid & ~3;
-              if (lane == 0 && done > 0) mbar_expect_tx(full, (uint32_t)done * (2u * D));
-              __syncwarp();
-              for (int i = lane; i < done / 4 * NB; i += 32) {
-                const int blk = i % NB, r = i / NB * 4;
-                int r0, r1, r2, r3;
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(ids_sm + r * 4));
-                tma_gather4(buf + blk * C::KV_BLOCK + r * 128, rows_map, kvh * (int)s1 + 64 * blk, r0, r1, r2, r3, full);
-              }
-            } else {
-              __syncwarp();
-            }
-            // what is left, 16 bytes at a time; of V zeros up to the next 16 rows
-            const int end = is_k ? valid : (valid + 15) & ~15, c16 = lane % C::CPR;
-            for (int r = done + lane / C::CPR; r < end; r += 32 / C::CPR) {
-              int row_id;
-              asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(row_id) : "r"(ids_sm + r * 4));
-              const bool ok = (uint32_t)row_id < row_lim;  // (behind the last token -1)
-              cp_async16_zfill(buf + (uint32_t)((c16 >> 3) * C::KV_BLOCK) + tc_swz(r, c16 & 7, 0), base + (int64_t)(ok ? row_id : 0) * s0 + c16 * 8, ok);
-            }
-            if (!in_pool && lane == 0) flag_error(FT_DEV_BAD_KV_INDEX);
-            mbar_arrive_on_cp_async(full);
           }
-#pragma unroll
-          for (int h = 0; h < TILE / 32; ++h) id[h] = nxt[h];
+          // what is left, 16 bytes at a time; of V zeros up to the next 16 rows
+          const T* base = base0 + (int64_t)x.kvh * s1;
+          const int end = is_k ? valid : (valid + 15) & ~15, c16 = lane % C::CPR;
+          for (int r = done + lane / C::CPR; r < end; r += 32 / C::CPR) {
+            int row_id;
+            asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(row_id) : "r"(ids_sm + r * 4));
+            const bool ok = (uint32_t)row_id < row_lim;  // (behind the last token -1)
+            cp_async16_zfill(buf + (uint32_t)((c16 >> 3) * C::KV_BLOCK) + tc_swz(r, c16 & 7, 0), base + (int64_t)(ok ? row_id : 0) * s0 + c16 * 8, ok);
+          }
+          if (!in_pool && lane == 0) flag_error(FT_DEV_BAD_KV_INDEX);
+          mbar_arrive_on_cp_async(full);
         }
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      };
+      Ids x0, x1, x2;
+      advance_entries();
+      refill(x0);
+      refill(x1);
+      refill(x2);
+      while (x0.valid != 0 && !dead) {  // (three copies of the body: ids under way stay in the registers that they go to)
+        load_tile(x0);
+        refill(x0);
+        if (x1.valid == 0 || dead) break;
+        load_tile(x1);
+        refill(x1);
+        if (x2.valid == 0 || dead) break;
+        load_tile(x2);
+        refill(x2);
       }
       cp_async_wait<0>();
+      };
+      if (role == 1)
+        load_all(std::true_type{});
+      else
+        load_all(std::false_type{});
     } else {
       // ==================================================================== Q loads
       int items = 0;
       for (int n = task_lo; n < task_hi && !dead; ++n, ++items) {
         int kvh;
         const int32_t* item = item_of(n, kvh);
-        const int q_tiles = __ldg(item + 5);
+        const int q_tiles = __ldg(item + 3);
         if (!ext_wait<D>(bar(C::Q_EMPTY), ((uint32_t)items & 1u) ^ 1u, abort_flag)) {
           give_up();
           break;
@@ -735,7 +772,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
   // ---- release tensor memory
   tc_fence_before();
   __syncthreads();
-  if (*abort_flag != 0)  // copies that nobody waits for any more land before the CTA ends
+  if (ext_aborted(abort_flag) != 0)  // copies that nobody waits for any more land before the CTA ends
     for (int i = 0; i < 2000; ++i) __nanosleep(1000);
   if (warp == 0) {
     tc_fence_after();

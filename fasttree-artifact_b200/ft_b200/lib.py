@@ -109,9 +109,9 @@ class AppendArgs(ctypes.Structure):
 
 class ExtendPlanInfo(ctypes.Structure):
     """Mirror of ``struct ft_extend_plan_info``."""
-    _fields_ = [(n, ctypes.c_int64) for n in ("table_ints", "items_off", "segments_off", "tokens_off", "sm_offs_off", "sm_tasks_off",
-                                              "merge_off", "merge_rows_off", "kv_entries_len", "q_rows", "pieces")] + [
-        (n, ctypes.c_int32) for n in ("num_items", "num_segments", "num_tokens", "num_merged", "partial_rows", "num_sms",
+    _fields_ = [(n, ctypes.c_int64) for n in ("table_ints", "items_off", "tokens_off", "tiles_off", "extra_off", "sms_off", "sm_tasks_off",
+                                              "merge_off", "merge_rows_off", "kv_entries_len", "q_rows")] + [
+        (n, ctypes.c_int32) for n in ("num_items", "num_tiles", "num_tokens", "num_merged", "partial_rows", "num_sms",
                                       "num_qo_heads", "num_kv_heads", "head_dim", "window", "elem_bytes", "rows_per_tile",
                                       "tile_tokens", "reserved")]
 

@@ -415,11 +415,10 @@ typedef struct ft_extend_plan ft_extend_plan;
 
 typedef struct ft_extend_plan_info {
   int64_t table_ints;     /* length of the table that ft_extend_plan_copy fills */
-  int64_t items_off, segments_off, tokens_off, sm_offs_off, sm_tasks_off, merge_off, merge_rows_off; /* its parts */
+  int64_t items_off, tokens_off, tiles_off, extra_off, sms_off, sm_tasks_off, merge_off, merge_rows_off; /* its parts */
   int64_t kv_entries_len; /* entries of kv_entries that the plan names: at least as many have to be there */
   int64_t q_rows;         /* one more than the largest row of q that it names */
-  int64_t pieces;         /* work items */
-  int32_t num_items, num_segments, num_tokens, num_merged; /* num_merged: query tokens whose K/V is split over items */
+  int32_t num_items, num_tiles, num_tokens, num_merged; /* num_merged: query tokens whose K/V is split over items */
   int32_t partial_rows;   /* rows of mid_o / mid_lse */
   int32_t num_sms;        /* CTAs of the scheduled form */
   int32_t num_qo_heads, num_kv_heads, head_dim, window, elem_bytes;

@@ -8,38 +8,49 @@ import torch
 import extend_cases
 from ft_b200 import extend, lib
 
-ITEM, SEG = 24, 8
+ITEM, TILE = 32, 8
 
 
 def shown(info, table, entries):
-    """Per q row: the pool rows it is shown, in the order of the items (with repetitions, were there any), its writers and the
-    partial rows of its merge list."""
+    """Per q row: the pool rows it is shown (with repetitions, were there any), its writers and the partial rows of its merge
+    list."""
     t = table.tolist()
     items = [t[info.items_off + ITEM * i:info.items_off + ITEM * (i + 1)] for i in range(info.num_items)]
+    words, group = info.tile_tokens // 32, info.num_qo_heads // info.num_kv_heads
+
+    def offsets(rec):
+        lo, hi, n, place = rec[:4]
+        if place < 0:
+            return [((hi << 32) | (lo & 0xffffffff)) + i for i in range(n)]
+        e = info.extra_off + place
+        return [(t[e + 2 * i + 1] << 32) | (t[e + 2 * i] & 0xffffffff) for i in range(n)]
+
     seen, writers, parts = {}, {}, {}
     for it in items:
-        seg0, nseg, t0, t1, step, q_tiles, length = it[:7]
+        t0, t1, step, q_tiles, length, tile0 = it[:6]
+        recs = {k: t[info.tiles_off + TILE * (tile0 + k):info.tiles_off + TILE * (tile0 + k + 1)] for k in range(t0, t1)}
+        offs = {k: offsets(r) for k, r in recs.items()}
+        assert it[24:32] == recs[t0] and tile0 + t1 <= info.num_tiles
+        assert all(r[2] == min(info.tile_tokens, length - k * info.tile_tokens) > 0 for k, r in recs.items())
         for w in range(2):
-            tok0, ntok, lo, hi, part, q_tile, first = it[8 + 8 * w:15 + 8 * w]
-            assert 0 <= q_tile < q_tiles
+            tok0, ntok, lo, hi, part, q_tile, first, block_tile = it[8 + 8 * w:16 + 8 * w]
+            assert 0 <= q_tile < q_tiles and block_tile in (0, 1)
             if ntok:
-                assert t0 <= lo < hi <= t1 and ntok * (info.num_qo_heads // info.num_kv_heads) <= max(
-                    info.rows_per_tile, info.num_qo_heads // info.num_kv_heads)
+                assert t0 <= lo < hi <= t1 and ntok * group <= max(info.rows_per_tile, group)
             for tok in range(ntok):
-                q_row, pos = t[info.tokens_off + 2 * (tok0 + tok):info.tokens_off + 2 * (tok0 + tok) + 2]
+                q_row = t[info.tokens_off + 2 * (tok0 + tok)]
                 got = []
-                for s in range(seg0, seg0 + nseg):
-                    lo32, hi32, slen, pos0, tlo, thi, voff, _ = t[info.segments_off + SEG * s:info.segments_off + SEG * (s + 1)]
-                    off = (hi32 << 32) | (lo32 & 0xffffffff)
-                    assert 0 <= voff and voff + slen <= length
-                    if not tlo <= first + tok < thi:
-                        continue
-                    a = max(pos - info.window + 1 - pos0, 0) if info.window else 0
-                    for j in range(a, min(slen, pos + 1 - pos0)):
-                        tile = (voff + j) // info.tile_tokens
-                        if lo <= tile < hi and (step == 1 or (tile - lo) % 2 == 0):
-                            got.append(int(entries[off + j]))
-                seen.setdefault(q_row, []).extend(got)
+                for k in range(lo, hi, step):
+                    place = recs[k][4 + block_tile]
+                    if place < 0:
+                        assert recs[k][2] == info.tile_tokens
+                        got += offs[k]
+                    else:
+                        m = info.extra_off + place + (first + tok) * words
+                        bits = [(t[m + i // 32] >> (i % 32)) & 1 for i in range(info.tile_tokens)]
+                        assert not any(bits[recs[k][2]:])
+                        got += [x for x, bit in zip(offs[k], bits) if bit]
+                seen.setdefault(q_row, []).extend(int(entries[x]) for x in got)
                 if part >= 0:
                     parts.setdefault(q_row, []).append(part + tok)
                 else:
@@ -72,9 +83,11 @@ def check(seq, ext, shared, hq, hkv, d, dtype=torch.float16, window=0, sms=148):
     used = sorted(x for p in parts.values() for x in p)
     assert used == list(range(info.partial_rows))                  # no partial row has two writers
     # every task is dealt once
-    offs = plan[info.sm_offs_off:info.sm_offs_off + info.num_sms + 1]
+    sms = plan[info.sms_off:info.sms_off + 4 * info.num_sms].reshape(-1, 4)
     tasks = plan[info.sm_tasks_off:info.sm_tasks_off + info.num_items * hkv]
-    assert offs[0] == 0 and (np.diff(offs) >= 0).all() and offs[-1] == info.num_items * hkv
+    assert sms[0, 0] == 0 and sms[-1, 1] == info.num_items * hkv
+    assert (sms[:, 0] <= sms[:, 1]).all() and (sms[1:, 0] == sms[:-1, 1]).all()
+    assert all(first == (tasks[a] if a < b else -1) for a, b, first, _ in sms.tolist())
     assert sorted(tasks.tolist()) == list(range(info.num_items * hkv))
     return info
 
@@ -112,9 +125,9 @@ def test_a_shared_prefix_stands_once():
     n = 16
     alone = check([4100] * n, [2] * n, [], 8, 2, 128)
     together = check([4100] * n, [2] * n, [(list(range(n)), 4098)], 8, 2, 128)
-    assert together.num_segments < alone.num_segments * 2 + n
+    assert together.num_tiles < alone.num_tiles
     def tokens(info, plan):
-        return sum(plan[info.segments_off + SEG * s + 2] for s in range(info.num_segments))
+        return sum(plan[info.tiles_off + TILE * k + 2] for k in range(info.num_tiles))
 
     table, _ = extend_cases.pool([4100] * n, [2] * n, [(list(range(n)), 4098)])
     starts = [r * table.shape[1] for r in range(n)]
@@ -145,9 +158,16 @@ def test_random_steps():
 def test_offsets_beyond_32_bits():
     start = [3 << 32, (3 << 32) + 1000]
     info, plan, _, _ = extend.host_plan([300, 200], [5, 6], start, 8, 2, 128, torch.float16)
-    offs = {int((int(plan[info.segments_off + SEG * s + 1]) << 32) | (int(plan[info.segments_off + SEG * s]) & 0xffffffff))
-            for s in range(info.num_segments)}
-    assert offs == set(start) and info.kv_entries_len == (3 << 32) + 1200
+    places = set()
+    for k in range(info.num_tiles):
+        lo, hi, n, place = (int(x) for x in plan[info.tiles_off + TILE * k:info.tiles_off + TILE * k + 4])
+        if place < 0:
+            places |= {((hi << 32) | (lo & 0xffffffff)) + i for i in range(n)}
+        else:
+            e = plan[info.extra_off + place:info.extra_off + place + 2 * n].reshape(-1, 2).astype(np.int64)
+            places |= set(((e[:, 1] << 32) | (e[:, 0] & 0xffffffff)).tolist())
+    assert places == set(range(start[0], start[0] + 300)) | set(range(start[1], start[1] + 200))
+    assert info.kv_entries_len == (3 << 32) + 1200
 
 
 def test_refusals():
