@@ -50,17 +50,21 @@ __device__ __forceinline__ ExtendStream extend_stream(const int32_t* item, int w
   return {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 }
 
-// Where a stream's row goes: a row of o, or a partial row.
+// Where the rows of token `tok` of a stream go: to o (-1), to a partial row, or nowhere (-2: the token sees nothing there).
+__device__ __forceinline__ int extend_part(const ExtendParams& p, const ExtendStream& st, int tok) {
+  return st.part < 0 ? -1 : __ldg(p.extra + st.part + tok);
+}
+
 template <typename T>
-__device__ __forceinline__ void extend_store(const ExtendParams& p, int part, int tok, int q_row, int head, int d, float x) {
+__device__ __forceinline__ void extend_store(const ExtendParams& p, int part, int q_row, int head, int d, float x) {
   if (part >= 0)
-    p.mid_o[((int64_t)(part + tok) * p.heads + head) * p.head_dim + d] = x;
+    p.mid_o[((int64_t)part * p.heads + head) * p.head_dim + d] = x;
   else
     reinterpret_cast<T*>(p.o)[(int64_t)q_row * p.o_s0 + (int64_t)head * p.o_s1 + d] = from_float<T>(x);
 }
-__device__ __forceinline__ void extend_store_lse(const ExtendParams& p, int part, int tok, int q_row, int head, float lse) {
+__device__ __forceinline__ void extend_store_lse(const ExtendParams& p, int part, int q_row, int head, float lse) {
   if (part >= 0)
-    p.mid_lse[(int64_t)(part + tok) * p.heads + head] = lse;
+    p.mid_lse[(int64_t)part * p.heads + head] = lse;
   else if (p.o_lse != nullptr)
     p.o_lse[(int64_t)q_row * p.heads + head] = lse;
 }
@@ -84,6 +88,8 @@ __device__ __noinline__ void extend_row(const ExtendParams& p, const int32_t* it
     if (lane == 0) flag_error(FT_DEV_BAD_Q_INDEX);
     return;
   }
+  const int part = extend_part(p, st, tok);
+  if (part == -2) return;
   const T* __restrict__ qp = reinterpret_cast<const T*>(p.q) + (int64_t)q_row * p.q_s0 + (int64_t)head * p.q_s1;
   const T* __restrict__ kbase = reinterpret_cast<const T*>(p.k) + (int64_t)kvh * p.k_s1;
   const T* __restrict__ vbase = reinterpret_cast<const T*>(p.v) + (int64_t)kvh * p.v_s1;
@@ -118,16 +124,16 @@ __device__ __noinline__ void extend_row(const ExtendParams& p, const int32_t* it
         if (bad && lane == 0) flag_error(FT_DEV_BAD_KV_INDEX);
 #pragma unroll
         for (int u = 0; u < TB; ++u) {
-          float part = 0.f;
+          float dot = 0.f;
           if (row[u] >= 0) {
             const T* __restrict__ kp = kbase + row[u] * p.k_s0;
 #pragma unroll
             for (int j = 0; j < MAXJ; ++j) {
               const int d = lane + 32 * j;
-              if (d < D) part = fmaf(qreg[j], to_float<T>(kp[d]), part);
+              if (d < D) dot = fmaf(qreg[j], to_float<T>(kp[d]), dot);
             }
           }
-          s[u] = part;
+          s[u] = dot;
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
@@ -173,9 +179,9 @@ __device__ __noinline__ void extend_row(const ExtendParams& p, const int32_t* it
 #pragma unroll
   for (int j = 0; j < MAXJ; ++j) {
     const int d = lane + 32 * j;
-    if (d < D) extend_store<T>(p, st.part, tok, q_row, head, d, acc[j] * inv);
+    if (d < D) extend_store<T>(p, part, q_row, head, d, acc[j] * inv);
   }
-  if (lane == 0) extend_store_lse(p, st.part, tok, q_row, head, l == 0.f ? -INFINITY : logf(l) + m);
+  if (lane == 0) extend_store_lse(p, part, q_row, head, l == 0.f ? -INFINITY : logf(l) + m);
 }
 
 // Any type and head size: a CTA per (item, KV head), a warp per query row in turn.
@@ -325,9 +331,9 @@ __global__ void __launch_bounds__(128) extend_merge_kernel(const ExtendParams p)
 #pragma unroll
     for (int c = 0; c < PIECES; ++c)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) extend_store<T>(p, -1, 0, rec.x, head, c * 128 + at + e, acc[c][e] * inv);
+      for (int e = 0; e < VEC; ++e) extend_store<T>(p, -1, rec.x, head, c * 128 + at + e, acc[c][e] * inv);
   }
-  if (lane == 0) extend_store_lse(p, -1, 0, rec.x, head, l == 0.f ? -INFINITY : logf(l) + m);
+  if (lane == 0) extend_store_lse(p, -1, rec.x, head, l == 0.f ? -INFINITY : logf(l) + m);
 }
 
 }  // namespace ft

@@ -22,28 +22,28 @@ bool vector_rows(const void* p, int64_t s0, int64_t s1, int elems, int size) {
   return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(elems * size - 1)) == 0 && s0 % elems == 0 && s1 % elems == 0;
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool PAIRS>
 int launch_append(const ft::AppendParams& p, cudaStream_t st) {
   const int units = p.head_dim / (2 * VEC), heads = (p.q != nullptr ? p.q_heads : 0) + 2 * p.kv_heads;
-  // enough threads for a token's units, two heads each, in whole warps and at most 256
-  int threads = (units * ((heads + 1) / 2) + 31) / 32 * 32;
-  threads = threads < units ? units : threads;
-  threads = threads > 256 ? 256 : threads;
-  ft::append_kernel<T, VEC><<<(unsigned)p.tokens, (unsigned)threads, 0, st>>>(p);
+  // a thread per unit, in whole warps, at most 128 (which hold every unit of a head: units is at most 128)
+  int threads = (units * heads + 31) / 32 * 32;
+  threads = threads > 128 ? 128 : threads;
+  ft::append_kernel<T, VEC, PAIRS><<<(unsigned)p.tokens, (unsigned)threads, 0, st>>>(p);
   FT_CUDA_OK(cudaGetLastError());
   count_launch();
   return FT_OK;
 }
 
 template <typename T>
-int launch_append_for(const ft::AppendParams& p, cudaStream_t st) {
+int launch_append_for(const ft::AppendParams& p, bool pairs, cudaStream_t st) {
   constexpr int VEC = 16 / (int)sizeof(T);
   const int size = (int)sizeof(T), half = p.rot / 2;
   bool vec = p.head_dim % (2 * VEC) == 0 && half % VEC == 0 && (p.head_dim - p.rot) % (2 * VEC) == 0 &&
              vector_rows(p.k, p.k_s0, p.k_s1, VEC, size) && vector_rows(p.v, p.v_s0, p.v_s1, VEC, size) &&
              vector_rows(p.k_buffer, p.kb_s0, p.kb_s1, VEC, size) && vector_rows(p.v_buffer, p.vb_s0, p.vb_s1, VEC, size);
   if (p.q != nullptr) vec = vec && vector_rows(p.q, p.q_s0, p.q_s1, VEC, size) && vector_rows(p.q_out, p.qo_s0, p.qo_s1, VEC, size);
-  return vec ? launch_append<T, VEC>(p, st) : launch_append<T, 1>(p, st);
+  if (pairs) return vec ? launch_append<T, VEC, true>(p, st) : launch_append<T, 1, true>(p, st);
+  return vec ? launch_append<T, VEC, false>(p, st) : launch_append<T, 1, false>(p, st);
 }
 
 // Can the tensor-core kernel take these arguments?  A reason, or NULL.
@@ -189,11 +189,11 @@ int ft_append(const ft_append_args* a) {
   p.kv_rows = a->kv_rows, p.positions_s0 = a->positions_stride0, p.cos_sin_rows = a->cos_sin_rows, p.cos_sin_s0 = a->cos_sin_stride0;
   p.tokens = a->tokens, p.q_heads = a->num_qo_heads, p.kv_heads = a->num_kv_heads, p.head_dim = a->head_dim, p.rot = a->rot_dim;
   p.axes = a->rot_dim > 0 ? a->num_axes : 0;
-  p.slots_64 = a->slots_64, p.positions_64 = a->positions_64, p.interleaved = a->interleaved != 0;
+  p.slots_64 = a->slots_64, p.positions_64 = a->positions_64;
   cudaStream_t st = static_cast<cudaStream_t>(a->stream);
-  if (a->dtype == FT_F16) return launch_append_for<__half>(p, st);
-  if (a->dtype == FT_BF16) return launch_append_for<__nv_bfloat16>(p, st);
-  return launch_append_for<float>(p, st);
+  if (a->dtype == FT_F16) return launch_append_for<__half>(p, a->interleaved != 0, st);
+  if (a->dtype == FT_BF16) return launch_append_for<__nv_bfloat16>(p, a->interleaved != 0, st);
+  return launch_append_for<float>(p, a->interleaved != 0, st);
 }
 
 int ft_extend(const ft_extend_args* a) {

@@ -12,9 +12,11 @@
 // taken.
 //
 // Layout of the table, in ints.
-// CTA (4): its first task in sm_tasks, one past its last, the first task itself, 0.
+// CTA (16): its first task in sm_tasks, one past its last, the first task itself, 0, that task's first and last K/V tile, its block's
+//   first record in the tile table, 0, the first four ints of its first tile's record, then 4 zeros.
 // Item (32): first and last K/V tile, step, query tiles, virtual length, the block's first record in the tile table, 0, 0, then two
-//   streams of {first token, tokens, first tile, last tile, first partial row or -1 (the output itself), query tile of the item,
+//   streams of {first token, tokens, first tile, last tile, -1 if the tokens' rows go to the output itself, else the place in the
+//   extra table of each token's partial row (-2: it sees nothing there and has none), query tile of the item,
 //   first token within the block, query tile of the block}, then the record of its first tile.  Two streams are two query tiles
 //   over the same K/V tiles (step 1), or one query tile whose even and odd K/V tiles run as two streams with partial rows of
 //   their own (step 2).
@@ -70,7 +72,7 @@ struct Costs {  // microseconds, B200: per K/V tile of two query tiles, of one i
 
 struct Problem {
   const int64_t *seq, *ext, *start, *qstart, *shared;
-  int batch, group, kv_heads, rows, tile;
+  int batch, group, kv_heads, head_dim, rows, tile;
   int64_t window;
   bool two_tiles, streams;
   int tokens_per_tile;
@@ -301,6 +303,15 @@ class Builder {
     return end;
   }
 
+  // about how many of the block's tokens see something of an item
+  int seen_by(const Item& it) const {
+    const Block& b = blocks[it.block];
+    int n = 0;
+    for (int s = b.seg0; s < b.seg0 + b.nseg; ++s)
+      if (segs[s].voff < it.t1 * p_.tile && segs[s].voff + segs[s].len > it.t0 * p_.tile) n += segs[s].tok_hi - segs[s].tok_lo;
+    return std::min(n, it.which == 3 ? b.ntok : it.which == 1 ? b.split : b.ntok - b.split);
+  }
+
   void choose_items() {
     const int nb = (int)blocks.size();
     std::vector<std::vector<uint8_t>> act(nb);
@@ -350,7 +361,7 @@ class Builder {
           }
         }
         if (out.size() - from > 1 || (out.size() > from && out[from].alternate))
-          for (size_t i = from; i < out.size(); ++i) parts += (out[i].alternate ? 2.0 : 1.0) * blocks[b].ntok;
+          for (size_t i = from; i < out.size(); ++i) parts += (out[i].alternate ? 2.0 : 1.0) * seen_by(out[i]);
       }
       return parts;
     };
@@ -359,14 +370,14 @@ class Builder {
     for (const Item& it : trial) total += it.cost * p_.kv_heads;
     const double even = total / p_.slots;
     auto merge_cost = [&](double parts) {  // a launch, and the partial rows written and read back
-      return parts > 0 ? 3.0 + parts * p_.kv_heads * p_.group * 8.0 * 128 / 4e6 : 0.0;
+      return parts > 0 ? 4.0 + parts * p_.kv_heads * p_.group * 8.0 * p_.head_dim / 4e6 : 0.0;
     };
     double best = -1;
-    static const double pieces[] = {0, 1.0, 0.5, 0.34, 0.25, 0.12};
+    static const double pieces[] = {0, 2.0, 1.5, 1.25, 1.15, 1.08, 1.04, 1.0, 0.75, 0.5, 0.34, 0.25};
     for (double f : pieces) {
       const double parts = cut(f * even, trial);
       const double end = deal(trial, nullptr, nullptr) + merge_cost(parts);
-      if (best < 0 || end < best * 0.98) {
+      if (best < 0 || end < best * 0.99) {
         best = end;
         items = trial;
       }
@@ -396,7 +407,7 @@ void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
     for (const Item& it : b.items) ++n_items[it.block];
     for (const Item& it : b.items) partial[it.block] |= (char)(n_items[it.block] > 1 || it.alternate);
   }
-  std::vector<std::vector<std::pair<int, int>>> runs(b.blocks.size());  // per block: {first partial row, first token | tokens << 16}
+  std::vector<std::vector<int32_t>> rows_of(b.tokens.size());  // per token its partial rows
   int64_t rows = 0;
   // records of the blocks' tiles
   std::vector<int32_t> tiles, extra, tile0(b.blocks.size(), 0);
@@ -485,9 +496,17 @@ void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
       s[6] = first;
       s[7] = of;
       if (partial[it.block]) {
-        s[4] = (int32_t)rows;
-        runs[it.block].push_back({(int)rows, first | n << 16});
-        rows += n;
+        s[4] = (int32_t)extra.size();
+        for (int i = first; i < first + n; ++i) {
+          bool sees = false;
+          for (int k = s[2]; k < s[3] && !sees; k += x[2]) {
+            const int32_t at = tiles[8 * ((size_t)tile0[it.block] + k) + 4 + of];
+            sees = at < 0;
+            for (int wd = 0; wd < words && !sees; ++wd) sees = extra[(size_t)at + i * words + wd] != 0;
+          }
+          extra.push_back(sees ? (int32_t)rows : -2);
+          if (sees) rows_of[blk.tok0 + i].push_back((int32_t)rows++);
+        }
       }
       ++q_tile;
     }
@@ -509,8 +528,14 @@ void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
   align();
   info.sms_off = (int64_t)t.size();
   for (int c = 0; c < p.slots; ++c) {
-    const int32_t x[4] = {b.sm_offs[c], b.sm_offs[c + 1], b.sm_offs[c] < b.sm_offs[c + 1] ? b.sm_tasks[b.sm_offs[c]] : -1, 0};
-    t.insert(t.end(), x, x + 4);
+    int32_t x[16] = {b.sm_offs[c], b.sm_offs[c + 1], -1, 0};
+    if (x[0] < x[1]) {
+      x[2] = b.sm_tasks[x[0]];
+      const Item& it = b.items[x[2] / p.kv_heads];
+      x[4] = it.t0, x[5] = it.t1, x[6] = tile0[it.block];
+      std::memcpy(x + 8, tiles.data() + 8 * ((size_t)tile0[it.block] + it.t0), 4 * sizeof(int32_t));
+    }
+    t.insert(t.end(), x, x + 16);
   }
   info.sm_tasks_off = (int64_t)t.size();
   t.insert(t.end(), b.sm_tasks.begin(), b.sm_tasks.end());
@@ -519,13 +544,9 @@ void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
   std::vector<int32_t> merged, lists;
   for (size_t k = 0; k < b.blocks.size(); ++k) {
     if (!partial[k]) continue;
-    for (int i = 0; i < b.blocks[k].ntok; ++i) {
-      const int32_t from = (int32_t)lists.size();
-      for (const auto& r : runs[k]) {
-        const int first = r.second & 0xffff, n = r.second >> 16;
-        if (i >= first && i < first + n) lists.push_back(r.first + i - first);
-      }
-      const int32_t x[4] = {b.tokens[b.blocks[k].tok0 + i].q_row, from, (int32_t)lists.size() - from, 0};
+    for (int i = b.blocks[k].tok0; i < b.blocks[k].tok0 + b.blocks[k].ntok; ++i) {
+      const int32_t x[4] = {b.tokens[i].q_row, (int32_t)lists.size(), (int32_t)rows_of[i].size(), 0};
+      lists.insert(lists.end(), rows_of[i].begin(), rows_of[i].end());
       merged.insert(merged.end(), x, x + 4);
     }
   }
@@ -575,6 +596,7 @@ int ft_extend_plan_build(const int64_t* seq_lens, const int64_t* extend_lens, co
     p.batch = batch;
     p.group = num_qo_heads / num_kv_heads;
     p.kv_heads = num_kv_heads;
+    p.head_dim = head_dim;
     p.window = window > most ? 0 : window;  // a window that hides nothing is none
     const bool tensor = elem_bytes == 2 && head_dim >= 64 && p.group <= 128;
     p.rows = tensor ? 128 : 16;
@@ -583,6 +605,24 @@ int ft_extend_plan_build(const int64_t* seq_lens, const int64_t* extend_lens, co
     p.tokens_per_tile = std::max(1, p.rows / p.group);
     p.slots = tensor ? num_sms : 4 * num_sms;
     p.cost = tensor ? (head_dim == 256 ? Costs{1.0, 0, 1.0, 1.0, 3.0} : Costs{0.6, 0.15, 0.75, 1.1, 2.5}) : Costs{2.0, 0, 2.0, 2.0, 3.0};
+    if (tensor) {
+      // Where the step is bound by the distinct K/V rows that come from memory rather than by products, a tile costs an SM its share
+      // of the copy rate.
+      double distinct = 0, pairs = 0;
+      for (int i = 0; i < batch; ++i) {
+        const int64_t cached = seq_lens[i] - extend_lens[i], reach = p.window > 0 ? std::min(seq_lens[i], p.window + extend_lens[i]) : seq_lens[i];
+        if (extend_lens[i] == 0) continue;
+        distinct += (double)std::min(reach, seq_lens[i] - shared_with_previous[i]);
+        pairs += (double)extend_lens[i] * (double)std::min(reach, cached + (extend_lens[i] + 1) / 2);
+      }
+      const double bytes = distinct * num_kv_heads * 2.0 * head_dim * elem_bytes, flops = pairs * num_qo_heads * 4.0 * head_dim;
+      if (bytes / 6.2e6 > flops / 1.0e9) {
+        const double share = p.tile * 2.0 * head_dim * elem_bytes / (6.2e6 / num_sms);
+        p.cost.alternate = std::max(p.cost.alternate, share);
+        p.cost.single = std::max(p.cost.single, share);
+        p.cost.load = std::max(p.cost.load, share - 2 * p.cost.pair);
+      }
+    }
     Builder b(p);
     b.run();
     // what the tables' 32-bit fields hold

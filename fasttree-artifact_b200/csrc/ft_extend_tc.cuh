@@ -57,7 +57,7 @@ struct ExtCfg {
   static constexpr int Q_BYTES = NB * 16384;        // one query tile
   static constexpr int KV_BLOCK = TILE * 128;       // one column block of a K/V tile
   static constexpr int KV_BYTES = NB * KV_BLOCK;
-  static constexpr int NSK = D == 64 ? 5 : 3, NSV = D == 64 ? 5 : 2;
+  static constexpr int NSK = D == 64 ? 5 : D == 128 ? 2 : 3, NSV = D == 64 ? 5 : D == 128 ? 3 : 2;
   static constexpr int Q_OFF = 0, K_OFF = NW * Q_BYTES, V_OFF = K_OFF + NSK * KV_BYTES;
   static constexpr int IDS_OFF = V_OFF + NSV * KV_BYTES;  // row ids of the tile being gathered, K's and V's
   static constexpr int BAR_OFF = IDS_OFF + 2 * TILE * 4;
@@ -71,7 +71,7 @@ struct ExtCfg {
   static constexpr int PV_N = D == 128 ? 128 : 64;  // columns of O per product
   static constexpr int CPR = D / 8;                 // 16-byte chunks of a row
   static constexpr int REGS_SOFTMAX = 208, REGS_OTHER = 88, REGS_LAUNCH = 168;
-  static constexpr int WAIT_LIMIT = 1 << 22;
+  static constexpr int WAIT_LIMIT = 1 << 25;        // a softmax warp that computes rows again keeps the others waiting
   static_assert(SMEM_BYTES <= 232448, "one CTA must fit in one SM's shared memory");
   static_assert(NW != 2 || (2 * REGS_SOFTMAX + REGS_OTHER) * 128 <= REGS_LAUNCH * THREADS, "register trade must balance");
 };
@@ -146,12 +146,18 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   allow_dependent_launch();
   wait_for_prior_grid();
-  const int4 share = __ldg(reinterpret_cast<const int4*>(p.sms) + blockIdx.x);
+  const int4* my_share = reinterpret_cast<const int4*>(p.sms) + 4 * blockIdx.x;
+  const int4 share = __ldg(my_share);
   const int task_lo = share.x, task_hi = share.y;
   if (task_lo >= task_hi) return;
   if ((sm & 1023u) != 0u) {  // the swizzled operand layout needs a 1024-byte aligned window
     if (tid == 0) flag_error(FT_DEV_WAIT_TIMEOUT);
     return;
+  }
+  if (tid == C::THREADS - 32) {  // the first copies would otherwise pay for fetching their descriptors
+    const CUtensorMap* maps[] = {&tp.k_map, &tp.v_map, &tp.q_map, &tp.q_map_tile, &tp.k_rows_map, &tp.v_rows_map};
+#pragma unroll
+    for (int i = 0; i < 6; ++i) asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(maps[i])) : "memory");
   }
   if (tid == 0) {
     for (int b = 0; b < C::NSK; ++b) {
@@ -178,10 +184,13 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(sm + C::TMEM_SLOT_OFF), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  // Each role passes the end of the set-up where it needs it: the loaders have their first row ids under way by then.
+  auto set_up = [&]() {
+    tc_fence_before();
+    asm volatile("bar.sync 0;\n" ::: "memory");
+    tc_fence_after();
+    return *tmem_slot;
+  };
   const int G = p.group;
   bool dead = false;
   auto give_up = [&]() {
@@ -196,6 +205,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
   };
 
   if (warp < 4 * NW) {
+    const uint32_t tmem = set_up();
     // ====================================================================== softmax, one query row per thread
     if constexpr (NW == 2) reg_grow<C::REGS_SOFTMAX>();
     const int w = warp >> 2, row = tid & 127;
@@ -375,15 +385,16 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       const bool live = row < rows;
       const int tok = live ? row / G : 0, head = kvh * G + (live ? row - tok * G : 0);
       const int2 tk = __ldg(reinterpret_cast<const int2*>(p.tokens) + st.tok0 + tok);
-      const bool store = live && tk.x >= 0 && tk.x < p.q_rows;
-      if (live && !store) flag_error(FT_DEV_BAD_Q_INDEX);
+      const int part = live ? extend_part(p, st, tok) : -2;
+      const bool store = part != -2 && tk.x >= 0 && tk.x < p.q_rows;
+      if (part != -2 && !store) flag_error(FT_DEV_BAD_Q_INDEX);
       const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
       float2 finite = make_float2(0.f, 0.f);  // 0 x every element: 0, or NaN
-      float* mid = st.part >= 0 ? p.mid_o + ((int64_t)(st.part + tok) * p.heads + head) * D : nullptr;
-      T* out = reinterpret_cast<T*>(p.o) + (int64_t)(store ? tk.x : 0) * p.o_s0 + (int64_t)head * p.o_s1;
-#pragma unroll
-      for (int cb = 0; cb < D / 32; ++cb) {
-        float o[32];
+      uint8_t* dst = nullptr;
+      if (store)
+        dst = part >= 0 ? reinterpret_cast<uint8_t*>(p.mid_o + ((int64_t)part * p.heads + head) * D)
+                           : reinterpret_cast<uint8_t*>(reinterpret_cast<T*>(p.o) + (int64_t)tk.x * p.o_s0 + (int64_t)head * p.o_s1);
+      auto load_32 = [&](int cb, float (&o)[32]) {
         tmem_ld32(o_col + cb * 32, o);
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
@@ -392,21 +403,26 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
           o[2 * c] = x.x;
           o[2 * c + 1] = x.y;
         }
-        if (store) {
-          if (mid != nullptr) {
+      };
+#pragma unroll
+      for (int cb = 0; cb < D / 32; ++cb) {
+        float o[32];
+        load_32(cb, o);
+        if (dst != nullptr) {
+          if (st.part >= 0) {
 #pragma unroll
             for (int c = 0; c < 8; ++c)
-              reinterpret_cast<float4*>(mid + cb * 32)[c] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+              reinterpret_cast<float4*>(dst + cb * 128)[c] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
           } else {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-              reinterpret_cast<uint4*>(out + cb * 32)[c] = make_uint4(pack2<T>(o[8 * c], o[8 * c + 1]), pack2<T>(o[8 * c + 2], o[8 * c + 3]),
+              reinterpret_cast<uint4*>(dst + cb * 64)[c] = make_uint4(pack2<T>(o[8 * c], o[8 * c + 1]), pack2<T>(o[8 * c + 2], o[8 * c + 3]),
                                                                      pack2<T>(o[8 * c + 4], o[8 * c + 5]), pack2<T>(o[8 * c + 6], o[8 * c + 7]));
           }
         }
       }
       if (store)
-        extend_store_lse(p, st.part, tok, tk.x, head, l_run == 0.f ? -INFINITY : (m_used + log2f(l_run)) * 0.6931471805599453f);
+        extend_store_lse(p, part, tk.x, head, l_run == 0.f ? -INFINITY : (m_used + log2f(l_run)) * 0.6931471805599453f);
       const bool spoiled = store && hidden && !(finite.x + finite.y == 0.f);
       for (uint32_t todo = __ballot_sync(0xffffffffu, spoiled); todo != 0; todo &= todo - 1) {
         const int r = (row & ~31) + __ffs(todo) - 1;
@@ -418,6 +434,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
     if constexpr (NW == 2) reg_shrink<C::REGS_OTHER>();
     const int role = warp - 4 * NW;
     if (role == 0) {
+      const uint32_t tmem = set_up();
       // ==================================================================== MMA issue
       // The whole warp walks the loop, on values that are the same in every lane (broadcast where they come from memory), so that
       // the operands of an MMA stand in uniform registers; one lane issues.  With a loop for one lane alone, every MMA waits
@@ -593,7 +610,8 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
         return h;
       };
       int n_next = task_lo;                 // the task whose head is in `next`
-      Head cur = head_of(task_lo), next = cur;
+      const int4 first_head = __ldg(my_share + 1);
+      Head cur = {first_head.x, first_head.y, first_head.z, share.z % p.kv_heads, __ldg(my_share + 2)}, next = cur;
       int t_rec = cur.t0;                   // tile of `rec`
       int4 rec = cur.rec;
       bool rec_here = true;
@@ -699,6 +717,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       Ids x0, x1, x2;
       advance_entries();
       refill(x0);
+      set_up();
       refill(x1);
       refill(x2);
       while (x0.valid != 0 && !dead) {  // (three copies of the body: ids under way stay in the registers that they go to)
@@ -718,6 +737,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       else
         load_all(std::false_type{});
     } else {
+      set_up();
       // ==================================================================== Q loads
       int items = 0;
       for (int n = task_lo; n < task_hi && !dead; ++n, ++items) {
@@ -776,7 +796,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
     for (int i = 0; i < 2000; ++i) __nanosleep(1000);
   if (warp == 0) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(*tmem_slot), "r"(512) : "memory");
   }
 }
 

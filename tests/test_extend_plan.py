@@ -52,7 +52,10 @@ def shown(info, table, entries):
                         got += [x for x, bit in zip(offs[k], bits) if bit]
                 seen.setdefault(q_row, []).extend(int(entries[x]) for x in got)
                 if part >= 0:
-                    parts.setdefault(q_row, []).append(part + tok)
+                    row = t[info.extra_off + part + tok]
+                    assert (row == -2) == (not got)
+                    if got:
+                        parts.setdefault(q_row, []).append(row)
                 else:
                     writers[q_row] = writers.get(q_row, 0) + 1
     merged = {}
@@ -83,11 +86,15 @@ def check(seq, ext, shared, hq, hkv, d, dtype=torch.float16, window=0, sms=148):
     used = sorted(x for p in parts.values() for x in p)
     assert used == list(range(info.partial_rows))                  # no partial row has two writers
     # every task is dealt once
-    sms = plan[info.sms_off:info.sms_off + 4 * info.num_sms].reshape(-1, 4)
+    sms = plan[info.sms_off:info.sms_off + 16 * info.num_sms].reshape(-1, 16)
     tasks = plan[info.sm_tasks_off:info.sm_tasks_off + info.num_items * hkv]
     assert sms[0, 0] == 0 and sms[-1, 1] == info.num_items * hkv
     assert (sms[:, 0] <= sms[:, 1]).all() and (sms[1:, 0] == sms[:-1, 1]).all()
-    assert all(first == (tasks[a] if a < b else -1) for a, b, first, _ in sms.tolist())
+    for a, b, first, _, t0, t1, tile0, _, *rec in sms.tolist():
+        assert first == (tasks[a] if a < b else -1)
+        if a < b:
+            it = plan[info.items_off + ITEM * (first // hkv):info.items_off + ITEM * (first // hkv + 1)].tolist()
+            assert [t0, t1, tile0] == [it[0], it[1], it[5]] and rec[:4] == it[24:28]
     assert sorted(tasks.tolist()) == list(range(info.num_items * hkv))
     return info
 
