@@ -3,6 +3,7 @@
 
 #include "ft_append.cuh"
 #include "ft_extend.cuh"
+#include "ft_extend_f32.cuh"
 #include "ft_extend_tc.cuh"
 
 namespace {
@@ -108,6 +109,30 @@ int try_extend_tc(const ft::ExtendParams& p, const ft_extend_args* a, cudaStream
   return rc == FT_OK ? 1 : rc;
 }
 
+// fp32 rows that the tiled kernel can copy 16 bytes at a time
+bool extend_f32_ok(const ft_extend_args* a) {
+  return (a->plan.rows_per_tile == 64 || a->plan.rows_per_tile == 16) && vector_rows(a->q, a->q_stride0, a->num_qo_heads > 1 ? a->q_stride1 : 0, 4, 4) &&
+         vector_rows(a->o, a->o_stride0, a->num_qo_heads > 1 ? a->o_stride1 : 0, 4, 4) &&
+         vector_rows(a->k_buffer, a->k_stride0, a->num_kv_heads > 1 ? a->k_stride1 : 0, 4, 4) &&
+         vector_rows(a->v_buffer, a->v_stride0, a->num_kv_heads > 1 ? a->v_stride1 : 0, 4, 4);
+}
+
+template <int D, int RPT>
+int launch_extend_f32_as(const ft::ExtendParams& p, int ctas, cudaStream_t st) {
+  auto kernel = ft::extend_f32_kernel<D, RPT>;
+  static OncePerDevice once;
+  FT_CUDA_OK(raise_smem_limit(once, kernel, ft::ExtF32Cfg<D, RPT>::SMEM_BYTES));
+  kernel<<<(unsigned)ctas, 256, ft::ExtF32Cfg<D, RPT>::SMEM_BYTES, st>>>(p);
+  FT_CUDA_OK(cudaGetLastError());
+  count_launch();
+  return FT_OK;
+}
+
+template <int D>
+int launch_extend_f32(const ft::ExtendParams& p, const ft_extend_args* a, cudaStream_t st) {
+  return a->plan.rows_per_tile == 64 ? launch_extend_f32_as<D, 4>(p, a->plan.num_sms, st) : launch_extend_f32_as<D, 1>(p, a->plan.num_sms, st);
+}
+
 // scheduled early: it reads the plan's lists, which the launch before it reads too, before it waits for that launch
 template <typename T, int D>
 int launch_extend_merge(const ft::ExtendParams& p, cudaStream_t st) {
@@ -128,6 +153,19 @@ int launch_extend(const ft::ExtendParams& p, const ft_extend_args* a, bool tenso
     if (tensor) done = p.head_dim == 64 ? try_extend_tc<T, 64>(p, a, st) : p.head_dim == 128 ? try_extend_tc<T, 128>(p, a, st) : try_extend_tc<T, 256>(p, a, st);
     if (done < 0) return done;
     if (tensor && done == 0 && a->path == FT_EXTEND_TCGEN05) return fail(FT_ERR_UNSUPPORTED, "tcgen05 path: no TMA descriptor for the layout of q");
+  }
+  if constexpr (sizeof(T) == 4) {
+    if (a->path == FT_EXTEND_AUTO && extend_f32_ok(a)) {
+      done = 1;
+      if (!dry_run("extend_f32_kernel")) {
+        const int rc = p.head_dim == 16   ? launch_extend_f32<16>(p, a, st)
+                       : p.head_dim == 32 ? launch_extend_f32<32>(p, a, st)
+                       : p.head_dim == 64 ? launch_extend_f32<64>(p, a, st)
+                       : p.head_dim == 128 ? launch_extend_f32<128>(p, a, st)
+                                           : launch_extend_f32<256>(p, a, st);
+        if (rc != FT_OK) return rc;
+      }
+    }
   }
   if (done == 0 && !dry_run("extend_generic_kernel")) {
     ft::extend_generic_kernel<T><<<(unsigned)(p.num_items * p.kv_heads), 128, 0, st>>>(p);

@@ -28,6 +28,7 @@
 #include <climits>
 #include <cstdint>
 #include <cstring>
+#include <memory>
 #include <new>
 #include <queue>
 #include <vector>
@@ -85,6 +86,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 class Builder {
  public:
   explicit Builder(const Problem& p) : p_(p) {}
+  double end = 0;  // of the simulated schedule, in microseconds
 
   void run() {
     place_tokens();
@@ -100,7 +102,7 @@ class Builder {
   std::vector<int32_t> sm_offs, sm_tasks;
 
  private:
-  const Problem& p_;
+  const Problem p_;
   std::vector<int> req_of_, first_tok_;
 
   int64_t prefix(int i) const { return p_.seq[i] - p_.ext[i]; }
@@ -376,12 +378,12 @@ class Builder {
     static const double pieces[] = {0, 2.0, 1.5, 1.25, 1.15, 1.08, 1.04, 1.0, 0.75, 0.5, 0.34, 0.25};
     for (double f : pieces) {
       const double parts = cut(f * even, trial);
-      const double end = deal(trial, nullptr, nullptr) + merge_cost(parts);
-      if (best < 0 || end < best * 0.99) {
-        best = end;
+      const double finish = deal(trial, nullptr, nullptr) + merge_cost(parts);
+      if (best < 0 || finish < best * 0.99) {
+        best = end = finish;
         items = trial;
       }
-      if (f == 0 && end <= 1.04 * even + 1.0) break;  // nothing to gain
+      if (f == 0 && finish <= 1.04 * even + 1.0) break;  // nothing to gain
     }
     std::vector<int> order, slot;
     deal(items, &order, &slot);
@@ -393,6 +395,24 @@ class Builder {
     for (size_t i = 0; i < order.size(); ++i) sm_tasks[at[slot[i]]++] = order[i];
   }
 };
+
+// Where the step is bound by the distinct K/V rows that come from memory rather than by products, a tile costs an SM its share of
+// the copy rate.
+void memory_bound_costs(Problem& p, int elem_bytes, int num_sms) {
+  double distinct = 0, pairs = 0;
+  for (int i = 0; i < p.batch; ++i) {
+    if (p.ext[i] == 0) continue;
+    const int64_t cached = p.seq[i] - p.ext[i], reach = p.window > 0 ? std::min(p.seq[i], p.window + p.ext[i]) : p.seq[i];
+    distinct += (double)std::min(reach, p.seq[i] - p.shared[i]);
+    pairs += (double)p.ext[i] * (double)std::min(reach, cached + (p.ext[i] + 1) / 2);
+  }
+  const double bytes = distinct * p.kv_heads * 2.0 * p.head_dim * elem_bytes, flops = pairs * p.kv_heads * p.group * 4.0 * p.head_dim;
+  if (bytes / 6.2e6 <= flops / 1.0e9) return;
+  const double share = p.tile * 2.0 * p.head_dim * elem_bytes / (6.2e6 / num_sms);
+  p.cost.alternate = std::max(p.cost.alternate, share);
+  p.cost.single = std::max(p.cost.single, share);
+  p.cost.load = std::max(p.cost.load, share - 2 * p.cost.pair);
+}
 
 void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
   ft_extend_plan_info& info = out->info;
@@ -599,32 +619,35 @@ int ft_extend_plan_build(const int64_t* seq_lens, const int64_t* extend_lens, co
     p.head_dim = head_dim;
     p.window = window > most ? 0 : window;  // a window that hides nothing is none
     const bool tensor = elem_bytes == 2 && head_dim >= 64 && p.group <= 128;
-    p.rows = tensor ? 128 : 16;
-    p.tile = tensor ? (head_dim == 256 ? 64 : 128) : 32;
     p.two_tiles = p.streams = tensor && head_dim <= 128;
-    p.tokens_per_tile = std::max(1, p.rows / p.group);
-    p.slots = tensor ? num_sms : 4 * num_sms;
-    p.cost = tensor ? (head_dim == 256 ? Costs{1.0, 0, 1.0, 1.0, 3.0} : Costs{0.6, 0.15, 0.75, 1.1, 2.5}) : Costs{2.0, 0, 2.0, 2.0, 3.0};
-    if (tensor) {
-      // Where the step is bound by the distinct K/V rows that come from memory rather than by products, a tile costs an SM its share
-      // of the copy rate.
-      double distinct = 0, pairs = 0;
-      for (int i = 0; i < batch; ++i) {
-        const int64_t cached = seq_lens[i] - extend_lens[i], reach = p.window > 0 ? std::min(seq_lens[i], p.window + extend_lens[i]) : seq_lens[i];
-        if (extend_lens[i] == 0) continue;
-        distinct += (double)std::min(reach, seq_lens[i] - shared_with_previous[i]);
-        pairs += (double)extend_lens[i] * (double)std::min(reach, cached + (extend_lens[i] + 1) / 2);
-      }
-      const double bytes = distinct * num_kv_heads * 2.0 * head_dim * elem_bytes, flops = pairs * num_qo_heads * 4.0 * head_dim;
-      if (bytes / 6.2e6 > flops / 1.0e9) {
-        const double share = p.tile * 2.0 * head_dim * elem_bytes / (6.2e6 / num_sms);
-        p.cost.alternate = std::max(p.cost.alternate, share);
-        p.cost.single = std::max(p.cost.single, share);
-        p.cost.load = std::max(p.cost.load, share - 2 * p.cost.pair);
+    p.tile = tensor && head_dim <= 128 ? 128 : 64;
+    p.slots = tensor ? num_sms : elem_bytes == 4 && head_dim == 256 ? num_sms : 2 * num_sms;
+    // Query tiles: 128 rows on the tensor cores; 64 or 16 on the CUDA cores, whichever schedule ends first.
+    const double d = head_dim / 128.0;
+    const Costs tc = head_dim == 256 ? Costs{1.0, 0, 1.0, 1.0, 3.0} : Costs{0.6, 0.15, 0.75, 1.1, 2.5};
+    const Costs many = {0, 0, 0, 1.0 + 13.0 * d, 4.0}, few = {0, 0, 0, 1.0 + 4.0 * d, 3.0};
+    struct Form {
+      int rows;
+      Costs cost;
+    };
+    const Form forms[2] = {{tensor ? 128 : 64, tensor ? tc : many}, {16, few}};
+    std::unique_ptr<Builder> built;
+    Problem best_p = p;
+    for (int f = 0; f < (tensor ? 1 : 2); ++f) {
+      Problem trial = p;
+      trial.rows = forms[f].rows;
+      trial.cost = forms[f].cost;
+      trial.tokens_per_tile = std::max(1, trial.rows / p.group);
+      if (tensor) memory_bound_costs(trial, elem_bytes, num_sms);
+      std::unique_ptr<Builder> b(new Builder(trial));
+      b->run();
+      if (!built || b->end < built->end) {
+        best_p = trial;
+        built = std::move(b);
       }
     }
-    Builder b(p);
-    b.run();
+    p = best_p;
+    const Builder& b = *built;
     // what the tables' 32-bit fields hold
     int64_t virt = 0, rows = 0;
     for (const Block& blk : b.blocks) virt = std::max<int64_t>(virt, blk.len);
