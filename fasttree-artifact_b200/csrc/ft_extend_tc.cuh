@@ -9,7 +9,7 @@
 // half of tensor memory, there is one stream, and the scores of a tile are computed beside the softmax of the one before.
 //
 // Roles (warps): one softmax warpgroup per stream (thread = query row = TMEM lane), then one warp each for the MMA issue,
-// K loads, V loads and Q loads.  All of them walk the same task list on their own; mbarriers (full / empty per buffer) are
+// K loads, V loads, and the tiles' row ids and Q loads.  All of them walk the same task list on their own; mbarriers (full / empty per buffer) are
 // the only hand-offs, and the counters behind their phases run on from task to task, so the next task's Q and K are loaded
 // and its first scores computed while the last rows of the task before are normalised and stored.  Every wait is bounded
 // and unwinds the CTA through an abort flag.
@@ -59,11 +59,13 @@ struct ExtCfg {
   static constexpr int KV_BYTES = NB * KV_BLOCK;
   static constexpr int NSK = D == 64 ? 5 : D == 128 ? 2 : 3, NSV = D == 64 ? 5 : D == 128 ? 3 : 2;
   static constexpr int Q_OFF = 0, K_OFF = NW * Q_BYTES, V_OFF = K_OFF + NSK * KV_BYTES;
-  static constexpr int IDS_OFF = V_OFF + NSV * KV_BYTES;  // row ids of the tile being gathered, K's and V's
-  static constexpr int BAR_OFF = IDS_OFF + 2 * TILE * 4;
+  static constexpr int NSI = 4;                           // tiles whose row ids are known or under way
+  static constexpr int IDS_OFF = V_OFF + NSV * KV_BYTES;  // NSI x {TILE row ids}, then NSI x {tokens, KV head}
+  static constexpr int META_OFF = IDS_OFF + NSI * TILE * 4;
+  static constexpr int BAR_OFF = META_OFF + NSI * 8;
   static constexpr int K_FULL = 0, K_EMPTY = K_FULL + NSK, V_FULL = K_EMPTY + NSK, V_EMPTY = V_FULL + NSV, S_FULL = V_EMPTY + NSV,
                        P_HALF = S_FULL + 2, P_FULL = P_HALF + 2, O_FULL = P_FULL + 2, PV_DONE = O_FULL + 2, Q_FULL = PV_DONE + 2, Q_EMPTY = Q_FULL + 1,
-                       NBARS = Q_EMPTY + 1;
+                       IDS_FULL = Q_EMPTY + 1, IDS_EMPTY = IDS_FULL + NSI, NBARS = IDS_EMPTY + NSI;
   static constexpr int ABORT_OFF = BAR_OFF + NBARS * 8, TMEM_SLOT_OFF = ABORT_OFF + 4, SMEM_BYTES = TMEM_SLOT_OFF + 4;
   // tensor memory columns.  Two streams: S_w, then O_w, then (head_dim 64) P_w.  One: two S buffers, O.
   static constexpr int S_COL = 0, O_COL = 256, P_COL = D == 64 ? 384 : S_COL;
@@ -89,6 +91,12 @@ __device__ __forceinline__ bool elect_one() {
   uint32_t one;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(one));
   return one != 0;
+}
+
+__device__ __forceinline__ int lds_int(uint32_t addr) {
+  int x;
+  asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(x) : "r"(addr) : "memory");
+  return x;
 }
 
 // Operand descriptors as two words: the low one holds the address and the leading offset, the high one the stride of 8 rows (1024
@@ -177,6 +185,10 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
     }
     mbar_init(bar(C::Q_FULL), 1);
     mbar_init(bar(C::Q_EMPTY), 1);
+    for (int b = 0; b < C::NSI; ++b) {
+      mbar_init(bar(C::IDS_FULL + b), 33);  // the copies of 32 lanes, and what lane 0 writes beside them
+      mbar_init(bar(C::IDS_EMPTY + b), 2);  // both loaders
+    }
     set_abort(0);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -447,13 +459,13 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       auto wait = [&](uint32_t b, uint32_t phase) {
         if (!__all_sync(0xffffffffu, ext_wait<D>(b, phase, abort_flag))) give_up();
       };
+      // (Loops are kept short on purpose: the roles run at the same time from one instruction cache.)
       int k_stage = 0, v_stage = 0;
-      uint32_t k_phase = 0, v_phase = 0;
-      int tiles_done[2] = {0, 0};
-      uint32_t q_phase = 0;
+      uint32_t k_phase = 0, v_phase = 0, q_phase = 0, p_phases = 0;  // p_phases: a bit per P buffer
+      int s_count = 0;
       const int tasks_u = __shfl_sync(0xffffffffu, task_hi - task_lo, 0);
       for (int n = 0; n < tasks_u && !dead; ++n) {
-        int t0, t1, step, len, lo[2], hi[2], q_tile[2];
+        int t0, t1, step, len, lo0, hi0, lo1 = 0, hi1 = 0, tile1 = 0;
         {
           int kvh;
           const int32_t* item = item_of(task_lo + n, kvh);
@@ -461,15 +473,16 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
           t1 = __shfl_sync(0xffffffffu, __ldg(item + 1), 0);
           step = __shfl_sync(0xffffffffu, __ldg(item + 2), 0);
           len = __shfl_sync(0xffffffffu, __ldg(item + 4), 0);
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const ExtendStream st = extend_stream(item, w);
-            lo[w] = __shfl_sync(0xffffffffu, st.lo, 0);
-            hi[w] = __shfl_sync(0xffffffffu, st.hi, 0);
-            q_tile[w] = __shfl_sync(0xffffffffu, st.q_tile, 0);
+          const ExtendStream a = extend_stream(item, 0);
+          lo0 = __shfl_sync(0xffffffffu, a.lo, 0);
+          hi0 = __shfl_sync(0xffffffffu, a.hi, 0);
+          if constexpr (NW == 2) {
+            const ExtendStream b = extend_stream(item, 1);
+            lo1 = __shfl_sync(0xffffffffu, b.lo, 0);
+            hi1 = __shfl_sync(0xffffffffu, b.hi, 0);
+            tile1 = __shfl_sync(0xffffffffu, b.q_tile, 0);
           }
         }
-        auto active = [&](int w, int t) { return t >= lo[w] && t < hi[w] && (step == 1 || ((t - lo[w]) & 1) == 0); };
         wait(ubar(C::Q_FULL), q_phase);
         q_phase ^= 1u;
         if (dead) break;
@@ -487,46 +500,54 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
           if (dead) return;
           proxy_fence();
           tc_fence_after();
-          const uint32_t a = desc_lo(sm_u + C::Q_OFF + tile * C::Q_BYTES, 16), b = desc_lo(sm_u + C::K_OFF + k_stage * C::KV_BYTES, 16);
-          const uint32_t d = tmem_u + C::S_COL + buf * C::S_STEP, done = ubar(C::S_FULL + buf);
+          uint32_t a = desc_lo(sm_u + C::Q_OFF + tile * C::Q_BYTES, 16), b = desc_lo(sm_u + C::K_OFF + k_stage * C::KV_BYTES, 16);
+          const uint32_t d = tmem_u + C::S_COL + buf * C::S_STEP;
           if (issuer) {
+#pragma unroll 1
+            for (int blk = 0; blk < NB; ++blk) {  // k-steps of 16 along head_dim: +32 B inside a block, +1 block after 4
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks)  // k-steps of 16 along head_dim: +32 B inside a block, +1 block after 4
-              mma_ss(d, a + (uint32_t)((ks >> 2) * (16384 >> 4) + (ks & 3) * 2), b + (uint32_t)((ks >> 2) * (C::KV_BLOCK >> 4) + (ks & 3) * 2),
-                     idesc_s, ks > 0);
-            tc_commit(done);
+              for (int ks = 0; ks < 4; ++ks) mma_ss(d, a + ks * 2, b + ks * 2, idesc_s, (uint32_t)(blk | ks));
+              a += 16384 >> 4;
+              b += C::KV_BLOCK >> 4;
+            }
+            tc_commit(ubar(C::S_FULL + buf));
           }
           __syncwarp();
         };
-        auto issue_pv = [&](int w, int t, bool first, bool last) {
-          const int g = tiles_done[w]++, buf = NW == 2 ? w : g & 1;
-          const uint32_t phase = NW == 2 ? (uint32_t)g & 1u : (uint32_t)(g >> 1) & 1u;
+        auto issue_pv = [&](int w, int buf, int t, bool first, bool last) {
           const uint32_t a = tmem_u + C::P_COL + buf * C::P_STEP, b = desc_lo(sm_u + C::V_OFF + v_stage * C::KV_BYTES, C::KV_BLOCK);
-          const uint32_t d = tmem_u + C::O_COL + w * D, pv_done = ubar(C::PV_DONE + buf), o_full = ubar(C::O_FULL + w);
+          const uint32_t d = tmem_u + C::O_COL + w * D;
           const int ksteps = min(TILE, len - t * TILE + 15) >> 4;  // the rows of V behind the next 16 are not defined
-          const bool whole = ksteps == TILE / 16;
-#pragma unroll
+          constexpr int HALF = TILE / 32;                          // k-steps of 16 tokens in half a tile
+#pragma unroll 1
           for (int half = 0; half < 2; ++half) {
-            wait(ubar((half == 0 ? C::P_HALF : C::P_FULL) + buf), phase);
+            wait(ubar((half == 0 ? C::P_HALF : C::P_FULL) + buf), (p_phases >> buf) & 1u);
             if (half == 0 && !dead) wait_v();
             if (dead) return;
             proxy_fence();
             tc_fence_after();
             if (issuer) {
+#pragma unroll 1
+              for (int h = 0; h < D / C::PV_N; ++h) {
+                const uint32_t ah = a + half * (HALF * 8), bh = b + h * (C::KV_BLOCK >> 4) + half * (HALF * 128);
+                if (ksteps >= (half + 1) * HALF) {
 #pragma unroll
-              for (int h = 0; h < D / C::PV_N; ++h)
-#pragma unroll
-                for (int ks = half * TILE / 32; ks < (half + 1) * TILE / 32; ++ks)
-                  if (whole || ks < ksteps)
-                    mma_ts(d + h * C::PV_N, a + (uint32_t)(ks * 8), b + (uint32_t)(h * (C::KV_BLOCK >> 4) + ks * 128), idesc_o,
-                           ks > 0 ? 1u : (first ? 0u : 1u));
+                  for (int ks = 0; ks < HALF; ++ks)
+                    mma_ts(d + h * C::PV_N, ah + ks * 8, bh + ks * 128, idesc_o, !first || half + ks > 0 ? 1u : 0u);
+                } else {
+#pragma unroll 1
+                  for (int ks = 0; ks < ksteps - half * HALF; ++ks)
+                    mma_ts(d + h * C::PV_N, ah + ks * 8, bh + ks * 128, idesc_o, !first || half + ks > 0 ? 1u : 0u);
+                }
+              }
               if (half == 1) {
-                if (NW == 1) tc_commit(pv_done);
-                if (last) tc_commit(o_full);
+                if (NW == 1) tc_commit(ubar(C::PV_DONE + buf));
+                if (last) tc_commit(ubar(C::O_FULL + w));
               }
             }
             __syncwarp();
           }
+          p_phases ^= 1u << buf;
         };
         auto release_k = [&]() {
           wait_k();
@@ -550,12 +571,15 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
         };
         if constexpr (NW == 2) {
           // iteration t: the products with V of tile t - step, then the scores of tile t, stream by stream
+#pragma unroll 1
           for (int t = t0; t < t1 + step && !dead; ++t) {
             const int before = t - step;
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              if (before >= t0 && active(w, before)) issue_pv(w, before, before == lo[w], before + step >= hi[w]);
-              if (!dead && t < t1 && active(w, t)) issue_qk(w, q_tile[w]);
+#pragma unroll 1
+            for (int w = 0; w < 2 && !dead; ++w) {
+              const int lo = w == 0 ? lo0 : lo1, hi = w == 0 ? hi0 : hi1;
+              if (step == 2 && ((t - lo) & 1) != 0) continue;  // (t and t - step are the same stream's)
+              if (before >= lo && before < hi) issue_pv(w, w, before, before == lo, before + step >= hi);
+              if (!dead && t >= lo && t < hi) issue_qk(w, w == 0 ? 0 : tile1);
             }
             if (dead) break;
             if (t < t1) release_k();
@@ -563,14 +587,16 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
             if (before >= t0 && before < t1 && !dead) release_v();
           }
         } else {
+          // (buffers by the tile's number over all tasks: its parity is s_count's)
+#pragma unroll 1
           for (int t = t0; t <= t1 && !dead; ++t) {
             if (t < t1) {
-              issue_qk((tiles_done[0] + (t > t0 ? 1 : 0)) & 1, 0);
+              issue_qk(s_count++ & 1, 0);
               if (!dead) release_k();
               if (t == t1 - 1 && !dead && issuer) tc_commit(ubar(C::Q_EMPTY));
             }
             if (t > t0 && !dead) {
-              issue_pv(0, t - 1, t - 1 == t0, t == t1);
+              issue_pv(0, (s_count - (t < t1 ? 2 : 1)) & 1, t - 1, t - 1 == lo0, t == t1);
               if (!dead) release_v();
             }
           }
@@ -579,205 +605,180 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       __syncwarp();
     } else if (role <= 2) {
       // ==================================================================== K loads (role 1), V loads (role 2)
-      auto load_all = [&](auto which) {
-      constexpr bool is_k = decltype(which)::value;
+      const bool is_k = role == 1;
       const CUtensorMap* map = is_k ? &tp.k_map : &tp.v_map;
       const CUtensorMap* rows_map = is_k ? &tp.k_rows_map : &tp.v_rows_map;
-      const int64_t s0 = is_k ? p.k_s0 : p.v_s0, s1 = is_k ? p.k_s1 : p.v_s1;
+      const int64_t s0 = is_k ? p.k_s0 : p.v_s0;
+      const int s1 = (int)(is_k ? p.k_s1 : p.v_s1);
       const T* base0 = reinterpret_cast<const T*>(is_k ? p.k : p.v);
-      constexpr int full0 = is_k ? C::K_FULL : C::V_FULL, empty0 = is_k ? C::K_EMPTY : C::V_EMPTY, stages = is_k ? C::NSK : C::NSV;
+      const uint32_t full0 = bar(is_k ? C::K_FULL : C::V_FULL), empty0 = bar(is_k ? C::K_EMPTY : C::V_EMPTY);
       const uint32_t ring = sm + (is_k ? C::K_OFF : C::V_OFF);
-      const uint32_t ids_sm = sm + C::IDS_OFF + (is_k ? 0 : TILE * 4);
+      const int stages = is_k ? C::NSK : C::NSV;
       const uint32_t row_lim = (uint32_t)(p.kv_rows < 0x7fffffffLL ? p.kv_rows : 0x7fffffffLL);
-      // The tiles of the CTA's tasks, one after the other, on a conveyor: the record of the tile after next but two is read, the
-      // table entries of the next but two are known, the row ids of three tiles are under way.  (A plain load that is sent off
-      // beside a hundred kilobytes of tile copies comes back after them; and a mixed tile's ids are two loads deep.)
-      struct Head {  // of a task: its tiles and where their records are
-        int t0, t1, tile0, kvh;
-        int4 rec;
-      };
-      struct Ids {  // row ids of a tile in flight; valid 0: there is no such tile
-        int id[TILE / 32], valid, kvh;
-      };
-      auto head_of = [&](int n) {
-        Head h;
-        const int32_t* item = item_of(n, h.kvh);
-        const int4 x = __ldg(reinterpret_cast<const int4*>(item)), y = __ldg(reinterpret_cast<const int4*>(item + 4));
-        h.t0 = x.x;
-        h.t1 = x.y;
-        h.tile0 = y.y;
-        h.rec = __ldg(reinterpret_cast<const int4*>(item + 24));
-        return h;
-      };
-      int n_next = task_lo;                 // the task whose head is in `next`
-      const int4 first_head = __ldg(my_share + 1);
-      Head cur = {first_head.x, first_head.y, first_head.z, share.z % p.kv_heads, __ldg(my_share + 2)}, next = cur;
-      int t_rec = cur.t0;                   // tile of `rec`
-      int4 rec = cur.rec;
-      bool rec_here = true;
-      ++n_next;
-      if (n_next < task_hi) next = head_of(n_next);
-      int rec_kvh = cur.kvh;
-      auto advance_rec = [&]() {            // rec becomes the record of the following tile
-        if (++t_rec < cur.t1) {
-          rec = __ldg(reinterpret_cast<const int4*>(p.tiles) + 2 * ((int64_t)cur.tile0 + t_rec));
-        } else if (n_next < task_hi) {
-          cur = next;
-          t_rec = cur.t0;
-          rec = cur.rec;
-          rec_kvh = cur.kvh;
-          ++n_next;
-          if (n_next < task_hi) next = head_of(n_next);
-        } else {
-          rec_here = false;
+      int stage = 0, slot = 0;
+      uint32_t phase = 1, ids_phase = 0;
+      set_up();
+      while (true) {
+        if (!__all_sync(0xffffffffu, ext_wait<D>(bar(C::IDS_FULL + slot), ids_phase, abort_flag))) {
+          give_up();
+          break;
         }
-      };
-      int64_t entry[TILE / 32];
-      int entry_valid = 0, entry_kvh = 0;
-      auto advance_entries = [&]() {        // the entries become those of rec's tile
-        entry_valid = rec_here ? rec.z : 0;
-        entry_kvh = rec_kvh;
-        if (rec_here) {
-#pragma unroll
-          for (int h = 0; h < TILE / 32; ++h) entry[h] = lane + 32 * h < rec.z ? extend_entry(p, rec, lane + 32 * h) : 0;
-          advance_rec();
-        }
-      };
-      auto refill = [&](Ids& x) {
-        x.valid = entry_valid;
-        x.kvh = entry_kvh;
-#pragma unroll
-        for (int h = 0; h < TILE / 32; ++h) {
-          x.id[h] = -1;
-          if (lane + 32 * h < entry_valid) x.id[h] = __ldg(p.kv_entries + entry[h]);
-        }
-        advance_entries();
-      };
-      int stage = 0;
-      uint32_t phase = 1;
-      auto load_tile = [&](const Ids& x) {
-        const int valid = x.valid, first = __shfl_sync(0xffffffffu, x.id[0], 0);
+        const uint32_t ids = sm + C::IDS_OFF + slot * (TILE * 4);
+        int valid, kvh, id[TILE / 32];
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];\n" : "=r"(valid), "=r"(kvh) : "r"(sm + C::META_OFF + slot * 8) : "memory");
+        if (valid == 0) break;  // the end
+        const int first = __shfl_sync(0xffffffffu, lds_int(ids), 0);
         bool dense = true, in_pool = true;
 #pragma unroll
         for (int h = 0; h < TILE / 32; ++h) {
-          dense &= x.id[h] == first + lane + 32 * h;
-          in_pool &= lane + 32 * h >= valid || (uint32_t)x.id[h] < row_lim;
+          id[h] = lds_int(ids + (lane + 32 * h) * 4);
+          dense &= id[h] == first + lane + 32 * h;
+          in_pool &= lane + 32 * h >= valid || (uint32_t)id[h] < row_lim;
         }
         in_pool = __all_sync(0xffffffffu, in_pool);
         dense = tp.has_tma && valid == TILE && in_pool && __all_sync(0xffffffffu, dense);
-        if (!__all_sync(0xffffffffu, ext_wait<D>(bar(empty0 + stage), phase, abort_flag))) {
+        if (!__all_sync(0xffffffffu, ext_wait<D>(empty0 + 8u * stage, phase, abort_flag))) {
           give_up();
-          return;
+          break;
         }
-        const uint32_t buf = ring + stage * C::KV_BYTES, full = bar(full0 + stage);
+        const uint32_t buf = ring + stage * C::KV_BYTES, full = full0 + 8u * stage;
         if (dense) {
           if (lane == 0) {
             mbar_arrive_expect_tx(full, C::KV_BYTES);
 #pragma unroll
-            for (int h = 0; h < NB; ++h) tma_load_3d(buf + h * C::KV_BLOCK, map, 64 * h, x.kvh, first, full);
+            for (int h = 0; h < NB; ++h) tma_load_3d(buf + h * C::KV_BLOCK, map, 64 * h, kvh, first, full);
           } else {
             mbar_arrive(full);
           }
         } else {
-          __syncwarp();
-#pragma unroll
-          for (int h = 0; h < TILE / 32; ++h)
-            asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(ids_sm + (lane + 32 * h) * 4), "r"(x.id[h]) : "memory");
           int done = 0;
           if (tp.has_gather4 && in_pool) {
             done = valid & ~3;
             if (lane == 0 && done > 0) mbar_expect_tx(full, (uint32_t)done * (2u * D));
             __syncwarp();
+#pragma unroll 1
             for (int i = lane; i < done / 4 * NB; i += 32) {
               const int blk = i % NB, r = i / NB * 4;
               int r0, r1, r2, r3;
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(ids_sm + r * 4));
-              tma_gather4(buf + blk * C::KV_BLOCK + r * 128, rows_map, x.kvh * (int)s1 + 64 * blk, r0, r1, r2, r3, full);
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(ids + r * 4));
+              tma_gather4(buf + blk * C::KV_BLOCK + r * 128, rows_map, kvh * s1 + 64 * blk, r0, r1, r2, r3, full);
             }
-          } else {
-            __syncwarp();
           }
           // what is left, 16 bytes at a time; of V zeros up to the next 16 rows
-          const T* base = base0 + (int64_t)x.kvh * s1;
+          const T* base = base0 + (int64_t)kvh * s1;
           const int end = is_k ? valid : (valid + 15) & ~15, c16 = lane % C::CPR;
+#pragma unroll 1
           for (int r = done + lane / C::CPR; r < end; r += 32 / C::CPR) {
-            int row_id;
-            asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(row_id) : "r"(ids_sm + r * 4));
-            const bool ok = (uint32_t)row_id < row_lim;  // (behind the last token -1)
+            const int row_id = lds_int(ids + r * 4);
+            const bool ok = r < valid && (uint32_t)row_id < row_lim;
             cp_async16_zfill(buf + (uint32_t)((c16 >> 3) * C::KV_BLOCK) + tc_swz(r, c16 & 7, 0), base + (int64_t)(ok ? row_id : 0) * s0 + c16 * 8, ok);
           }
           if (!in_pool && lane == 0) flag_error(FT_DEV_BAD_KV_INDEX);
           mbar_arrive_on_cp_async(full);
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(bar(C::IDS_EMPTY + slot));
+        if (++slot == C::NSI) {
+          slot = 0;
+          ids_phase ^= 1u;
         }
         if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }
-      };
-      Ids x0, x1, x2;
-      advance_entries();
-      refill(x0);
-      set_up();
-      refill(x1);
-      refill(x2);
-      while (x0.valid != 0 && !dead) {  // (three copies of the body: ids under way stay in the registers that they go to)
-        load_tile(x0);
-        refill(x0);
-        if (x1.valid == 0 || dead) break;
-        load_tile(x1);
-        refill(x1);
-        if (x2.valid == 0 || dead) break;
-        load_tile(x2);
-        refill(x2);
       }
       cp_async_wait<0>();
-      };
-      if (role == 1)
-        load_all(std::true_type{});
-      else
-        load_all(std::false_type{});
     } else {
+      // ==================================================================== row ids of the K/V tiles, Q loads
+      // The ids of a tile go to a slot of a ring that both loaders read, NSI tiles ahead of them: a plain load that is sent off
+      // beside a hundred kilobytes of tile copies comes back after them.  A task's first tiles come before its Q, for which
+      // this warp may have to wait until the task before is through with its own.
+      int slot = 0, items = 0;
+      uint32_t ids_phase = 1;
+      auto put_ids = [&](const int4 rec, int kvh) {  // rec.z 0: the end
+        if (!__all_sync(0xffffffffu, ext_wait<D>(bar(C::IDS_EMPTY + slot), ids_phase, abort_flag))) {
+          give_up();
+          return;
+        }
+        const uint32_t ids = sm + C::IDS_OFF + slot * (TILE * 4);
+#pragma unroll
+        for (int h = 0; h < TILE / 32; ++h)
+          if (lane + 32 * h < rec.z) cp_async4(ids + (lane + 32 * h) * 4, p.kv_entries + extend_entry(p, rec, lane + 32 * h));
+        if (lane == 0) {
+          asm volatile("st.shared.v2.b32 [%0], {%1, %2};\n" ::"r"(sm + C::META_OFF + slot * 8), "r"(rec.z), "r"(kvh) : "memory");
+          mbar_arrive(bar(C::IDS_FULL + slot));
+        }
+        mbar_arrive_on_cp_async(bar(C::IDS_FULL + slot));
+        if (++slot == C::NSI) {
+          slot = 0;
+          ids_phase ^= 1u;
+        }
+      };
       set_up();
-      // ==================================================================== Q loads
-      int items = 0;
       for (int n = task_lo; n < task_hi && !dead; ++n, ++items) {
-        int kvh;
+        int kvh, t0, t1, tile0;
+        int4 rec;
         const int32_t* item = item_of(n, kvh);
+        if (n == task_lo) {
+          const int4 head = __ldg(my_share + 1);
+          t0 = head.x;
+          t1 = head.y;
+          tile0 = head.z;
+          rec = __ldg(my_share + 2);
+        } else {
+          t0 = __ldg(item);
+          t1 = __ldg(item + 1);
+          tile0 = __ldg(item + 5);
+          rec = __ldg(reinterpret_cast<const int4*>(item + 24));
+        }
+        int t = t0;
+        auto put_until = [&](int end) {
+#pragma unroll 1
+          for (; t < end && !dead; ++t) {
+            const int4 next = t + 1 < t1 ? __ldg(reinterpret_cast<const int4*>(p.tiles) + 2 * ((int64_t)tile0 + t + 1)) : rec;
+            put_ids(rec, kvh);
+            rec = next;
+          }
+        };
+        put_until(min(t1, t0 + 2));
+        if (dead) break;
         const int q_tiles = __ldg(item + 3);
-        if (!ext_wait<D>(bar(C::Q_EMPTY), ((uint32_t)items & 1u) ^ 1u, abort_flag)) {
+        if (!__all_sync(0xffffffffu, ext_wait<D>(bar(C::Q_EMPTY), ((uint32_t)items & 1u) ^ 1u, abort_flag))) {
           give_up();
           break;
         }
         // bytes first: a whole tile if its tokens' rows are consecutive, else a box per token
-        uint32_t bytes = 0;
-        bool in_order[2] = {false, false};
-        int first[2] = {0, 0};
+        uint32_t bytes = 0, in_order = 0;
+#pragma unroll 1
         for (int w = 0; w < q_tiles; ++w) {
           const ExtendStream st = extend_stream(item, w);
-          first[w] = __ldg(p.tokens + 2 * st.tok0);
-          bool mine = true, valid = true;
+          const int first = __ldg(p.tokens + 2 * st.tok0);
+          bool mine = true;
           int rows = 0;
           for (int i = lane; i < st.ntok; i += 32) {
             const int r = __ldg(p.tokens + 2 * (st.tok0 + i));
-            mine &= r == first[w] + i;
-            if (r >= 0 && r < p.q_rows) ++rows;
-            else valid = false;
+            mine &= r == first + i && r >= 0 && r < p.q_rows;
+            rows += r >= 0 && r < p.q_rows;
           }
-          in_order[w] = __all_sync(0xffffffffu, mine && valid);
+          const bool whole = __all_sync(0xffffffffu, mine);
           rows = __reduce_add_sync(0xffffffffu, rows);
-          bytes += in_order[w] ? (uint32_t)(128 / G * G) * (2u * D) : (uint32_t)rows * G * (2u * D);
+          in_order |= whole ? 1u << w : 0u;
+          bytes += whole ? (uint32_t)(128 / G * G) * (2u * D) : (uint32_t)rows * G * (2u * D);
         }
         if (lane == 0) mbar_arrive_expect_tx(bar(C::Q_FULL), bytes);
         __syncwarp();
+#pragma unroll 1
         for (int w = 0; w < q_tiles; ++w) {
           const ExtendStream st = extend_stream(item, w);
           const uint32_t dst = sm + C::Q_OFF + w * C::Q_BYTES;
-          if (in_order[w]) {
-            if (lane < NB) tma_load_3d(dst + lane * 16384, &tp.q_map_tile, 64 * lane, kvh * G, first[w], bar(C::Q_FULL));
+          if ((in_order >> w & 1u) != 0) {
+            if (lane < NB) tma_load_3d(dst + lane * 16384, &tp.q_map_tile, 64 * lane, kvh * G, __ldg(p.tokens + 2 * st.tok0), bar(C::Q_FULL));
           } else {
+#pragma unroll 1
             for (int i = lane; i < st.ntok; i += 32) {
               const int r = __ldg(p.tokens + 2 * (st.tok0 + i));
               if (r < 0 || r >= p.q_rows) continue;
+#pragma unroll 1
               for (int sub = 0; sub < G; sub += tp.q_box_heads)
 #pragma unroll
                 for (int h = 0; h < NB; ++h)
@@ -785,7 +786,10 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
             }
           }
         }
+        put_until(t1);
       }
+      if (!dead) put_ids(make_int4(0, 0, 0, -1), 0);
+      cp_async_wait<0>();
     }
   }
 
