@@ -278,7 +278,7 @@ int ft_extend(const ft_extend_args* a) {
   p.num_items = pl.num_items, p.num_merged = pl.num_merged, p.partial_rows = pl.partial_rows;
   p.heads = a->num_qo_heads, p.kv_heads = a->num_kv_heads, p.group = a->num_qo_heads / a->num_kv_heads, p.head_dim = a->head_dim;
   p.tile = pl.tile_tokens;
-  p.sm_scale = a->sm_scale, p.logit_cap = a->logit_cap > 0.f ? a->logit_cap : 0.f;
+  p.sm_scale = a->sm_scale, p.logit_cap = a->logit_cap > 0.f && a->logit_cap < INFINITY ? a->logit_cap : 0.f;  // (an infinite cap is none)
   cudaStream_t st = static_cast<cudaStream_t>(a->stream);
   if (a->dtype == FT_F16) return launch_extend<__half>(p, a, tensor, st);
   if (a->dtype == FT_BF16) return launch_extend<__nv_bfloat16>(p, a, tensor, st);

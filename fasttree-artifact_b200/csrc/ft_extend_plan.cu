@@ -336,10 +336,11 @@ class Builder {
       c.push_back(n);
     }
     double total = 0;
-    auto cut = [&](double limit, std::vector<Item>& out) {
+    auto cut = [&](double most, std::vector<Item>& out, int from_block = 0) {
       out.clear();
       double parts = 0;  // partial rows of the cut
       for (int b = 0; b < nb; ++b) {
+        const double limit = b < from_block ? 0 : most;
         const size_t from = out.size();
         for (size_t s = 0; s + 1 < cuts[b].size(); ++s) {
           const int t0 = cuts[b][s], t1 = cuts[b][s + 1];
@@ -384,6 +385,22 @@ class Builder {
         items = trial;
       }
       if (f == 0 && finish <= 1.04 * even + 1.0) break;  // nothing to gain
+    }
+    // Tasks that fill some rounds of the slots and leave a part of one: only the blocks of that part are cut.
+    const int64_t tasks = (int64_t)nb * p_.kv_heads, left = tasks % p_.slots;
+    if (best > 1.04 * even + 1.0 && tasks > p_.slots && tasks < 16 * p_.slots && left > 0) {
+      const int few = (int)std::min<int64_t>(nb, ceil_div(left, p_.kv_heads));
+      double typical = 0;
+      for (int b = nb - few; b < nb; ++b) typical += make_item(b, act[b], 0, (int)act[b].size(), false).cost / few;
+      static const int ways[] = {2, 3, 4, 6};
+      for (int n : ways) {
+        const double parts = cut(typical / n, trial, nb - few);
+        const double finish = deal(trial, nullptr, nullptr) + merge_cost(parts);
+        if (finish < best * 0.98) {
+          best = end = finish;
+          items = trial;
+        }
+      }
     }
     std::vector<int> order, slot;
     deal(items, &order, &slot);

@@ -25,8 +25,6 @@
 // there P has columns of its own.  When a stream's scores are ready all its earlier products are done (tcgen05.commit covers
 // every MMA issued before it), so no wait is needed before O is rescaled with two streams; with one there is a barrier for it.
 //
-// Capped scores: cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap)).
-//
 // Rows of V that a query does not see are multiplied by P = 0, and 0 x Inf is NaN: a row that is not shown everything and did
 // not come out finite is computed again from its own tokens (extend_row).
 #pragma once
@@ -72,7 +70,7 @@ struct ExtCfg {
   static constexpr int S_STEP = NW == 2 ? 128 : 64, P_STEP = D == 64 ? 64 : S_STEP;
   static constexpr int PV_N = D == 128 ? 128 : 64;  // columns of O per product
   static constexpr int CPR = D / 8;                 // 16-byte chunks of a row
-  static constexpr int REGS_SOFTMAX = 208, REGS_OTHER = 88, REGS_LAUNCH = 168;
+  static constexpr int REGS_SOFTMAX = 224, REGS_OTHER = 56, REGS_LAUNCH = 168;
   static constexpr int WAIT_LIMIT = 1 << 25;        // a softmax warp that computes rows again keeps the others waiting
   static_assert(SMEM_BYTES <= 232448, "one CTA must fit in one SM's shared memory");
   static_assert(NW != 2 || (2 * REGS_SOFTMAX + REGS_OTHER) * 128 <= REGS_LAUNCH * THREADS, "register trade must balance");
@@ -139,6 +137,65 @@ __device__ __forceinline__ bool ext_wait(uint32_t bar, uint32_t parity, uint32_t
   }
   return false;
 }
+
+// Capped scores in powers of two, c2 tanh(x), x = S scale / cap, c2 = cap log2(e).
+//
+// Up to |x| = 1.25 by the minimax polynomial tanh(x) = x (q0 + q1 x^2 + ... + q6 x^12), fitted with the Remez exchange: off by
+// at most 2.9e-7.  Two tanh or one exponential more per score on the special-function unit, which the softmax already keeps busy,
+// cost more than eight packed FMAs for two scores (2048 on 2048 tokens, 32/4 heads of 128, capped: 221 us, so NNN; not capped 111).
+// A warp that meets a larger |x| goes over to tanh(x) = 1 - 2 / (1 + e^(2 x)), one reciprocal for two scores.
+struct Capped {
+  float a[7], c2, k2, u_most;
+  __device__ __forceinline__ Capped(float scale, float cap) {
+    constexpr float LOG2E = 1.4426950408889634f;
+    constexpr float q[7] = {0.9999964833259583f,    -0.33324214816093445f,  0.1326480358839035f,   -0.051644690334796906f,
+                            0.017636235803365707f, -0.004325489979237318f, 0.0005254826974123716f};
+    const float k = scale / cap;
+    c2 = cap * LOG2E;
+    k2 = 2.f * LOG2E * k;
+    u_most = (1.25f / k) * (1.25f / k);
+    float f = c2 * k;
+#pragma unroll
+    for (int i = 0; i < 7; ++i) {
+      a[i] = f * q[i];
+      f *= k * k;
+    }
+  }
+  // in place; returns the largest square of a score
+  template <int N>
+  __device__ __forceinline__ float polynomial(float (&s)[N]) const {
+    float most[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const float2 x = make_float2(s[2 * i], s[2 * i + 1]), u = __fmul2_rn(x, x);
+      asm("max.f32 %0, %0, %1, %2;" : "+f"(most[i & 1]) : "f"(u.x), "f"(u.y));
+      float2 y = make_float2(a[6], a[6]);
+#pragma unroll
+      for (int k = 5; k >= 0; --k) y = __ffma2_rn(y, u, make_float2(a[k], a[k]));
+      y = __fmul2_rn(y, x);
+      s[2 * i] = y.x;
+      s[2 * i + 1] = y.y;
+    }
+    return fmaxf(most[0], most[1]);
+  }
+  template <int N>
+  __device__ __forceinline__ void exact(float (&s)[N]) const {
+    const float2 one = make_float2(1.f, 1.f), n2 = make_float2(-2.f * c2, -2.f * c2), p2 = make_float2(c2, c2);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      // (2^60 and above is as good as infinite: 1 + 2^60 squared still is a number)
+      float2 y = __fmul2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(k2, k2));
+      asm("min.NaN.f32 %0, %0, %1;" : "+f"(y.x) : "f"(60.f));
+      asm("min.NaN.f32 %0, %0, %1;" : "+f"(y.y) : "f"(60.f));
+      y = __fadd2_rn(make_float2(fast_exp2(y.x), fast_exp2(y.y)), one);
+      float r;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y.x * y.y));
+      y = __ffma2_rn(__fmul2_rn(make_float2(r, r), make_float2(y.y, y.x)), n2, p2);
+      s[2 * i] = y.x;
+      s[2 * i + 1] = y.y;
+    }
+  }
+};
 
 template <typename T, int D, bool CAP>
 __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const __grid_constant__ ExtendTcParams tp) {
@@ -225,15 +282,10 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
     const uint32_t o_col = t_lane + C::O_COL + w * D;
     const float scale = p.sm_scale == 0.f ? 1.17549435e-38f : fabsf(p.sm_scale);
     constexpr float LOG2E = 1.4426950408889634f;
-    // scores in powers of two: S x scale2; capped ones c2 - 2 c2 / (1 + 2^(S x k2))
+    // scores in powers of two: S x scale2, or what Capped makes of S
     const float scale2 = CAP ? 1.f : scale * LOG2E;
-    const float c2 = CAP ? p.logit_cap * LOG2E : 0.f, k2 = CAP ? 2.f * LOG2E * scale / p.logit_cap : 0.f;
-    auto capped = [&](float x) {
-      float y, r;
-      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * k2));
-      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y + 1.f));
-      return fmaf(-2.f * c2, r, c2);
-    };
+    const Capped capped = CAP ? Capped(scale, p.logit_cap) : Capped(0.f, 1.f);
+    bool steep = false;  // capped scores: this warp has met one that the polynomial is not for
     int tiles_done = 0, items_done = 0;
     for (int n = task_lo; n < task_hi && !dead; ++n) {
       int lo, hi, step, rows;    // of the stream: K/V tiles lo, lo + step, ... below hi, rows of the query tile
@@ -285,6 +337,18 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
 #pragma unroll
         for (int c = 0; c < TILE / 32; ++c) tmem_ld32_nowait(s_col + 32 * c, *reinterpret_cast<float(*)[32]>(&s[32 * c]));
         tmem_wait_ld();
+        if constexpr (CAP) {
+          if (!steep) {
+            const float most = capped.polynomial(s);
+            steep = __any_sync(0xffffffffu, row < rows && most > capped.u_most);
+            if (steep) {
+#pragma unroll
+              for (int c = 0; c < TILE / 32; ++c) tmem_ld32_nowait(s_col + 32 * c, *reinterpret_cast<float(*)[32]>(&s[32 * c]));
+              tmem_wait_ld();
+            }
+          }
+          if (steep) capped.exact(s);
+        }
         if constexpr (MASKED) {
 #pragma unroll
           for (int k = 0; k < TILE / 32; ++k)
@@ -298,10 +362,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
 #pragma unroll
           for (int k = 0; k < 4; ++k) asm("max.f32 %0, %0, %1, %2;" : "+f"(mx4[k]) : "f"(s[c + 2 * k]), "f"(s[c + 2 * k + 1]));
         float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-        if constexpr (CAP)
-          mx = !MASKED || any ? capped(mx) : -INFINITY;
-        else
-          mx *= scale2;
+        if constexpr (!CAP) mx *= scale2;
         float corr = 1.f;
         bool grow = false;
         if (mx > m_used + 8.f || m_used == -INFINITY) {  // the offset may lag the true maximum by up to 2^8
@@ -322,11 +383,6 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
 #pragma unroll
           for (int i = 0; i < TILE / 4; ++i) {
             float2 x = make_float2(s[h * (TILE / 2) + 2 * i], s[h * (TILE / 2) + 2 * i + 1]);
-            if constexpr (CAP) {
-              // (a masked score, -inf, stays one)
-              x.x = MASKED && x.x == -INFINITY ? x.x : capped(x.x);
-              x.y = MASKED && x.y == -INFINITY ? x.y : capped(x.y);
-            }
             x = __ffma2_rn(x, sc2, no2);
             x.x = fast_exp2(x.x);
             x.y = fast_exp2(x.y);
@@ -503,7 +559,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
           uint32_t a = desc_lo(sm_u + C::Q_OFF + tile * C::Q_BYTES, 16), b = desc_lo(sm_u + C::K_OFF + k_stage * C::KV_BYTES, 16);
           const uint32_t d = tmem_u + C::S_COL + buf * C::S_STEP;
           if (issuer) {
-#pragma unroll 1
+#pragma unroll
             for (int blk = 0; blk < NB; ++blk) {  // k-steps of 16 along head_dim: +32 B inside a block, +1 block after 4
 #pragma unroll
               for (int ks = 0; ks < 4; ++ks) mma_ss(d, a + ks * 2, b + ks * 2, idesc_s, (uint32_t)(blk | ks));
@@ -519,7 +575,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
           const uint32_t d = tmem_u + C::O_COL + w * D;
           const int ksteps = min(TILE, len - t * TILE + 15) >> 4;  // the rows of V behind the next 16 are not defined
           constexpr int HALF = TILE / 32;                          // k-steps of 16 tokens in half a tile
-#pragma unroll 1
+#pragma unroll
           for (int half = 0; half < 2; ++half) {
             wait(ubar((half == 0 ? C::P_HALF : C::P_FULL) + buf), (p_phases >> buf) & 1u);
             if (half == 0 && !dead) wait_v();
@@ -527,7 +583,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
             proxy_fence();
             tc_fence_after();
             if (issuer) {
-#pragma unroll 1
+#pragma unroll
               for (int h = 0; h < D / C::PV_N; ++h) {
                 const uint32_t ah = a + half * (HALF * 8), bh = b + h * (C::KV_BLOCK >> 4) + half * (HALF * 128);
                 if (ksteps >= (half + 1) * HALF) {
