@@ -82,6 +82,7 @@ struct Problem {
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+uint32_t bits_below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
 class Builder {
  public:
@@ -120,7 +121,8 @@ class Builder {
   }
 
   // Query tiles: a request joins the tile that the one before it has not filled where that costs less K/V than a tile of
-  // its own - whole if it fits, in part if what it shares is the most of what it reads.
+  // its own - whole if it fits and does not read long stretches alone (those would only become tiles with masks), in part if
+  // what it shares is the most of what it reads.
   void pack_blocks() {
     std::vector<std::pair<int, int>> tiles;  // [first, last) token
     const int cap = p_.tokens_per_tile;
@@ -134,7 +136,8 @@ class Builder {
         int64_t common = INT64_MAX;  // with the request before it that has tokens
         for (int k = last + 1; k <= i; ++k) common = std::min(common, p_.shared[k]);
         const int64_t part = std::min<int64_t>(e, room), own = prefix(i) - common + part;
-        const bool join = e <= room || (common > 0 && own * cap < part * p_.seq[i]);
+        const bool alone = own > 4 * p_.tile && own > 4 * common;
+        const bool join = (e <= room && !alone) || (common > 0 && own * cap < part * p_.seq[i]);
         if (join) {
           end = at + (int)part;
           at = end;
@@ -336,7 +339,7 @@ class Builder {
       c.push_back(n);
     }
     double total = 0;
-    auto cut = [&](double most, std::vector<Item>& out, int from_block = 0) {
+    auto cut = [&](double most, std::vector<Item>& out, int from_block = 0, bool remainder = false) {
       out.clear();
       double parts = 0;  // partial rows of the cut
       for (int b = 0; b < nb; ++b) {
@@ -358,7 +361,14 @@ class Builder {
             }
           }
           for (int k = 0; k < n; ++k) {
-            const int a = one.t0 + (int)((int64_t)(one.t1 - one.t0) * k / n), e = one.t0 + (int)((int64_t)(one.t1 - one.t0) * (k + 1) / n);
+            const int all = one.t1 - one.t0;
+            int a = one.t0 + (int)((int64_t)all * k / n), e = one.t0 + (int)((int64_t)all * (k + 1) / n);
+            if (remainder && n > 1) {  // pieces as long as the limit allows, and what is left
+              const int len = std::max(1, (int)(limit * all / (one.cost - p_.cost.item)));
+              a = std::min(one.t1, one.t0 + k * len);
+              e = k + 1 == n ? one.t1 : std::min(one.t1, a + len);
+              if (a >= e) continue;
+            }
             const Item it = make_item(b, act[b], a, e, p_.streams && !(whole && limit <= 0));
             if (it.which != 0) out.push_back(it);
           }
@@ -375,10 +385,22 @@ class Builder {
     auto merge_cost = [&](double parts) {  // a launch, and the partial rows written and read back
       return parts > 0 ? 4.0 + parts * p_.kv_heads * p_.group * 8.0 * p_.head_dim / 4e6 : 0.0;
     };
+    // no schedule of these items ends sooner: their work spread evenly, the dearest of them, the merge
+    auto at_least = [&](const std::vector<Item>& its, double parts) {
+      double sum = 0, dearest = 0;
+      for (const Item& it : its) {
+        sum += it.cost * p_.kv_heads;
+        dearest = std::max(dearest, it.cost);
+      }
+      return std::max(sum / p_.slots, dearest) + merge_cost(parts);
+    };
     double best = -1;
     static const double pieces[] = {0, 2.0, 1.5, 1.25, 1.15, 1.08, 1.04, 1.0, 0.75, 0.5, 0.34, 0.25};
-    for (double f : pieces) {
-      const double parts = cut(f * even, trial);
+    for (int form = 0; form < 2 * (int)(sizeof(pieces) / sizeof(pieces[0])); ++form) {
+      const double f = pieces[form / 2];
+      if (form % 2 == 1 && (f < 1.0 || f > 1.3)) continue;  // in equal pieces, or long ones and a remainder
+      const double parts = cut(f * even, trial, 0, form % 2 == 1);
+      if (best >= 0 && at_least(trial, parts) >= best * 0.99) continue;
       const double finish = deal(trial, nullptr, nullptr) + merge_cost(parts);
       if (best < 0 || finish < best * 0.99) {
         best = end = finish;
@@ -395,6 +417,7 @@ class Builder {
       static const int ways[] = {2, 3, 4, 6};
       for (int n : ways) {
         const double parts = cut(typical / n, trial, nb - few);
+        if (at_least(trial, parts) >= best * 0.98) continue;
         const double finish = deal(trial, nullptr, nullptr) + merge_cost(parts);
         if (finish < best * 0.98) {
           best = end = finish;
@@ -501,8 +524,9 @@ void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
             for (int t = b.segs[s].tok_lo; t < b.segs[s].tok_hi; ++t) {
               int64_t from, to;
               sight(b.segs[s], t, from, to);
-              for (int64_t v = std::max<int64_t>(from, v0); v < std::min<int64_t>(to, v1); ++v)
-                extra[bits_at + t * words + (v - v0) / 32] |= (int32_t)(1u << ((v - v0) & 31));
+              const int lo = (int)(std::max<int64_t>(from, v0) - v0), hi = (int)(std::min<int64_t>(to, v1) - v0);
+              for (int wd = 0; wd < words && lo < hi; ++wd)
+                extra[bits_at + t * words + wd] |= (int32_t)(bits_below(hi - 32 * wd) & ~bits_below(lo - 32 * wd));
             }
         }
         x[4 + w] = bits_at;

@@ -664,8 +664,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       const bool is_k = role == 1;
       const CUtensorMap* map = is_k ? &tp.k_map : &tp.v_map;
       const CUtensorMap* rows_map = is_k ? &tp.k_rows_map : &tp.v_rows_map;
-      const int64_t s0 = is_k ? p.k_s0 : p.v_s0;
-      const int s1 = (int)(is_k ? p.k_s1 : p.v_s1);
+      const int64_t s0 = is_k ? p.k_s0 : p.v_s0, s1 = is_k ? p.k_s1 : p.v_s1;
       const T* base0 = reinterpret_cast<const T*>(is_k ? p.k : p.v);
       const uint32_t full0 = bar(is_k ? C::K_FULL : C::V_FULL), empty0 = bar(is_k ? C::K_EMPTY : C::V_EMPTY);
       const uint32_t ring = sm + (is_k ? C::K_OFF : C::V_OFF);
@@ -717,7 +716,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
               const int blk = i % NB, r = i / NB * 4;
               int r0, r1, r2, r3;
               asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(ids + r * 4));
-              tma_gather4(buf + blk * C::KV_BLOCK + r * 128, rows_map, kvh * s1 + 64 * blk, r0, r1, r2, r3, full);
+              tma_gather4(buf + blk * C::KV_BLOCK + r * 128, rows_map, kvh * (int)s1 + 64 * blk, r0, r1, r2, r3, full);
             }
           }
           // what is left, 16 bytes at a time; of V zeros up to the next 16 rows
