@@ -389,6 +389,7 @@ void fill_extend(PyObject* const* x, ft_extend_args& a, at::Tensor& hold) {
   a.dtype = dtype_code(q.scalar_type());
   if (k.sizes() != v.sizes()) refuse("%s", "k_buffer and v_buffer differ in shape");
   if (o.sizes() != q.sizes()) refuse("%s", "o must have the shape of q");
+  if (o.numel() > 0 && o.data_ptr() == q.data_ptr()) refuse("%s", "o must not be q: rows of q are read after rows of o are written");
   if (q.size(2) != k.size(2)) refuse("%s", "head_dim of q and k_buffer differ");
   const at::Tensor& entries = on_device_of("kv_entries", table("kv_entries", x[4]), q);
   const at::Tensor& plan = on_device_of("the plan", table("the plan", x[5]), q);
@@ -420,6 +421,21 @@ void fill_extend(PyObject* const* x, ft_extend_args& a, at::Tensor& hold) {
     hold = at::empty({lse * (a.head_dim + 1)}, q.options().dtype(at::kFloat));
     a.mid_o = static_cast<float*>(hold.data_ptr());
     a.mid_lse = a.mid_o + lse * a.head_dim;
+  }
+}
+
+// extend_args(...as extend()) -> bytes of the filled ft_extend_args; its scratch is gone when the call returns
+PyObject* py_extend_args(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  if (n != 11) return PyErr_Format(PyExc_TypeError, "extend_args() takes 11 arguments");
+  try {
+    ft_extend_args a;
+    at::Tensor hold;
+    fill_extend(x, a, hold);
+    return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(&a), sizeof(a));
+  } catch (const Refused&) {
+    return nullptr;
+  } catch (const std::exception& e) {
+    return PyErr_Format(PyExc_RuntimeError, "%s", e.what());
   }
 }
 
@@ -455,6 +471,7 @@ PyMethodDef methods[] = {
     {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_call)), METH_FASTCALL, "check, fill and launch"},
     {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_append)), METH_FASTCALL, "check, fill and launch ft_append"},
     {"extend", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_extend)), METH_FASTCALL, "check, fill and launch ft_extend"},
+    {"extend_args", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_extend_args)), METH_FASTCALL, "filled ft_extend_args as bytes"},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_bind)), METH_FASTCALL, "addresses of the C ABI"},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -158,16 +158,30 @@ def tree_prefixes(tree_info):
 
 def extend(q, k_buffer, v_buffer, o, kv_entries, plan, sm_scale, logit_cap=-1, o_lse=None, path="auto"):
     """Causal attention of a step's new tokens over the paged cache, which holds their prefixes and themselves (append
-    first).  ``q``, ``o`` ``[tokens, q heads, head_dim]``, the pool ``[rows, kv heads, head_dim]``, ``kv_entries`` the int32
+    first).  ``q``, ``o`` ``[tokens, q heads, head_dim]`` (which must not overlap), the pool ``[rows, kv heads, head_dim]``, ``kv_entries`` the int32
     table that the plan's ``kv_starts`` index (flat or ``[requests, positions]``).  ``logit_cap`` > 0: scores become
     ``logit_cap * tanh(score / logit_cap)``.  ``o_lse``: optional fp32 ``[tokens, q heads]``.  Rows of ``o`` behind the plan's
     tokens are left as they are.  Partial results, where the plan has them, live in memory that the call takes from torch's
     allocator on the current stream."""
+    rc = _lib.call_module().extend(*_extend_call(q, k_buffer, v_buffer, o, kv_entries, plan, sm_scale, logit_cap, o_lse, path))
+    if rc != 0:
+        _lib.check(rc)
+
+
+def _extend_call(q, k_buffer, v_buffer, o, kv_entries, plan, sm_scale, logit_cap, o_lse, path):
     if not isinstance(plan, ExtendPlan):
         raise ValueError("plan must come from fasttree_extend_preparation")
     code = _lib.EXTEND_PATHS.get(path)
     if code is None:
         raise ValueError(f"path must be one of {sorted(_lib.EXTEND_PATHS)}")
-    rc = _lib.call_module().extend(q, k_buffer, v_buffer, o, kv_entries, plan.table, plan._raw, sm_scale, logit_cap, o_lse, code)
-    if rc != 0:
-        _lib.check(rc)
+    return q, k_buffer, v_buffer, o, kv_entries, plan.table, plan._raw, sm_scale, logit_cap, o_lse, code
+
+
+def path_name(q, k_buffer, v_buffer, o, kv_entries, plan, sm_scale, logit_cap=-1, o_lse=None, path="auto"):
+    """Names of the kernels that :func:`extend` would launch, joined by '+'."""
+    call = _extend_call(q, k_buffer, v_buffer, o, kv_entries, plan, sm_scale, logit_cap, o_lse, path)
+    args = _lib.ExtendArgs.from_buffer_copy(_lib.call_module().extend_args(*call))
+    name = _lib.load().ft_extend_path_name(ctypes.byref(args))
+    if name is None:
+        _lib.check(-1)
+    return name.decode()
