@@ -22,8 +22,20 @@
 // rows see whole has none), keeps a running maximum that may lag by 2^8 before O is rescaled in
 // tensor memory, and writes P in the storage type; the row's sum is of the unrounded probabilities in fp32.  P takes the
 // place of S, except at head_dim 64, where the products have different shapes and their order is not the order of issue:
-// there P has columns of its own.  When a stream's scores are ready all its earlier products are done (tcgen05.commit covers
-// every MMA issued before it), so no wait is needed before O is rescaled with two streams; with one there is a barrier for it.
+// there P has columns of its own, and a stream's next scores are computed as soon as the ones before are in registers (2048 on
+// 2048 tokens, 32/4 heads of 64: 101 -> 94 us).  At head_dim 128 a stream's scores are ready only when its earlier products are
+// done (tcgen05.commit covers every MMA issued before it), so nothing is waited for before O is rescaled; at 64 and 256 there is
+// a barrier for that.
+//
+// What bounds it: at head_dim 128 the chain scores -> softmax -> product of a stream, which the other stream hides but for a
+// third (the tensor pipe is busy 60 to 65 % of the time): 4096 tokens behind 12288 cached ones, 64/8 heads, bf16 1476 us =
+// 1304 TFLOP/s, 0.78 of what a large library product reaches in a burst; 2048 on 2048, 32/4 heads 109 us = 950.  At 64 the
+// exponentials, 16 a clock and SM: 94 us = 550 TFLOP/s for the same.  At 256 the products, whose 64-column shapes read shared
+// memory more often than they multiply: 251 to 266 us = 770 to 820 TFLOP/s.  Few tokens: the K/V rows' way from memory, 4.0 to
+// 4.6 TB/s where each request has a cache of its own, and below about 30 us the chain of dependent reads at the start
+// (schedule, tile record, row ids, first tile) and the merge's launch.  Scattered pools: the TMA unit's row gathers, about 27 ns
+// for four rows of 128 bytes and SM (sixteen prompts 330 us, with consecutive rows 283); 16-byte copies beside or instead of
+// them were slower in every mixture (half of the rows 375).
 //
 // Rows of V that a query does not see are multiplied by P = 0, and 0 x Inf is NaN: a row that is not shown everything and did
 // not come out finite is computed again from its own tokens (extend_row).
@@ -62,12 +74,13 @@ struct ExtCfg {
   static constexpr int META_OFF = IDS_OFF + NSI * TILE * 4;
   static constexpr int BAR_OFF = META_OFF + NSI * 8;
   static constexpr int K_FULL = 0, K_EMPTY = K_FULL + NSK, V_FULL = K_EMPTY + NSK, V_EMPTY = V_FULL + NSV, S_FULL = V_EMPTY + NSV,
-                       P_HALF = S_FULL + 2, P_FULL = P_HALF + 2, O_FULL = P_FULL + 2, PV_DONE = O_FULL + 2, Q_FULL = PV_DONE + 2, Q_EMPTY = Q_FULL + 1,
+                       P_HALF = S_FULL + 2, P_FULL = P_HALF + 2, O_FULL = P_FULL + 2, PV_DONE = O_FULL + 2, S_READ = PV_DONE + 2, Q_FULL = S_READ + 2, Q_EMPTY = Q_FULL + 1,
                        IDS_FULL = Q_EMPTY + 1, IDS_EMPTY = IDS_FULL + NSI, NBARS = IDS_EMPTY + NSI;
   static constexpr int ABORT_OFF = BAR_OFF + NBARS * 8, TMEM_SLOT_OFF = ABORT_OFF + 4, SMEM_BYTES = TMEM_SLOT_OFF + 4;
   // tensor memory columns.  Two streams: S_w, then O_w, then (head_dim 64) P_w.  One: two S buffers, O.
   static constexpr int S_COL = 0, O_COL = 256, P_COL = D == 64 ? 384 : S_COL;
   static constexpr int S_STEP = NW == 2 ? 128 : 64, P_STEP = D == 64 ? 64 : S_STEP;
+  static constexpr bool EARLY = D == 64;            // scores of a stream's next tile as soon as those before are read: P is elsewhere
   static constexpr int PV_N = D == 128 ? 128 : 64;  // columns of O per product
   static constexpr int CPR = D / 8;                 // 16-byte chunks of a row
   static constexpr int REGS_SOFTMAX = 224, REGS_OTHER = 56, REGS_LAUNCH = 168;
@@ -142,7 +155,7 @@ __device__ __forceinline__ bool ext_wait(uint32_t bar, uint32_t parity, uint32_t
 //
 // Up to |x| = 1.25 by the minimax polynomial tanh(x) = x (q0 + q1 x^2 + ... + q6 x^12), fitted with the Remez exchange: off by
 // at most 2.9e-7.  Two tanh or one exponential more per score on the special-function unit, which the softmax already keeps busy,
-// cost more than eight packed FMAs for two scores (2048 on 2048 tokens, 32/4 heads of 128, capped: 221 us, so NNN; not capped 111).
+// cost more than eight packed FMAs for two scores (2048 on 2048 tokens, 32/4 heads of 128, capped: 221 us, so 167; not capped 109).
 // A warp that meets a larger |x| goes over to tanh(x) = 1 - 2 / (1 + e^(2 x)), one reciprocal for two scores.
 struct Capped {
   float a[7], c2, k2, u_most;
@@ -239,6 +252,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       mbar_init(bar(C::P_FULL + b), 128);
       mbar_init(bar(C::O_FULL + b), 1);
       mbar_init(bar(C::PV_DONE + b), 1);
+      mbar_init(bar(C::S_READ + b), 128);
     }
     mbar_init(bar(C::Q_FULL), 1);
     mbar_init(bar(C::Q_EMPTY), 1);
@@ -319,7 +333,18 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
           return;
         }
         tc_fence_after();
+        // P's columns, and O if it is rescaled: the product with V of the stream's tile before has to be done with them
+        auto wait_pv = [&]() {
+          const int before = tiles_done - 2, b = NW == 2 ? w : before & 1;
+          const uint32_t ph = NW == 2 ? (uint32_t)before & 1u : (uint32_t)(before >> 1) & 1u;
+          if (before >= 0 && !ext_wait<D>(bar(C::PV_DONE + b), ph, abort_flag)) give_up();
+          tc_fence_after();
+        };
         if (MASKED && !__any_sync(0xffffffffu, any)) {  // nothing in sight of the warp's rows
+          if constexpr (C::EARLY) {
+            mbar_arrive(bar(C::S_READ + buf));
+            wait_pv();
+          }
           if (warp_live) {
             float zero[32];
 #pragma unroll
@@ -348,6 +373,10 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
             }
           }
           if (steep) capped.exact(s);
+        }
+        if constexpr (C::EARLY) {
+          tc_fence_before();
+          mbar_arrive(bar(C::S_READ + buf));
         }
         if constexpr (MASKED) {
 #pragma unroll
@@ -389,15 +418,13 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
             sum2[i & 1] = __fadd2_rn(sum2[i & 1], x);
             wds[i] = pack2<T>(x.x, x.y);
           }
+          if (C::EARLY && h == 0) wait_pv();
           if constexpr (TILE == 128)
             tmem_st32(p_col + 32 * h, *reinterpret_cast<float(*)[32]>(&wds[0]));
           else
             tmem_st16(p_col + 16 * h, *reinterpret_cast<uint32_t(*)[16]>(&wds[0]));
           if (h == 0 && t > lo && __any_sync(0xffffffffu, grow)) {
-            if constexpr (NW == 1) {  // P.V of the tile before has to be done
-              if (!ext_wait<D>(bar(C::PV_DONE + (buf ^ 1)), (uint32_t)((tiles_done - 2) >> 1) & 1u, abort_flag)) give_up();
-              tc_fence_after();
-            }
+            if constexpr (NW == 1) wait_pv();
 #pragma unroll
             for (int cb = 0; cb < D / 32; ++cb) {
               float o[32];
@@ -414,7 +441,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
         l_run += (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
       };
       // Two loops, so that the one over tiles that every row sees whole has no masks in it: with one loop the scores do not all fit
-      // the registers (4096 tokens behind 12288, 64/8 heads: 1910 us, with two NNN).  Where the next tile's bits are is read a
+      // the registers (4096 tokens behind 12288, 64/8 heads: 1910 us, with two 1620).  Where the next tile's bits are is read a
       // tile ahead.
       auto mask_at = [&](int t) { return t < hi ? __ldg(mask_of + 8 * t) : -1; };
       int mask = mask_at(lo);
@@ -518,7 +545,8 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       // (Loops are kept short on purpose: the roles run at the same time from one instruction cache.)
       int k_stage = 0, v_stage = 0;
       uint32_t k_phase = 0, v_phase = 0, q_phase = 0, p_phases = 0;  // p_phases: a bit per P buffer
-      int s_count = 0;
+      int s_count = 0;        // score tiles issued (one stream)
+      uint32_t s_phases = 0;  // a bit per stream
       const int tasks_u = __shfl_sync(0xffffffffu, task_hi - task_lo, 0);
       for (int n = 0; n < tasks_u && !dead; ++n) {
         int t0, t1, step, len, lo0, hi0, lo1 = 0, hi1 = 0, tile1 = 0;
@@ -597,7 +625,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
                 }
               }
               if (half == 1) {
-                if (NW == 1) tc_commit(ubar(C::PV_DONE + buf));
+                if (NW == 1 || C::EARLY) tc_commit(ubar(C::PV_DONE + buf));
                 if (last) tc_commit(ubar(C::O_FULL + w));
               }
             }
@@ -625,7 +653,30 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
           }
           v_here = false;
         };
-        if constexpr (NW == 2) {
+        if constexpr (C::EARLY) {
+          // iteration t: the scores of tile t for both streams, then the products with V of tile t - step
+#pragma unroll 1
+          for (int t = t0; t < t1 + step && !dead; ++t) {
+            const int before = t - step;
+#pragma unroll 1
+            for (int w = 0; w < 2 && !dead; ++w) {
+              const int lo = w == 0 ? lo0 : lo1, hi = w == 0 ? hi0 : hi1;
+              if (t < lo || t >= hi || (step == 2 && ((t - lo) & 1) != 0)) continue;
+              wait(ubar(C::S_READ + w), ((s_phases >> w) & 1u) ^ 1u);
+              s_phases ^= 1u << w;
+              if (!dead) issue_qk(w, w == 0 ? 0 : tile1);
+            }
+            if (t < t1 && !dead) release_k();
+            if (t == t1 - 1 && !dead && issuer) tc_commit(ubar(C::Q_EMPTY));
+#pragma unroll 1
+            for (int w = 0; w < 2 && !dead; ++w) {
+              const int lo = w == 0 ? lo0 : lo1, hi = w == 0 ? hi0 : hi1;
+              if (before < lo || before >= hi || (step == 2 && ((before - lo) & 1) != 0)) continue;
+              issue_pv(w, w, before, before == lo, before + step >= hi);
+            }
+            if (before >= t0 && before < t1 && !dead) release_v();
+          }
+        } else if constexpr (NW == 2) {
           // iteration t: the products with V of tile t - step, then the scores of tile t, stream by stream
 #pragma unroll 1
           for (int t = t0; t < t1 + step && !dead; ++t) {
