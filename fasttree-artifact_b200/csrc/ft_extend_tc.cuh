@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(sm + C::TMEM_SLOT_OFF), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
-  // Each role passes the end of the set-up where it needs it: the loaders have their first row ids under way by then.
+  // the end of the set-up, which every role passes once, before it waits for or touches anything that was set up
   auto set_up = [&]() {
     tc_fence_before();
     asm volatile("bar.sync 0;\n" ::: "memory");
@@ -328,7 +328,8 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
         const uint32_t phase = NW == 2 ? (uint32_t)tiles_done & 1u : (uint32_t)(tiles_done >> 1) & 1u;
         ++tiles_done;
         const uint32_t s_col = t_lane + C::S_COL + buf * C::S_STEP, p_col = t_lane + C::P_COL + buf * C::P_STEP;
-        if (!ext_wait<D>(bar(C::S_FULL + buf), phase, abort_flag)) {
+        // (one answer for the warp: it goes on, or gives up, as a whole)
+        if (!__all_sync(0xffffffffu, ext_wait<D>(bar(C::S_FULL + buf), phase, abort_flag))) {
           give_up();
           return;
         }
@@ -337,7 +338,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
         auto wait_pv = [&]() {
           const int before = tiles_done - 2, b = NW == 2 ? w : before & 1;
           const uint32_t ph = NW == 2 ? (uint32_t)before & 1u : (uint32_t)(before >> 1) & 1u;
-          if (before >= 0 && !ext_wait<D>(bar(C::PV_DONE + b), ph, abort_flag)) give_up();
+          if (before >= 0 && !__all_sync(0xffffffffu, ext_wait<D>(bar(C::PV_DONE + b), ph, abort_flag))) give_up();
           tc_fence_after();
         };
         if (MASKED && !__any_sync(0xffffffffu, any)) {  // nothing in sight of the warp's rows
@@ -467,7 +468,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       }
       if (dead) break;
       // ---- the row's result: normalised, to o or to its partial row
-      if (!ext_wait<D>(bar(C::O_FULL + w), (uint32_t)items_done & 1u, abort_flag)) {
+      if (!__all_sync(0xffffffffu, ext_wait<D>(bar(C::O_FULL + w), (uint32_t)items_done & 1u, abort_flag))) {
         give_up();
         break;
       }
