@@ -641,17 +641,25 @@ int ft_extend_plan_build(const int64_t* seq_lens, const int64_t* extend_lens, co
   if (!(head_dim == 16 || head_dim == 32 || head_dim == 64 || head_dim == 128 || head_dim == 256)) return FT_ERR_UNSUPPORTED;
   int64_t total = 0, most = 0;
   for (int i = 0; i < batch; ++i) {
-    const int64_t cached = seq_lens[i] - extend_lens[i];
-    if (extend_lens[i] < 0 || cached < 0 || kv_starts[i] < 0 || q_starts[i] < 0 || shared_with_previous[i] < 0)
+    if (extend_lens[i] < 0 || seq_lens[i] < extend_lens[i] || kv_starts[i] < 0 || q_starts[i] < 0 || shared_with_previous[i] < 0)
       return FT_ERR_INVALID_ARGUMENT;
+    const int64_t cached = seq_lens[i] - extend_lens[i];
     if (shared_with_previous[i] > cached || (shared_with_previous[i] > 0 && (i == 0 || shared_with_previous[i] > seq_lens[i - 1] - extend_lens[i - 1])))
       return FT_ERR_INVALID_ARGUMENT;
-    if (seq_lens[i] > INT32_MAX / 2 || q_starts[i] + extend_lens[i] > INT32_MAX / 2) return FT_ERR_TOO_LARGE;
+    if (seq_lens[i] > INT32_MAX / 2 || q_starts[i] > INT32_MAX / 2 || q_starts[i] + extend_lens[i] > INT32_MAX / 2 || kv_starts[i] > INT64_MAX / 2)
+      return FT_ERR_TOO_LARGE;
     total += extend_lens[i];
     most = std::max(most, seq_lens[i]);
   }
   if (total > INT32_MAX / 64 || window > INT32_MAX) return FT_ERR_TOO_LARGE;
   try {
+    // a row of q is one request's: two writers of a row of o would race
+    std::vector<std::pair<int64_t, int64_t>> q_rows;
+    for (int i = 0; i < batch; ++i)
+      if (extend_lens[i] > 0) q_rows.push_back({q_starts[i], q_starts[i] + extend_lens[i]});
+    std::sort(q_rows.begin(), q_rows.end());
+    for (size_t i = 1; i < q_rows.size(); ++i)
+      if (q_rows[i].first < q_rows[i - 1].second) return FT_ERR_INVALID_ARGUMENT;
     Problem p;
     p.seq = seq_lens, p.ext = extend_lens, p.start = kv_starts, p.qstart = q_starts, p.shared = shared_with_previous;
     p.batch = batch;

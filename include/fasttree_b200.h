@@ -406,11 +406,12 @@ int ft_append_args_size(void);
 int ft_append(const ft_append_args* args);
 
 /* The schedule of one extend-attention step: which query rows run together, over which K/V, on which SM.  Pure host code,
- * like ft_plan.  `batch` requests; request i has seq_lens[i] tokens in the cache, of which the last extend_lens[i] are the
- * step's queries (rows q_starts[i] .. of q); its tokens' pool rows are kv_entries[kv_starts[i] ..].  Requests that share a
- * prefix stand next to one another: the first shared_with_previous[i] entries of request i are those of request i - 1
- * (0: nothing is known; at most the cached part seq_len - extend_len of either), and such a prefix is read once for all of
- * them.  window > 0: a query sees the newest `window` positions up to its own.  elem_bytes: 2 or 4. */
+ * like ft_plan.  `batch` requests; request i has seq_lens[i] tokens in the cache, of which the last extend_lens[i] are
+ * the step's queries (rows q_starts[i] .. of q, of no other request); its tokens' pool rows are
+ * kv_entries[kv_starts[i] ..].  Requests that share a prefix stand next to one another: the first
+ * shared_with_previous[i] entries of request i are those of request i - 1 (0: nothing is known; at most the cached
+ * part seq_len - extend_len of either), and such a prefix is read once for all of them.  window > 0: a query sees the
+ * newest `window` positions up to its own.  elem_bytes: 2 or 4. */
 typedef struct ft_extend_plan ft_extend_plan;
 
 typedef struct ft_extend_plan_info {

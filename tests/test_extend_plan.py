@@ -1,4 +1,5 @@
 """The schedule of extend attention, checked on the host: what every query token is shown, exactly once, and nothing else."""
+import ctypes
 import random
 
 import numpy as np
@@ -192,3 +193,28 @@ def test_refusals():
         extend.host_plan(**{**ok, "seq_lens": [2 ** 31, 6]})
     with pytest.raises(ValueError):
         extend.prepare(**ok, device="cpu")
+
+
+def build(seq, ext, kv, q, shared, batch=None):
+    """ft_extend_plan_build as a C program calls it: its status (a plan that it makes is freed)."""
+    i64 = ctypes.c_int64 * len(seq)
+    handle = ctypes.c_void_p()
+    clib = lib.load()
+    rc = clib.ft_extend_plan_build(i64(*seq), i64(*ext), i64(*kv), i64(*q), i64(*shared), len(seq), 8, 2, 128, 2, 0, 148,
+                                   ctypes.byref(handle))
+    assert (rc == 0) == bool(handle.value)
+    if handle.value:
+        clib.ft_extend_plan_free(handle)
+    return rc
+
+
+def test_refusals_at_the_c_entry():
+    top = 2 ** 63 - 1
+    assert build([5, 6], [1, 2], [0, 10], [0, 1], [0, 0]) == 0
+    assert build([5, 6], [1, 2], [0, 10], [7, 2], [0, 0]) == 0       # rows in any order, with gaps
+    assert build([5, 6, 4], [1, 2, 0], [0, 10, 20], [0, 1, 1], [0, 0, 0]) == 0  # a request without queries has no rows
+    assert build([5, 6], [1, 2], [0, 10], [1, 0], [0, 0]) != 0       # row 1 twice
+    assert build([5, 6], [1, 2], [0, 10], [0, 0], [0, 0]) != 0
+    assert build([-2 ** 63, 6], [1, 2], [0, 10], [0, 1], [0, 0]) != 0
+    assert build([5, 6], [1, 2], [top, 10], [0, 1], [0, 0]) != 0     # kv_start + seq_len would wrap
+    assert build([5, 6], [1, 2], [0, 10], [top, 1], [0, 0]) != 0
