@@ -248,6 +248,20 @@ int ft_extend(const ft_extend_args* a) {
   if (pl.num_items < 0 || pl.num_tokens < 0 || pl.num_merged < 0 || pl.partial_rows < 0)
     return fail(FT_ERR_INVALID_ARGUMENT, "the plan's counts are negative");
   if (pl.num_items == 0) return FT_OK;  // no query
+  const struct {
+    int64_t off, ints;
+  } parts[] = {{pl.items_off, (int64_t)pl.num_items * ft::EXT_ITEM_INTS}, {pl.tokens_off, 2LL * pl.num_tokens}, {pl.tiles_off, 8LL * pl.num_tiles},
+               {pl.extra_off, 0}, {pl.sms_off, 16LL * pl.num_sms}, {pl.sm_tasks_off, (int64_t)pl.num_items * pl.num_kv_heads},
+               {pl.merge_off, 4LL * pl.num_merged}, {pl.merge_rows_off, 0}};
+  for (const auto& part : parts)
+    if (part.off < 0 || part.off % 4 != 0 || part.ints < 0 || part.off + part.ints > pl.table_ints)
+      return fail(FT_ERR_INVALID_ARGUMENT, "the plan's parts do not lie in its table");
+  // the sizes that the kernels are compiled for, as ft_extend_plan_build chooses them
+  const int group = a->num_qo_heads / a->num_kv_heads;
+  const bool tensor_form = pl.elem_bytes == 2 && a->head_dim >= 64 && group <= 128;
+  if (a->num_qo_heads % a->num_kv_heads != 0 || pl.num_sms <= 0 || pl.tile_tokens != (tensor_form && a->head_dim <= 128 ? 128 : 64) ||
+      !(pl.rows_per_tile == (tensor_form ? 128 : 64) || (!tensor_form && pl.rows_per_tile == 16)))
+    return fail(FT_ERR_INVALID_ARGUMENT, "the plan's sizes are not a plan's");
   if (a->q == nullptr || a->k_buffer == nullptr || a->v_buffer == nullptr || a->o == nullptr || a->kv_entries == nullptr || a->plan_table == nullptr)
     return fail(FT_ERR_INVALID_ARGUMENT, "q / k_buffer / v_buffer / o / kv_entries / plan_table is NULL");
   if (!aligned16(a->plan_table)) return fail(FT_ERR_UNSUPPORTED, "plan_table must be 16-byte aligned");

@@ -218,3 +218,34 @@ def test_refusals_at_the_c_entry():
     assert build([-2 ** 63, 6], [1, 2], [0, 10], [0, 1], [0, 0]) != 0
     assert build([5, 6], [1, 2], [top, 10], [0, 1], [0, 0]) != 0     # kv_start + seq_len would wrap
     assert build([5, 6], [1, 2], [0, 10], [top, 1], [0, 0]) != 0
+
+
+def test_descriptions_that_are_no_plan_are_refused():
+    """ft_extend reads only the host's description before it launches: one whose parts do not lie in its table, or whose sizes
+    no kernel is compiled for, is an error of the call."""
+    info = extend.host_plan([9000, 60], [2, 7], [0, 9000], 8, 2, 128, torch.float16)[0]
+    clib = lib.load()
+
+    def call(**changes):
+        a = lib.ExtendArgs()
+        a.dtype, a.num_qo_heads, a.num_kv_heads, a.head_dim = 0, 8, 2, 128  # FT_F16
+        ctypes.memmove(ctypes.byref(a.plan), ctypes.byref(info), ctypes.sizeof(info))
+        for k, v in changes.items():
+            setattr(a.plan, k, v)
+        rc = clib.ft_extend(ctypes.byref(a))
+        return rc, clib.ft_last_error().decode()
+
+    assert info.num_merged > 0
+    assert "is NULL" in call()[1]  # the description itself passes
+    for part in ("items_off", "tokens_off", "tiles_off", "extra_off", "sms_off", "sm_tasks_off", "merge_off", "merge_rows_off"):
+        for value in (-4, info.table_ints + 4, getattr(info, part) + 1):
+            rc, text = call(**{part: value})
+            assert rc != 0 and "do not lie in its table" in text, part
+    for count in ("num_items", "num_tiles", "num_sms", "num_merged"):
+        rc, text = call(**{count: 2 ** 28})
+        assert rc != 0 and "do not lie in its table" in text, count
+    for sizes in (dict(num_sms=0), dict(tile_tokens=64), dict(tile_tokens=0), dict(rows_per_tile=64), dict(rows_per_tile=0)):
+        rc, text = call(**sizes)
+        assert rc != 0 and "sizes are not a plan's" in text, sizes
+    rc, text = call(num_items=-1)
+    assert rc != 0 and "negative" in text
