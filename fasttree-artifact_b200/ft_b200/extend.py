@@ -31,7 +31,9 @@ def append(q, k, v, k_buffer, v_buffer, slots, q_out=None, positions=None, cos_s
 
 class ExtendPlan:
     """Schedule of one step's extend attention, for all layers: a host description and one device table.  Read-only once
-    made: any number of calls, streams and captured graphs may use it at once."""
+    made: any number of calls, streams and captured graphs may use it at once.  Like every tensor of a call, its table has to
+    live until the work that reads it is done: keep the plan as long as a graph that was captured with it, and until other
+    streams than the one it was made on are through with it."""
 
     def __init__(self, info, table, seq_lens, extend_lens):
         self.info = info

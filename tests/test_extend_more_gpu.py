@@ -1,6 +1,8 @@
 """ft_extend where it can go wrong beside the ordinary shapes: which kernel runs, odd head groups, values that are no numbers,
 far rows of a large pool, empty calls, one plan for many layers, trees."""
 import math
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -208,3 +210,37 @@ def test_beside_decode_steps_on_one_stream():
     torch.cuda.synchronize()
     assert all(torch.equal(o[:n], first[:n]) for o in outs)
     assert all(torch.equal(x.float().cpu(), want) for x in decoded) and math.isfinite(want.sum().item())
+
+
+FIRST_CALLS = """
+import sys
+sys.path[:0] = {path!r}
+import torch
+import fasttree
+from test_extend_gpu import Step
+steps = [Step([5000, 90], [1, 9], [], 8, 2, d, t) for d, t in
+         ((64, torch.float16), (128, torch.bfloat16), (256, torch.float16), (32, torch.float16), (128, torch.float32))]
+outs, pools = [torch.zeros_like(s.gq) for s in steps], [(torch.zeros_like(s.gk), torch.zeros_like(s.gv)) for s in steps]
+slots = torch.arange(4, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    for s, o, (k, v) in zip(steps, outs, pools):
+        fasttree.fasttree_append(None, s.gk[:4], s.gv[:4], k, v, slots)
+        fasttree.fasttree_extend(s.gq, s.gk, s.gv, o, s.gt, s.plan, s.scale)
+graph.replay()
+torch.cuda.synchronize()
+for s, o, (k, v) in zip(steps, outs, pools):
+    want, _ = s.run()
+    n = sum(s.ext)
+    assert torch.equal(o[:n], want[:n]) and not (o[n:] != 0).any()
+    assert torch.equal(k[:4], s.gk[:4]) and torch.equal(v[:4], s.gv[:4]) and not (k[4:] != 0).any()
+print("first calls captured")
+"""
+
+
+def test_first_calls_of_a_process_in_a_captured_graph():
+    """Nothing that a kernel's first call sets up (its code, its shared memory limit, its descriptors) needs the stream."""
+    path = [p for p in sys.path if p]
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS.format(path=path)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "first calls captured" in r.stdout, r.stderr[-2000:]
