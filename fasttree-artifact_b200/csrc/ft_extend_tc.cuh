@@ -30,7 +30,8 @@
 // What bounds it: at head_dim 128 the chain scores -> softmax -> product of a stream, which the other stream hides but for a
 // third (the tensor pipe is busy 60 to 65 % of the time): 4096 tokens behind 12288 cached ones, 64/8 heads, bf16 1476 us =
 // 1304 TFLOP/s, 0.78 of what a large library product reaches in a burst; 2048 on 2048, 32/4 heads 109 us = 950.  At 64 the
-// exponentials, 16 a clock and SM: 94 us = 550 TFLOP/s for the same.  At 256 the products, whose 64-column shapes read shared
+// exponentials, 16 a clock and SM, at 63 % of the active cycles: 94 us = 550 TFLOP/s for the same (the two softmax warps of a
+// scheduler taking turns at them: 111).  At 256 the products, whose 64-column shapes read shared
 // memory more often than they multiply: 251 to 266 us = 770 to 820 TFLOP/s.  Few tokens: the K/V rows' way from memory, 4.0 to
 // 4.6 TB/s where each request has a cache of its own, and below about 30 us the chain of dependent reads at the start
 // (schedule, tile record, row ids, first tile) and the merge's launch.  Scattered pools: the TMA unit's row gathers, about 27 ns
