@@ -152,41 +152,37 @@ __device__ __forceinline__ bool ext_wait(uint32_t bar, uint32_t parity, uint32_t
   return false;
 }
 
-// Capped scores in powers of two, c2 tanh(x), x = S scale / cap, c2 = cap log2(e).
+// Capped scores: tanh(x), x = S scale / cap, which the softmax multiplies by cap log2(e).
 //
-// Up to |x| = 1.25 by the minimax polynomial tanh(x) = x (q0 + q1 x^2 + ... + q6 x^12), fitted with the Remez exchange: off by
-// at most 2.9e-7.  Two tanh or one exponential more per score on the special-function unit, which the softmax already keeps busy,
-// cost more than eight packed FMAs for two scores (2048 on 2048 tokens, 32/4 heads of 128, capped: 221 us, so 167; not capped 109).
+// Up to |x| = 1 by tanh(x) = x (1 + x^2 r(x^2)), r of six coefficients fitted with the Remez exchange for the smallest relative
+// error: 6e-8, about fp32's half step, so a cap far above the scores changes nothing near 0.  The coefficients are those of x and
+// stay normal numbers whatever scale and cap are: with the powers of scale / cap multiplied into them, which saves one
+// multiplication in nine, the thirteenth is 0 from about scale / cap = 8e-4 on (sm_scale 1/128, cap 30: scores off by 0.3).
+// Two tanh or one exponential more per score on the special-function unit, which the softmax already keeps busy, cost more than
+// nine packed FMAs for two scores.
 // A warp that meets a larger |x| goes over to tanh(x) = 1 - 2 / (1 + e^(2 x)), one reciprocal for two scores.
 struct Capped {
-  float a[7], c2, k2, u_most;
+  static constexpr float LOG2E = 1.4426950408889634f, MOST = 1.f;
+  float k, c2;
+  // (limits that keep k and c2 finite; a cap of 1e36 hides nothing from fp32 that 1e38 would show)
   __device__ __forceinline__ Capped(float scale, float cap) {
-    constexpr float LOG2E = 1.4426950408889634f;
-    constexpr float q[7] = {0.9999964833259583f,    -0.33324214816093445f,  0.1326480358839035f,   -0.051644690334796906f,
-                            0.017636235803365707f, -0.004325489979237318f, 0.0005254826974123716f};
-    const float k = scale / cap;
+    cap = fminf(cap, 1e36f);
+    k = fminf(scale / cap, 1e36f);
     c2 = cap * LOG2E;
-    k2 = 2.f * LOG2E * k;
-    u_most = (1.25f / k) * (1.25f / k);
-    float f = c2 * k;
-#pragma unroll
-    for (int i = 0; i < 7; ++i) {
-      a[i] = f * q[i];
-      f *= k * k;
-    }
   }
-  // in place; returns the largest square of a score
+  // in place; returns the largest x^2
   template <int N>
   __device__ __forceinline__ float polynomial(float (&s)[N]) const {
+    constexpr float q[6] = {-0.33332987f, 0.13326409f, -0.053498708f, 0.02035976f, -0.0062593398f, 0.0010582648f};
     float most[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
-      const float2 x = make_float2(s[2 * i], s[2 * i + 1]), u = __fmul2_rn(x, x);
+      const float2 x = __fmul2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(k, k)), u = __fmul2_rn(x, x);
       asm("max.f32 %0, %0, %1, %2;" : "+f"(most[i & 1]) : "f"(u.x), "f"(u.y));
-      float2 y = make_float2(a[6], a[6]);
+      float2 y = make_float2(q[5], q[5]);
 #pragma unroll
-      for (int k = 5; k >= 0; --k) y = __ffma2_rn(y, u, make_float2(a[k], a[k]));
-      y = __fmul2_rn(y, x);
+      for (int j = 4; j >= 0; --j) y = __ffma2_rn(y, u, make_float2(q[j], q[j]));
+      y = __fmul2_rn(__ffma2_rn(y, u, make_float2(1.f, 1.f)), x);
       s[2 * i] = y.x;
       s[2 * i + 1] = y.y;
     }
@@ -194,7 +190,8 @@ struct Capped {
   }
   template <int N>
   __device__ __forceinline__ void exact(float (&s)[N]) const {
-    const float2 one = make_float2(1.f, 1.f), n2 = make_float2(-2.f * c2, -2.f * c2), p2 = make_float2(c2, c2);
+    const float k2 = 2.f * LOG2E * k;
+    const float2 one = make_float2(1.f, 1.f), n2 = make_float2(-2.f, -2.f);
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
       // (2^60 and above is as good as infinite: 1 + 2^60 squared still is a number)
@@ -204,7 +201,7 @@ struct Capped {
       y = __fadd2_rn(make_float2(fast_exp2(y.x), fast_exp2(y.y)), one);
       float r;
       asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y.x * y.y));
-      y = __ffma2_rn(__fmul2_rn(make_float2(r, r), make_float2(y.y, y.x)), n2, p2);
+      y = __ffma2_rn(__fmul2_rn(make_float2(r, r), make_float2(y.y, y.x)), n2, one);
       s[2 * i] = y.x;
       s[2 * i + 1] = y.y;
     }
@@ -297,9 +294,9 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
     const uint32_t o_col = t_lane + C::O_COL + w * D;
     const float scale = p.sm_scale == 0.f ? 1.17549435e-38f : fabsf(p.sm_scale);
     constexpr float LOG2E = 1.4426950408889634f;
-    // scores in powers of two: S x scale2, or what Capped makes of S
-    const float scale2 = CAP ? 1.f : scale * LOG2E;
     const Capped capped = CAP ? Capped(scale, p.logit_cap) : Capped(0.f, 1.f);
+    // scores in powers of two: scale2 x S, or x what Capped makes of S
+    const float scale2 = CAP ? capped.c2 : scale * LOG2E;
     bool steep = false;  // capped scores: this warp has met one that the polynomial is not for
     int tiles_done = 0, items_done = 0;
     for (int n = task_lo; n < task_hi && !dead; ++n) {
@@ -367,7 +364,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
         if constexpr (CAP) {
           if (!steep) {
             const float most = capped.polynomial(s);
-            steep = __any_sync(0xffffffffu, row < rows && most > capped.u_most);
+            steep = __any_sync(0xffffffffu, row < rows && most > Capped::MOST * Capped::MOST);
             if (steep) {
 #pragma unroll
               for (int c = 0; c < TILE / 32; ++c) tmem_ld32_nowait(s_col + 32 * c, *reinterpret_cast<float(*)[32]>(&s[32 * c]));
@@ -393,7 +390,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
 #pragma unroll
           for (int k = 0; k < 4; ++k) asm("max.f32 %0, %0, %1, %2;" : "+f"(mx4[k]) : "f"(s[c + 2 * k]), "f"(s[c + 2 * k + 1]));
         float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-        if constexpr (!CAP) mx *= scale2;
+        mx *= scale2;
         float corr = 1.f;
         bool grow = false;
         if (mx > m_used + 8.f || m_used == -INFINITY) {  // the offset may lag the true maximum by up to 2^8
