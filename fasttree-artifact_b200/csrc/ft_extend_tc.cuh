@@ -16,7 +16,9 @@
 //
 // A K/V tile whose rows are consecutive in the pool is one TMA box per 64 columns; any other is gathered four rows at a
 // time through the TMA unit, its last rows with 16-byte copies.  Rows of V behind the last token are zeroed up to the next
-// 16, where the product ends; rows of K are not: their scores are masked.
+// 16, where the product ends; rows of K are not: their scores are masked.  Row ids outside the pool become zeros, which would count
+// as keys of score 0: the K loader notes the task, and its rows are computed again one by one (extend_row), which leaves such ids
+// out.  That is slow, and the call is flagged; a check of every tile instead costs all calls 1 to 8 %.
 //
 // Softmax: a thread reads its row of S, masks what the row does not see (bits from the plan; a tile that all of the query tile's
 // rows see whole has none), keeps a running maximum that may lag by 2^8 before O is rescaled in
@@ -71,9 +73,10 @@ struct ExtCfg {
   static constexpr int NSK = D == 64 ? 5 : D == 128 ? 2 : 3, NSV = D == 64 ? 5 : D == 128 ? 3 : 2;
   static constexpr int Q_OFF = 0, K_OFF = NW * Q_BYTES, V_OFF = K_OFF + NSK * KV_BYTES;
   static constexpr int NSI = 4;                           // tiles whose row ids are known or under way
-  static constexpr int IDS_OFF = V_OFF + NSV * KV_BYTES;  // NSI x {TILE row ids}, then NSI x {tokens, KV head}
+  static constexpr int IDS_OFF = V_OFF + NSV * KV_BYTES;  // NSI x {TILE row ids}, then NSI x {tokens, KV head, task, 0}
   static constexpr int META_OFF = IDS_OFF + NSI * TILE * 4;
-  static constexpr int BAR_OFF = META_OFF + NSI * 8;
+  static constexpr int BAD_OFF = META_OFF + NSI * 16;     // first and last task with a row id outside the pool
+  static constexpr int BAR_OFF = BAD_OFF + 8;
   static constexpr int K_FULL = 0, K_EMPTY = K_FULL + NSK, V_FULL = K_EMPTY + NSK, V_EMPTY = V_FULL + NSV, S_FULL = V_EMPTY + NSV,
                        P_HALF = S_FULL + 2, P_FULL = P_HALF + 2, O_FULL = P_FULL + 2, PV_DONE = O_FULL + 2, S_READ = PV_DONE + 2, Q_FULL = S_READ + 2, Q_EMPTY = Q_FULL + 1,
                        IDS_FULL = Q_EMPTY + 1, IDS_EMPTY = IDS_FULL + NSI, NBARS = IDS_EMPTY + NSI;
@@ -108,6 +111,12 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ int lds_int(uint32_t addr) {
   int x;
   asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(x) : "r"(addr) : "memory");
+  return x;
+}
+
+__device__ __forceinline__ int2 lds_int2(uint32_t addr) {
+  int2 x;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];\n" : "=r"(x.x), "=r"(x.y) : "r"(addr) : "memory");
   return x;
 }
 
@@ -256,6 +265,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       mbar_init(bar(C::IDS_FULL + b), 33);  // the copies of 32 lanes, and what lane 0 writes beside them
       mbar_init(bar(C::IDS_EMPTY + b), 2);  // both loaders
     }
+    asm volatile("st.shared.v2.b32 [%0], {%1, %2};\n" ::"r"(sm + C::BAD_OFF), "r"(0x7fffffff), "r"(-1) : "memory");
     set_abort(0);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -516,7 +526,9 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       }
       if (store)
         extend_store_lse(p, part, tk.x, head, l_run == 0.f ? -INFINITY : (m_used + log2f(l_run)) * 0.6931471805599453f);
-      const bool spoiled = store && hidden && !(finite.x + finite.y == 0.f);
+      // (noted by the K loader before the tile was handed over; the tasks between the first and the last are taken with them)
+      const int2 bad = lds_int2(sm + C::BAD_OFF);
+      const bool spoiled = store && ((n >= bad.x && n <= bad.y) || (hidden && !(finite.x + finite.y == 0.f)));
       for (uint32_t todo = __ballot_sync(0xffffffffu, spoiled); todo != 0; todo &= todo - 1) {
         const int r = (row & ~31) + __ffs(todo) - 1;
         __syncwarp();
@@ -728,8 +740,9 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
           break;
         }
         const uint32_t ids = sm + C::IDS_OFF + slot * (TILE * 4);
-        int valid, kvh, id[TILE / 32];
-        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];\n" : "=r"(valid), "=r"(kvh) : "r"(sm + C::META_OFF + slot * 8) : "memory");
+        int id[TILE / 32];
+        const int2 meta = lds_int2(sm + C::META_OFF + slot * 16);
+        const int valid = meta.x, kvh = meta.y;
         if (valid == 0) break;  // the end
         const int first = __shfl_sync(0xffffffffu, lds_int(ids), 0);
         bool dense = true, in_pool = true;
@@ -777,7 +790,14 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
             const bool ok = r < valid && (uint32_t)row_id < row_lim;
             cp_async16_zfill(buf + (uint32_t)((c16 >> 3) * C::KV_BLOCK) + tc_swz(r, c16 & 7, 0), base + (int64_t)(ok ? row_id : 0) * s0 + c16 * 8, ok);
           }
-          if (!in_pool && lane == 0) flag_error(FT_DEV_BAD_KV_INDEX);
+          if (!in_pool && lane == 0) {
+            if (is_k) {
+              const int task = lds_int(sm + C::META_OFF + slot * 16 + 8), before = lds_int(sm + C::BAD_OFF);
+              asm volatile("st.shared.v2.b32 [%0], {%1, %2};\n" ::"r"(sm + C::BAD_OFF), "r"(min(task, before)), "r"(task) : "memory");
+              __threadfence_block();
+            }
+            flag_error(FT_DEV_BAD_KV_INDEX);
+          }
           mbar_arrive_on_cp_async(full);
           __syncwarp();
         }
@@ -799,7 +819,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       // this warp may have to wait until the task before is through with its own.
       int slot = 0, items = 0;
       uint32_t ids_phase = 1;
-      auto put_ids = [&](const int4 rec, int kvh) {  // rec.z 0: the end
+      auto put_ids = [&](const int4 rec, int kvh, int task) {  // rec.z 0: the end
         if (!__all_sync(0xffffffffu, ext_wait<D>(bar(C::IDS_EMPTY + slot), ids_phase, abort_flag))) {
           give_up();
           return;
@@ -809,7 +829,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
         for (int h = 0; h < TILE / 32; ++h)
           if (lane + 32 * h < rec.z) cp_async4(ids + (lane + 32 * h) * 4, p.kv_entries + extend_entry(p, rec, lane + 32 * h));
         if (lane == 0) {
-          asm volatile("st.shared.v2.b32 [%0], {%1, %2};\n" ::"r"(sm + C::META_OFF + slot * 8), "r"(rec.z), "r"(kvh) : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %3};\n" ::"r"(sm + C::META_OFF + slot * 16), "r"(rec.z), "r"(kvh), "r"(task) : "memory");
           mbar_arrive(bar(C::IDS_FULL + slot));
         }
         mbar_arrive_on_cp_async(bar(C::IDS_FULL + slot));
@@ -840,7 +860,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
 #pragma unroll 1
           for (; t < end && !dead; ++t) {
             const int4 next = t + 1 < t1 ? __ldg(reinterpret_cast<const int4*>(p.tiles) + 2 * ((int64_t)tile0 + t + 1)) : rec;
-            put_ids(rec, kvh);
+            put_ids(rec, kvh, n);
             rec = next;
           }
         };
@@ -892,7 +912,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
         }
         put_until(t1);
       }
-      if (!dead) put_ids(make_int4(0, 0, 0, -1), 0);
+      if (!dead) put_ids(make_int4(0, 0, 0, -1), 0, 0);
       cp_async_wait<0>();
     }
   }
