@@ -77,9 +77,11 @@ __device__ __forceinline__ int64_t extend_entry(const ExtendParams& p, const int
 }
 
 // Query row (token `tok` of the stream, query head `head`) over the stream's K/V tiles lo, lo + step, ..., by one warp: lanes
-// span the head dimension, four tokens in flight, online softmax with warp-shuffle sums.
+// span the head dimension, four tokens in flight, online softmax with warp-shuffle sums.  steps: a counter in shared memory that
+// goes up with every tile, for those who wait for this warp (0: none does).
 template <typename T>
-__device__ __noinline__ void extend_row(const ExtendParams& p, const int32_t* item, const ExtendStream st, const int tok, const int head) {
+__device__ __noinline__ void extend_row(const ExtendParams& p, const int32_t* item, const ExtendStream st, const int tok, const int head,
+                                        const uint32_t steps = 0) {
   constexpr int MAXJ = 8, TB = 4;  // 8 x 32 lanes = head_dim up to 256
   const int lane = threadIdx.x & 31, D = p.head_dim, kvh = head / p.group;
   const int step = item[2], tile0 = item[5], words = p.tile / 32;
@@ -105,6 +107,7 @@ __device__ __noinline__ void extend_row(const ExtendParams& p, const int32_t* it
     const int32_t* tile = p.tiles + 8 * ((int64_t)tile0 + t);
     const int4 rec = __ldg(reinterpret_cast<const int4*>(tile));
     const int bits_at = __ldg(tile + 4 + st.block_tile);
+    if (steps != 0 && lane == 0) asm volatile("red.shared.add.u32 [%0], 1;\n" ::"r"(steps) : "memory");
     for (int k = 0; k < words; ++k) {
       uint32_t todo = bits_at < 0 ? 0xffffffffu : (uint32_t)__ldg(p.extra + bits_at + (st.first + tok) * words + k);
       while (todo != 0) {

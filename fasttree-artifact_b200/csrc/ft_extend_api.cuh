@@ -184,9 +184,76 @@ int launch_extend(const ft::ExtendParams& p, const ft_extend_args* a, bool tenso
   return FT_OK;
 }
 
+// Two warps.  The first waits as the roles of extend_tc_kernel do: (1) for a barrier that nothing arrives at; (2) for the same with the
+// abort flag raised, with probes for seconds; (3) as a whole warp for a completed barrier, with no probe
+// in half of its lanes; (4) for a barrier that the second warp arrives at after `limit` probes and more, counting steps until
+// then; (5) for one that it does not arrive at while it takes no step.  No copy, MMA or tensor memory is involved.
+__global__ void extend_wait_selftest_kernel(int limit, int* result) {
+  __shared__ __align__(8) unsigned long long barrier_word[3];
+  __shared__ __align__(8) int words[2];
+  const uint32_t never = ft::smem_u32(barrier_word), done = never + 8, late = never + 16, flag = ft::smem_u32(words);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 3; ++i) ft::mbar_init(never + 8 * i, 1);
+    words[0] = words[1] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    ft::mbar_arrive(done);
+  }
+  __syncthreads();
+  bool plain = false, aborted = false, split = false;
+  if (warp == 0) plain = __any_sync(0xffffffffu, ft::ext_wait(never, 0, flag, limit));
+  __syncthreads();
+  if (threadIdx.x == 0) words[0] = 1;
+  __syncthreads();
+  if (warp == 0) aborted = __any_sync(0xffffffffu, ft::ext_wait(never, 0, flag, 1 << 20));
+  __syncthreads();
+  if (threadIdx.x == 0) words[0] = 0;
+  __syncthreads();
+  if (warp == 0) split = __all_sync(0xffffffffu, ft::ext_wait(done, 0, flag, lane < 16 ? 0 : limit));
+  __syncthreads();
+  bool patient = true;
+  if (warp == 0) {
+    patient = __all_sync(0xffffffffu, ft::ext_wait(late, 0, flag, limit));
+  } else if (lane == 0) {
+    // as long as four waits that run out: each probe of a barrier that nothing arrives at takes the time that theirs take
+    for (int i = 0; i < 32; ++i) {
+      for (int n = 0; n < (limit + 7) / 8; ++n) {
+        if (ft::ext_wait(never, 0, flag, 1)) break;
+      }
+      asm volatile("red.shared.add.u32 [%0], 1;\n" ::"r"(flag + 4) : "memory");
+    }
+    ft::mbar_arrive(late);
+  }
+  __syncwarp();
+  __syncthreads();
+  bool last = false;
+  if (warp == 0) last = __any_sync(0xffffffffu, ft::ext_wait(late, 1, flag, limit));
+  if (threadIdx.x == 0) {
+    ft::flag_error(FT_DEV_WAIT_TIMEOUT);
+    result[0] = (plain ? 1 : 0) + (aborted ? 2 : 0) + (split ? 4 : 0) + (patient ? 0 : 8) + (last ? 16 : 0);
+    result[1] = ft::EXT_WAIT_LIMIT;
+  }
+}
+
 }  // namespace
 
 extern "C" {
+
+int ft_selftest_extend_wait(int limit, int* result_host, void* stream) {
+  if (result_host == nullptr) return fail(FT_ERR_INVALID_ARGUMENT, "result_host is NULL");
+  if (limit < 64 || limit > (1 << 16)) return fail(FT_ERR_INVALID_ARGUMENT, "limit must be in [64, 2^16] probes");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int* dev = nullptr;
+  FT_CUDA_OK(cudaMalloc(&dev, 2 * sizeof(int)));
+  extend_wait_selftest_kernel<<<1, 64, 0, st>>>(limit, dev);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) e = cudaMemcpyAsync(result_host, dev, 2 * sizeof(int), cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  cudaFree(dev);
+  if (e != cudaSuccess) return fail(FT_ERR_CUDA, "extend wait self-test failed: %s", cudaGetErrorString(e));
+  count_launch();
+  return FT_OK;
+}
 
 int ft_append_args_size(void) { return static_cast<int>(sizeof(ft_append_args)); }
 int ft_extend_args_size(void) { return static_cast<int>(sizeof(ft_extend_args)); }

@@ -27,7 +27,7 @@ EXPORTS = ["ft_version", "ft_decode_args_size", "ft_last_error", "ft_decode", "f
            "ft_plan_copy_aux_segments",
            "ft_plan_free",
            "ft_append_args_size", "ft_append", "ft_extend_plan_build", "ft_extend_plan_get_info", "ft_extend_plan_copy",
-           "ft_extend_plan_free", "ft_extend_args_size", "ft_extend", "ft_extend_path_name"]
+           "ft_extend_plan_free", "ft_extend_args_size", "ft_extend", "ft_extend_path_name", "ft_selftest_extend_wait"]
 
 EXTEND_PATHS = {"auto": 0, "generic": 1, "tcgen05": 2}
 
@@ -172,6 +172,8 @@ def load():
         lib.ft_decode_host_io.restype = ctypes.c_int
         lib.ft_selftest_bounded_wait.argtypes = [ctypes.c_int, ctypes.POINTER(ctypes.c_int), ctypes.c_void_p]
         lib.ft_selftest_bounded_wait.restype = ctypes.c_int
+        lib.ft_selftest_extend_wait.argtypes = [ctypes.c_int, ctypes.POINTER(ctypes.c_int), ctypes.c_void_p]
+        lib.ft_selftest_extend_wait.restype = ctypes.c_int
         lib.ft_bump_kv_lens.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p]
         lib.ft_bump_kv_lens.restype = ctypes.c_int
         vp, i32, i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
