@@ -23,6 +23,47 @@ bool vector_rows(const void* p, int64_t s0, int64_t s1, int elems, int size) {
   return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(elems * size - 1)) == 0 && s0 % elems == 0 && s1 % elems == 0;
 }
 
+// A [rows, heads, head_dim] tensor's place in memory, strides in bytes; an axis of one entry has stride 0.
+struct Place {
+  int64_t at, n[2], s[2], inner;
+  Place(const void* p, int64_t rows, int heads, int d, int64_t s0, int64_t s1, int size)
+      : at((int64_t) reinterpret_cast<uintptr_t>(p)), n{rows, heads}, s{rows > 1 ? s0 * size : 0, heads > 1 ? s1 * size : 0}, inner((int64_t)d * size) {}
+  bool operator==(const Place& b) const {
+    return at == b.at && n[0] == b.n[0] && n[1] == b.n[1] && s[0] == b.s[0] && s[1] == b.s[1] && inner == b.inner;
+  }
+  int64_t edge(bool high) const {  // lowest address, or one past the highest
+    int64_t x = at + (high ? inner : 0);
+    for (int i = 0; i < 2; ++i) {
+      const int64_t far = (n[i] - 1) * s[i];
+      if ((far > 0) == high) x += far;
+    }
+    return x;
+  }
+  // bytes from the tensor's start that it touches in each period, or -1: its strides are not of that period
+  int64_t in_period(int64_t period) const {
+    int64_t x = inner;
+    for (int i = 0; i < 2; ++i) {
+      if (s[i] < 0) return -1;
+      if (s[i] % period != 0) x += (n[i] - 1) * s[i];
+    }
+    return x <= period ? x : -1;
+  }
+};
+
+// May two tensors share a byte?  No, if their address ranges are apart, or if they touch different bytes of a period that both are
+// laid out in (columns of one buffer, heads in turn).  Layouts that this does not tell apart count as overlapping.
+bool may_overlap(const Place& a, const Place& b) {
+  if (a.n[0] <= 0 || a.n[1] <= 0 || b.n[0] <= 0 || b.n[1] <= 0) return false;
+  if (a.edge(true) <= b.edge(false) || b.edge(true) <= a.edge(false)) return false;
+  const int64_t periods[] = {a.s[0], a.s[1], b.s[0], b.s[1]};
+  for (const int64_t p : periods) {
+    if (p <= 0) continue;
+    const int64_t ea = a.in_period(p), eb = b.in_period(p), r = ((b.at - a.at) % p + p) % p;
+    if (ea >= 0 && eb >= 0 && r >= ea && r + eb <= p) return false;
+  }
+  return true;
+}
+
 template <typename T, int VEC, bool PAIRS>
 int launch_append(const ft::AppendParams& p, cudaStream_t st) {
   const int units = p.head_dim / (2 * VEC), heads = (p.q != nullptr ? p.q_heads : 0) + 2 * p.kv_heads;
@@ -286,6 +327,21 @@ int ft_append(const ft_append_args* a) {
   if (a->kv_rows <= 0) return fail(FT_ERR_INVALID_ARGUMENT, "kv_rows must be positive");
   if (a->rot_dim > 0 && (a->positions == nullptr || a->cos_sin == nullptr || a->cos_sin_rows <= 0))
     return fail(FT_ERR_INVALID_ARGUMENT, "a rotation needs positions and a table of cosines and sines");
+  const int size = a->dtype == FT_F32 ? 4 : 2;
+  if (a->q != nullptr) {
+    const Place out(a->q_out, a->tokens, a->num_qo_heads, a->head_dim, a->q_out_stride0, a->q_out_stride1, size),
+        q(a->q, a->tokens, a->num_qo_heads, a->head_dim, a->q_stride0, a->q_stride1, size);
+    const struct {
+      const char* name;
+      Place place;
+    } others[] = {{"k", Place(a->k, a->tokens, a->num_kv_heads, a->head_dim, a->k_stride0, a->k_stride1, size)},
+                  {"v", Place(a->v, a->tokens, a->num_kv_heads, a->head_dim, a->v_stride0, a->v_stride1, size)},
+                  {"k_buffer", Place(a->k_buffer, a->kv_rows, a->num_kv_heads, a->head_dim, a->k_buffer_stride0, a->k_buffer_stride1, size)},
+                  {"v_buffer", Place(a->v_buffer, a->kv_rows, a->num_kv_heads, a->head_dim, a->v_buffer_stride0, a->v_buffer_stride1, size)}};
+    if (!(out == q) && may_overlap(out, q)) return fail(FT_ERR_INVALID_ARGUMENT, "q_out overlaps q and is not q");
+    for (const auto& other : others)
+      if (may_overlap(out, other.place)) return fail(FT_ERR_INVALID_ARGUMENT, "q_out overlaps %s", other.name);
+  }
   p.q = a->q, p.k = a->k, p.v = a->v, p.q_out = a->q_out, p.k_buffer = a->k_buffer, p.v_buffer = a->v_buffer;
   p.slots = a->slots, p.positions = a->positions, p.cos_sin = a->cos_sin;
   p.q_s0 = a->q_stride0, p.q_s1 = a->q_stride1, p.k_s0 = a->k_stride0, p.k_s1 = a->k_stride1;
@@ -342,6 +398,14 @@ int ft_extend(const ft_extend_args* a) {
     return fail(FT_ERR_INVALID_ARGUMENT, "the plan has partial rows: mid_o (16-byte aligned) and mid_lse are needed");
   if ((int64_t)pl.num_items * a->num_kv_heads > 0x7fffffffLL || (int64_t)pl.num_merged * a->num_qo_heads > 0x7fffffffLL)
     return fail(FT_ERR_TOO_LARGE, "more tasks than one launch takes");
+  // (rows of q are read after rows of o are written)
+  const int size = pl.elem_bytes;
+  const Place out(a->o, pl.q_rows, a->num_qo_heads, a->head_dim, a->o_stride0, a->o_stride1, size);
+  if (may_overlap(out, Place(a->q, pl.q_rows, a->num_qo_heads, a->head_dim, a->q_stride0, a->q_stride1, size)))
+    return fail(FT_ERR_INVALID_ARGUMENT, "o overlaps q");
+  if (may_overlap(out, Place(a->k_buffer, a->kv_rows, a->num_kv_heads, a->head_dim, a->k_stride0, a->k_stride1, size)) ||
+      may_overlap(out, Place(a->v_buffer, a->kv_rows, a->num_kv_heads, a->head_dim, a->v_stride0, a->v_stride1, size)))
+    return fail(FT_ERR_INVALID_ARGUMENT, "o overlaps the pool");
   const char* obstacle = extend_tc_obstacle(a);
   if (a->path == FT_EXTEND_TCGEN05 && obstacle != nullptr) return fail(FT_ERR_UNSUPPORTED, "tcgen05 path: %s", obstacle);
   const bool tensor = a->path != FT_EXTEND_GENERIC && obstacle == nullptr;

@@ -19,11 +19,11 @@ def append(q, k, v, k_buffer, v_buffer, slots, q_out=None, positions=None, cos_s
     ``q`` ``[tokens, q heads, head_dim]`` (or None), ``k`` and ``v`` ``[tokens, kv heads, head_dim]``, the pool
     ``[rows, kv heads, head_dim]``; fp16, bf16 or fp32, any strides with a contiguous head_dim axis.  ``slots`` (int32 or
     int64): -1 is a padding token, which is not stored; no row twice.  The turned queries go to ``q_out``, which may be ``q``
-    (the default) but must not overlap it otherwise.  ``cos_sin`` (fp32 ``[positions, rot_dim]``): cosines of the rot_dim / 2
-    pairs, then their sines; elements from ``rot_dim`` on stay as they are.  ``positions``: ``[tokens]``, or ``[axes,
-    tokens]`` with ``sections``, the number of consecutive pairs that each axis turns.  Pairs are elements (i, i + rot_dim /
-    2), or (2 i, 2 i + 1) if ``interleaved``.  Without ``positions`` and ``cos_sin`` nothing is turned (``q``, if given, is
-    copied to ``q_out``)."""
+    (the default) but must not overlap it, ``k``, ``v`` or the pool otherwise.  ``cos_sin`` (fp32 ``[positions,
+    rot_dim]``): cosines of the rot_dim / 2 pairs, then their sines; elements from ``rot_dim`` on stay as they are.
+    ``positions``: ``[tokens]``, or ``[axes, tokens]`` with ``sections``, the number of consecutive pairs that each axis turns.
+    Pairs are elements (i, i + rot_dim / 2), or (2 i, 2 i + 1) if ``interleaved``.  Without ``positions`` and ``cos_sin``
+    nothing is turned (``q``, if given, is copied to ``q_out``)."""
     rc = _lib.call_module().append(q, k, v, k_buffer, v_buffer, slots, q_out, positions, cos_sin, sections, interleaved)
     if rc != 0:
         _lib.check(rc)
@@ -160,11 +160,11 @@ def tree_prefixes(tree_info):
 
 def extend(q, k_buffer, v_buffer, o, kv_entries, plan, sm_scale, logit_cap=-1, o_lse=None, path="auto"):
     """Causal attention of a step's new tokens over the paged cache, which holds their prefixes and themselves (append
-    first).  ``q``, ``o`` ``[tokens, q heads, head_dim]`` (which must not overlap), the pool ``[rows, kv heads, head_dim]``, ``kv_entries`` the int32
-    table that the plan's ``kv_starts`` index (flat or ``[requests, positions]``).  ``logit_cap`` > 0: scores become
-    ``logit_cap * tanh(score / logit_cap)``.  ``o_lse``: optional fp32 ``[tokens, q heads]``.  Rows of ``o`` behind the plan's
-    tokens are left as they are.  Partial results, where the plan has them, live in memory that the call takes from torch's
-    allocator on the current stream."""
+    first).  ``q``, ``o`` ``[tokens, q heads, head_dim]``, the pool ``[rows, kv heads, head_dim]`` (``o`` must overlap neither ``q``
+    nor the pool), ``kv_entries`` the int32 table that the plan's ``kv_starts`` index (flat or ``[requests, positions]``).
+    ``logit_cap`` > 0: scores become ``logit_cap * tanh(score / logit_cap)``.  ``o_lse``: optional fp32 ``[tokens, q heads]``.
+    Rows of ``o`` behind the plan's tokens are left as they are.  Partial results, where the plan has them, live in memory that
+    the call takes from torch's allocator on the current stream."""
     rc = _lib.call_module().extend(*_extend_call(q, k_buffer, v_buffer, o, kv_entries, plan, sm_scale, logit_cap, o_lse, path))
     if rc != 0:
         _lib.check(rc)

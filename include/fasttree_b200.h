@@ -369,7 +369,7 @@ typedef struct ft_append_args {
   const void* q;       /* [tokens, num_qo_heads, head_dim], or NULL: keys and values only */
   const void* k;       /* [tokens, num_kv_heads, head_dim]                                 */
   const void* v;       /* same shape as k                                                  */
-  void* q_out;         /* shape of q; may be q itself, must not overlap it otherwise       */
+  void* q_out;         /* shape of q; may be q itself, else must overlap none of the others */
   void* k_buffer;      /* [kv_rows, num_kv_heads, head_dim], written at the slots          */
   void* v_buffer;
   const void* slots;   /* [tokens] pool rows, int32 or int64; -1: a padding token, which is not stored.  A row named twice
@@ -448,7 +448,7 @@ typedef struct ft_extend_args {
   const void* q;         /* [q_rows, num_qo_heads, head_dim] */
   const void* k_buffer;  /* [kv_rows, num_kv_heads, head_dim] */
   const void* v_buffer;
-  void* o;               /* shape of q, written */
+  void* o;               /* shape of q, written; must overlap neither q nor the pool */
   float* o_lse;          /* optional [q_rows, num_qo_heads] log(sum)+max, or NULL */
   int32_t dtype;
   int32_t num_qo_heads, num_kv_heads, head_dim;
