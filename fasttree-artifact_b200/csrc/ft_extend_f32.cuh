@@ -10,6 +10,9 @@
 // Bound by shared-memory reads and FMAs in about equal parts: 512 tokens on 2048, 8/2 heads of 128, 180 us = 27 TFLOP/s (the
 // CUDA cores' nominal rate is 72), heads of 256 the same; steps of few tokens by the chain of reads at the start.  64 rows where
 // the step has them, 16 (a quarter of the work per tile, four times the tiles) where requests have few: the plan tries both.
+// With 16 rows a score is summed in blocks of 32 products, which makes its error two to three times smaller (single tokens, heads of
+// 256, scores capped at 50: outputs off by 9.1e-7, in blocks 3.3e-7) and takes no more time; with 64 rows the registers that it needs
+// cost 7 %, and the error of one chain is that of a matrix product.
 #pragma once
 
 #include "ft_extend.cuh"
@@ -114,8 +117,7 @@ __global__ void __launch_bounds__(256, ExtF32Cfg<D, RPT>::CTAS) extend_f32_kerne
         for (int i = 0; i < RPT; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
-#pragma unroll 4
-        for (int c = 0; c < CH; ++c) {
+        auto products = [&](int c, float (&to)[RPT][4]) {
           float4 q[RPT], k[4];
 #pragma unroll
           for (int i = 0; i < RPT; ++i) q[i] = at4(ext_chunk<CH>(ty * RPT + i, c));
@@ -125,7 +127,20 @@ __global__ void __launch_bounds__(256, ExtF32Cfg<D, RPT>::CTAS) extend_f32_kerne
           for (int i = 0; i < RPT; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              s[i][j] = fmaf(q[i].w, k[j].w, fmaf(q[i].z, k[j].z, fmaf(q[i].y, k[j].y, fmaf(q[i].x, k[j].x, s[i][j]))));
+              to[i][j] = fmaf(q[i].w, k[j].w, fmaf(q[i].z, k[j].z, fmaf(q[i].y, k[j].y, fmaf(q[i].x, k[j].x, to[i][j]))));
+        };
+        if constexpr (RPT == 1 && CH > 8) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < CH; c0 += 8) {
+            float part[RPT][4] = {};
+#pragma unroll 4
+            for (int c = c0; c < c0 + 8; ++c) products(c, part);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[0][j] += part[0][j];
+          }
+        } else {
+#pragma unroll 4
+          for (int c = 0; c < CH; ++c) products(c, s);
         }
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
