@@ -225,53 +225,49 @@ int launch_extend(const ft::ExtendParams& p, const ft_extend_args* a, bool tenso
   return FT_OK;
 }
 
-// Two warps.  The first waits as the roles of extend_tc_kernel do: (1) for a barrier that nothing arrives at; (2) for the same with the
-// abort flag raised, with probes for seconds; (3) as a whole warp for a completed barrier, with no probe
-// in half of its lanes; (4) for a barrier that the second warp arrives at after `limit` probes and more, counting steps until
-// then; (5) for one that it does not arrive at while it takes no step.  No copy, MMA or tensor memory is involved.
+// Two warps.  The first waits as the roles of extend_tc_kernel do: (1) for a barrier that nothing arrives at; (2) for the same where
+// another role has given up, with probes for seconds; (3) for a completed barrier, with no probe to spare; (4) for a barrier that
+// the second warp arrives at long after `limit` probes, counting steps until then; (5) for its next phase, which nothing completes, after the last
+// step.  No copy, MMA or tensor memory is involved.
 __global__ void extend_wait_selftest_kernel(int limit, int* result) {
   __shared__ __align__(8) unsigned long long barrier_word[3];
-  __shared__ __align__(8) int words[2];
-  const uint32_t never = ft::smem_u32(barrier_word), done = never + 8, late = never + 16, flag = ft::smem_u32(words);
+  __shared__ int state_word;
+  const uint32_t never = ft::smem_u32(barrier_word), done = never + 8, late = never + 16, state = ft::smem_u32(&state_word);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 3; ++i) ft::mbar_init(never + 8 * i, 1);
-    words[0] = words[1] = 0;
+    state_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     ft::mbar_arrive(done);
   }
   __syncthreads();
-  bool plain = false, aborted = false, split = false;
-  if (warp == 0) plain = __any_sync(0xffffffffu, ft::ext_wait(never, 0, flag, limit));
+  bool plain = false, gone = false, there = true, patient = true, last = false;
+  if (warp == 0) plain = ft::ext_wait(never, 0, state, limit);
   __syncthreads();
-  if (threadIdx.x == 0) words[0] = 1;
+  if (threadIdx.x == 0) state_word = INT_MIN;
   __syncthreads();
-  if (warp == 0) aborted = __any_sync(0xffffffffu, ft::ext_wait(never, 0, flag, 1 << 20));
+  if (warp == 0) gone = ft::ext_wait(never, 0, state, 1 << 20);
   __syncthreads();
-  if (threadIdx.x == 0) words[0] = 0;
+  if (threadIdx.x == 0) state_word = 0;
   __syncthreads();
-  if (warp == 0) split = __all_sync(0xffffffffu, ft::ext_wait(done, 0, flag, lane < 16 ? 0 : limit));
+  if (warp == 0) there = ft::ext_wait(done, 0, state, 0);
   __syncthreads();
-  bool patient = true;
   if (warp == 0) {
-    patient = __all_sync(0xffffffffu, ft::ext_wait(late, 0, flag, limit));
-  } else if (lane == 0) {
-    // as long as four waits that run out: each probe of a barrier that nothing arrives at takes the time that theirs take
-    for (int i = 0; i < 32; ++i) {
-      for (int n = 0; n < (limit + 7) / 8; ++n) {
-        if (ft::ext_wait(never, 0, flag, 1)) break;
-      }
-      asm volatile("red.shared.add.u32 [%0], 1;\n" ::"r"(flag + 4) : "memory");
+    patient = ft::ext_wait(late, 0, state, limit);
+  } else {
+    for (int i = 0; i < 32; ++i) {  // (8 `limit` probes, of the time that the first warp's take, and more)
+      for (int n = 0; n < (limit + 7) / 8; ++n)
+        if (ft::ext_wait(never, 0, state, 1)) break;
+      if (lane == 0) asm volatile("red.shared.add.u32 [%0], 1;\n" ::"r"(state) : "memory");
+      __syncwarp();
     }
-    ft::mbar_arrive(late);
+    if (lane == 0) ft::mbar_arrive(late);
   }
-  __syncwarp();
   __syncthreads();
-  bool last = false;
-  if (warp == 0) last = __any_sync(0xffffffffu, ft::ext_wait(late, 1, flag, limit));
+  if (warp == 0) last = ft::ext_wait(late, 1, state, limit);
   if (threadIdx.x == 0) {
     ft::flag_error(FT_DEV_WAIT_TIMEOUT);
-    result[0] = (plain ? 1 : 0) + (aborted ? 2 : 0) + (split ? 4 : 0) + (patient ? 0 : 8) + (last ? 16 : 0);
+    result[0] = (plain ? 1 : 0) + (gone ? 2 : 0) + (there ? 0 : 4) + (patient ? 0 : 8) + (last ? 16 : 0);
     result[1] = ft::EXT_WAIT_LIMIT;
   }
 }

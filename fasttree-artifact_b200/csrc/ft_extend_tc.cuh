@@ -12,7 +12,7 @@
 // K loads, V loads, and the tiles' row ids and Q loads.  All of them walk the same task list on their own; mbarriers (full / empty per buffer) are
 // the only hand-offs, and the counters behind their phases run on from task to task, so the next task's Q and K are loaded
 // and its first scores computed while the last rows of the task before are normalised and stored.  Every wait is bounded
-// and unwinds the CTA through an abort flag.
+// and unwinds the CTA through a state word.
 //
 // A K/V tile whose rows are consecutive in the pool is one TMA box per 64 columns; any other is gathered four rows at a
 // time through the TMA unit, its last rows with 16-byte copies.  Rows of V behind the last token are zeroed up to the next
@@ -80,8 +80,7 @@ struct ExtCfg {
   static constexpr int K_FULL = 0, K_EMPTY = K_FULL + NSK, V_FULL = K_EMPTY + NSK, V_EMPTY = V_FULL + NSV, S_FULL = V_EMPTY + NSV,
                        P_HALF = S_FULL + 2, P_FULL = P_HALF + 2, O_FULL = P_FULL + 2, PV_DONE = O_FULL + 2, S_READ = PV_DONE + 2, Q_FULL = S_READ + 2, Q_EMPTY = Q_FULL + 1,
                        IDS_FULL = Q_EMPTY + 1, IDS_EMPTY = IDS_FULL + NSI, NBARS = IDS_EMPTY + NSI;
-  static constexpr int ABORT_OFF = BAR_OFF + NBARS * 8;  // abort flag, then the CTA's steps: see ext_wait
-  static constexpr int TMEM_SLOT_OFF = ABORT_OFF + 8, SMEM_BYTES = TMEM_SLOT_OFF + 4;
+  static constexpr int STATE_OFF = BAR_OFF + NBARS * 8, TMEM_SLOT_OFF = STATE_OFF + 4, SMEM_BYTES = TMEM_SLOT_OFF + 4;
   // tensor memory columns.  Two streams: S_w, then O_w, then (head_dim 64) P_w.  One: two S buffers, O.
   static constexpr int S_COL = 0, O_COL = 256, P_COL = D == 64 ? 384 : S_COL;
   static constexpr int S_STEP = NW == 2 ? 128 : 64, P_STEP = D == 64 ? 64 : S_STEP;
@@ -140,38 +139,42 @@ __device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_
       : "memory");
 }
 
-__device__ __forceinline__ int ext_aborted(uint32_t flag) {
+// A CTA's state word: negative once a role has given up, else the count of its steps: K/V tiles whose row ids were sent for, and tiles
+// of rows that are computed again one by one.
+__device__ __forceinline__ int ext_state(uint32_t state) {
   int x;
-  asm volatile("ld.volatile.shared.b32 %0, [%1];\n" : "=r"(x) : "r"(flag) : "memory");
+  asm volatile("ld.volatile.shared.b32 %0, [%1];\n" : "=r"(x) : "r"(state) : "memory");
   return x;
+}
+__device__ __forceinline__ bool ext_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return __all_sync(0xffffffffu, ok != 0);
 }
 
 // Probes of mbarrier.try_wait before a wait gives up, about 4 us each where nothing comes: 0.26 s.
 constexpr int EXT_WAIT_LIMIT = 1 << 16;
 
-// Bounded wait for the phase of `bar` with the given parity: false after `limit` probes without a step of the CTA, or once another
-// role has raised the abort flag.  Steps are counted beside the flag: K/V tiles whose row ids were sent for, and tiles of rows that
-// are computed again one by one.  A stream may have nothing to do for many long tasks, and others wait for rows computed again,
-// so the time alone does not tell a long wait from one that nothing will end.
-__device__ __forceinline__ bool ext_wait(uint32_t bar, uint32_t parity, uint32_t abort_flag, int limit = EXT_WAIT_LIMIT) {
-  int seen = 0;
-  for (int it = 0; it < limit; ++it) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    if ((it & 15) == 15) {
-      int aborted, now;
-      asm volatile("ld.volatile.shared.v2.b32 {%0, %1}, [%2];\n" : "=r"(aborted), "=r"(now) : "r"(abort_flag) : "memory");
-      if (aborted != 0) return false;
-      if (now != seen) it = -1;
-      seen = now;
-    }
+// Bounded wait of a whole warp for the phase of `bar` with the given parity, with one answer for its lanes: false after `limit` probes
+// without a step of the CTA, or once another role has given up.  A stream may have nothing to do for many long tasks, and others wait
+// for rows computed again, so the time alone does not tell a long wait from one that nothing will end.
+// The form counts: the first probe stands apart because most waits end with it, and the warp's vote keeps its lanes together (2048 on
+// 2048 tokens at head_dim 256: 255 us; a loop that each lane left by itself, with a look at the state in every sixteenth probe, 283).
+__device__ __forceinline__ bool ext_wait(uint32_t bar, uint32_t parity, uint32_t state, int limit = EXT_WAIT_LIMIT) {
+  if (ext_try(bar, parity)) return true;
+  int seen = 0, left = limit;
+#pragma unroll 1
+  while (true) {
+    if (ext_try(bar, parity)) return true;
+    const int now = ext_state(state);
+    left = __any_sync(0xffffffffu, now != seen) ? limit : left - 1;
+    seen = now;
+    if (__any_sync(0xffffffffu, now < 0) || left <= 0) return false;
   }
-  return false;
 }
 
 // Capped scores: tanh(x), x = S scale / cap, which the softmax multiplies by cap log2(e).
@@ -242,9 +245,8 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
   extern __shared__ __align__(1024) uint8_t smem[];
   const ExtendParams& p = tp.p;
   const uint32_t sm = smem_u32(smem), bars = sm + C::BAR_OFF;
-  const uint32_t abort_flag = sm + C::ABORT_OFF;
-  auto set_abort = [&](int x) { asm volatile("st.volatile.shared.b32 [%0], %1;\n" ::"r"(abort_flag), "r"(x) : "memory"); };
-  const uint32_t steps = abort_flag + 4;
+  const uint32_t state = sm + C::STATE_OFF;
+  auto set_state = [&](int x) { asm volatile("st.volatile.shared.b32 [%0], %1;\n" ::"r"(state), "r"(x) : "memory"); };
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::TMEM_SLOT_OFF);
   auto bar = [&](int i) { return bars + 8u * i; };
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -287,8 +289,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       mbar_init(bar(C::IDS_EMPTY + b), 2);  // both loaders
     }
     asm volatile("st.shared.v2.b32 [%0], {%1, %2};\n" ::"r"(sm + C::BAD_OFF), "r"(0x7fffffff), "r"(-1) : "memory");
-    asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(steps), "r"(0) : "memory");
-    set_abort(0);
+    set_state(0);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 0) {
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
   const int G = p.group;
   bool dead = false;
   auto give_up = [&]() {
-    set_abort(1);
+    set_state(INT_MIN);
     flag_error(FT_DEV_WAIT_TIMEOUT);
     dead = true;
   };
@@ -356,7 +357,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
         ++tiles_done;
         const uint32_t s_col = t_lane + C::S_COL + buf * C::S_STEP, p_col = t_lane + C::P_COL + buf * C::P_STEP;
         // (one answer for the warp: it goes on, or gives up, as a whole)
-        if (!__all_sync(0xffffffffu, ext_wait(bar(C::S_FULL + buf), phase, abort_flag))) {
+        if (!ext_wait(bar(C::S_FULL + buf), phase, state)) {
           give_up();
           return;
         }
@@ -365,7 +366,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
         auto wait_pv = [&]() {
           const int before = tiles_done - 2, b = NW == 2 ? w : before & 1;
           const uint32_t ph = NW == 2 ? (uint32_t)before & 1u : (uint32_t)(before >> 1) & 1u;
-          if (before >= 0 && !__all_sync(0xffffffffu, ext_wait(bar(C::PV_DONE + b), ph, abort_flag))) give_up();
+          if (before >= 0 && !ext_wait(bar(C::PV_DONE + b), ph, state)) give_up();
           tc_fence_after();
         };
         if (MASKED && !__any_sync(0xffffffffu, any)) {  // nothing in sight of the warp's rows
@@ -497,7 +498,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       }
       if (dead) break;
       // ---- the row's result: normalised, to o or to its partial row
-      if (!__all_sync(0xffffffffu, ext_wait(bar(C::O_FULL + w), (uint32_t)items_done & 1u, abort_flag))) {
+      if (!ext_wait(bar(C::O_FULL + w), (uint32_t)items_done & 1u, state)) {
         give_up();
         break;
       }
@@ -554,7 +555,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       for (uint32_t todo = __ballot_sync(0xffffffffu, spoiled); todo != 0; todo &= todo - 1) {
         const int r = (row & ~31) + __ffs(todo) - 1;
         __syncwarp();
-        extend_row<T>(p, item, st, r / G, kvh * G + r % G, steps);
+        extend_row<T>(p, item, st, r / G, kvh * G + r % G, state);
       }
     }
   } else {
@@ -572,7 +573,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       const bool issuer = elect_one();
       auto ubar = [&](int i) { return bars_u + 8u * (uint32_t)i; };
       auto wait = [&](uint32_t b, uint32_t phase) {
-        if (!__all_sync(0xffffffffu, ext_wait(b, phase, abort_flag))) give_up();
+        if (!ext_wait(b, phase, state)) give_up();
       };
       // (Loops are kept short on purpose: the roles run at the same time from one instruction cache.)
       int k_stage = 0, v_stage = 0;
@@ -757,7 +758,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       uint32_t phase = 1, ids_phase = 0;
       set_up();
       while (true) {
-        if (!__all_sync(0xffffffffu, ext_wait(bar(C::IDS_FULL + slot), ids_phase, abort_flag))) {
+        if (!ext_wait(bar(C::IDS_FULL + slot), ids_phase, state)) {
           give_up();
           break;
         }
@@ -776,7 +777,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
         }
         in_pool = __all_sync(0xffffffffu, in_pool);
         dense = tp.has_tma && valid == TILE && in_pool && __all_sync(0xffffffffu, dense);
-        if (!__all_sync(0xffffffffu, ext_wait(empty0 + 8u * stage, phase, abort_flag))) {
+        if (!ext_wait(empty0 + 8u * stage, phase, state)) {
           give_up();
           break;
         }
@@ -842,7 +843,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       int slot = 0, items = 0;
       uint32_t ids_phase = 1;
       auto put_ids = [&](const int4 rec, int kvh, int task) {  // rec.z 0: the end
-        if (!__all_sync(0xffffffffu, ext_wait(bar(C::IDS_EMPTY + slot), ids_phase, abort_flag))) {
+        if (!ext_wait(bar(C::IDS_EMPTY + slot), ids_phase, state)) {
           give_up();
           return;
         }
@@ -853,7 +854,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
         if (lane == 0) {
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %3};\n" ::"r"(sm + C::META_OFF + slot * 16), "r"(rec.z), "r"(kvh), "r"(task) : "memory");
           mbar_arrive(bar(C::IDS_FULL + slot));
-          asm volatile("red.shared.add.u32 [%0], 1;\n" ::"r"(steps) : "memory");
+          asm volatile("red.shared.add.u32 [%0], 1;\n" ::"r"(state) : "memory");
         }
         mbar_arrive_on_cp_async(bar(C::IDS_FULL + slot));
         if (++slot == C::NSI) {
@@ -890,7 +891,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
         put_until(min(t1, t0 + 2));
         if (dead) break;
         const int q_tiles = __ldg(item + 3);
-        if (!__all_sync(0xffffffffu, ext_wait(bar(C::Q_EMPTY), ((uint32_t)items & 1u) ^ 1u, abort_flag))) {
+        if (!ext_wait(bar(C::Q_EMPTY), ((uint32_t)items & 1u) ^ 1u, state)) {
           give_up();
           break;
         }
@@ -943,7 +944,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
   // ---- release tensor memory
   tc_fence_before();
   __syncthreads();
-  if (ext_aborted(abort_flag) != 0)  // copies that nobody waits for any more land before the CTA ends
+  if (ext_state(state) < 0)  // copies that nobody waits for any more land before the CTA ends
     for (int i = 0; i < 2000; ++i) __nanosleep(1000);
   if (warp == 0) {
     tc_fence_after();

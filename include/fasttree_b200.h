@@ -474,8 +474,8 @@ int ft_extend_args_size(void);
 int ft_extend(const ft_extend_args* args);
 /* Runs the bounded waits of ft_extend's tensor-core kernel against barriers that nothing arrives at, with `limit` probes (64 to
  * 2^16, about 4 us each), and synchronises: a health check as ft_selftest_bounded_wait.  result_host[0]: 0 as expected, else the sum of 1
- * (a wait did not run out), 2 (the abort flag did not end one), 4 (lanes of one warp got different answers), 8 (one ran out
- * although the CTA took steps), 16 (one did not run out after the last step); result_host[1]: the probes of the kernel's own
+ * (a wait did not run out), 2 (it went on where another role had given up), 4 (it did not see a completed barrier), 8 (it ran out
+ * although the CTA took steps), 16 (it did not run out after the last step); result_host[1]: the probes of the kernel's own
  * waits.  Raises FT_DEV_WAIT_TIMEOUT in the device status word. */
 int ft_selftest_extend_wait(int limit, int* result_host, void* stream);
 /* names of the kernels that ft_extend would launch, as ft_stage1_path_name gives them */
