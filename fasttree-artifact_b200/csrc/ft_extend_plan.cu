@@ -673,6 +673,8 @@ int ft_extend_plan_build(const int64_t* seq_lens, const int64_t* extend_lens, co
     p.slots = tensor ? num_sms : elem_bytes == 4 && head_dim == 256 ? num_sms : 2 * num_sms;
     // Query tiles: 128 rows on the tensor cores; 64 or 16 on the CUDA cores, whichever schedule ends first.
     const double d = head_dim / 128.0;
+    // (The tensor-core costs for head_dim 64 are those measured at 128, and a cap is not known here, although a capped tile costs half
+    // as much again: such steps are cut as if their tiles cost the same, so only the tasks' order and number can suffer.)
     const Costs tc = head_dim == 256 ? Costs{1.0, 0, 1.0, 1.0, 3.0} : Costs{0.6, 0.15, 0.75, 1.1, 2.5};
     const Costs many = {0, 0, 0, 1.0 + 13.0 * d, 4.0}, few = {0, 0, 0, 1.0 + 4.0 * d, 3.0};
     struct Form {

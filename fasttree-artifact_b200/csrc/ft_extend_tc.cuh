@@ -30,15 +30,15 @@
 // a barrier for that.
 //
 // What bounds it: at head_dim 128 the chain scores -> softmax -> product of a stream, which the other stream hides but for a
-// third (the tensor pipe is busy 60 to 65 % of the time): 4096 tokens behind 12288 cached ones, 64/8 heads, bf16 1476 us =
-// 1304 TFLOP/s, 0.78 of what a large library product reaches in a burst; 2048 on 2048, 32/4 heads 109 us = 950.  At 64 the
-// exponentials, 16 a clock and SM, at 63 % of the active cycles: 94 us = 550 TFLOP/s for the same (the two softmax warps of a
-// scheduler taking turns at them: 111).  At 256 the products, whose 64-column shapes read shared
-// memory more often than they multiply: 251 to 266 us = 770 to 820 TFLOP/s.  Few tokens: the K/V rows' way from memory, 4.0 to
-// 4.6 TB/s where each request has a cache of its own, and below about 30 us the chain of dependent reads at the start
-// (schedule, tile record, row ids, first tile) and the merge's launch.  Scattered pools: the TMA unit's row gathers, about 27 ns
-// for four rows of 128 bytes and SM (sixteen prompts 330 us, with consecutive rows 283); 16-byte copies beside or instead of
-// them were slower in every mixture (half of the rows 375).
+// third (the tensor pipe is busy 55 % of an SM's active cycles in 2048 on 2048 tokens), and power: 4096 tokens behind 12288
+// cached ones, 64/8 heads, bf16, 1710 us = 1125 TFLOP/s run on end, 0.81 of what a large library product settles at; 1486 us =
+// 1295 in short runs; 2048 on 2048, 32/4 heads 109 us = 950.  At 64 the exponentials, 16 a clock and SM, at 63 % of the active
+// cycles: 94 us = 548 TFLOP/s for the same (the two softmax warps of a scheduler taking turns at them: 111 for 94).  At 256 the products,
+// whose 64-column shapes read shared memory more often than they multiply: 254 us = 811 TFLOP/s.  Few tokens: the K/V rows' way from
+// memory, 4.0 to 4.6 TB/s where each request has a cache of its own, and below about 30 us the chain of dependent reads at the
+// start (schedule, tile record, row ids, first tile) and the merge's launch.  Scattered pools: the TMA unit's row gathers, about
+// 27 ns for four rows of 128 bytes and SM (sixteen prompts 332 us, with consecutive rows 297); 16-byte copies beside or instead
+// of them were slower in every mixture (half of the rows 375).
 //
 // Rows of V that a query does not see are multiplied by P = 0, and 0 x Inf is NaN: a row that is not shown everything and did
 // not come out finite is computed again from its own tokens (extend_row).

@@ -1,7 +1,8 @@
 """New tokens of a serving step: into the paged cache (``append``) and their attention over it (``extend``).
 
 Same call contract as :mod:`ft_b200.engine`: the caller owns every tensor, kernels are enqueued on torch's current CUDA
-stream of the tensors' device, nothing synchronises with the host.  Bad arguments raise ``ValueError`` or
+stream of the tensors' device, and ``append`` and ``extend`` do not synchronise with the host.  ``prepare``, once per step, does: it
+copies the plan from ordinary host memory and returns when the copy is done.  Bad arguments raise ``ValueError`` or
 ``FastTreeError``.  The reference leaves both to its host (SGLang's rotary embedding, ``store_kv_cache`` and extend
 attention); they have no counterpart in it.
 """
@@ -33,7 +34,8 @@ class ExtendPlan:
     """Schedule of one step's extend attention, for all layers: a host description and one device table.  Read-only once
     made: any number of calls, streams and captured graphs may use it at once.  Like every tensor of a call, its table has to
     live until the work that reads it is done: keep the plan as long as a graph that was captured with it, and until other
-    streams than the one it was made on are through with it."""
+    streams than the one it was made on are through with it.  A plan is of one step's lengths, and so is a graph that was
+    captured with it."""
 
     def __init__(self, info, table, seq_lens, extend_lens):
         self.info = info
@@ -138,7 +140,8 @@ def prepare(seq_lens, extend_lens, kv_starts, num_qo_heads, num_kv_heads, head_d
     (in SGLang: row ``req_pool_indices[r]`` of ``req_to_token``, flattened).  ``shared_prefixes``: pairs ``(requests,
     length)`` - these requests' first ``length`` cached tokens are the same pool rows, and their attention reads them once;
     nested pairs describe a tree (:func:`tree_prefixes`).  ``window`` > 0: a token sees the newest ``window`` positions up
-    to its own.  Integers on the host; one copy to ``device``."""
+    to its own.  Integers on the host; one copy to ``device``, for which the host waits.  Steps of single tokens without window
+    and cap are ``fasttree_decode``'s: it takes them faster and without a plan per step."""
     dev = torch.device(device)
     if dev.type != "cuda":
         raise ValueError("the plan is uploaded to a CUDA device; the engine has no CPU path")

@@ -182,6 +182,7 @@ def fasttree_extend_preparation(seq_lens, extend_lens, kv_starts, num_qo_heads, 
 
 
 def fasttree_extend(q, k_buffer, v_buffer, o, kv_entries, plan, sm_scale, logit_cap=-1, o_lse=None):
-    """Causal attention of a step's new tokens - one per request, a question, a whole prompt - over the paged cache; writes
-    ``o`` on the current CUDA stream (:func:`ft_b200.extend.extend`).  Here ``logit_cap`` is applied."""
+    """Causal attention of a step's new tokens - a question, a whole prompt, or one per request where scores are capped or a window
+    hides old positions (else :func:`fasttree_decode` is faster) - over the paged cache; writes ``o`` on the current CUDA stream
+    (:func:`ft_b200.extend.extend`).  Here ``logit_cap`` is applied."""
     _extend.extend(q, k_buffer, v_buffer, o, kv_entries, plan, sm_scale, logit_cap=logit_cap, o_lse=o_lse)
