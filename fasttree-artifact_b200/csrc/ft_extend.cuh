@@ -187,6 +187,25 @@ __device__ __noinline__ void extend_row(const ExtendParams& p, const int32_t* it
   if (lane == 0) extend_store_lse(p, part, q_row, head, l == 0.f ? -INFINITY : logf(l) + m);
 }
 
+// How many row ids outside the pool a stream shows to a token: each lane for its own, by a whole warp.  steps as above.
+__device__ __noinline__ int extend_bad_in_sight(const ExtendParams& p, const int32_t* item, const ExtendStream st, const int tok, const uint32_t steps) {
+  const int lane = threadIdx.x & 31, step = item[2], tile0 = item[5], words = p.tile / 32;
+  int n = 0;
+  for (int t = st.lo; t < st.hi; t += step) {
+    const int32_t* tile = p.tiles + 8 * ((int64_t)tile0 + t);
+    const int4 rec = __ldg(reinterpret_cast<const int4*>(tile));
+    const int bits_at = __ldg(tile + 4 + st.block_tile);
+    if (lane == 0) asm volatile("red.shared.add.u32 [%0], 1;\n" ::"r"(steps) : "memory");
+#pragma unroll 4
+    for (int k = 0; k < words; ++k) {
+      const int i = 32 * k + lane, id = i < rec.z ? __ldg(p.kv_entries + extend_entry(p, rec, i)) : 0;
+      const uint32_t out = __ballot_sync(0xffffffffu, i < rec.z && (id < 0 || id >= p.kv_rows));
+      if (out != 0) n += __popc(out & (bits_at < 0 ? 0xffffffffu : (uint32_t)__ldg(p.extra + bits_at + (st.first + tok) * words + k)));
+    }
+  }
+  return n;
+}
+
 // Any type and head size: a CTA per (item, KV head), a warp per query row in turn.
 template <typename T>
 __global__ void __launch_bounds__(128) extend_generic_kernel(const ExtendParams p) {

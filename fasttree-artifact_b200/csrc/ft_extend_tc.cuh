@@ -16,9 +16,9 @@
 //
 // A K/V tile whose rows are consecutive in the pool is one TMA box per 64 columns; any other is gathered four rows at a
 // time through the TMA unit, its last rows with 16-byte copies.  Rows of V behind the last token are zeroed up to the next
-// 16, where the product ends; rows of K are not: their scores are masked.  Row ids outside the pool become zeros, which would count
-// as keys of score 0: the K loader notes the task, and its rows are computed again one by one (extend_row), which leaves such ids
-// out.  That is slow, and the call is flagged; a check of every tile instead costs all calls 1 to 8 %.
+// 16, where the product ends; rows of K are not: their scores are masked.  Row ids outside the pool become zeros; the K loader notes
+// the task, and what such keys of score 0 have put into a row's sum is taken out of it at the task's end (a check of every tile instead
+// costs all calls 1 to 8 %).
 //
 // Softmax: a thread reads its row of S, masks what the row does not see (bits from the plan; a tile that all of the query tile's
 // rows see whole has none), keeps a running maximum that may lag by 2^8 before O is rescaled in
@@ -514,6 +514,19 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       const int part = live ? extend_part(p, st, tok) : -2;
       const bool store = part != -2 && tk.x >= 0 && tk.x < p.q_rows;
       if (part != -2 && !store) flag_error(FT_DEV_BAD_Q_INDEX);
+      // Row ids outside the pool were zeros: keys of score 0 and no value, which nothing but the row's sum has met.  What they put
+      // there is taken out, if the offset is a real key's (then P has its full precision) and enough of the sum is left.
+      // (The K loader notes the task before it hands the tile over; the tasks between the first and the last are looked at too.)
+      bool again = false;
+      const int2 bad = lds_int2(sm + C::BAD_OFF);
+      if (n >= bad.x && n <= bad.y) {
+        const int in_sight = extend_bad_in_sight(p, item, st, tok, state);
+        if (in_sight > 0) {
+          const float rest = l_run - (float)in_sight * fast_exp2(-m_used);
+          again = !(m_used > 0.f && rest >= 0.015625f * l_run);
+          l_run = rest;
+        }
+      }
       const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
       float2 finite = make_float2(0.f, 0.f);  // 0 x every element: 0, or NaN
       uint8_t* dst = nullptr;
@@ -549,9 +562,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
       }
       if (store)
         extend_store_lse(p, part, tk.x, head, l_run == 0.f ? -INFINITY : (m_used + log2f(l_run)) * 0.6931471805599453f);
-      // (noted by the K loader before the tile was handed over; the tasks between the first and the last are taken with them)
-      const int2 bad = lds_int2(sm + C::BAD_OFF);
-      const bool spoiled = store && ((n >= bad.x && n <= bad.y) || (hidden && !(finite.x + finite.y == 0.f)));
+      const bool spoiled = store && (again || (hidden && !(finite.x + finite.y == 0.f)));
       for (uint32_t todo = __ballot_sync(0xffffffffu, spoiled); todo != 0; todo &= todo - 1) {
         const int r = (row & ~31) + __ffs(todo) - 1;
         __syncwarp();

@@ -93,3 +93,27 @@ def test_over_many_tasks_of_a_block(dtype, d, window):
     hits = [(r, p, -1) for r in (4, 5, 6, 7, 8) for p in (7, 299)] + [(9, 480, s.k.shape[0]), (11, 400, -1), (2, 560, -9), (0, 499, -1)]
     check(s, hits, plan=plan)
     check(s, hits, plan=plan, cap=5.0)
+
+
+@pytest.mark.parametrize("dtype,d", FORMS)
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_scores_far_from_zero(dtype, d, sign):
+    """A key of zeros would outweigh all others, or none: every score lies far below or above 0."""
+    s = Step([900, 200], [40, 3], [], 8, 2, d, DTYPES[dtype])
+    s.q = (s.q.abs() + 0.5).to(s.dtype)
+    s.k = (sign * (s.k.abs() + 0.5)).to(s.dtype)
+    s.gq, s.gk = s.q.cuda(), s.k.cuda()
+    check(s, [(0, 50, -1), (0, 300, -1), (0, 860, -1), (1, 7, s.k.shape[0])])
+
+
+@pytest.mark.parametrize("dtype,d", FORMS)
+def test_rows_that_see_none_keep_their_bits(dtype, d):
+    s = Step([700, 300, 260], [200, 40, 1], [([0, 1], 250)], 8, 2, d, DTYPES[dtype])
+    want, want_lse = s.run()
+    table = s.gt.clone()
+    table[0, 600] = -1                                           # seen by request 0's queries from the hundredth on
+    o, lse = torch.empty_like(s.gq), torch.empty_like(want_lse)
+    extend.extend(s.gq, s.gk, s.gv, o, table, s.plan, s.scale, o_lse=lse)
+    assert lib.read_device_status() == lib.FT_DEV_BAD_KV_INDEX
+    rows = list(range(100)) + list(range(200, 241))
+    assert torch.equal(o[rows], want[rows]) and torch.equal(lse[rows], want_lse[rows])

@@ -4,9 +4,9 @@ import ctypes
 import pytest
 import torch
 
-from ft_b200 import extend, lib
-from test_extend_bad_rows_gpu import check
+from ft_b200 import lib
 from test_extend_gpu import Step
+from test_extend_queues_gpu import checker, replan
 
 
 def test_self_test_refuses_bad_arguments():
@@ -31,10 +31,11 @@ def test_waits_run_out_end_on_the_abort_flag_and_follow_steps():
 @pytest.mark.gpu
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_rows_computed_again_for_longer_than_a_wait_lasts(d):
-    """A row id outside the pool in a long context on one CTA: its rows go one by one, and the other roles, and the next task,
-    wait for them."""
+    """NaN in the newest token's value, in a long context on one CTA: the rows that do not see it go one by one, and the other
+    roles, and the next task, wait for them for seconds."""
     n, e = 40000, 64
     s = Step([n], [e], [], 4, 2, d, torch.bfloat16)
-    info, table, _, _ = extend.host_plan([n], [e], [0], 4, 2, d, s.dtype, num_sms=1)
-    plan = extend.ExtendPlan(info, torch.from_numpy(table).cuda(), [n], [e])
-    check(s, [(0, 20000, -1), (0, 5, s.k.shape[0])], plan=plan)
+    replan(s, 1)
+    check = checker(s, -1.0)
+    s.gv[s.table[0, n - 1].long()] = float("nan")
+    check(list(range(e - 1)))
