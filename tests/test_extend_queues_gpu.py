@@ -42,7 +42,7 @@ def replan(s, made_for, num_sms=None, seed=0):
     return kinds, int((ends[:, 1] - ends[:, 0]).max())
 
 
-def checker(s, cap):
+def against_oracle(s, cap):
     """Runs the step and holds it to the oracle, which is computed once."""
     out, want_lse, absv, size = expected(s, s.table, cap)
     tol, tol_lse = extend_cases.bounds(s.dtype, out, absv, size, cap, s.d)
@@ -71,7 +71,7 @@ def mixed(dtype, d, window=0, layout="scattered", seed=0):
 @pytest.mark.parametrize("cap", [-1.0, 6.0])
 def test_queues_against_the_oracle(dtype, d, window, cap):
     s = mixed(dtype, d, window, layout="prefill" if cap > 0 else "scattered", seed=d + window)
-    kinds, check = set(), checker(s, cap)
+    kinds, check = set(), against_oracle(s, cap)
     for made_for, num_sms in ((1, None), (3, None), (148, 1), (148, 5), (10, 2)):
         some, longest = replan(s, made_for, num_sms, seed=made_for)
         assert longest >= 8
@@ -101,7 +101,7 @@ def test_queues_repeat_and_do_not_depend_on_the_queue(dtype, d):
 def test_values_that_are_no_numbers_out_of_sight_in_queues(dtype, d, cap):
     """Every request's newest token holds them: all other queries stay within their bounds."""
     s = mixed(dtype, d)
-    check = checker(s, cap)
+    check = against_oracle(s, cap)
     last = [sum(s.ext[:r + 1]) - 1 for r in range(len(s.ext)) if s.ext[r]]
     good = [i for i in range(sum(s.ext)) if i not in last]
     newest = torch.stack([s.table[r, s.seq[r] - 1] for r in range(len(s.seq)) if s.ext[r]]).long()
@@ -127,7 +127,7 @@ def test_query_tiles_of_rows_that_are_not_consecutive(dtype, d):
 @pytest.mark.parametrize("dtype,d", [("bf16", 64), ("fp16", 128), ("bf16", 256), ("fp32", 128)])
 def test_positions_beyond_16_bits(dtype, d):
     s = Step([70001, 66000], [2, 1], [([0, 1], 65500)], 2, 1, d, DTYPES[dtype])
-    check = checker(s, -1.0)
+    check = against_oracle(s, -1.0)
     for made_for, num_sms in ((148, None), (2, None), (148, 3)):
         replan(s, made_for, num_sms)
         check()

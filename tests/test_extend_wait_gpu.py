@@ -6,7 +6,7 @@ import torch
 
 from ft_b200 import lib
 from test_extend_gpu import Step
-from test_extend_queues_gpu import checker, replan
+from test_extend_queues_gpu import against_oracle, replan
 
 
 def test_self_test_refuses_bad_arguments():
@@ -36,6 +36,6 @@ def test_rows_computed_again_for_longer_than_a_wait_lasts(d):
     n, e = 40000, 64
     s = Step([n], [e], [], 4, 2, d, torch.bfloat16)
     replan(s, 1)
-    check = checker(s, -1.0)
+    check = against_oracle(s, -1.0)
     s.gv[s.table[0, n - 1].long()] = float("nan")
     check(list(range(e - 1)))
