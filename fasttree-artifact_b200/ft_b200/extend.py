@@ -19,7 +19,8 @@ def append(q, k, v, k_buffer, v_buffer, slots, q_out=None, positions=None, cos_s
 
     ``q`` ``[tokens, q heads, head_dim]`` (or None), ``k`` and ``v`` ``[tokens, kv heads, head_dim]``, the pool
     ``[rows, kv heads, head_dim]``; fp16, bf16 or fp32, any strides with a contiguous head_dim axis.  ``slots`` (int32 or
-    int64): -1 is a padding token, which is not stored; no row twice.  The turned queries go to ``q_out``, which may be ``q``
+    int64): -1 is a padding token, which is not stored; no row twice.  ``k`` and ``v`` may be views of the pool only where each
+    token stands at its own slot.  The turned queries go to ``q_out``, which may be ``q``
     (the default) but must not overlap it, ``k``, ``v`` or the pool otherwise.  ``cos_sin`` (fp32 ``[positions,
     rot_dim]``): cosines of the rot_dim / 2 pairs, then their sines; elements from ``rot_dim`` on stay as they are.
     ``positions``: ``[tokens]``, or ``[axes, tokens]`` with ``sections``, the number of consecutive pairs that each axis turns.

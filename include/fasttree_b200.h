@@ -367,7 +367,7 @@ void ft_plan_free(ft_plan* plan);
  * All pointers are device pointers, strides are in elements, the innermost stride is 1. */
 typedef struct ft_append_args {
   const void* q;       /* [tokens, num_qo_heads, head_dim], or NULL: keys and values only */
-  const void* k;       /* [tokens, num_kv_heads, head_dim]                                 */
+  const void* k;       /* [tokens, num_kv_heads, head_dim]; in the pool, as v, only where each token stands at its own slot */
   const void* v;       /* same shape as k                                                  */
   void* q_out;         /* shape of q; may be q itself, else must overlap none of the others */
   void* k_buffer;      /* [kv_rows, num_kv_heads, head_dim], written at the slots          */

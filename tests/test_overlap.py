@@ -97,3 +97,19 @@ def test_append_into_memory_that_it_reads():
     assert torch.equal(buf, keep) and torch.equal(kb[:t], k) and torch.equal(vb[:t], v)
     fasttree.fasttree_append(buf[:t, 4:Q], k, v, kb, vb, slots, q_out=out[:, :Q - 4])
     assert torch.equal(out[:, :Q - 4], keep[:t, 4:Q])
+
+
+@gpu
+@pytest.mark.parametrize("hkv,dtype", [(2, torch.float16), (40, torch.bfloat16), (3, torch.float32)])
+def test_keys_turned_in_the_pool(hkv, dtype):
+    """k and v are the pool's own rows: the same as from a copy of them."""
+    t, rows = 37, 50
+    g = torch.Generator().manual_seed(hkv)
+    kb, vb = (torch.randn(rows, hkv, D, generator=g).to(dtype).cuda() for _ in range(2))
+    angle = torch.randn(rows, D // 2, generator=g)
+    table, pos = torch.cat([angle.cos(), angle.sin()], 1).cuda(), torch.randint(0, rows, (t,), generator=g).cuda()
+    slots = torch.arange(5, 5 + t, device="cuda")
+    want_k, want_v = kb.clone(), vb.clone()
+    fasttree.fasttree_append(None, kb[5:5 + t].clone(), vb[5:5 + t].clone(), want_k, want_v, slots, positions=pos, cos_sin=table)
+    fasttree.fasttree_append(None, kb[5:5 + t], vb[5:5 + t], kb, vb, slots, positions=pos, cos_sin=table)
+    assert torch.equal(kb, want_k) and torch.equal(vb, want_v)
