@@ -1163,3 +1163,4 @@ int ft_read_device_status(void* stream, int32_t* flags) {
 }  // extern "C"
 
 #include "ft_extend_api.cuh"
+#include "ft_branch_api.cuh"

@@ -1,0 +1,246 @@
+// C entry points for branching continuations: ft_draft_tree, ft_draft_accept, ft_beam_select, ft_beam_reorder (part of ft_api.cu, as
+// ft_extend_api.cuh).
+#pragma once
+
+#include "ft_beam.cuh"
+#include "ft_draft.cuh"
+
+namespace {
+
+// A draft plan's parts lie in its table, and its requests' rows within `rows`.
+int check_draft_plan(const ft_extend_plan_info& pl, const int32_t* table, int64_t rows) {
+  if (pl.draft != 1) return fail(FT_ERR_INVALID_ARGUMENT, "the plan was not made for drafted tokens");
+  if (pl.num_drafts < 0 || pl.num_spans < 0 || pl.longest_draft < 0 || pl.longest_draft > FT_MAX_DRAFT || pl.num_tokens < 0)
+    return fail(FT_ERR_INVALID_ARGUMENT, "the plan's counts are not a plan's");
+  if (pl.drafts_off < 0 || pl.drafts_off % 4 != 0 || pl.drafts_off + 8LL * pl.num_drafts > pl.table_ints || pl.spans_off < 0 || pl.spans_off % 4 != 0 ||
+      pl.spans_off + 8LL * pl.num_spans > pl.table_ints || pl.extra_off < 0 || pl.extra_off % 4 != 0 || pl.extra_off > pl.table_ints)
+    return fail(FT_ERR_INVALID_ARGUMENT, "the plan's parts do not lie in its table");
+  if (pl.tile_tokens != 64 && pl.tile_tokens != 128) return fail(FT_ERR_INVALID_ARGUMENT, "the plan's sizes are not a plan's");
+  if (pl.num_tokens == 0) return FT_OK;
+  if (table == nullptr) return fail(FT_ERR_INVALID_ARGUMENT, "plan_table is NULL");
+  if (!aligned16(table)) return fail(FT_ERR_UNSUPPORTED, "plan_table must be 16-byte aligned");
+  if (pl.q_rows > rows) return fail(FT_ERR_INVALID_ARGUMENT, "the plan names %lld tokens, the call has %lld", (long long)pl.q_rows, (long long)rows);
+  return FT_OK;
+}
+
+int current_sms() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess ? sm_count(dev) : 148;
+}
+
+template <typename T>
+int launch_accept(const ft::AcceptParams& p, int requests, int64_t row_bytes, bool vec, cudaStream_t st) {
+  // CTAs per request: as many as the SMs hold two of, as long as each has 8 KB of a row to read (fewer bytes come no sooner)
+  int ranks = 1;
+  const int room = 2 * current_sms();
+  while (p.targets == nullptr && ranks < 8 && (int64_t)requests * ranks * 2 <= room && row_bytes / (2 * ranks) >= 8192) ranks *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(requests * ranks));
+  cfg.blockDim = dim3(ft::ACCEPT_THREADS);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ranks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  FT_CUDA_OK(cudaLaunchKernelEx(&cfg, ft::draft_accept_kernel<T>, p, (int)vec));
+  count_launch();
+  return FT_OK;
+}
+
+struct BeamShape {
+  int pieces, slices, slice_len;
+  int64_t keys, bytes;  // of the workspace: keys, then sums
+};
+
+int dtype_size(int dtype) { return dtype == FT_F32 ? 4 : 2; }
+
+int check_beam_select(const ft_beam_select_args* a) {
+  if (a == nullptr) return fail(FT_ERR_INVALID_ARGUMENT, "args is NULL");
+  if (a->dtype != FT_F16 && a->dtype != FT_BF16 && a->dtype != FT_F32)
+    return fail(FT_ERR_INVALID_ARGUMENT, "dtype %d is not one of FT_F16/FT_BF16/FT_F32", a->dtype);
+  if (a->batch < 0 || a->beams <= 0 || a->beams > FT_MAX_BEAMS || a->best <= 0 || a->best > FT_MAX_BEAMS)
+    return fail(FT_ERR_INVALID_ARGUMENT, "beams %d and best %d must be 1 to %d", a->beams, a->best, FT_MAX_BEAMS);
+  if (a->vocab <= 0) return fail(FT_ERR_INVALID_ARGUMENT, "vocab must be positive");
+  return FT_OK;
+}
+
+// Slices of a row.  Eight 16-byte pieces a thread where that leaves every SM CTAs enough to hide each other's waits, fewer where the
+// call is small and its length is what one slice takes.  (148 SMs whatever the device: the workspace's size goes by this.)
+BeamShape beam_shape(const ft_beam_select_args* a) {
+  BeamShape s;
+  const int n = 16 / dtype_size(a->dtype), sms = 148;
+  const int64_t rows = (int64_t)a->batch * a->beams;
+  for (s.pieces = 8; s.pieces > 1; s.pieces /= 2) {
+    const int64_t slice = (int64_t)ft::BEAM_THREADS * s.pieces * n;
+    if (rows * ((a->vocab + slice - 1) / slice) >= 3LL * sms) break;
+  }
+  const int64_t most = (int64_t)ft::BEAM_THREADS * s.pieces * n;
+  s.slices = (int)((a->vocab + most - 1) / most);
+  s.slice_len = (int)((((int64_t)a->vocab + s.slices - 1) / s.slices + n - 1) / n * n);
+  s.keys = rows * s.slices * a->best;
+  s.bytes = s.keys * 8 + rows * s.slices * 8;
+  return s;
+}
+
+int pow2_at_least(int n, int low) {
+  while (low < n) low *= 2;
+  return low;
+}
+
+template <typename T, int NV>
+void launch_scan(const ft::BeamParams& p, int groups, bool vec, cudaStream_t st) {
+  const unsigned ctas = (unsigned)((int64_t)p.batch * p.beams * p.slices);
+  if (vec)
+    ft::beam_scan_kernel<T, NV, true><<<ctas, ft::BEAM_THREADS, 0, st>>>(p, groups);
+  else
+    ft::beam_scan_kernel<T, NV, false><<<ctas, ft::BEAM_THREADS, 0, st>>>(p, groups);
+}
+
+template <typename T>
+int launch_beam_select(const ft::BeamParams& p, int pieces, bool vec, cudaStream_t st) {
+  const int groups = pow2_at_least(p.best, ft::BEAM_WARPS);
+  switch (pieces) {
+    case 1: launch_scan<T, 1>(p, groups, vec, st); break;
+    case 2: launch_scan<T, 2>(p, groups, vec, st); break;
+    case 4: launch_scan<T, 4>(p, groups, vec, st); break;
+    default: launch_scan<T, 8>(p, groups, vec, st); break;
+  }
+  FT_CUDA_OK(cudaGetLastError());
+  count_launch();
+  FT_CUDA_OK(launch_early(ft::beam_merge_kernel, dim3((unsigned)p.batch), ft::BEAM_THREADS, 0, st, p, groups));
+  count_launch();
+  return FT_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ft_draft_tree_args_size(void) { return static_cast<int>(sizeof(ft_draft_tree_args)); }
+int ft_draft_accept_args_size(void) { return static_cast<int>(sizeof(ft_draft_accept_args)); }
+int ft_beam_select_args_size(void) { return static_cast<int>(sizeof(ft_beam_select_args)); }
+int ft_beam_reorder_args_size(void) { return static_cast<int>(sizeof(ft_beam_reorder_args)); }
+
+int ft_draft_tree(const ft_draft_tree_args* a) {
+  if (a == nullptr) return fail(FT_ERR_INVALID_ARGUMENT, "args is NULL");
+  const int rc = check_draft_plan(a->plan, a->plan_table, a->rows);
+  if (rc != FT_OK) return rc;
+  if (a->plan.num_tokens == 0) return FT_OK;
+  if (a->parents == nullptr) return fail(FT_ERR_INVALID_ARGUMENT, "parents is NULL");
+  ft::DraftParams p;
+  memset(&p, 0, sizeof(p));
+  p.drafts = a->plan_table + a->plan.drafts_off;
+  p.spans = reinterpret_cast<const DraftSpan*>(a->plan_table + a->plan.spans_off);
+  p.extra = a->plan_table + a->plan.extra_off;
+  p.parents = a->parents, p.positions = a->positions;
+  p.parents_64 = a->parents_64, p.positions_64 = a->positions_64;
+  p.window = a->plan.window, p.words = a->plan.tile_tokens / 32;
+  ft::draft_tree_kernel<<<(unsigned)a->plan.num_drafts, ft::DRAFT_THREADS, 0, static_cast<cudaStream_t>(a->stream)>>>(p);
+  FT_CUDA_OK(cudaGetLastError());
+  count_launch();
+  return FT_OK;
+}
+
+int ft_draft_accept(const ft_draft_accept_args* a) {
+  if (a == nullptr) return fail(FT_ERR_INVALID_ARGUMENT, "args is NULL");
+  const int rc = check_draft_plan(a->plan, a->plan_table, a->rows);
+  if (rc != FT_OK) return rc;
+  const ft_extend_plan_info& pl = a->plan;
+  if ((a->logits == nullptr) == (a->targets == nullptr) && pl.num_tokens > 0)
+    return fail(FT_ERR_INVALID_ARGUMENT, "one of logits and targets must be given");
+  if (a->dtype != FT_F16 && a->dtype != FT_BF16 && a->dtype != FT_F32)
+    return fail(FT_ERR_INVALID_ARGUMENT, "dtype %d is not one of FT_F16/FT_BF16/FT_F32", a->dtype);
+  if (a->logits != nullptr && a->vocab <= 0) return fail(FT_ERR_INVALID_ARGUMENT, "vocab must be positive");
+  if (a->num_requests < pl.num_drafts) return fail(FT_ERR_INVALID_ARGUMENT, "the plan has %d requests, the results %d", pl.num_drafts, a->num_requests);
+  if (a->accepted_width < pl.longest_draft)
+    return fail(FT_ERR_INVALID_ARGUMENT, "accepted has %d entries a request, the longest draft %d tokens", a->accepted_width, pl.longest_draft);
+  if (pl.num_drafts == 0) return FT_OK;
+  if (a->plan_table == nullptr || !aligned16(a->plan_table)) return fail(FT_ERR_INVALID_ARGUMENT, "plan_table is NULL or not 16-byte aligned");
+  if (a->accepted == nullptr || a->counts == nullptr || a->next_tokens == nullptr ||
+      (pl.num_tokens > 0 && (a->tokens == nullptr || a->parents == nullptr)))
+    return fail(FT_ERR_INVALID_ARGUMENT, "tokens / parents / accepted / counts / next_tokens is NULL");
+  if ((a->slots == nullptr) != (a->kv_entries == nullptr) && pl.num_tokens > 0)
+    return fail(FT_ERR_INVALID_ARGUMENT, "slots and kv_entries go together");
+  if (a->slots != nullptr && pl.kv_entries_len > a->kv_entries_len)
+    return fail(FT_ERR_INVALID_ARGUMENT, "the plan names %lld entries of kv_entries, which has %lld", (long long)pl.kv_entries_len,
+                (long long)a->kv_entries_len);
+  ft::AcceptParams p;
+  memset(&p, 0, sizeof(p));
+  p.drafts = a->plan_table + pl.drafts_off;
+  p.logits = a->logits, p.targets = a->targets, p.tokens = a->tokens, p.parents = a->parents;
+  p.accepted = a->accepted, p.counts = a->counts, p.next_tokens = a->next_tokens;
+  p.slots = a->kv_entries != nullptr ? a->slots : nullptr, p.kv_entries = a->kv_entries;
+  p.logits_s0 = a->logits_stride0, p.accepted_s0 = a->accepted_stride0, p.kv_entries_len = a->kv_entries_len;
+  p.vocab = a->vocab, p.width = a->accepted_width;
+  p.targets_64 = a->targets_64, p.tokens_64 = a->tokens_64, p.parents_64 = a->parents_64, p.next_64 = a->next_64, p.slots_64 = a->slots_64;
+  const int size = dtype_size(a->dtype), n = 16 / size;
+  const bool vec = aligned16(a->logits) && a->logits_stride0 % n == 0;
+  const int64_t row_bytes = (int64_t)a->vocab * size;
+  cudaStream_t st = static_cast<cudaStream_t>(a->stream);
+  if (a->dtype == FT_F16) return launch_accept<__half>(p, pl.num_drafts, row_bytes, vec, st);
+  if (a->dtype == FT_BF16) return launch_accept<__nv_bfloat16>(p, pl.num_drafts, row_bytes, vec, st);
+  return launch_accept<float>(p, pl.num_drafts, row_bytes, vec, st);
+}
+
+int64_t ft_beam_select_workspace(const ft_beam_select_args* a) {
+  const int rc = check_beam_select(a);
+  return rc != FT_OK ? rc : beam_shape(a).bytes;
+}
+
+int ft_beam_select(const ft_beam_select_args* a) {
+  const int rc = check_beam_select(a);
+  if (rc != FT_OK) return rc;
+  if (a->batch == 0) return FT_OK;
+  if (a->logits == nullptr || a->scores == nullptr || a->out_scores == nullptr || a->out_beams == nullptr || a->out_tokens == nullptr)
+    return fail(FT_ERR_INVALID_ARGUMENT, "logits / scores / out_scores / out_beams / out_tokens is NULL");
+  if (a->workspace == nullptr || !aligned16(a->workspace)) return fail(FT_ERR_INVALID_ARGUMENT, "workspace is NULL or not 16-byte aligned");
+  const BeamShape s = beam_shape(a);
+  if ((int64_t)a->batch * a->beams * s.slices > 0x7fffffffLL || (int64_t)a->beams * s.slices * a->best > 0x7fffffffLL / 2)
+    return fail(FT_ERR_TOO_LARGE, "more slices of logits than one launch takes");
+  ft::BeamParams p;
+  memset(&p, 0, sizeof(p));
+  p.logits = a->logits, p.scores = a->scores, p.out_scores = a->out_scores, p.out_beams = a->out_beams, p.out_tokens = a->out_tokens;
+  p.keys = static_cast<unsigned long long*>(a->workspace);
+  p.sums = reinterpret_cast<float2*>(p.keys + s.keys);
+  p.logits_s0 = a->logits_stride0, p.logits_s1 = a->logits_stride1, p.scores_s0 = a->scores_stride0, p.scores_s1 = a->scores_stride1;
+  p.out_scores_s0 = a->out_scores_stride0, p.out_beams_s0 = a->out_beams_stride0, p.out_tokens_s0 = a->out_tokens_stride0;
+  p.batch = a->batch, p.beams = a->beams, p.vocab = a->vocab, p.best = a->best, p.slices = s.slices, p.slice_len = s.slice_len;
+  p.beams_64 = a->beams_64, p.tokens_64 = a->tokens_64;
+  const int n = 16 / dtype_size(a->dtype);
+  const bool vec = aligned16(a->logits) && (a->batch == 1 || a->logits_stride0 % n == 0) && (a->beams == 1 || a->logits_stride1 % n == 0);
+  cudaStream_t st = static_cast<cudaStream_t>(a->stream);
+  if (a->dtype == FT_F16) return launch_beam_select<__half>(p, s.pieces, vec, st);
+  if (a->dtype == FT_BF16) return launch_beam_select<__nv_bfloat16>(p, s.pieces, vec, st);
+  return launch_beam_select<float>(p, s.pieces, vec, st);
+}
+
+int ft_beam_reorder(const ft_beam_reorder_args* a) {
+  if (a == nullptr) return fail(FT_ERR_INVALID_ARGUMENT, "args is NULL");
+  if (a->elem_bytes != 4 && a->elem_bytes != 8) return fail(FT_ERR_INVALID_ARGUMENT, "elements of %d bytes, not 4 or 8", a->elem_bytes);
+  if (a->batch < 0 || a->from <= 0 || a->from > FT_MAX_BEAMS || a->to <= 0 || a->to > FT_MAX_BEAMS)
+    return fail(FT_ERR_INVALID_ARGUMENT, "rows of %d and %d beams a request must be 1 to %d", a->from, a->to, FT_MAX_BEAMS);
+  if (a->table_rows < 0 || a->width < 0) return fail(FT_ERR_INVALID_ARGUMENT, "the table's sizes are negative");
+  if (a->batch == 0 || a->table_rows == 0 || a->width == 0) return FT_OK;
+  if (a->table == nullptr || a->rows == nullptr || a->beams == nullptr || a->out_rows == nullptr)
+    return fail(FT_ERR_INVALID_ARGUMENT, "table / rows / beams / out_rows is NULL");
+  if (a->batch > 65535) return fail(FT_ERR_TOO_LARGE, "more than 65535 requests");
+  ft::ReorderParams p;
+  memset(&p, 0, sizeof(p));
+  p.words = a->elem_bytes / 4;
+  p.table = static_cast<uint32_t*>(a->table);
+  p.rows = a->rows, p.beams = a->beams, p.out_rows = a->out_rows, p.starts = a->starts, p.ends = a->ends;
+  p.table_rows = a->table_rows, p.width = a->width * p.words, p.table_s0 = a->table_stride0 * p.words;
+  p.rows_s0 = a->rows_stride0, p.beams_s0 = a->beams_stride0, p.out_rows_s0 = a->out_rows_stride0;
+  p.from = a->from, p.to = a->to;
+  p.rows_64 = a->rows_64, p.beams_64 = a->beams_64, p.out_rows_64 = a->out_rows_64, p.starts_64 = a->starts_64, p.ends_64 = a->ends_64;
+  p.columns = ft::REORDER_WORDS * ft::BEAM_THREADS / a->to;
+  const int64_t chunks = (p.width + p.columns - 1) / p.columns;
+  if (chunks > 0x7fffffffLL) return fail(FT_ERR_TOO_LARGE, "the table's rows are too long for one launch");
+  FT_CUDA_OK(launch_early(ft::beam_reorder_kernel, dim3((unsigned)chunks, (unsigned)a->batch), ft::BEAM_THREADS, 0, static_cast<cudaStream_t>(a->stream), p));
+  count_launch();
+  return FT_OK;
+}
+
+}  // extern "C"

@@ -27,6 +27,11 @@ typedef int (*DecodeFn)(const ft_decode_args*);
 DecodeFn g_entry[3] = {nullptr, nullptr, nullptr};  // ft_decode, ft_stage1, ft_stage2
 int (*g_append)(const ft_append_args*) = nullptr;
 int (*g_extend)(const ft_extend_args*) = nullptr;
+int (*g_draft_tree)(const ft_draft_tree_args*) = nullptr;
+int (*g_draft_accept)(const ft_draft_accept_args*) = nullptr;
+int64_t (*g_beam_workspace)(const ft_beam_select_args*) = nullptr;
+int (*g_beam_select)(const ft_beam_select_args*) = nullptr;
+int (*g_beam_reorder)(const ft_beam_reorder_args*) = nullptr;
 
 struct Refused {};  // a Python error has been set
 
@@ -453,6 +458,190 @@ PyObject* py_extend(PyObject*, PyObject* const* x, Py_ssize_t n) {
   }
 }
 
+// ---- branching continuations (ft_draft_tree, ft_draft_accept, ft_beam_select, ft_beam_reorder)
+
+template <typename Fn>
+PyObject* guarded(Fn fn) {
+  try {
+    return fn();
+  } catch (const Refused&) {
+    return nullptr;
+  } catch (const std::exception& e) {
+    return PyErr_Format(PyExc_RuntimeError, "%s", e.what());
+  }
+}
+
+// a [n] tensor of whole numbers
+const at::Tensor& index_row(const char* name, PyObject* o, const at::Tensor& like, int64_t n) {
+  const at::Tensor& t = indices(name, o, like);
+  if (t.dim() != 1 || t.size(0) != n) refuse("%s has another number of entries than the call's other tensors", name);
+  return t;
+}
+
+// a [rows, columns] tensor of whole numbers
+const at::Tensor& index_rows(const char* name, PyObject* o, const at::Tensor& like) {
+  const at::Tensor& t = indices(name, o, like);
+  if (t.dim() != 2) refuse("%s must have two axes: requests, beams", name);
+  return t;
+}
+
+int is_long(const at::Tensor& t) { return t.scalar_type() == at::kLong; }
+
+void plan_of(PyObject* table_obj, PyObject* info_obj, const at::Tensor& like, ft_extend_plan_info& info, const int32_t*& table_at) {
+  const at::Tensor& plan = on_device_of("the plan", table("the plan", table_obj), like);
+  char* raw = nullptr;
+  Py_ssize_t len = 0;
+  if (PyBytes_AsStringAndSize(info_obj, &raw, &len) != 0) throw Refused();
+  if (len != (Py_ssize_t)sizeof(info)) refuse("%s", "the plan's description has another size than the library's");
+  memcpy(&info, raw, sizeof(info));
+  if (info.table_ints > plan.numel()) refuse("%s", "the plan's table is shorter than its description says");
+  table_at = static_cast<const int32_t*>(plan.data_ptr());
+}
+
+// draft_tree(parents, plan table, plan info, positions | None)
+PyObject* py_draft_tree(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  if (n != 4) return PyErr_Format(PyExc_TypeError, "draft_tree() takes 4 arguments");
+  return guarded([&] {
+    ft_draft_tree_args a;
+    memset(&a, 0, sizeof(a));
+    const at::Tensor& parents = tensor("parents", x[0]);
+    index_row("parents", x[0], parents, parents.dim() == 1 ? parents.size(0) : -1);
+    const int32_t* at = nullptr;
+    plan_of(x[1], x[2], parents, a.plan, at);
+    a.plan_table = const_cast<int32_t*>(at);
+    a.parents = parents.data_ptr(), a.parents_64 = is_long(parents), a.rows = parents.size(0);
+    if (x[3] != Py_None) {
+      const at::Tensor& pos = index_row("positions", x[3], parents, parents.size(0));
+      if (pos.numel() > 0 && pos.data_ptr() == parents.data_ptr()) refuse("%s", "positions must not be parents");
+      a.positions = pos.data_ptr(), a.positions_64 = is_long(pos);
+    }
+    return launch_on(parents, a, g_draft_tree);
+  });
+}
+
+// draft_accept(logits | None, targets | None, tokens, parents, plan table, plan info, accepted, counts, next_tokens, slots | None,
+//              kv_entries | None)
+PyObject* py_draft_accept(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  if (n != 11) return PyErr_Format(PyExc_TypeError, "draft_accept() takes 11 arguments");
+  return guarded([&] {
+    ft_draft_accept_args a;
+    memset(&a, 0, sizeof(a));
+    const at::Tensor& tokens = tensor("tokens", x[2]);
+    const int64_t rows = tokens.dim() == 1 ? tokens.size(0) : -1;
+    index_row("tokens", x[2], tokens, rows);
+    const at::Tensor& parents = index_row("parents", x[3], tokens, rows);
+    if ((x[0] == Py_None) == (x[1] == Py_None)) refuse("%s", "one of logits and targets must be given");
+    if (x[0] != Py_None) {
+      const at::Tensor& logits = on_device_of("logits", tensor("logits", x[0]), tokens);
+      a.dtype = dtype_code(logits.scalar_type());
+      if (logits.dim() != 2 || logits.size(0) != rows) refuse("%s", "logits must be [tokens, vocabulary]");
+      if (logits.size(1) < 1 || logits.size(1) > INT32_MAX) refuse("%s", "the vocabulary must have 1 to 2^31 - 1 entries");
+      if (logits.size(1) > 1 && logits.stride(1) != 1) refuse("%s", "logits must be contiguous along the vocabulary");
+      a.logits = logits.data_ptr(), a.vocab = (int32_t)logits.size(1);
+      a.logits_stride0 = rows > 1 ? logits.stride(0) : 0;
+    } else {
+      const at::Tensor& targets = index_row("targets", x[1], tokens, rows);
+      a.targets = targets.data_ptr(), a.targets_64 = is_long(targets);
+    }
+    plan_of(x[4], x[5], tokens, a.plan, a.plan_table);
+    const at::Tensor& accepted = on_device_of("accepted", tensor("accepted", x[6]), tokens);
+    const at::Tensor& counts = on_device_of("counts", tensor("counts", x[7]), tokens);
+    if (accepted.scalar_type() != at::kInt || accepted.dim() != 2 || (accepted.size(1) > 1 && accepted.stride(1) != 1))
+      refuse("%s", "accepted must be an int32 [requests, tokens] tensor with contiguous rows");
+    const int64_t reqs = accepted.size(0);
+    if (reqs > INT32_MAX || accepted.size(1) > INT32_MAX) refuse("%s", "accepted is too large");
+    if (reqs > 1 && accepted.stride(0) < accepted.size(1)) refuse("%s", "rows of accepted overlap");
+    if (counts.scalar_type() != at::kInt || counts.dim() != 1 || counts.size(0) != reqs || !counts.is_contiguous())
+      refuse("%s", "counts must be a contiguous int32 tensor with one entry per request");
+    const at::Tensor& next = index_row("next_tokens", x[8], tokens, reqs);
+    if ((x[9] == Py_None) != (x[10] == Py_None)) refuse("%s", "slots and kv_entries go together");
+    if (x[9] != Py_None) {
+      const at::Tensor& slots = index_row("slots", x[9], tokens, rows);
+      const at::Tensor& entries = on_device_of("kv_entries", table("kv_entries", x[10]), tokens);
+      a.slots = slots.data_ptr(), a.slots_64 = is_long(slots);
+      a.kv_entries = static_cast<int32_t*>(entries.data_ptr()), a.kv_entries_len = entries.numel();
+    }
+    a.tokens = tokens.data_ptr(), a.tokens_64 = is_long(tokens), a.parents = parents.data_ptr(), a.parents_64 = is_long(parents);
+    a.accepted = static_cast<int32_t*>(accepted.data_ptr()), a.accepted_stride0 = accepted.stride(0), a.accepted_width = (int32_t)accepted.size(1);
+    a.counts = static_cast<int32_t*>(counts.data_ptr()), a.next_tokens = next.data_ptr(), a.next_64 = is_long(next);
+    a.num_requests = (int32_t)reqs, a.rows = rows;
+    return launch_on(tokens, a, g_draft_accept);
+  });
+}
+
+// beam_select(logits, scores, out_scores, out_beams, out_tokens); the workspace is the call's own, from torch's allocator
+PyObject* py_beam_select(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  if (n != 5) return PyErr_Format(PyExc_TypeError, "beam_select() takes 5 arguments");
+  return guarded([&]() -> PyObject* {
+    ft_beam_select_args a;
+    memset(&a, 0, sizeof(a));
+    const at::Tensor& logits = tensor("logits", x[0]);
+    a.dtype = dtype_code(logits.scalar_type());
+    if (logits.dim() != 3) refuse("%s", "logits must be [batch, beams, vocabulary]");
+    if (logits.size(2) > 1 && logits.stride(2) != 1) refuse("%s", "logits must be contiguous along the vocabulary");
+    for (int i = 0; i < 3; ++i)
+      if (logits.size(i) > INT32_MAX) refuse("%s", "logits are too many for one call");
+    const int64_t batch = logits.size(0), beams = logits.size(1);
+    const at::Tensor& scores = on_device_of("scores", tensor("scores", x[1]), logits);
+    if (scores.scalar_type() != at::kFloat || scores.dim() != 2 || scores.size(0) != batch || scores.size(1) != beams)
+      refuse("%s", "scores must be a float32 [batch, beams] tensor");
+    const at::Tensor& out = on_device_of("out_scores", tensor("out_scores", x[2]), logits);
+    if (out.scalar_type() != at::kFloat || out.dim() != 2 || out.size(0) != batch || (out.size(1) > 1 && out.stride(1) != 1))
+      refuse("%s", "out_scores must be a float32 [batch, results] tensor with contiguous rows");
+    const at::Tensor &ob = index_rows("out_beams", x[3], logits), &ot = index_rows("out_tokens", x[4], logits);
+    if (ob.sizes() != out.sizes() || ot.sizes() != out.sizes()) refuse("%s", "out_scores, out_beams and out_tokens differ in shape");
+    if (out.size(1) > INT32_MAX) refuse("%s", "too many results");
+    if (batch > 1 && (out.stride(0) < out.size(1) || ob.stride(0) < out.size(1) || ot.stride(0) < out.size(1)))
+      refuse("%s", "rows of the results overlap");
+    a.logits = logits.data_ptr(), a.scores = static_cast<const float*>(scores.data_ptr());
+    a.out_scores = static_cast<float*>(out.data_ptr()), a.out_beams = ob.data_ptr(), a.out_tokens = ot.data_ptr();
+    a.batch = (int32_t)batch, a.beams = (int32_t)beams, a.vocab = (int32_t)logits.size(2), a.best = (int32_t)out.size(1);
+    a.beams_64 = is_long(ob), a.tokens_64 = is_long(ot);
+    a.logits_stride0 = logits.stride(0), a.logits_stride1 = logits.stride(1);
+    a.scores_stride0 = scores.stride(0), a.scores_stride1 = scores.stride(1);
+    a.out_scores_stride0 = out.stride(0), a.out_beams_stride0 = ob.stride(0), a.out_tokens_stride0 = ot.stride(0);
+    const int64_t bytes = g_beam_workspace(&a);
+    if (bytes < 0) return PyLong_FromLong((long)bytes);
+    const at::Tensor hold = at::empty({bytes}, logits.options().dtype(at::kByte));
+    a.workspace = hold.data_ptr();
+    return launch_on(logits, a, g_beam_select);
+  });
+}
+
+// beam_reorder(table, rows, beams, out_rows | None, starts | None, ends | None)
+PyObject* py_beam_reorder(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  if (n != 6) return PyErr_Format(PyExc_TypeError, "beam_reorder() takes 6 arguments");
+  return guarded([&] {
+    ft_beam_reorder_args a;
+    memset(&a, 0, sizeof(a));
+    const at::Tensor& t = tensor("table", x[0]);
+    if (t.dim() != 2 || (t.size(1) > 1 && t.stride(1) != 1)) refuse("%s", "table must be [rows, width] with contiguous rows");
+    const int64_t bytes = t.element_size();
+    if (bytes != 4 && bytes != 8) refuse("%s", "table must have elements of 4 or 8 bytes");
+    if (t.size(0) > 1 && t.stride(0) < t.size(1)) refuse("%s", "rows of table overlap");
+    const at::Tensor &rows = index_rows("rows", x[1], t), &beams = index_rows("beams", x[2], t);
+    const at::Tensor& out = x[3] != Py_None ? index_rows("out_rows", x[3], t) : rows;
+    const int64_t batch = rows.size(0);
+    if (beams.size(0) != batch || out.size(0) != batch) refuse("%s", "rows, beams and out_rows differ in requests");
+    if (out.size(1) != beams.size(1)) refuse("%s", "beams and out_rows differ in beams");
+    if (batch > INT32_MAX || rows.size(1) > INT32_MAX || beams.size(1) > INT32_MAX) refuse("%s", "too many beams for one call");
+    if (x[4] != Py_None) {
+      const at::Tensor& s = index_row("starts", x[4], t, batch);
+      a.starts = s.data_ptr(), a.starts_64 = is_long(s);
+    }
+    if (x[5] != Py_None) {
+      const at::Tensor& s = index_row("ends", x[5], t, batch);
+      a.ends = s.data_ptr(), a.ends_64 = is_long(s);
+    }
+    a.table = t.data_ptr(), a.rows = rows.data_ptr(), a.beams = beams.data_ptr(), a.out_rows = out.data_ptr();
+    a.elem_bytes = (int32_t)bytes, a.batch = (int32_t)batch, a.from = (int32_t)rows.size(1), a.to = (int32_t)beams.size(1);
+    a.rows_64 = is_long(rows), a.beams_64 = is_long(beams), a.out_rows_64 = is_long(out);
+    a.table_rows = t.size(0), a.width = t.size(1), a.table_stride0 = t.stride(0);
+    a.rows_stride0 = rows.stride(0), a.beams_stride0 = beams.stride(0), a.out_rows_stride0 = out.stride(0);
+    return launch_on(t, a, g_beam_reorder);
+  });
+}
+
 // bind(addresses of ft_decode, ft_stage1, ft_stage2, ft_append, ft_extend, sizes of their argument blocks in the library)
 PyObject* py_bind(PyObject*, PyObject* const* x, Py_ssize_t n) {
   if (n != 8) return PyErr_Format(PyExc_TypeError, "bind() takes 8 arguments");
@@ -466,12 +655,33 @@ PyObject* py_bind(PyObject*, PyObject* const* x, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+// bind_branches(addresses of ft_draft_tree, ft_draft_accept, ft_beam_select_workspace, ft_beam_select, ft_beam_reorder, sizes of the
+// argument blocks of tree, accept, select, reorder in the library)
+PyObject* py_bind_branches(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  if (n != 9) return PyErr_Format(PyExc_TypeError, "bind_branches() takes 9 arguments");
+  if (PyLong_AsLong(x[5]) != (long)sizeof(ft_draft_tree_args) || PyLong_AsLong(x[6]) != (long)sizeof(ft_draft_accept_args) ||
+      PyLong_AsLong(x[7]) != (long)sizeof(ft_beam_select_args) || PyLong_AsLong(x[8]) != (long)sizeof(ft_beam_reorder_args))
+    return PyErr_Format(PyExc_RuntimeError, "the library's argument blocks differ from those this module was built with");
+  g_draft_tree = reinterpret_cast<int (*)(const ft_draft_tree_args*)>(PyLong_AsVoidPtr(x[0]));
+  g_draft_accept = reinterpret_cast<int (*)(const ft_draft_accept_args*)>(PyLong_AsVoidPtr(x[1]));
+  g_beam_workspace = reinterpret_cast<int64_t (*)(const ft_beam_select_args*)>(PyLong_AsVoidPtr(x[2]));
+  g_beam_select = reinterpret_cast<int (*)(const ft_beam_select_args*)>(PyLong_AsVoidPtr(x[3]));
+  g_beam_reorder = reinterpret_cast<int (*)(const ft_beam_reorder_args*)>(PyLong_AsVoidPtr(x[4]));
+  if (PyErr_Occurred()) return nullptr;
+  Py_RETURN_NONE;
+}
+
 PyMethodDef methods[] = {
     {"args", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_args)), METH_FASTCALL, "filled ft_decode_args as bytes"},
     {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_call)), METH_FASTCALL, "check, fill and launch"},
     {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_append)), METH_FASTCALL, "check, fill and launch ft_append"},
     {"extend", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_extend)), METH_FASTCALL, "check, fill and launch ft_extend"},
     {"extend_args", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_extend_args)), METH_FASTCALL, "filled ft_extend_args as bytes"},
+    {"draft_tree", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_draft_tree)), METH_FASTCALL, "check, fill and launch ft_draft_tree"},
+    {"draft_accept", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_draft_accept)), METH_FASTCALL, "check, fill and launch ft_draft_accept"},
+    {"beam_select", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_beam_select)), METH_FASTCALL, "check, fill and launch ft_beam_select"},
+    {"beam_reorder", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_beam_reorder)), METH_FASTCALL, "check, fill and launch ft_beam_reorder"},
+    {"bind_branches", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_bind_branches)), METH_FASTCALL, "addresses of the C ABI"},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_bind)), METH_FASTCALL, "addresses of the C ABI"},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -1,0 +1,314 @@
+// Drafted tokens: their trees into a plan's masks, and which of them the model agrees with.
+//
+// Kernels here and in ft_beam.cuh that write tables let no later launch start early: others read their tables before they wait.
+//
+// A request's drafted tokens are numbered so that a parent comes before its children.  The attention itself is ft_extend's: its
+// kernels read what a row sees from bits of the plan, and ft_draft_tree sets the few words of them that trees decide.
+#pragma once
+
+#include "ft_common.cuh"
+#include "ft_draft_span.cuh"
+
+namespace ft {
+
+struct DraftParams {
+  const int32_t* drafts;  // the plan's requests (ft_extend_plan.cu)
+  const DraftSpan* spans;
+  int32_t* extra;
+  const void* parents;
+  void* positions;
+  int32_t parents_64, positions_64, window, words;  // words: of a token's bits in a tile
+};
+
+struct Draft {
+  int row, n, cached, id, span0, spans;
+  int64_t entries;
+};
+
+__device__ __forceinline__ Draft load_draft(const int32_t* drafts, int i) {
+  const int4 a = __ldg(reinterpret_cast<const int4*>(drafts) + 2 * i), b = __ldg(reinterpret_cast<const int4*>(drafts) + 2 * i + 1);
+  return {a.x, a.y, a.z, b.y, b.z, b.w, (int64_t)(((uint64_t)(uint32_t)b.x << 32) | (uint32_t)a.w)};
+}
+
+__device__ __forceinline__ int64_t load_index(const void* p, int is_64, int64_t i) {
+  return is_64 ? __ldg(static_cast<const long long*>(p) + i) : (int64_t)__ldg(static_cast<const int*>(p) + i);
+}
+
+// The tree of a request into shared memory: parent[i] is -1 (a root), -2 (padding) or an earlier token; what is none of these, and
+// what hangs on padding, becomes padding.  depth: filled if not NULL.  A whole block; ends with a barrier.
+__device__ __forceinline__ void load_tree(const void* parents, int is_64, const Draft& d, int16_t* parent, int16_t* depth) {
+  bool bad = false;
+  for (int i = threadIdx.x; i < d.n; i += blockDim.x) {
+    const int64_t p = load_index(parents, is_64, (int64_t)d.row + i);
+    const bool ok = p >= -2 && p < i;
+    bad |= !ok;
+    parent[i] = (int16_t)(ok ? (int)p : -2);
+  }
+  __syncthreads();
+  // climbs see the parents as they were given, so what hangs on padding is marked afterwards
+  uint32_t lost = 0;
+  for (int i = threadIdx.x, k = 0; i < d.n; i += blockDim.x, ++k) {
+    int at = i, steps = 0;
+    for (int up = parent[at]; up >= 0; up = parent[at]) {
+      at = up;
+      ++steps;
+    }
+    if (at != i && parent[at] == -2) {
+      lost |= 1u << k;
+      steps = 0;
+    }
+    if (depth != nullptr) depth[i] = (int16_t)steps;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x, k = 0; i < d.n; i += blockDim.x, ++k)
+    if ((lost >> k & 1u) != 0) parent[i] = -2;
+  if (bad || lost != 0) flag_error(FT_DEV_BAD_PARENT);
+  __syncthreads();
+}
+
+constexpr int DRAFT_THREADS = 128;
+static_assert(FT_MAX_DRAFT <= 32 * DRAFT_THREADS, "a bit per token that a thread looks at");
+
+// A CTA per request: positions of its tokens, and the words that its tree decides.  Bound by a chain of three reads (request, parents
+// and spans, words) and a climb.  Two stretches of a tile may share a word, in different bits: clearing and setting are
+// atomic, and their order does not matter.
+__global__ void __launch_bounds__(DRAFT_THREADS) draft_tree_kernel(const DraftParams p) {
+  __shared__ int16_t parent[FT_MAX_DRAFT], depth[FT_MAX_DRAFT];
+  const Draft d = load_draft(p.drafts, blockIdx.x);
+  if (d.n == 0) return;
+  load_tree(p.parents, p.parents_64, d, parent, depth);
+  if (p.positions != nullptr)
+    for (int i = threadIdx.x; i < d.n; i += DRAFT_THREADS) {
+      const int64_t at = (int64_t)d.row + i;
+      if (p.positions_64)
+        static_cast<long long*>(p.positions)[at] = d.cached + depth[i];
+      else
+        static_cast<int*>(p.positions)[at] = d.cached + depth[i];
+    }
+  for (int s = threadIdx.x >> 5; s < d.spans; s += DRAFT_THREADS / 32) {
+    const int4* raw = reinterpret_cast<const int4*>(p.spans + d.span0 + s);
+    const int4 a = __ldg(raw), b = __ldg(raw + 1);
+    const DraftSpan span = {a.x, a.y, a.z, a.w, b.x, b.y, 0, 0};
+    for (int k = threadIdx.x & 31; k < span.tokens; k += 32)
+      draft_span_words(span, k, p.window, parent, depth, [&](int word, uint32_t mask, uint32_t bits) {
+        int32_t* at = p.extra + span.bits + k * p.words + word;
+        if (mask == 0xffffffffu) {
+          *at = (int32_t)bits;
+        } else {
+          atomicAnd(at, (int32_t)(~mask | bits));
+          atomicOr(at, (int32_t)bits);
+        }
+      });
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ acceptance
+
+struct AcceptParams {
+  const int32_t* drafts;
+  const void* logits;
+  const void* targets;
+  const void* tokens;
+  const void* parents;
+  int32_t* accepted;
+  int32_t* counts;
+  void* next_tokens;
+  const void* slots;
+  int32_t* kv_entries;
+  int64_t logits_s0, accepted_s0, kv_entries_len;
+  int32_t vocab, width, targets_64, tokens_64, parents_64, next_64, slots_64;
+};
+
+// Whole numbers in the order of floats; -0 and 0 are one, NaN stands below all.
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return x != x ? 0u : (b & 0x80000000u) != 0 ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float from_ordered(uint32_t k) { return __uint_as_float((k & 0x80000000u) != 0 ? k & 0x7fffffffu : ~k); }
+
+// 16 bytes of a row as floats
+template <typename T>
+struct Vec {
+  static constexpr int N = 16 / (int)sizeof(T);
+};
+__device__ __forceinline__ uint4 load_stream(const void* p) {
+  uint4 x;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(p));
+  return x;
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+// the larger of each half; a number and NaN: the number
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b, __half) {
+  const __half2 m = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b, __nv_bfloat16) {
+  const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+// largest of a vector's elements
+template <typename T>
+__device__ __forceinline__ float vec_max(const uint4& v) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  } else {
+    const float2 m = unpack2<T>(max2(max2(v.x, v.y, T()), max2(v.z, v.w, T()), T()));
+    return fmaxf(m.x, m.y);
+  }
+}
+template <typename T>
+__device__ __forceinline__ float vec_at(const uint4& v, int e) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(w[e]);
+  } else {
+    const float2 x = unpack2<T>(w[e >> 1]);
+    return (e & 1) != 0 ? x.y : x.x;
+  }
+}
+
+constexpr int ACCEPT_THREADS = 512;
+
+// Largest logit of one rank's share of a row, as {ordered value, ~index}: a thread's candidates come in rising
+// order, so a larger one only replaces the first of equals.
+template <typename T>
+__device__ __forceinline__ unsigned long long row_argmax(const T* __restrict__ row, int vocab, bool vec, int rank, int ranks) {
+  constexpr int N = Vec<T>::N, U = 4;
+  float best = -INFINITY;
+  uint32_t at = 0xffffffffu;
+  auto take = [&](float x, int i) {
+    if (x > best) {
+      best = x;
+      at = (uint32_t)i;
+    }
+  };
+  if (vec) {
+    const int nv = vocab / N, lo = (int)((int64_t)nv * rank / ranks), hi = (int)((int64_t)nv * (rank + 1) / ranks);
+    for (int v0 = lo + (int)threadIdx.x; v0 < hi; v0 += U * ACCEPT_THREADS) {
+      uint4 x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) x[u] = load_stream(row + (int64_t)min(v0 + u * ACCEPT_THREADS, hi - 1) * N);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (v0 + u * ACCEPT_THREADS < hi && vec_max<T>(x[u]) > best)
+#pragma unroll
+          for (int e = 0; e < N; ++e) take(vec_at<T>(x[u], e), (v0 + u * ACCEPT_THREADS) * N + e);
+      }
+    }
+    if (rank == ranks - 1 && nv * N + (int)threadIdx.x < vocab) take(to_float<T>(row[nv * N + threadIdx.x]), nv * N + (int)threadIdx.x);
+  } else {
+    constexpr int E = 8;
+    const int lo = (int)((int64_t)vocab * rank / ranks), hi = (int)((int64_t)vocab * (rank + 1) / ranks);
+    for (int i0 = lo + (int)threadIdx.x; i0 < hi; i0 += E * ACCEPT_THREADS) {
+      float x[E];
+#pragma unroll
+      for (int u = 0; u < E; ++u) x[u] = to_float<T>(row[min(i0 + u * ACCEPT_THREADS, hi - 1)]);
+#pragma unroll
+      for (int u = 0; u < E; ++u)
+        if (i0 + u * ACCEPT_THREADS < hi) take(x[u], i0 + u * ACCEPT_THREADS);
+    }
+  }
+  // (nothing above -inf: the row's first element will do)
+  return at == 0xffffffffu ? 0xffffffffull - (rank == 0 ? 0u : 1u) : ((unsigned long long)ordered(best) << 32) | (0xffffffffu - at);
+}
+
+__device__ __forceinline__ void cluster_arrive_wait() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+
+// A cluster of CTAs per request walks down its tree: the row of the token it stands at is split among them, each gives its largest
+// logit to all (through the cluster's shared memory, in two sets by turns: a CTA that is ahead writes the next step's), and all
+// go on to the same child.  So only the rows along the path are read: one to a handful of, say, 32.  Each step costs a row's
+// way from memory and the exchange.
+template <typename T>
+__global__ void __launch_bounds__(ACCEPT_THREADS) draft_accept_kernel(const AcceptParams p, const int vec) {
+  __shared__ int16_t parent[FT_MAX_DRAFT];
+  __shared__ int32_t token[FT_MAX_DRAFT];
+  __shared__ int16_t path[FT_MAX_DRAFT];
+  __shared__ unsigned long long from_cta[2][8], from_warp[ACCEPT_THREADS / 32];
+  __shared__ int child_at[3];  // by turns: a step's, the next one's, which is cleared before the step's barrier, and the one before's
+  uint32_t rank, ranks;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+  const Draft d = load_draft(p.drafts, blockIdx.x / ranks);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < d.n; i += ACCEPT_THREADS) {
+    const int64_t t = load_index(p.tokens, p.tokens_64, (int64_t)d.row + i);
+    token[i] = t >= 0 && t <= 0x7fffffff ? (int)t : -1;
+  }
+  if (threadIdx.x < 3) child_at[threadIdx.x] = FT_MAX_DRAFT;
+  load_tree(p.parents, p.parents_64, d, parent, nullptr);
+  if (ranks > 1) cluster_arrive_wait();  // all of them run before any writes to another
+  int count = 0;
+  int64_t next = -1;
+  if (d.n > 0 && parent[0] == -1) {
+    for (int cur = 0; cur < FT_MAX_DRAFT;) {
+      if (threadIdx.x == 0) path[count] = (int16_t)cur;
+      ++count;
+      if (p.targets != nullptr) {
+        next = load_index(p.targets, p.targets_64, (int64_t)d.row + cur);
+      } else {
+        unsigned long long key = row_argmax(static_cast<const T*>(p.logits) + ((int64_t)d.row + cur) * p.logits_s0, p.vocab, vec != 0, (int)rank, (int)ranks);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
+        if (lane == 0) from_warp[warp] = key;
+        __syncthreads();
+        const int set = count & 1;
+        key = from_warp[lane & (ACCEPT_THREADS / 32 - 1)];
+#pragma unroll
+        for (int o = ACCEPT_THREADS / 64; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
+        if (ranks > 1) {
+          if (threadIdx.x < ranks) {
+            uint32_t there;
+            const uint32_t here = (uint32_t)__cvta_generic_to_shared(&from_cta[set][rank]);
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(there) : "r"(here), "r"(threadIdx.x));
+            asm volatile("st.shared::cluster.u64 [%0], %1;\n" ::"r"(there), "l"(key) : "memory");
+          }
+          cluster_arrive_wait();
+          key = 0;
+          for (uint32_t r = 0; r < ranks; ++r) key = max(key, from_cta[set][r]);
+        }
+        next = (int64_t)(0xffffffffu - (uint32_t)key);
+      }
+      // the first child that holds it
+      const int turn = count % 3;
+      int found = FT_MAX_DRAFT;
+      for (int i = cur + 1 + (int)threadIdx.x; i < d.n; i += ACCEPT_THREADS)
+        if (parent[i] == cur && (int64_t)token[i] == next) found = min(found, i);
+      found = __reduce_min_sync(0xffffffffu, found);
+      if (lane == 0 && found < FT_MAX_DRAFT) atomicMin(&child_at[turn], found);
+      if (threadIdx.x == 0) child_at[(count + 1) % 3] = FT_MAX_DRAFT;
+      __syncthreads();
+      cur = child_at[turn];
+    }
+  }
+  if (rank != 0) return;
+  __syncthreads();
+  const int64_t out = d.id;
+  if (threadIdx.x == 0) {
+    p.counts[out] = count;
+    if (p.next_64)
+      static_cast<long long*>(p.next_tokens)[out] = next;
+    else
+      static_cast<int*>(p.next_tokens)[out] = (int)next;
+  }
+  for (int i = threadIdx.x; i < p.width; i += ACCEPT_THREADS) p.accepted[out * p.accepted_s0 + i] = i < count ? path[i] : -1;
+  if (p.slots == nullptr) return;
+  // the path's rows first, then the others', each in order: the path rises
+  for (int i = threadIdx.x; i < d.n; i += ACCEPT_THREADS) {
+    int before = 0;
+    while (before < count && path[before] < i) ++before;
+    const int to = before < count && path[before] == i ? before : count + i - before;
+    const int64_t entry = d.entries + d.cached + to;
+    if (entry < p.kv_entries_len) p.kv_entries[entry] = (int32_t)load_index(p.slots, p.slots_64, (int64_t)d.row + i);
+  }
+}
+
+}  // namespace ft

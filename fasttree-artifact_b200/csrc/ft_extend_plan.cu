@@ -24,6 +24,14 @@
 //   their offsets (low, high each) in the extra table; per query tile of the block -1 if each of its tokens sees the whole tile of
 //   tile_tokens, else the place of the bits of those that the block's tokens see, a word per 32 and token; 0, 0.
 // Token (2): row of q, position.  Merged token (4): row of q, first entry of its list of partial rows, entries, 0.
+//
+// Plans of drafted tokens (a tree per request, whose parents only the device knows) are made for every tree of their sizes: a
+// token may see any drafted token before it and, behind a window, any cached one that depth 0 would show it, and tiles where that
+// differs from tree to tree have bits for ft_draft_tree to fill in.  Until then the tokens are chains.
+// Draft (8), one per request with tokens: first row of q, tokens, cached tokens, start of its entries of the row-id table (low, high),
+// its number, its first span, spans.  Span (8), a stretch of a tile that some tokens of one request see differently from tree to
+// tree: place of the first token's bits in the extra table, tokens, the first one's number among the request's, first and last bit,
+// position of the first bit less the cached tokens, 0, 0.
 #include <algorithm>
 #include <climits>
 #include <cstdint>
@@ -34,6 +42,7 @@
 #include <vector>
 
 #include "fasttree_b200.h"
+#include "ft_draft_span.cuh"
 
 struct ft_extend_plan {
   std::vector<int32_t> table;
@@ -50,7 +59,7 @@ struct Segment {
 };
 
 struct Token {
-  int32_t q_row, pos;
+  int32_t q_row, pos, cached, req;
 };
 
 struct Block {
@@ -73,12 +82,28 @@ struct Costs {  // microseconds, B200: per K/V tile of two query tiles, of one i
 
 struct Problem {
   const int64_t *seq, *ext, *start, *qstart, *shared;
+  const int32_t* ids;  // of drafts: the requests' numbers
   int batch, group, kv_heads, head_dim, rows, tile;
   int64_t window;
+  bool draft;
   bool two_tiles, streams;
   int tokens_per_tile;
   int slots;
   Costs cost;
+};
+
+// The positions that a token may see, and those that it sees whatever its request's tree is.
+struct Sight {
+  int64_t from, to, sure_from, sure_to;
+  Sight(const Problem& p, const Token& t) {
+    to = t.pos + 1;
+    sure_to = p.draft ? t.cached : to;
+    from = sure_from = 0;
+    if (p.window > 0) {
+      from = std::max<int64_t>((p.draft ? t.cached : t.pos) - p.window + 1, 0);
+      sure_from = std::max<int64_t>(t.pos - p.window + 1, 0);
+    }
+  }
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -113,7 +138,7 @@ class Builder {
     for (int i = 0; i < p_.batch; ++i) {
       first_tok_[i] = (int)tokens.size();
       for (int64_t t = 0; t < p_.ext[i]; ++t) {
-        tokens.push_back({(int32_t)(p_.qstart[i] + t), (int32_t)(prefix(i) + t)});
+        tokens.push_back({(int32_t)(p_.qstart[i] + t), (int32_t)(prefix(i) + t), (int32_t)prefix(i), i});
         req_of_.push_back(i);
       }
     }
@@ -207,10 +232,10 @@ class Builder {
     const std::pair<int, int> tk = toks(b, lo, hi);
     if (tk.first >= tk.second) return;
     int64_t first = INT64_MAX, common = INT64_MAX;
-    for (int t = tk.first; t < tk.second; ++t) first = std::min<int64_t>(first, tokens[t].pos);
+    for (int t = tk.first; t < tk.second; ++t) first = std::min(first, Sight(p_, tokens[t]).from);
     if (lo == hi) common = tokens[tk.second - 1].pos + 1;
     for (int k = lo + 1; k <= hi; ++k) common = std::min(common, p_.shared[k]);
-    const int64_t begin = std::max(depth, p_.window > 0 ? first - p_.window + 1 : 0);
+    const int64_t begin = std::max(depth, first);
     if (begin < common) {
       segs.push_back({p_.start[lo] + begin, (int32_t)(common - begin), (int32_t)begin, tk.first - b.tok0, tk.second - b.tok0, b.len});
       b.len += (int32_t)(common - begin);
@@ -236,9 +261,9 @@ class Builder {
         if (lo >= hi) continue;
         int64_t from = INT64_MAX, to = 0;
         for (int t = lo; t < hi; ++t) {
-          const int64_t pos = tokens[b.tok0 + t].pos;
-          from = std::min(from, p_.window > 0 ? pos - p_.window + 1 : 0);
-          to = std::max(to, pos + 1);
+          const Sight see(p_, tokens[b.tok0 + t]);
+          from = std::min(from, see.from);
+          to = std::max(to, see.to);
         }
         from = std::max<int64_t>(from - g.pos0, 0);
         to = std::min<int64_t>(to - g.pos0, g.len);
@@ -454,6 +479,29 @@ void memory_bound_costs(Problem& p, int elem_bytes, int num_sms) {
   p.cost.load = std::max(p.cost.load, share - 2 * p.cost.pair);
 }
 
+// The stretches of the tile [v0, v1) of a block that tokens of a request see differently from tree to tree.
+void add_spans(const Problem& p, const Builder& b, const Block& blk, int sg, int v0, int v1, int bits_at,
+               std::vector<std::vector<DraftSpan>>& spans_of) {
+  const int words = p.tile / 32;
+  for (int s = sg; s < blk.seg0 + blk.nseg && b.segs[s].voff < v1; ++s) {
+    const Segment& g = b.segs[s];
+    const int lo = std::max(v0, (int)g.voff), hi = std::min(v1, g.voff + g.len);
+    const int64_t pos_lo = g.pos0 + (lo - g.voff), pos_hi = g.pos0 + (hi - g.voff);
+    for (int t = g.tok_lo; t < g.tok_hi;) {
+      const Token& first = b.tokens[blk.tok0 + t];
+      int e = t;
+      bool differs = false;
+      for (; e < g.tok_hi && b.tokens[blk.tok0 + e].req == first.req; ++e) {
+        const Sight see(p, b.tokens[blk.tok0 + e]);
+        differs |= std::max(pos_lo, see.from) < std::min(pos_hi, see.to) && (pos_lo < see.sure_from || pos_hi > see.sure_to);
+      }
+      if (differs && lo < hi)
+        spans_of[first.req].push_back({bits_at + t * words, e - t, first.pos - first.cached, lo - v0, hi - v0, (int32_t)(pos_lo - first.cached), 0, 0});
+      t = e;
+    }
+  }
+}
+
 void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
   ft_extend_plan_info& info = out->info;
   std::vector<int32_t>& t = out->table;
@@ -472,15 +520,21 @@ void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
   // records of the blocks' tiles
   std::vector<int32_t> tiles, extra, tile0(b.blocks.size(), 0);
   const int words = p.tile / 32;
+  std::vector<std::vector<DraftSpan>> spans_of(p.draft ? p.batch : 0);  // per request
   info.kv_entries_len = 0;
   for (size_t k = 0; k < b.blocks.size(); ++k) {
     const Block& blk = b.blocks[k];
     tile0[k] = (int32_t)(tiles.size() / 8);
-    // what token t of the block sees of segment g, as virtual positions
+    // what token t of the block may see of segment g, and what it surely does, as virtual positions
     auto sight = [&](const Segment& g, int t, int64_t& from, int64_t& to) {
-      const int64_t pos = b.tokens[blk.tok0 + t].pos;
-      from = g.voff + std::max<int64_t>(p.window > 0 ? pos - p.window + 1 - g.pos0 : 0, 0);
-      to = g.voff + std::min<int64_t>(g.len, pos + 1 - g.pos0);
+      const Sight see(p, b.tokens[blk.tok0 + t]);
+      from = g.voff + std::max<int64_t>(see.from - g.pos0, 0);
+      to = g.voff + std::min<int64_t>(g.len, see.to - g.pos0);
+    };
+    auto sure = [&](const Segment& g, int t, int64_t& from, int64_t& to) {
+      const Sight see(p, b.tokens[blk.tok0 + t]);
+      from = g.voff + std::max<int64_t>(see.sure_from - g.pos0, 0);
+      to = g.voff + std::min<int64_t>(g.len, see.sure_to - g.pos0);
     };
     int sg = blk.seg0, sg_known = -1;
     int64_t all_lo[2] = {0, 0}, all_hi[2] = {0, 0};  // what all tokens of query tile w see of segment sg
@@ -508,7 +562,7 @@ void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
           all_hi[w] = g.tok_lo <= lo && g.tok_hi >= hi ? INT64_MAX : 0;
           for (int t = lo; t < hi && all_hi[w] > 0; ++t) {
             int64_t from, to;
-            sight(g, t, from, to);
+            sure(g, t, from, to);
             all_lo[w] = std::max(all_lo[w], from);
             all_hi[w] = std::min(all_hi[w], to);
           }
@@ -531,11 +585,15 @@ void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
         }
         x[4 + w] = bits_at;
       }
+      if (p.draft && bits_at >= 0) add_spans(p, b, blk, sg, v0, v1, bits_at, spans_of);
       tiles.insert(tiles.end(), x, x + 8);
       if (extra.size() > (size_t)INT32_MAX / 2) throw std::bad_alloc();
     }
   }
   for (const Segment& g : b.segs) info.kv_entries_len = std::max(info.kv_entries_len, g.kv_off + g.len);
+  if (p.draft)  // (a window may hide all but the newest entries, which ft_draft_accept writes)
+    for (int i = 0; i < p.batch; ++i)
+      if (p.ext[i] > 0) info.kv_entries_len = std::max(info.kv_entries_len, p.start[i] + p.seq[i]);
   info.items_off = 0;
   for (const Item& it : b.items) {
     const Block& blk = b.blocks[it.block];
@@ -572,6 +630,21 @@ void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
       ++q_tile;
     }
     t.insert(t.end(), x, x + ITEM_INTS);
+  }
+  if (p.draft) {  // until the trees are known
+    std::vector<int16_t> chain, depth;
+    for (int i = 0; i < p.batch; ++i) {
+      while ((int64_t)chain.size() < p.ext[i]) {
+        chain.push_back((int16_t)chain.size() - 1);
+        depth.push_back((int16_t)depth.size());
+      }
+      for (const DraftSpan& s : spans_of[i])
+        for (int k = 0; k < s.tokens; ++k)
+          draft_span_words(s, k, (int)p.window, chain.data(), depth.data(), [&](int word, uint32_t mask, uint32_t bits) {
+            int32_t& x = extra[(size_t)s.bits + k * words + word];
+            x = (int32_t)(((uint32_t)x & ~mask) | bits);
+          });
+    }
   }
   align();
   info.tokens_off = (int64_t)t.size();
@@ -616,6 +689,24 @@ void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
   info.merge_rows_off = (int64_t)t.size();
   t.insert(t.end(), lists.begin(), lists.end());
   align();
+  if (p.draft) {
+    info.draft = 1;
+    std::vector<DraftSpan> spans;
+    info.drafts_off = (int64_t)t.size();
+    for (int i = 0; i < p.batch; ++i) {
+      const int32_t x[8] = {(int32_t)p.qstart[i], (int32_t)p.ext[i], (int32_t)(p.seq[i] - p.ext[i]), (int32_t)(uint32_t)(p.start[i] & 0xffffffffll),
+                            (int32_t)(p.start[i] >> 32), p.ids[i], (int32_t)spans.size(), (int32_t)spans_of[i].size()};
+      t.insert(t.end(), x, x + 8);
+      spans.insert(spans.end(), spans_of[i].begin(), spans_of[i].end());
+      info.longest_draft = std::max(info.longest_draft, (int32_t)p.ext[i]);
+    }
+    info.num_drafts = p.batch;
+    info.num_spans = (int32_t)spans.size();
+    info.spans_off = (int64_t)t.size();
+    static_assert(sizeof(DraftSpan) == 8 * sizeof(int32_t), "a span is eight ints of the table");
+    const int32_t* raw = reinterpret_cast<const int32_t*>(spans.data());
+    t.insert(t.end(), raw, raw + 8 * spans.size());
+  }
   info.table_ints = (int64_t)t.size();
   info.num_items = (int32_t)b.items.size();
   info.num_tiles = (int32_t)(tiles.size() / 8);
@@ -625,13 +716,9 @@ void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
   info.num_sms = p.slots;
 }
 
-}  // namespace
-
-extern "C" {
-
-int ft_extend_plan_build(const int64_t* seq_lens, const int64_t* extend_lens, const int64_t* kv_starts, const int64_t* q_starts,
-                         const int64_t* shared_with_previous, int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
-                         int32_t head_dim, int32_t elem_bytes, int64_t window, int32_t num_sms, ft_extend_plan** out) {
+int build(const int64_t* seq_lens, const int64_t* extend_lens, const int64_t* kv_starts, const int64_t* q_starts,
+          const int64_t* shared_with_previous, const int32_t* draft_ids, int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
+          int32_t head_dim, int32_t elem_bytes, int64_t window, int32_t num_sms, ft_extend_plan** out) {
   if (out == nullptr) return FT_ERR_INVALID_ARGUMENT;
   *out = nullptr;
   if (batch < 0 || num_qo_heads <= 0 || num_kv_heads <= 0 || num_qo_heads % num_kv_heads != 0 || num_sms <= 0 || window < 0 ||
@@ -648,6 +735,8 @@ int ft_extend_plan_build(const int64_t* seq_lens, const int64_t* extend_lens, co
       return FT_ERR_INVALID_ARGUMENT;
     if (seq_lens[i] > INT32_MAX / 2 || q_starts[i] > INT32_MAX / 2 || q_starts[i] + extend_lens[i] > INT32_MAX / 2 || kv_starts[i] > INT64_MAX / 2)
       return FT_ERR_TOO_LARGE;
+    if (draft_ids != nullptr && (draft_ids[i] < 0 || draft_ids[i] >= batch)) return FT_ERR_INVALID_ARGUMENT;
+    if (draft_ids != nullptr && extend_lens[i] > FT_MAX_DRAFT) return FT_ERR_TOO_LARGE;
     total += extend_lens[i];
     most = std::max(most, seq_lens[i]);
   }
@@ -662,6 +751,8 @@ int ft_extend_plan_build(const int64_t* seq_lens, const int64_t* extend_lens, co
       if (q_rows[i].first < q_rows[i - 1].second) return FT_ERR_INVALID_ARGUMENT;
     Problem p;
     p.seq = seq_lens, p.ext = extend_lens, p.start = kv_starts, p.qstart = q_starts, p.shared = shared_with_previous;
+    p.draft = draft_ids != nullptr;
+    p.ids = draft_ids;
     p.batch = batch;
     p.group = num_qo_heads / num_kv_heads;
     p.kv_heads = num_kv_heads;
@@ -726,6 +817,27 @@ int ft_extend_plan_build(const int64_t* seq_lens, const int64_t* extend_lens, co
     return FT_ERR_INVALID_ARGUMENT;
   }
   return FT_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ft_extend_plan_build(const int64_t* seq_lens, const int64_t* extend_lens, const int64_t* kv_starts, const int64_t* q_starts,
+                         const int64_t* shared_with_previous, int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
+                         int32_t head_dim, int32_t elem_bytes, int64_t window, int32_t num_sms, ft_extend_plan** out) {
+  return build(seq_lens, extend_lens, kv_starts, q_starts, shared_with_previous, nullptr, batch, num_qo_heads, num_kv_heads, head_dim,
+               elem_bytes, window, num_sms, out);
+}
+
+int ft_draft_plan_build(const int64_t* seq_lens, const int64_t* draft_lens, const int64_t* kv_starts, const int64_t* q_starts,
+                        const int64_t* shared_with_previous, const int32_t* request_ids, int32_t batch, int32_t num_qo_heads,
+                        int32_t num_kv_heads, int32_t head_dim, int32_t elem_bytes, int64_t window, int32_t num_sms, ft_extend_plan** out) {
+  static const int32_t none = 0;
+  if (out != nullptr) *out = nullptr;
+  if (batch > 0 && request_ids == nullptr) return FT_ERR_INVALID_ARGUMENT;
+  return build(seq_lens, draft_lens, kv_starts, q_starts, shared_with_previous, batch > 0 ? request_ids : &none, batch, num_qo_heads,
+               num_kv_heads, head_dim, elem_bytes, window, num_sms, out);
 }
 
 int ft_extend_plan_get_info(const ft_extend_plan* plan, ft_extend_plan_info* info) {

@@ -96,7 +96,7 @@ def _order_by_prefix(n, cached, shared_prefixes):
 
 
 def host_plan(seq_lens, extend_lens, kv_starts, num_qo_heads, num_kv_heads, head_dim, dtype, shared_prefixes=None, window=0,
-              num_sms=148):
+              num_sms=148, draft=False):
     """Host half of :func:`prepare`: ``(info, numpy int32 table, seq_lens, extend_lens)``."""
     seq = _ints("seq_lens", seq_lens)
     n = seq.size
@@ -116,9 +116,15 @@ def host_plan(seq_lens, extend_lens, kv_starts, num_qo_heads, num_kv_heads, head
     arrays = [np.ascontiguousarray(a[order]) if n else a for a in (seq, ext, start, q_start)] + [shared]
     lib = _lib.load()
     i64p, handle = ctypes.POINTER(ctypes.c_int64), ctypes.c_void_p()
-    rc = lib.ft_extend_plan_build(*(a.ctypes.data_as(i64p) for a in arrays), n, int(num_qo_heads), int(num_kv_heads), int(head_dim),
-                                  4 if dtype == torch.float32 else 2, min(int(window), 2 ** 31 - 1), int(num_sms),
-                                  ctypes.byref(handle))
+    sizes = (n, int(num_qo_heads), int(num_kv_heads), int(head_dim), 4 if dtype == torch.float32 else 2, min(int(window), 2 ** 31 - 1),
+             int(num_sms), ctypes.byref(handle))
+    if draft:
+        if n and ext.max() > _lib.FT_MAX_DRAFT:
+            raise ValueError(f"a request has {int(ext.max())} drafted tokens, more than {_lib.FT_MAX_DRAFT}")
+        ids = np.asarray(order, dtype=np.int32)
+        rc = lib.ft_draft_plan_build(*(a.ctypes.data_as(i64p) for a in arrays), ids.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)), *sizes)
+    else:
+        rc = lib.ft_extend_plan_build(*(a.ctypes.data_as(i64p) for a in arrays), *sizes)
     if rc != 0:
         raise _lib.FastTreeError(rc, "ft_extend_plan_build refused the step: head_dim must be one of 16, 32, 64, 128, 256 and the "
                                      "step's tables must fit 32-bit fields")
@@ -133,7 +139,7 @@ def host_plan(seq_lens, extend_lens, kv_starts, num_qo_heads, num_kv_heads, head
 
 
 def prepare(seq_lens, extend_lens, kv_starts, num_qo_heads, num_kv_heads, head_dim, dtype, shared_prefixes=None, window=0,
-            device="cuda"):
+            device="cuda", draft=False):
     """Plan a step's extend attention; the plan serves every layer of the step.
 
     Request r has ``seq_lens[r]`` tokens in the cache, the last ``extend_lens[r]`` of them the step's new ones, whose
@@ -142,13 +148,19 @@ def prepare(seq_lens, extend_lens, kv_starts, num_qo_heads, num_kv_heads, head_d
     length)`` - these requests' first ``length`` cached tokens are the same pool rows, and their attention reads them once;
     nested pairs describe a tree (:func:`tree_prefixes`).  ``window`` > 0: a token sees the newest ``window`` positions up
     to its own.  Integers on the host; one copy to ``device``, for which the host waits.  Steps of single tokens without window
-    and cap are ``fasttree_decode``'s: it takes them faster and without a plan per step."""
+    and cap are ``fasttree_decode``'s: it takes them faster and without a plan per step.
+
+    ``draft``: a request's new tokens are the nodes of a tree (at most 1024, parents first), not a chain: a token sees the cached
+    tokens, its ancestors and itself; with a window those of the newest ``window`` positions up to its own, which is cached + depth.
+    The plan goes by the sizes; the trees, which may live on the device alone, are given to :func:`ft_b200.branch.draft_tree` before
+    the step's first :func:`extend` (until then tokens are chains).  That changes the plan's table, so such a plan belongs to one
+    stream, or the caller orders what uses it."""
     dev = torch.device(device)
     if dev.type != "cuda":
         raise ValueError("the plan is uploaded to a CUDA device; the engine has no CPU path")
     sms = torch.cuda.get_device_properties(dev).multi_processor_count
     info, table, seq, ext = host_plan(seq_lens, extend_lens, kv_starts, num_qo_heads, num_kv_heads, head_dim, dtype,
-                                      shared_prefixes, window, sms)
+                                      shared_prefixes, window, sms, draft)
     return ExtendPlan(info, torch.from_numpy(table).to(dev), seq, ext)
 
 

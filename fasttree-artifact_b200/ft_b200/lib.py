@@ -18,6 +18,9 @@ PATHS = {"auto": FT_PATH_AUTO, "generic": FT_PATH_GENERIC, "mma": FT_PATH_MMA, "
 FT_STATIC_SCRATCH_BYTES = 16 << 20      # capacity of the array behind ft_decode_static_scratch
 
 FT_DEV_BAD_KV_INDEX, FT_DEV_BAD_Q_INDEX, FT_DEV_BAD_ROW_INDEX, FT_DEV_WAIT_TIMEOUT, FT_DEV_BAD_POSITION = 1, 2, 4, 8, 16
+FT_DEV_BAD_PARENT = 32
+
+FT_MAX_DRAFT, FT_MAX_BEAMS = 1024, 64
 
 EXPORTS = ["ft_version", "ft_decode_args_size", "ft_last_error", "ft_decode", "ft_stage1", "ft_stage2",
            "ft_decode_static_scratch", "ft_decode_host_io", "ft_selftest_bounded_wait", "ft_read_wait_diagnostics", "ft_bump_kv_lens",
@@ -27,7 +30,9 @@ EXPORTS = ["ft_version", "ft_decode_args_size", "ft_last_error", "ft_decode", "f
            "ft_plan_copy_aux_segments",
            "ft_plan_free",
            "ft_append_args_size", "ft_append", "ft_extend_plan_build", "ft_extend_plan_get_info", "ft_extend_plan_copy",
-           "ft_extend_plan_free", "ft_extend_args_size", "ft_extend", "ft_extend_path_name", "ft_selftest_extend_wait"]
+           "ft_extend_plan_free", "ft_extend_args_size", "ft_extend", "ft_extend_path_name", "ft_selftest_extend_wait",
+           "ft_draft_plan_build", "ft_draft_tree_args_size", "ft_draft_tree", "ft_draft_accept_args_size", "ft_draft_accept",
+           "ft_beam_select_args_size", "ft_beam_select_workspace", "ft_beam_select", "ft_beam_reorder_args_size", "ft_beam_reorder"]
 
 EXTEND_PATHS = {"auto": 0, "generic": 1, "tcgen05": 2}
 
@@ -113,7 +118,9 @@ class ExtendPlanInfo(ctypes.Structure):
                                               "merge_off", "merge_rows_off", "kv_entries_len", "q_rows")] + [
         (n, ctypes.c_int32) for n in ("num_items", "num_tiles", "num_tokens", "num_merged", "partial_rows", "num_sms",
                                       "num_qo_heads", "num_kv_heads", "head_dim", "window", "elem_bytes", "rows_per_tile",
-                                      "tile_tokens", "reserved")]
+                                      "tile_tokens", "reserved")] + [
+        (n, ctypes.c_int64) for n in ("drafts_off", "spans_off")] + [
+        (n, ctypes.c_int32) for n in ("draft", "num_drafts", "num_spans", "longest_draft")]
 
 
 class ExtendArgs(ctypes.Structure):
@@ -125,6 +132,40 @@ class ExtendArgs(ctypes.Structure):
                                       "v_stride1", "o_stride0", "o_stride1")] + [
         ("kv_entries", ctypes.c_void_p), ("kv_entries_len", ctypes.c_int64), ("plan_table", ctypes.c_void_p),
         ("plan", ExtendPlanInfo), ("mid_o", ctypes.c_void_p), ("mid_lse", ctypes.c_void_p), ("stream", ctypes.c_void_p)]
+
+
+class DraftTreeArgs(ctypes.Structure):
+    """Mirror of ``struct ft_draft_tree_args``."""
+    _fields_ = [("parents", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("parents_64", ctypes.c_int32),
+                ("positions_64", ctypes.c_int32), ("rows", ctypes.c_int64), ("plan_table", ctypes.c_void_p),
+                ("plan", ExtendPlanInfo), ("stream", ctypes.c_void_p)]
+
+
+class DraftAcceptArgs(ctypes.Structure):
+    """Mirror of ``struct ft_draft_accept_args``."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("logits", "targets", "tokens", "parents", "accepted", "counts", "next_tokens", "slots",
+                                               "kv_entries")] + [
+        (n, ctypes.c_int32) for n in ("dtype", "vocab", "targets_64", "tokens_64", "parents_64", "next_64", "slots_64", "num_requests",
+                                      "accepted_width", "reserved")] + [
+        (n, ctypes.c_int64) for n in ("rows", "logits_stride0", "accepted_stride0", "kv_entries_len")] + [
+        ("plan_table", ctypes.c_void_p), ("plan", ExtendPlanInfo), ("stream", ctypes.c_void_p)]
+
+
+class BeamSelectArgs(ctypes.Structure):
+    """Mirror of ``struct ft_beam_select_args``."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("logits", "scores", "out_scores", "out_beams", "out_tokens", "workspace")] + [
+        (n, ctypes.c_int32) for n in ("dtype", "batch", "beams", "vocab", "best", "beams_64", "tokens_64", "reserved")] + [
+        (n, ctypes.c_int64) for n in ("logits_stride0", "logits_stride1", "scores_stride0", "scores_stride1", "out_scores_stride0",
+                                      "out_beams_stride0", "out_tokens_stride0")] + [("stream", ctypes.c_void_p)]
+
+
+class BeamReorderArgs(ctypes.Structure):
+    """Mirror of ``struct ft_beam_reorder_args``."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("table", "rows", "beams", "out_rows", "starts", "ends")] + [
+        (n, ctypes.c_int32) for n in ("elem_bytes", "batch", "from_", "to", "rows_64", "beams_64", "out_rows_64", "starts_64", "ends_64",
+                                      "reserved")] + [
+        (n, ctypes.c_int64) for n in ("table_rows", "width", "table_stride0", "rows_stride0", "beams_stride0", "out_rows_stride0")] + [
+        ("stream", ctypes.c_void_p)]
 
 
 _lock = threading.Lock()
@@ -226,6 +267,18 @@ def load():
         lib.ft_extend_plan_copy.restype = ctypes.c_int
         lib.ft_extend_plan_free.argtypes = [ctypes.c_void_p]
         lib.ft_extend_plan_free.restype = None
+        lib.ft_draft_plan_build.argtypes = [i64p] * 5 + [i32p] + [i32] * 5 + [i64, i32, ctypes.POINTER(ctypes.c_void_p)]
+        lib.ft_draft_plan_build.restype = ctypes.c_int
+        for name, struct in (("ft_draft_tree", DraftTreeArgs), ("ft_draft_accept", DraftAcceptArgs), ("ft_beam_select", BeamSelectArgs),
+                             ("ft_beam_reorder", BeamReorderArgs)):
+            size = getattr(lib, name + "_args_size")()
+            if size != ctypes.sizeof(struct):
+                raise FastTreeError(-1, "%s of the library (%d bytes) differs from the binding (%d)"
+                                    % (struct.__name__, size, ctypes.sizeof(struct)))
+            getattr(lib, name).argtypes = [ctypes.POINTER(struct)]
+            getattr(lib, name).restype = ctypes.c_int
+        lib.ft_beam_select_workspace.argtypes = [ctypes.POINTER(BeamSelectArgs)]
+        lib.ft_beam_select_workspace.restype = ctypes.c_int64
         _lib = lib
     return _lib
 
@@ -253,6 +306,10 @@ def call_module():
             mod.bind(*(ctypes.cast(getattr(handle, n), ctypes.c_void_p).value
                        for n in ("ft_decode", "ft_stage1", "ft_stage2", "ft_append", "ft_extend")),
                      handle.ft_decode_args_size(), handle.ft_append_args_size(), handle.ft_extend_args_size())
+            branches = ("ft_draft_tree", "ft_draft_accept", "ft_beam_select", "ft_beam_reorder")
+            mod.bind_branches(*(ctypes.cast(getattr(handle, n), ctypes.c_void_p).value
+                                for n in ("ft_draft_tree", "ft_draft_accept", "ft_beam_select_workspace", "ft_beam_select", "ft_beam_reorder")),
+                              *(getattr(handle, n + "_args_size")() for n in branches))
             _call = mod
     return _call
 

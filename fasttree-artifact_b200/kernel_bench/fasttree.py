@@ -18,6 +18,7 @@ _PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 if _PKG not in sys.path:
     sys.path.insert(0, _PKG)
 
+from ft_b200 import branch as _branch      # noqa: E402
 from ft_b200 import engine as _engine      # noqa: E402
 from ft_b200 import extend as _extend      # noqa: E402
 from ft_b200 import planner as _planner    # noqa: E402
@@ -175,10 +176,11 @@ def fasttree_append(q, k, v, k_buffer, v_buffer, slots, q_out=None, positions=No
 
 
 def fasttree_extend_preparation(seq_lens, extend_lens, kv_starts, num_qo_heads, num_kv_heads, head_dim, dtype,
-                                shared_prefixes=None, window=0, device="cuda"):
-    """Plan for :func:`fasttree_extend`, one per step, for every layer (:func:`ft_b200.extend.prepare`)."""
+                                shared_prefixes=None, window=0, device="cuda", draft=False):
+    """Plan for :func:`fasttree_extend`, one per step, for every layer (:func:`ft_b200.extend.prepare`).  ``draft``: the new tokens
+    are trees of drafted ones, which :func:`fasttree_draft_tree` gives to the plan."""
     return _extend.prepare(seq_lens, extend_lens, kv_starts, num_qo_heads, num_kv_heads, head_dim, dtype,
-                           shared_prefixes=shared_prefixes, window=window, device=device)
+                           shared_prefixes=shared_prefixes, window=window, device=device, draft=draft)
 
 
 def fasttree_extend(q, k_buffer, v_buffer, o, kv_entries, plan, sm_scale, logit_cap=-1, o_lse=None):
@@ -186,3 +188,24 @@ def fasttree_extend(q, k_buffer, v_buffer, o, kv_entries, plan, sm_scale, logit_
     hides old positions (else :func:`fasttree_decode` is faster) - over the paged cache; writes ``o`` on the current CUDA stream
     (:func:`ft_b200.extend.extend`).  Here ``logit_cap`` is applied."""
     _extend.extend(q, k_buffer, v_buffer, o, kv_entries, plan, sm_scale, logit_cap=logit_cap, o_lse=o_lse)
+
+
+def fasttree_draft_tree(parents, plan, positions=None):
+    """The trees of a step's drafted tokens enter a plan made with ``draft=True``; their positions come out
+    (:func:`ft_b200.branch.draft_tree`).  No counterpart in the reference."""
+    _branch.draft_tree(parents, plan, positions=positions)
+
+
+def fasttree_draft_accept(logits, tokens, parents, plan, accepted, counts, next_tokens, slots=None, kv_entries=None, targets=None):
+    """The drafted tokens that the model agrees with, and their rows first in the row table (:func:`ft_b200.branch.draft_accept`)."""
+    _branch.draft_accept(logits, tokens, parents, plan, accepted, counts, next_tokens, slots=slots, kv_entries=kv_entries, targets=targets)
+
+
+def fasttree_beam_select(logits, scores, out_scores, out_beams, out_tokens):
+    """The best continuations of each request's beams (:func:`ft_b200.branch.beam_select`)."""
+    _branch.beam_select(logits, scores, out_scores, out_beams, out_tokens)
+
+
+def fasttree_beam_reorder(table, rows, beams, starts=None, ends=None, out_rows=None):
+    """Rows of a table follow the beams (:func:`ft_b200.branch.beam_reorder`)."""
+    _branch.beam_reorder(table, rows, beams, starts=starts, ends=ends, out_rows=out_rows)

@@ -57,7 +57,8 @@ enum ft_device_flag {
   FT_DEV_BAD_Q_INDEX = 2,   /* a request id was outside [0, batch) */
   FT_DEV_BAD_ROW_INDEX = 4, /* a partial-row id was outside [0, num_partial_rows) */
   FT_DEV_WAIT_TIMEOUT = 8,  /* a bounded barrier wait gave up */
-  FT_DEV_BAD_POSITION = 16  /* ft_append: a position was outside the cosine / sine table */
+  FT_DEV_BAD_POSITION = 16, /* ft_append: a position was outside the cosine / sine table */
+  FT_DEV_BAD_PARENT = 32    /* drafted tokens: a parent is neither -1, -2 nor an earlier token of the request's tree */
 };
 
 /*
@@ -425,6 +426,9 @@ typedef struct ft_extend_plan_info {
   int32_t num_qo_heads, num_kv_heads, head_dim, window, elem_bytes;
   int32_t rows_per_tile, tile_tokens; /* query rows (tokens x GQA group) of a query tile, tokens of a K/V tile */
   int32_t reserved;
+  int64_t drafts_off, spans_off; /* plans of ft_draft_plan_build: their requests, and what their trees decide */
+  int32_t draft;                 /* 1: such a plan */
+  int32_t num_drafts, num_spans, longest_draft; /* requests, stretches of tiles, most tokens of a request */
 } ft_extend_plan_info;
 
 int ft_extend_plan_build(const int64_t* seq_lens, const int64_t* extend_lens, const int64_t* kv_starts, const int64_t* q_starts,
@@ -480,6 +484,109 @@ int ft_extend(const ft_extend_args* args);
 int ft_selftest_extend_wait(int limit, int* result_host, void* stream);
 /* names of the kernels that ft_extend would launch, as ft_stage1_path_name gives them */
 const char* ft_extend_path_name(const ft_extend_args* args);
+
+/* ---- branching continuations: drafted trees, beams -------------------------------------------------------- */
+
+#define FT_MAX_DRAFT 1024 /* drafted tokens of a request */
+
+/* ft_extend_plan_build for drafted tokens: the new tokens of request i are draft_lens[i] (at most FT_MAX_DRAFT) nodes of a tree,
+ * and a token sees the cached tokens, its ancestors and itself.  The plan is made for the sizes alone; the trees are given to
+ * ft_draft_tree, before which the tokens are chains.  request_ids[i] (below batch): the request's row in ft_draft_accept's results.
+ * window > 0: a token at position p = cached + depth sees positions p - window + 1 .. p of its path. */
+int ft_draft_plan_build(const int64_t* seq_lens, const int64_t* draft_lens, const int64_t* kv_starts, const int64_t* q_starts,
+                        const int64_t* shared_with_previous, const int32_t* request_ids, int32_t batch, int32_t num_qo_heads,
+                        int32_t num_kv_heads, int32_t head_dim, int32_t elem_bytes, int64_t window, int32_t num_sms, ft_extend_plan** out);
+
+/* A step's trees enter the plan's device table, for every ft_extend of the step; their tokens' positions come out.  parents[row of
+ * q]: the number of the token's parent among the request's tokens, which must be an earlier one; -1: a root, which hangs on the
+ * cached tokens; -2: padding, which sees the cached tokens alone and has no children.  Anything else is taken for padding and
+ * flagged (FT_DEV_BAD_PARENT).  positions[row of q]: cached tokens + depth (0 at a root and for padding). */
+typedef struct ft_draft_tree_args {
+  const void* parents;  /* [rows] int32 or int64 */
+  void* positions;      /* [rows] int32 or int64, or NULL */
+  int32_t parents_64, positions_64;
+  int64_t rows;         /* of parents and positions: at least the plan's q_rows */
+  int32_t* plan_table;  /* device copy of the table, changed */
+  ft_extend_plan_info plan;
+  void* stream;
+} ft_draft_tree_args;
+
+int ft_draft_tree_args_size(void);
+/* One launch on args->stream.  Calls that change one table, and ft_extend calls that read it, must be ordered by the caller. */
+int ft_draft_tree(const ft_draft_tree_args* args);
+
+/* Which drafted tokens the model agrees with: from a request's token 0 (its newest certain token, a root) on, the child that holds
+ * the token of the largest logit (of equal ones the lowest; NaN is passed over), the first such child, as long as there is one.
+ * Only the rows of logits along that path are read.  parents as in ft_draft_tree (what they take for padding is never accepted). */
+typedef struct ft_draft_accept_args {
+  const void* logits;   /* [rows, vocab], row t: the model's after token t; NULL if targets is given */
+  const void* targets;  /* [rows] the model's next token behind each token, in place of logits (sampled, say), or NULL */
+  const void* tokens;   /* [rows] drafted tokens */
+  const void* parents;  /* [rows] */
+  int32_t* accepted;    /* [num requests][accepted_stride0]: the accepted tokens' numbers in path order, then -1 */
+  int32_t* counts;      /* [num requests] accepted tokens */
+  void* next_tokens;    /* [num requests] the model's token behind the last accepted one; -1 without any */
+  const void* slots;    /* NULL, or [rows] the tokens' pool rows: with kv_entries, the request's entries behind its cached ones */
+  int32_t* kv_entries;  /*   become the accepted tokens' rows, in path order, then the others' */
+  int32_t dtype;        /* enum ft_dtype, of logits */
+  int32_t vocab;
+  int32_t targets_64, tokens_64, parents_64, next_64, slots_64, num_requests;
+  int32_t accepted_width;
+  int32_t reserved;
+  int64_t rows, logits_stride0, accepted_stride0, kv_entries_len;
+  const int32_t* plan_table;
+  ft_extend_plan_info plan;
+  void* stream;
+} ft_draft_accept_args;
+
+int ft_draft_accept_args_size(void);
+int ft_draft_accept(const ft_draft_accept_args* args);
+
+#define FT_MAX_BEAMS 64 /* beams of a request, and results */
+
+/* The `best` best continuations of each request's beams: score = scores[beam] + logits[beam][token] - log sum exp(logits[beam]),
+ * best first; of equal scores the lowest beam's first, then the larger logit, then the lowest token.  Logits of -inf are never chosen, nor is anything from a
+ * beam whose score is not finite (one that ended, say) or whose logits hold NaN or +inf; where too little is left the last
+ * results are score -inf, beam -1, token -1. */
+typedef struct ft_beam_select_args {
+  const void* logits;   /* [batch, beams, vocab] */
+  const float* scores;  /* [batch, beams] */
+  float* out_scores;    /* [batch, best] */
+  void* out_beams;      /* [batch, best] int32 or int64, as out_tokens */
+  void* out_tokens;
+  void* workspace;      /* ft_beam_select_workspace(args) bytes, 16-byte aligned; the call's own */
+  int32_t dtype;        /* enum ft_dtype, of logits */
+  int32_t batch, beams, vocab, best;
+  int32_t beams_64, tokens_64;
+  int32_t reserved;
+  int64_t logits_stride0, logits_stride1, scores_stride0, scores_stride1;
+  int64_t out_scores_stride0, out_beams_stride0, out_tokens_stride0;
+  void* stream;
+} ft_beam_select_args;
+
+int ft_beam_select_args_size(void);
+int64_t ft_beam_select_workspace(const ft_beam_select_args* args); /* negative: an error */
+int ft_beam_select(const ft_beam_select_args* args);
+
+/* Rows of a table follow the beams: columns starts[i] .. ends[i] - 1 of row out_rows[i][j] become those of row rows[i][beams[i][j]],
+ * as they were before the call (rows may change places within a request); beam -1 leaves its row alone.  A row that a call
+ * writes belongs to one request, and stands once among its out_rows.  Rows, beams and columns outside the table are left out and
+ * flagged (FT_DEV_BAD_ROW_INDEX). */
+typedef struct ft_beam_reorder_args {
+  void* table;           /* [table_rows, width], elements of 4 or 8 bytes */
+  const void* rows;      /* [batch, from] */
+  const void* beams;     /* [batch, to] */
+  const void* out_rows;  /* [batch, to] */
+  const void* starts;    /* [batch], or NULL: 0 */
+  const void* ends;      /* [batch], or NULL: width */
+  int32_t elem_bytes, batch, from, to;
+  int32_t rows_64, beams_64, out_rows_64, starts_64, ends_64, reserved;
+  int64_t table_rows, width, table_stride0, rows_stride0, beams_stride0, out_rows_stride0;
+  void* stream;
+} ft_beam_reorder_args;
+
+int ft_beam_reorder_args_size(void);
+int ft_beam_reorder(const ft_beam_reorder_args* args);
 
 #ifdef __cplusplus
 }
