@@ -3,10 +3,12 @@
 //   score(b, x) = scores[b] + logits[b][x] - log sum_y exp(logits[b][y])
 //
 // Within a beam the order of scores is that of the logits, so a beam's share of the results is among its `best` largest
-// logits.  beam_scan_kernel reads every logit once: a CTA holds a slice of a row in registers and leaves the slice's maximum, its
-// sum of exponentials and its `best` largest logits; beam_merge_kernel puts a request's slices together.  Scores are made and compared in 64
-// bits, from sums of at most 128 fp32 terms each, because scores of different beams may lie close: what decides is the logits' own value.
+// logits.  beam_scan_kernel reads every logit once: a CTA goes through a slice of a row and leaves its sum of exponentials and its
+// `best` largest logits; beam_merge_kernel puts a request's slices together.  Scores are made and compared in 64 bits, because those of
+// different beams may lie close: what decides is the logits' own value.
 #pragma once
+
+#include <type_traits>
 
 #include "ft_draft.cuh"
 
@@ -22,7 +24,7 @@ struct BeamParams {
   void* out_beams;
   void* out_tokens;
   unsigned long long* keys;  // [rows][slices][best] {ordered logit, ~token}, 0: none
-  float2* sums;              // [rows][slices] {maximum, sum of exp(logit - maximum)}
+  float2* sums;              // [rows][slices] {c, sum of 2^(logit log2(e) - c)}
   int64_t logits_s0, logits_s1, scores_s0, scores_s1, out_scores_s0, out_beams_s0, out_tokens_s0;
   int32_t batch, beams, vocab, best, slices, slice_len, beams_64, tokens_64;  // slice_len: a multiple of 16 bytes
 };
@@ -59,19 +61,54 @@ __device__ __forceinline__ unsigned long long warp_max_key(unsigned long long k)
   return k;
 }
 
-// One slice of one row: NV 16-byte pieces a thread, or as many elements one at a time where rows do not start on 16 bytes (a rule of
-// the call, not of the row, so that equal rows have equal sums).
+// log2(e) as the kernels multiply by it: what a sum's offset is divided by to give a logarithm, in 64 bits.
+constexpr float BEAM_LOG2E = 1.4426950408889634f;
+
+// The best of a list of n keys into out[0 .. best), 0 where the list ends: ranked by counting, or one at a time, whichever
+// takes fewer instructions.  A whole block, behind a barrier.
+__device__ __forceinline__ void best_of_list(const unsigned long long* keys, int n, unsigned long long* __restrict__ out, int best,
+                                             unsigned long long (&from_warp)[BEAM_WARPS]) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (n <= 128 + 16 * best) {
+    for (int i = threadIdx.x; i < n; i += BEAM_THREADS) {
+      const unsigned long long key = keys[i];
+      int rank = 0;
+#pragma unroll 4
+      for (int k = 0; k < n; ++k) rank += keys[k] > key;
+      if (rank < best) out[rank] = key;
+    }
+    for (int i = n + (int)threadIdx.x; i < best; i += BEAM_THREADS) out[i] = 0;
+    return;
+  }
+  unsigned long long last = ~0ull;
+  for (int r = 0; r < best; ++r) {
+    unsigned long long key = 0;
+    for (int i = threadIdx.x; i < n; i += BEAM_THREADS)
+      if (keys[i] < last) key = max(key, keys[i]);
+    key = warp_max_key(key);
+    if (lane == 0) from_warp[warp] = key;
+    __syncthreads();
+    last = warp_max_key(from_warp[lane & (BEAM_WARPS - 1)]);
+    if (threadIdx.x == 0) out[r] = last;
+    __syncthreads();
+  }
+}
+
+// One slice of one row, in chunks of NV 16-byte pieces a thread, or as many elements one at a time where rows do not start on 16
+// bytes (a rule of the call, not of the row, so that equal rows have equal sums).
 //
-// The `best` largest: each group of threads (a warp for up to 8 results) has a largest logit, and the least of them bounds the
-// `best`-th from below; what reaches it, 22 of 16 384 logits on average for 8 groups, is listed and ranked by counting.
+// The sum: each thread has its own running maximum and adds 2^(x log2(e) - c), c = maximum x log2(e).
+// The `best` largest: in the first chunk each group of threads (a warp for up to 8 results) has a largest logit, and the least of them
+// bounds the `best`-th from below; what reaches it, 22 of 8192 logits on average for 8 groups, is listed, and what of the other chunks
+// does.  Where equal logits overflow the list, the best of the list and the chunk are picked one at a time.
 template <typename T, int NV, bool VEC>
-__global__ void __launch_bounds__(BEAM_THREADS) beam_scan_kernel(const BeamParams p, const int groups) {
-  constexpr int N = Vec<T>::N, E = NV * N;
-  constexpr float LOG2E = 1.4426950408889634f;
+__global__ void __launch_bounds__(BEAM_THREADS, 4) beam_scan_kernel(const BeamParams p, const int groups) {
+  constexpr int N = Vec<T>::N, CHUNK = BEAM_THREADS * NV * N;
   __shared__ unsigned long long keys[BEAM_KEYS];
-  __shared__ float low[BEAM_WARPS], high[BEAM_WARPS], sums[BEAM_WARPS];
-  __shared__ unsigned long long from_warp[BEAM_WARPS];
-  __shared__ int listed;
+  __shared__ float low[BEAM_WARPS], high[BEAM_WARPS];
+  __shared__ float2 sums[BEAM_WARPS];
+  __shared__ unsigned long long from_warp[BEAM_WARPS], picked[FT_MAX_BEAMS];
+  __shared__ int more[3];  // listed by a chunk, by turns: the next chunk's is cleared before a chunk's last barrier
   allow_dependent_launch();
   wait_for_prior_grid();
   const int row = (int)(blockIdx.x / (unsigned)p.slices), slice = (int)(blockIdx.x - (unsigned)row * p.slices);
@@ -83,114 +120,136 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_scan_kernel(const BeamParam
     if (threadIdx.x == 0) p.sums[blockIdx.x] = make_float2(-INFINITY, 0.f);
     return;
   }
-  if (threadIdx.x == 0) listed = 0;
+  if (threadIdx.x < 3) more[threadIdx.x] = 0;
   const T* __restrict__ base = static_cast<const T*>(p.logits) + req * p.logits_s0 + beam * p.logits_s1;
-  const int first = slice * p.slice_len, end = min(p.vocab, first + p.slice_len);
-  // element e of piece j of a thread is number first + (j * BEAM_THREADS + thread) * N + e, either way
-  uint4 x[NV];
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int at = first + (j * BEAM_THREADS + (int)threadIdx.x) * N;
-    uint32_t w[4];
-    if (VEC && at + N <= end) {
-      x[j] = load_stream(base + at);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (sizeof(T) == 4) {
-          w[e] = at + e < end ? __float_as_uint(to_float<T>(base[at + e])) : 0xff800000u;
-        } else {
-          const uint16_t* raw = reinterpret_cast<const uint16_t*>(base);
-          const uint32_t none = sizeof(T) == 2 && unpack2<T>(0xfc00u).x == -INFINITY ? 0xfc00u : 0xff80u;  // -inf
-          const uint32_t a = at + 2 * e < end ? raw[at + 2 * e] : none, b = at + 2 * e + 1 < end ? raw[at + 2 * e + 1] : none;
-          w[e] = a | b << 16;
-        }
-      }
-      x[j] = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  }
-  float piece[NV], mine = -INFINITY;
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    piece[j] = vec_max<T>(x[j]);
-    mine = fmaxf(mine, piece[j]);
-  }
-  float top;
-  const float bound = group_bound(mine, groups, low, high, top);
-  // the sum of exp(x - top), 0 for a slice of nothing but -inf; NaN and +inf make it NaN
-  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-  const float off = top == -INFINITY ? 0.f : -top;
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
-#pragma unroll
-    for (int e = 0; e < N / 2; ++e) {
-      float2 y;
-      if constexpr (sizeof(T) == 4)
-        y = make_float2(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
-      else
-        y = unpack2<T>(w[e]);
-      y = __fmul2_rn(__fadd2_rn(y, make_float2(off, off)), make_float2(LOG2E, LOG2E));
-      sum[e & 1] = __fadd2_rn(sum[e & 1], make_float2(fast_exp2(y.x), fast_exp2(y.y)));
-    }
-  }
-  const float total = warp_sum((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
-  if (lane == 0) sums[warp] = total;
-  // what reaches the bound
-  const float least = fmaxf(bound, -3.4028234e38f);
-  if (__any_sync(0xffffffffu, mine >= least)) {
+  const int begin = slice * p.slice_len, end = min(p.vocab, begin + p.slice_len);
+  float top = -INFINITY, off = 0.f, sum = 0.f, least = -3.4028234e38f;
+  int listed = 0, turn = 0;
+#pragma unroll 1
+  for (int first = begin; first < end; first += CHUNK) {
+    // element e of piece j of a thread is number first + (j * BEAM_THREADS + thread) * N + e, either way
+    uint4 x[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (!__any_sync(0xffffffffu, piece[j] >= least)) continue;
       const int at = first + (j * BEAM_THREADS + (int)threadIdx.x) * N;
+      if (VEC && at + N <= end) {
+        x[j] = load_stream(base + at);
+      } else {
+        uint32_t w[4];
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float y = vec_at<T>(x[j], e);
-        if (y >= least) {
-          const int to = atomicAdd(&listed, 1);
-          if (to < BEAM_KEYS) keys[to] = ((unsigned long long)ordered(y) << 32) | (0xffffffffu - (uint32_t)(at + e));
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (sizeof(T) == 4) {
+            w[e] = at + e < end ? __float_as_uint(to_float<T>(base[at + e])) : 0xff800000u;
+          } else {
+            const uint16_t* raw = reinterpret_cast<const uint16_t*>(base);
+            const uint32_t none = std::is_same<T, __half>::value ? 0xfc00u : 0xff80u;  // -inf
+            const uint32_t a = at + 2 * e < end ? raw[at + 2 * e] : none, b = at + 2 * e + 1 < end ? raw[at + 2 * e + 1] : none;
+            w[e] = a | b << 16;
+          }
+        }
+        x[j] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    float piece[NV], mine = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      piece[j] = vec_max<T>(x[j]);
+      mine = fmaxf(mine, piece[j]);
+    }
+    if (mine > top) {  // (with +inf, c is it too and the sum NaN, as with NaN)
+      const float c = mine * BEAM_LOG2E;
+      sum = top == -INFINITY ? sum : sum * fast_exp2(off - c);
+      top = mine;
+      off = c;
+    }
+    float2 sum2[2] = {make_float2(sum, 0.f), make_float2(0.f, 0.f)};
+    const float2 scale2 = make_float2(BEAM_LOG2E, BEAM_LOG2E), off2 = make_float2(-off, -off);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) {
+        float2 y;
+        if constexpr (sizeof(T) == 4)
+          y = make_float2(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
+        else
+          y = unpack2<T>(w[e]);
+        y = __ffma2_rn(y, scale2, off2);
+        sum2[e & 1] = __fadd2_rn(sum2[e & 1], make_float2(fast_exp2(y.x), fast_exp2(y.y)));
+      }
+    }
+    sum = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
+    if (first == begin) {
+      float all;
+      least = fmaxf(least, group_bound(mine, groups, low, high, all));
+    }
+    // what reaches the bound (the pieces are unpacked anew: kept since the sum they would take 100 registers)
+    if (__any_sync(0xffffffffu, mine >= least)) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if (!__any_sync(0xffffffffu, piece[j] >= least)) continue;
+        asm volatile("" : "+r"(x[j].x), "+r"(x[j].y), "+r"(x[j].z), "+r"(x[j].w));
+        const int at = first + (j * BEAM_THREADS + (int)threadIdx.x) * N;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float y = vec_at<T>(x[j], e);
+          if (y >= least) {
+            const int to = listed + atomicAdd(&more[turn], 1);
+            if (to < BEAM_KEYS) keys[to] = ((unsigned long long)ordered(y) << 32) | (0xffffffffu - (uint32_t)(at + e));
+          }
         }
       }
     }
+    const int next = turn == 2 ? 0 : turn + 1;
+    if (threadIdx.x == 0) more[next] = 0;
+    __syncthreads();
+    const int now = listed + more[turn];
+    turn = next;
+    if (now <= BEAM_KEYS) {
+      listed = now;
+      continue;
+    }
+    unsigned long long last = ~0ull;
+#pragma unroll 1
+    for (int r = 0; r < p.best; ++r) {
+      unsigned long long key = 0;
+      for (int i = threadIdx.x; i < listed; i += BEAM_THREADS)
+        if (keys[i] < last) key = max(key, keys[i]);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        asm volatile("" : "+r"(x[j].x), "+r"(x[j].y), "+r"(x[j].z), "+r"(x[j].w));
+        const int at = first + (j * BEAM_THREADS + (int)threadIdx.x) * N;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float y = vec_at<T>(x[j], e);
+          const unsigned long long k = ((unsigned long long)ordered(y) << 32) | (0xffffffffu - (uint32_t)(at + e));
+          if (y >= least && k < last) key = max(key, k);
+        }
+      }
+      key = warp_max_key(key);
+      if (lane == 0) from_warp[warp] = key;
+      __syncthreads();
+      last = warp_max_key(from_warp[lane & (BEAM_WARPS - 1)]);
+      if (threadIdx.x == 0) picked[r] = last;
+      __syncthreads();
+    }
+    for (int i = threadIdx.x; i < p.best; i += BEAM_THREADS) keys[i] = picked[i];
+    listed = p.best;
+    least = from_ordered((uint32_t)(last >> 32));  // (more than `best` were there, so none is missing)
+    __syncthreads();
   }
+  // the threads' sums, over the largest offset
+  if (top == -INFINITY) off = -INFINITY;
+  const float warp_off = warp_max(off), from = warp_off == -INFINITY ? 0.f : warp_off;
+  const float total = warp_sum(sum == 0.f ? 0.f : sum * fast_exp2(off - from));
+  if (lane == 0) sums[warp] = make_float2(warp_off, total);
+  best_of_list(keys, listed, out, p.best, from_warp);
   __syncthreads();
-  if (threadIdx.x == 0) {
-    float all = 0.f;
-#pragma unroll
-    for (int w = 0; w < BEAM_WARPS; ++w) all += sums[w];
-    p.sums[blockIdx.x] = make_float2(top, all);
-  }
-  const int n = listed;
-  // ranked by counting, or one at a time, whichever takes fewer instructions
-  if (n <= BEAM_KEYS && (n / BEAM_WARPS) * n <= 11 * p.best * (5 * E + 100)) {
-    for (int i = threadIdx.x; i < n; i += BEAM_THREADS) {
-      const unsigned long long key = keys[i];
-      int rank = 0;
-      for (int k = 0; k < n; ++k) rank += keys[k] > key;
-      if (rank < p.best) out[rank] = key;
-    }
-    for (int i = n + (int)threadIdx.x; i < p.best; i += BEAM_THREADS) out[i] = 0;
-    return;
-  }
-  unsigned long long before = ~0ull;
-  for (int r = 0; r < p.best; ++r) {
-    unsigned long long key = 0;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int at = first + (j * BEAM_THREADS + (int)threadIdx.x) * N;
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float y = vec_at<T>(x[j], e);
-        const unsigned long long k = ((unsigned long long)ordered(y) << 32) | (0xffffffffu - (uint32_t)(at + e));
-        if (y >= least && k < before) key = max(key, k);
-      }
-    }
-    key = warp_max_key(key);
-    if (lane == 0) from_warp[warp] = key;
-    __syncthreads();
-    before = warp_max_key(from_warp[lane & (BEAM_WARPS - 1)]);
-    if (threadIdx.x == 0) out[r] = before;
-    __syncthreads();
+  if (warp == 0) {
+    const float2 x = lane < BEAM_WARPS ? sums[lane] : make_float2(-INFINITY, 0.f);
+    const float most = warp_max(x.x), from_all = most == -INFINITY ? 0.f : most;
+    const float all = warp_sum(x.y == 0.f ? 0.f : x.y * fast_exp2(x.x - from_all));
+    if (lane == 0) p.sums[blockIdx.x] = make_float2(most, all);
   }
 }
 
@@ -224,23 +283,26 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamPara
     double sum = 0;
     for (int s = lane; s < p.slices; s += 32) {
       const float2 x = __ldcg(&sums[b * p.slices + s]);
-      if (x.x != -INFINITY || x.y != 0.f) sum += (double)x.y * exp((double)x.x - (double)top);
+      if (x.y != 0.f) sum += (double)x.y * exp2((double)x.x - (double)top);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const float score = p.scores[req * p.scores_s0 + b * p.scores_s1];
     if (lane == 0) {
-      const double lse = (double)top + log(sum);
+      // (the terms' exponents were taken x BEAM_LOG2E, which is not log2(e): by it the offset is a logit again, and what is left of
+      // the difference, 1.3e-8 of the distance from the largest logit to the mean, is below fp32's half step)
+      const double lse = (double)top / (double)BEAM_LOG2E + log(sum);
       shift[b] = fabsf(score) < INFINITY && fabs(lse) < (double)INFINITY ? (double)score - lse : (double)NAN;
     }
   }
   __syncthreads();
-  const int per_beam = p.slices * p.best, total = p.beams * per_beam;
+  const int lists = p.beams * p.slices, total = lists * p.best;
   const unsigned long long* __restrict__ keys = p.keys + (int64_t)req * total;
-  // false: no candidate
+  // candidate i, the lists' first ones first (so that every group of threads has some of the best); false: there is none
   auto candidate = [&](int i, BeamCandidate& c) {
-    c.key = __ldcg(keys + i);
-    c.beam = i / per_beam;
+    const int rank = i / lists, list = i - rank * lists;
+    c.key = __ldcg(keys + list * p.best + rank);
+    c.beam = list / p.slices;
     c.score = (double)from_ordered((uint32_t)(c.key >> 32)) + shift[c.beam];
     return c.key != 0 && c.score == c.score;
   };

@@ -66,18 +66,16 @@ int check_beam_select(const ft_beam_select_args* a) {
   return FT_OK;
 }
 
-// Slices of a row.  Eight 16-byte pieces a thread where that leaves every SM CTAs enough to hide each other's waits, fewer where the
-// call is small and its length is what one slice takes.  (148 SMs whatever the device: the workspace's size goes by this.)
+// Slices of a row: of four chunks where that leaves every SM CTAs enough to hide each other's waits, of fewer and smaller ones where
+// the call is small and its length is what one slice takes.  (148 SMs whatever the device: the workspace's size goes by this.)
 BeamShape beam_shape(const ft_beam_select_args* a) {
   BeamShape s;
-  const int n = 16 / dtype_size(a->dtype), sms = 148;
+  const int n = 16 / dtype_size(a->dtype);
   const int64_t rows = (int64_t)a->batch * a->beams;
-  for (s.pieces = 8; s.pieces > 1; s.pieces /= 2) {
-    const int64_t slice = (int64_t)ft::BEAM_THREADS * s.pieces * n;
-    if (rows * ((a->vocab + slice - 1) / slice) >= 3LL * sms) break;
-  }
-  const int64_t most = (int64_t)ft::BEAM_THREADS * s.pieces * n;
-  s.slices = (int)((a->vocab + most - 1) / most);
+  int64_t slice = (int64_t)ft::BEAM_THREADS * n * 16;
+  while (slice > ft::BEAM_THREADS * n && rows * ((a->vocab + slice - 1) / slice) < 6 * 148) slice /= 2;
+  s.pieces = (int)std::min<int64_t>(4, slice / (ft::BEAM_THREADS * n));
+  s.slices = (int)((a->vocab + slice - 1) / slice);
   s.slice_len = (int)((((int64_t)a->vocab + s.slices - 1) / s.slices + n - 1) / n * n);
   s.keys = rows * s.slices * a->best;
   s.bytes = s.keys * 8 + rows * s.slices * 8;
@@ -104,8 +102,7 @@ int launch_beam_select(const ft::BeamParams& p, int pieces, bool vec, cudaStream
   switch (pieces) {
     case 1: launch_scan<T, 1>(p, groups, vec, st); break;
     case 2: launch_scan<T, 2>(p, groups, vec, st); break;
-    case 4: launch_scan<T, 4>(p, groups, vec, st); break;
-    default: launch_scan<T, 8>(p, groups, vec, st); break;
+    default: launch_scan<T, 4>(p, groups, vec, st); break;
   }
   FT_CUDA_OK(cudaGetLastError());
   count_launch();
