@@ -10,6 +10,7 @@
 
 #include <type_traits>
 
+#include "ft_async.cuh"
 #include "ft_draft.cuh"
 
 namespace ft {
@@ -94,57 +95,128 @@ __device__ __forceinline__ void best_of_list(const unsigned long long* keys, int
   }
 }
 
-// One slice of one row, in chunks of NV 16-byte pieces a thread, or as many elements one at a time where rows do not start on 16
-// bytes (a rule of the call, not of the row, so that equal rows have equal sums).
+// Shared memory of beam_scan_kernel: stages of a chunk each, as its bytes stand in memory from the 16-byte border below on.
+template <int NV>
+struct BeamScan {
+  static constexpr int STAGES = 3, CHUNK_BYTES = BEAM_THREADS * NV * 16, STAGE_BYTES = CHUNK_BYTES + 32, SMEM_BYTES = STAGES * STAGE_BYTES;
+  static constexpr int WAIT_LIMIT = 1 << 16;
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+// One slice of one row, in chunks of NV x 16 bytes a thread that come by bulk copies, three chunks ahead.
+//
+// VEC: rows start on 16 bytes, and a thread reads 16 bytes at a time; else it reads words of 4 (a rule of the call, not of the row, so
+// that equal rows have equal sums).  Copies are of whole 16-byte pieces inside the row; what stands at its ends is filled in.
 //
 // The sum: each thread has its own running maximum and adds 2^(x log2(e) - c), c = maximum x log2(e).
 // The `best` largest: in the first chunk each group of threads (a warp for up to 8 results) has a largest logit, and the least of them
 // bounds the `best`-th from below; what reaches it, 22 of 8192 logits on average for 8 groups, is listed, and what of the other chunks
 // does.  Where equal logits overflow the list, the best of the list and the chunk are picked one at a time.
 template <typename T, int NV, bool VEC>
-__global__ void __launch_bounds__(BEAM_THREADS, 4) beam_scan_kernel(const BeamParams p, const int groups) {
-  constexpr int N = Vec<T>::N, CHUNK = BEAM_THREADS * NV * N;
+__global__ void __launch_bounds__(BEAM_THREADS, 3) beam_scan_kernel(const BeamParams p, const int groups) {
+  using C = BeamScan<NV>;
+  constexpr int S = (int)sizeof(T), N = 16 / S, CHUNK = BEAM_THREADS * NV * N;
+  constexpr uint32_t NONE = S == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;  // -inf
+  extern __shared__ __align__(128) uint8_t stages[];
   __shared__ unsigned long long keys[BEAM_KEYS];
   __shared__ float low[BEAM_WARPS], high[BEAM_WARPS];
   __shared__ float2 sums[BEAM_WARPS];
   __shared__ unsigned long long from_warp[BEAM_WARPS], picked[FT_MAX_BEAMS];
+  __shared__ __align__(8) unsigned long long barrier[C::STAGES];
   __shared__ int more[3];  // listed by a chunk, by turns: the next chunk's is cleared before a chunk's last barrier
   allow_dependent_launch();
   wait_for_prior_grid();
   const int row = (int)(blockIdx.x / (unsigned)p.slices), slice = (int)(blockIdx.x - (unsigned)row * p.slices);
-  const int req = row / p.beams, beam = row - req * p.beams, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int req = row / p.beams, beam = row - req * p.beams, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   unsigned long long* __restrict__ out = p.keys + (int64_t)blockIdx.x * p.best;
+  const int begin = slice * p.slice_len, end = min(p.vocab, begin + p.slice_len);
   const float score = __ldg(p.scores + req * p.scores_s0 + beam * p.scores_s1);
-  if (!(fabsf(score) < INFINITY)) {  // nothing comes from this beam
-    for (int i = threadIdx.x; i < p.best; i += BEAM_THREADS) out[i] = 0;
-    if (threadIdx.x == 0) p.sums[blockIdx.x] = make_float2(-INFINITY, 0.f);
+  if (!(fabsf(score) < INFINITY) || begin >= end) {  // nothing comes from this beam
+    for (int i = tid; i < p.best; i += BEAM_THREADS) out[i] = 0;
+    if (tid == 0) p.sums[blockIdx.x] = make_float2(-INFINITY, 0.f);
     return;
   }
-  if (threadIdx.x < 3) more[threadIdx.x] = 0;
   const T* __restrict__ base = static_cast<const T*>(p.logits) + req * p.logits_s0 + beam * p.logits_s1;
-  const int begin = slice * p.slice_len, end = min(p.vocab, begin + p.slice_len);
+  const uintptr_t row_at = reinterpret_cast<uintptr_t>(base), row_end = row_at + (int64_t)p.vocab * S;
+  const uint32_t bars = (uint32_t)__cvta_generic_to_shared(barrier), ring = (uint32_t)__cvta_generic_to_shared(stages);
+  // a chunk's bytes: from `at` (its stage begins at the 16-byte border below), of which [from, to) are copied
+  struct Span {
+    uintptr_t at, from, to;
+  };
+  auto span_of = [&](int first) {
+    const uintptr_t a = row_at + (int64_t)first * S, b = row_at + (int64_t)min(end, first + CHUNK) * S;
+    Span s = {a, a & ~(uintptr_t)15, (b + 15) & ~(uintptr_t)15};
+    if (s.from < row_at) s.from += 16;
+    if (s.to > row_end) s.to -= 16;
+    if (s.to < s.from) s.to = s.from;
+    return s;
+  };
+  auto issue = [&](int chunk) {
+    const int first = begin + chunk * CHUNK;
+    if (first >= end) return;
+    const Span s = span_of(first);
+    const uint32_t bytes = (uint32_t)(s.to - s.from), bar = bars + 8 * (chunk % C::STAGES);
+    mbar_arrive_expect_tx(bar, bytes);
+    if (bytes > 0)
+      bulk_load(ring + (chunk % C::STAGES) * C::STAGE_BYTES + (uint32_t)(s.from - (s.at & ~(uintptr_t)15)), reinterpret_cast<const void*>(s.from), bytes, bar);
+  };
+  if (tid == 0) {
+    for (int i = 0; i < C::STAGES; ++i) mbar_init(bars + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    proxy_fence();
+    for (int i = 0; i < C::STAGES; ++i) issue(i);
+  }
+  if (tid < 3) more[tid] = 0;
+  __syncthreads();
   float top = -INFINITY, off = 0.f, sum = 0.f, least = -3.4028234e38f;
-  int listed = 0, turn = 0;
+  int listed = 0, turn = 0, chunk = 0;
+  uint32_t phase = 0;
+  bool late = false;
 #pragma unroll 1
-  for (int first = begin; first < end; first += CHUNK) {
-    // element e of piece j of a thread is number first + (j * BEAM_THREADS + thread) * N + e, either way
+  for (int first = begin; first < end; first += CHUNK, ++chunk) {
+    const int stage = chunk % C::STAGES;
+    const int len = min(end - first, CHUNK);
+    const Span s = span_of(first);
+    uint8_t* const bytes = stages + stage * C::STAGE_BYTES;
+    const uint32_t shift = (uint32_t)(s.at & 15);
+    late |= !mbar_wait_warp(bars + 8 * stage, phase, C::WAIT_LIMIT);
+    if (stage == C::STAGES - 1) phase ^= 1u;
+    const uintptr_t stop = s.at + (int64_t)len * S, whole = (stop + 15) & ~(uintptr_t)15;
+    if (s.from > s.at || s.to < whole) {  // the row's ends, and -inf up to the next 16 bytes
+      if (tid < 2 * N) {
+        const uintptr_t at = tid < N ? s.at + tid * S : s.to + (tid - N) * S;
+        if (tid < N ? at < s.from && at < stop : at < whole && at >= s.at && at >= s.from)
+          *reinterpret_cast<T*>(bytes + (at - (s.at & ~(uintptr_t)15))) = at < stop ? *reinterpret_cast<const T*>(at) : from_float<T>(-INFINITY);
+      }
+      proxy_fence();
+      __syncthreads();
+    }
+    // word w of piece j; number of its first element in the chunk
+    auto number = [&](int j, int e) {
+      if constexpr (VEC) return (j * BEAM_THREADS + tid) * N + e;
+      if constexpr (S == 4) return (4 * j + e) * BEAM_THREADS + tid;
+      return 2 * ((4 * j + (e >> 1)) * BEAM_THREADS + tid) + (e & 1);
+    };
     uint4 x[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int at = first + (j * BEAM_THREADS + (int)threadIdx.x) * N;
-      if (VEC && at + N <= end) {
-        x[j] = load_stream(base + at);
+      if constexpr (VEC) {
+        x[j] = number(j, 0) < len ? *reinterpret_cast<const uint4*>(bytes + number(j, 0) * S) : make_uint4(NONE, NONE, NONE, NONE);
       } else {
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if constexpr (sizeof(T) == 4) {
-            w[e] = at + e < end ? __float_as_uint(to_float<T>(base[at + e])) : 0xff800000u;
+          const int i = number(j, e * (4 / S));
+          const uint8_t* const from = bytes + shift + i * S;
+          if constexpr (S == 4) {
+            w[e] = i < len ? *reinterpret_cast<const uint32_t*>(from) : NONE;
           } else {
-            const uint16_t* raw = reinterpret_cast<const uint16_t*>(base);
-            const uint32_t none = std::is_same<T, __half>::value ? 0xfc00u : 0xff80u;  // -inf
-            const uint32_t a = at + 2 * e < end ? raw[at + 2 * e] : none, b = at + 2 * e + 1 < end ? raw[at + 2 * e + 1] : none;
-            w[e] = a | b << 16;
+            const uint32_t a = i < len ? *reinterpret_cast<const uint16_t*>(from) : NONE & 0xffffu;
+            w[e] = a | (i + 1 < len ? (uint32_t)*reinterpret_cast<const uint16_t*>(from + 2) << 16 : NONE & 0xffff0000u);
           }
         }
         x[j] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -170,7 +242,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4) beam_scan_kernel(const BeamPa
 #pragma unroll
       for (int e = 0; e < N / 2; ++e) {
         float2 y;
-        if constexpr (sizeof(T) == 4)
+        if constexpr (S == 4)
           y = make_float2(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
         else
           y = unpack2<T>(w[e]);
@@ -185,26 +257,29 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4) beam_scan_kernel(const BeamPa
     }
     // what reaches the bound (the pieces are unpacked anew: kept since the sum they would take 100 registers)
     if (__any_sync(0xffffffffu, mine >= least)) {
+      uint32_t hits = 0;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         if (!__any_sync(0xffffffffu, piece[j] >= least)) continue;
         asm volatile("" : "+r"(x[j].x), "+r"(x[j].y), "+r"(x[j].z), "+r"(x[j].w));
-        const int at = first + (j * BEAM_THREADS + (int)threadIdx.x) * N;
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float y = vec_at<T>(x[j], e);
-          if (y >= least) {
-            const int to = listed + atomicAdd(&more[turn], 1);
-            if (to < BEAM_KEYS) keys[to] = ((unsigned long long)ordered(y) << 32) | (0xffffffffu - (uint32_t)(at + e));
-          }
+        for (int e = 0; e < N; ++e) hits |= vec_at<T>(x[j], e) >= least ? 1u << (j * N + e) : 0u;
+      }
+      if (hits != 0) {
+        int to = listed + atomicAdd(&more[turn], __popc(hits));
+        for (; hits != 0; hits &= hits - 1, ++to) {
+          const int bit = __ffs(hits) - 1, i = number(bit / N, bit % N);
+          const float y = to_float<T>(*reinterpret_cast<const T*>(bytes + shift + i * S));
+          if (to < BEAM_KEYS) keys[to] = ((unsigned long long)ordered(y) << 32) | (0xffffffffu - (uint32_t)(first + i));
         }
       }
     }
     const int next = turn == 2 ? 0 : turn + 1;
-    if (threadIdx.x == 0) more[next] = 0;
+    if (tid == 0) more[next] = 0;
     __syncthreads();
     const int now = listed + more[turn];
     turn = next;
+    if (tid == 0) issue(chunk + C::STAGES);
     if (now <= BEAM_KEYS) {
       listed = now;
       continue;
@@ -213,16 +288,15 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4) beam_scan_kernel(const BeamPa
 #pragma unroll 1
     for (int r = 0; r < p.best; ++r) {
       unsigned long long key = 0;
-      for (int i = threadIdx.x; i < listed; i += BEAM_THREADS)
+      for (int i = tid; i < listed; i += BEAM_THREADS)
         if (keys[i] < last) key = max(key, keys[i]);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         asm volatile("" : "+r"(x[j].x), "+r"(x[j].y), "+r"(x[j].z), "+r"(x[j].w));
-        const int at = first + (j * BEAM_THREADS + (int)threadIdx.x) * N;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           const float y = vec_at<T>(x[j], e);
-          const unsigned long long k = ((unsigned long long)ordered(y) << 32) | (0xffffffffu - (uint32_t)(at + e));
+          const unsigned long long k = ((unsigned long long)ordered(y) << 32) | (0xffffffffu - (uint32_t)(first + number(j, e)));
           if (y >= least && k < last) key = max(key, k);
         }
       }
@@ -230,10 +304,10 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4) beam_scan_kernel(const BeamPa
       if (lane == 0) from_warp[warp] = key;
       __syncthreads();
       last = warp_max_key(from_warp[lane & (BEAM_WARPS - 1)]);
-      if (threadIdx.x == 0) picked[r] = last;
+      if (tid == 0) picked[r] = last;
       __syncthreads();
     }
-    for (int i = threadIdx.x; i < p.best; i += BEAM_THREADS) keys[i] = picked[i];
+    for (int i = tid; i < p.best; i += BEAM_THREADS) keys[i] = picked[i];
     listed = p.best;
     least = from_ordered((uint32_t)(last >> 32));  // (more than `best` were there, so none is missing)
     __syncthreads();
@@ -244,7 +318,10 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4) beam_scan_kernel(const BeamPa
   const float total = warp_sum(sum == 0.f ? 0.f : sum * fast_exp2(off - from));
   if (lane == 0) sums[warp] = make_float2(warp_off, total);
   best_of_list(keys, listed, out, p.best, from_warp);
-  __syncthreads();
+  if (__syncthreads_or(late)) {  // a copy that did not come: its bytes may not land in another CTA's memory
+    if (tid == 0) flag_error(FT_DEV_WAIT_TIMEOUT);
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+  }
   if (warp == 0) {
     const float2 x = lane < BEAM_WARPS ? sums[lane] : make_float2(-INFINITY, 0.f);
     const float most = warp_max(x.x), from_all = most == -INFINITY ? 0.f : most;
@@ -263,20 +340,29 @@ __device__ __forceinline__ bool before(const BeamCandidate& a, const BeamCandida
   return a.score != b.score ? a.score > b.score : a.beam != b.beam ? a.beam < b.beam : a.key > b.key;
 }
 
-// A CTA per request: each beam's sum from its slices (64 bits), each listed logit's score, and as in the slices a bound that keeps most
-// of them out of the ranking.
-__global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamParams p, const int groups) {
+// A CTA per request: each beam's sum from its slices (64 bits), each listed logit's score, and a threshold between the best
+// and the rest, found by halving, that leaves few to be ranked.  REGS scores a thread stay in registers, in fp32 rounded down, which
+// keeps their order; more are made anew each time.
+template <int REGS>
+__global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamParams p) {
   __shared__ double shift[FT_MAX_BEAMS];  // a beam's score less its logarithm; NaN: nothing comes from it
   __shared__ BeamCandidate list[BEAM_KEYS];
-  __shared__ float low[BEAM_WARPS], high[BEAM_WARPS];
+  __shared__ float high[BEAM_WARPS];
+  __shared__ int counts[3][BEAM_WARPS], place[BEAM_KEYS];
   __shared__ BeamCandidate from_warp[BEAM_WARPS];
   __shared__ int listed;
-  const int req = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) listed = 0;
+  const int req = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) listed = 0;
   allow_dependent_launch();
   wait_for_prior_grid();
   const float2* __restrict__ sums = p.sums + (int64_t)req * p.beams * p.slices;
+  const int per_beam = p.slices * p.best, total = p.beams * per_beam;
+  const unsigned long long* __restrict__ keys = p.keys + (int64_t)req * total;
+  unsigned long long mine[REGS];
+#pragma unroll
+  for (int k = 0; k < REGS; ++k) mine[k] = tid + k * BEAM_THREADS < total ? __ldcg(keys + tid + k * BEAM_THREADS) : 0;
   for (int b = warp; b < p.beams; b += BEAM_WARPS) {
+    const float score = p.scores[req * p.scores_s0 + b * p.scores_s1];
     float top = -INFINITY;
     for (int s = lane; s < p.slices; s += 32) top = fmaxf(top, __ldcg(&sums[b * p.slices + s]).x);
     top = warp_max(top);
@@ -287,7 +373,6 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamPara
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const float score = p.scores[req * p.scores_s0 + b * p.scores_s1];
     if (lane == 0) {
       // (the terms' exponents were taken x BEAM_LOG2E, which is not log2(e): by it the offset is a logit again, and what is left of
       // the difference, 1.3e-8 of the distance from the largest logit to the mean, is below fp32's half step)
@@ -296,27 +381,84 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamPara
     }
   }
   __syncthreads();
-  const int lists = p.beams * p.slices, total = lists * p.best;
-  const unsigned long long* __restrict__ keys = p.keys + (int64_t)req * total;
-  // candidate i, the lists' first ones first (so that every group of threads has some of the best); false: there is none
-  auto candidate = [&](int i, BeamCandidate& c) {
-    const int rank = i / lists, list = i - rank * lists;
-    c.key = __ldcg(keys + list * p.best + rank);
-    c.beam = list / p.slices;
-    c.score = (double)from_ordered((uint32_t)(c.key >> 32)) + shift[c.beam];
-    return c.key != 0 && c.score == c.score;
+  // candidate i with this key; false: there is none
+  auto candidate = [&](int i, unsigned long long key, BeamCandidate& c) {
+    c.key = key;
+    c.beam = i / per_beam;
+    c.score = (double)from_ordered((uint32_t)(key >> 32)) + shift[c.beam];
+    return key != 0 && c.score == c.score;
   };
   BeamCandidate c;
-  // (the bound in fp32, rounded towards -inf, so that it stays one)
-  float mine = -INFINITY, top;
-  for (int i = threadIdx.x; i < total; i += BEAM_THREADS)
-    if (candidate(i, c)) mine = fmaxf(mine, __double2float_rd(c.score));
-  const float bound = group_bound(mine, groups, low, high, top);
-  for (int i = threadIdx.x; i < total; i += BEAM_THREADS)
-    if (candidate(i, c) && c.score >= (double)bound) {
+  float score[REGS], top = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < REGS; ++k) {
+    const int i = tid + k * BEAM_THREADS;
+    score[k] = i < total && candidate(i, mine[k], c) ? __double2float_rd(c.score) : -INFINITY;
+    top = fmaxf(top, score[k]);
+  }
+  auto beyond = [&](auto fn) {  // those that no register holds
+    for (int i = tid + REGS * BEAM_THREADS; i < total; i += BEAM_THREADS)
+      if (candidate(i, __ldcg(keys + i), c)) fn(__double2float_rd(c.score));
+  };
+  beyond([&](float x) { top = fmaxf(top, x); });
+  top = warp_max(top);
+  if (lane == 0) high[warp] = top;
+  __syncthreads();
+  top = high[0];
+#pragma unroll
+  for (int w = 1; w < BEAM_WARPS; ++w) top = fmaxf(top, high[w]);
+  int turn = 0;
+  auto reach = [&](float least) {  // how many do
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < REGS; ++k) n += score[k] >= least;
+    beyond([&](float x) { n += x >= least; });
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) counts[turn][warp] = n;
+    __syncthreads();
+    n = 0;
+#pragma unroll
+    for (int w = 0; w < BEAM_WARPS; ++w) n += counts[turn][w];
+    turn = turn == 2 ? 0 : turn + 1;
+    return n;
+  };
+  // the threshold: steps that double away from the best until enough reach it, then halves between the last two
+  const int enough = 2 * p.best + 32;
+  float least = -3.4028234e38f;
+  int n = 0;
+  if (top > -INFINITY) {
+    float above = top, step = 1.f;
+    for (; step < 1e6f; step *= 4.f) {
+      n = reach(top - step);
+      if (n >= p.best) {
+        least = top - step;
+        break;
+      }
+      above = top - step;
+    }
+    if (step < 1e6f)
+      for (int i = 0; i < 24 && n > enough; ++i) {
+        const float middle = 0.5f * (above + least);
+        const int m = reach(middle);
+        if (m >= p.best) {
+          least = middle;
+          n = m;
+        } else {
+          above = middle;
+        }
+      }
+  }
+  auto put = [&](int i, unsigned long long key) {
+    if (candidate(i, key, c) && __double2float_rd(c.score) >= least) {
       const int to = atomicAdd(&listed, 1);
       if (to < BEAM_KEYS) list[to] = c;
     }
+  };
+#pragma unroll
+  for (int k = 0; k < REGS; ++k)
+    if (score[k] >= least) put(tid + k * BEAM_THREADS, mine[k]);
+  for (int i = tid + REGS * BEAM_THREADS; i < total; i += BEAM_THREADS) put(i, __ldcg(keys + i));
+  for (int i = tid; i < BEAM_KEYS; i += BEAM_THREADS) place[i] = 0;
   __syncthreads();
   auto store = [&](int at, float score, int64_t beam, int64_t token) {
     p.out_scores[req * p.out_scores_s0 + at] = score;
@@ -330,23 +472,29 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamPara
       static_cast<int*>(p.out_tokens)[req * p.out_tokens_s0 + at] = (int)token;
   };
   auto store_candidate = [&](int at, const BeamCandidate& x) { store(at, (float)x.score, x.beam, 0xffffffffu - (uint32_t)x.key); };
-  const int n = listed;
+  n = listed;
   if (n <= BEAM_KEYS) {
-    for (int i = threadIdx.x; i < n; i += BEAM_THREADS) {
+    // ranked by counting; where they are few, several threads share one's count
+    int parts = 1;
+    while (parts < 8 && n * parts * 2 <= BEAM_THREADS) parts *= 2;
+    for (int i = tid / parts; i < n; i += BEAM_THREADS / parts) {
       c = list[i];
       int rank = 0;
-      for (int k = 0; k < n; ++k) rank += before(list[k], c);
-      if (rank < p.best) store_candidate(rank, c);
+      for (int k = tid & (parts - 1); k < n; k += parts) rank += before(list[k], c);
+      if (rank != 0) atomicAdd(&place[i], rank);
     }
-    for (int i = n + (int)threadIdx.x; i < p.best; i += BEAM_THREADS) store(i, -INFINITY, -1, -1);
+    __syncthreads();
+    for (int i = tid; i < n; i += BEAM_THREADS)
+      if (place[i] < p.best) store_candidate(place[i], list[i]);
+    for (int i = n + tid; i < p.best; i += BEAM_THREADS) store(i, -INFINITY, -1, -1);
     return;
   }
-  // one at a time: the best of what comes behind the last one
+  // equal scores without end: one at a time, the best of what comes behind the last one
   BeamCandidate last = {(double)INFINITY, 0, -1};
   for (int r = 0; r < p.best; ++r) {
     BeamCandidate most = {-(double)INFINITY, 0, 0x7fffffff};
-    for (int i = threadIdx.x; i < total; i += BEAM_THREADS)
-      if (candidate(i, c) && before(last, c) && before(c, most)) most = c;
+    for (int i = tid; i < total; i += BEAM_THREADS)
+      if (candidate(i, __ldcg(keys + i), c) && before(last, c) && before(c, most)) most = c;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       BeamCandidate other;
@@ -361,7 +509,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamPara
 #pragma unroll
     for (int w = 1; w < BEAM_WARPS; ++w)
       if (before(from_warp[w], last)) last = from_warp[w];
-    if (threadIdx.x == 0) store_candidate(r, last);
+    if (tid == 0) store_candidate(r, last);
     __syncthreads();
   }
 }
@@ -379,7 +527,7 @@ struct ReorderParams {
   const void* ends;
   int64_t table_rows, width, table_s0, rows_s0, beams_s0, out_rows_s0;
   int32_t from, to, words, rows_64, beams_64, out_rows_64, starts_64, ends_64;  // words: of an element
-  int32_t columns;  // of a CTA, in words
+  int32_t shift;  // a CTA has 2^shift columns, in words
 };
 
 // A CTA has some columns of all of a request's rows: it reads every word that it moves before it writes any, so that rows may
@@ -393,7 +541,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_reorder_kernel(const Reorde
   bool bad = lo < 0 || lo > whole || hi < 0 || hi > whole;
   lo = (lo < 0 ? 0 : lo > whole ? whole : lo) * p.words;
   hi = (hi < 0 ? 0 : hi > whole ? whole : hi) * p.words;
-  const int64_t first = lo + (int64_t)blockIdx.x * p.columns;
+  const int64_t first = lo + ((int64_t)blockIdx.x << p.shift);
   if (first >= hi && blockIdx.x > 0) return;
   if ((int)threadIdx.x < p.to) {
     int64_t s = -1, t = -1;
@@ -411,17 +559,17 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_reorder_kernel(const Reorde
   }
   if (bad) flag_error(FT_DEV_BAD_ROW_INDEX);
   __syncthreads();
-  const int columns = first >= hi ? 0 : (int)(hi - first < p.columns ? hi - first : p.columns);
+  const int columns = first >= hi ? 0 : (int)(hi - first < (1 << p.shift) ? hi - first : 1 << p.shift);
   uint32_t x[REORDER_WORDS];
 #pragma unroll
   for (int j = 0; j < REORDER_WORDS; ++j) {
-    const int i = j * BEAM_THREADS + (int)threadIdx.x, r = i / p.columns, c = i - r * p.columns;
+    const int i = j * BEAM_THREADS + (int)threadIdx.x, r = i >> p.shift, c = i & ((1 << p.shift) - 1);
     if (r < p.to && c < columns && target[r] >= 0) x[j] = p.table[source[r] * p.table_s0 + first + c];
   }
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < REORDER_WORDS; ++j) {
-    const int i = j * BEAM_THREADS + (int)threadIdx.x, r = i / p.columns, c = i - r * p.columns;
+    const int i = j * BEAM_THREADS + (int)threadIdx.x, r = i >> p.shift, c = i & ((1 << p.shift) - 1);
     if (r < p.to && c < columns && target[r] >= 0) p.table[target[r] * p.table_s0 + first + c] = x[j];
   }
 }

@@ -66,17 +66,28 @@ int check_beam_select(const ft_beam_select_args* a) {
   return FT_OK;
 }
 
-// Slices of a row: of four chunks where that leaves every SM CTAs enough to hide each other's waits, of fewer and smaller ones where
-// the call is small and its length is what one slice takes.  (148 SMs whatever the device: the workspace's size goes by this.)
+// Slices of a row, of whole chunks but for the last: of those sizes the one whose rounds of CTAs, three to an SM, end first.  A CTA takes
+// 1.1 us per chunk of 16 KB with the others' share of memory and 2 us beside, with fewer on its SM less by as much; chunks are
+// smaller where the call would leave SMs without any.  (148 SMs whatever the device: the workspace's size goes by this.)
 BeamShape beam_shape(const ft_beam_select_args* a) {
   BeamShape s;
   const int n = 16 / dtype_size(a->dtype);
   const int64_t rows = (int64_t)a->batch * a->beams;
-  int64_t slice = (int64_t)ft::BEAM_THREADS * n * 16;
-  while (slice > ft::BEAM_THREADS * n && rows * ((a->vocab + slice - 1) / slice) < 6 * 148) slice /= 2;
-  s.pieces = (int)std::min<int64_t>(4, slice / (ft::BEAM_THREADS * n));
-  s.slices = (int)((a->vocab + slice - 1) / slice);
-  s.slice_len = (int)((((int64_t)a->vocab + s.slices - 1) / s.slices + n - 1) / n * n);
+  for (s.pieces = 4; s.pieces > 1; s.pieces /= 2) {
+    const int64_t chunk = (int64_t)ft::BEAM_THREADS * n * s.pieces;
+    if (rows * ((a->vocab + chunk - 1) / chunk) >= 2 * 148) break;
+  }
+  const int64_t chunk = (int64_t)ft::BEAM_THREADS * n * s.pieces, chunks = (a->vocab + chunk - 1) / chunk;
+  double best = -1;
+  for (int m = 1; m <= 16 && m <= chunks; ++m) {
+    const int64_t slices = (chunks + m - 1) / m, ctas = rows * slices, rounds = (ctas + 3 * 148 - 1) / (3 * 148);
+    const double t = rounds * (2.0 + 1.1 * m);
+    if (best < 0 || t < best) {
+      best = t;
+      s.slices = (int)slices;
+      s.slice_len = (int)(m * chunk);
+    }
+  }
   s.keys = rows * s.slices * a->best;
   s.bytes = s.keys * 8 + rows * s.slices * 8;
   return s;
@@ -87,26 +98,29 @@ int pow2_at_least(int n, int low) {
   return low;
 }
 
-template <typename T, int NV>
-void launch_scan(const ft::BeamParams& p, int groups, bool vec, cudaStream_t st) {
-  const unsigned ctas = (unsigned)((int64_t)p.batch * p.beams * p.slices);
-  if (vec)
-    ft::beam_scan_kernel<T, NV, true><<<ctas, ft::BEAM_THREADS, 0, st>>>(p, groups);
-  else
-    ft::beam_scan_kernel<T, NV, false><<<ctas, ft::BEAM_THREADS, 0, st>>>(p, groups);
+template <typename T, int NV, bool VEC>
+int launch_scan_as(const ft::BeamParams& p, int groups, cudaStream_t st) {
+  auto kernel = ft::beam_scan_kernel<T, NV, VEC>;
+  static OncePerDevice once;
+  FT_CUDA_OK(raise_smem_limit(once, kernel, ft::BeamScan<NV>::SMEM_BYTES));
+  kernel<<<(unsigned)((int64_t)p.batch * p.beams * p.slices), ft::BEAM_THREADS, ft::BeamScan<NV>::SMEM_BYTES, st>>>(p, groups);
+  FT_CUDA_OK(cudaGetLastError());
+  count_launch();
+  return FT_OK;
 }
 
 template <typename T>
 int launch_beam_select(const ft::BeamParams& p, int pieces, bool vec, cudaStream_t st) {
   const int groups = pow2_at_least(p.best, ft::BEAM_WARPS);
-  switch (pieces) {
-    case 1: launch_scan<T, 1>(p, groups, vec, st); break;
-    case 2: launch_scan<T, 2>(p, groups, vec, st); break;
-    default: launch_scan<T, 4>(p, groups, vec, st); break;
-  }
-  FT_CUDA_OK(cudaGetLastError());
-  count_launch();
-  FT_CUDA_OK(launch_early(ft::beam_merge_kernel, dim3((unsigned)p.batch), ft::BEAM_THREADS, 0, st, p, groups));
+  const int rc = pieces == 1   ? (vec ? launch_scan_as<T, 1, true>(p, groups, st) : launch_scan_as<T, 1, false>(p, groups, st))
+                 : pieces == 2 ? (vec ? launch_scan_as<T, 2, true>(p, groups, st) : launch_scan_as<T, 2, false>(p, groups, st))
+                               : (vec ? launch_scan_as<T, 4, true>(p, groups, st) : launch_scan_as<T, 4, false>(p, groups, st));
+  if (rc != FT_OK) return rc;
+  const int total = p.beams * p.slices * p.best;
+  if (total <= 2 * ft::BEAM_THREADS)
+    FT_CUDA_OK(launch_early(ft::beam_merge_kernel<2>, dim3((unsigned)p.batch), ft::BEAM_THREADS, 0, st, p));
+  else
+    FT_CUDA_OK(launch_early(ft::beam_merge_kernel<16>, dim3((unsigned)p.batch), ft::BEAM_THREADS, 0, st, p));
   count_launch();
   return FT_OK;
 }
@@ -232,8 +246,8 @@ int ft_beam_reorder(const ft_beam_reorder_args* a) {
   p.rows_s0 = a->rows_stride0, p.beams_s0 = a->beams_stride0, p.out_rows_s0 = a->out_rows_stride0;
   p.from = a->from, p.to = a->to;
   p.rows_64 = a->rows_64, p.beams_64 = a->beams_64, p.out_rows_64 = a->out_rows_64, p.starts_64 = a->starts_64, p.ends_64 = a->ends_64;
-  p.columns = ft::REORDER_WORDS * ft::BEAM_THREADS / a->to;
-  const int64_t chunks = (p.width + p.columns - 1) / p.columns;
+  for (p.shift = 12; pow2_at_least(a->to, 1) << p.shift > ft::REORDER_WORDS * ft::BEAM_THREADS;) --p.shift;
+  const int64_t chunks = (p.width + (1 << p.shift) - 1) >> p.shift;
   if (chunks > 0x7fffffffLL) return fail(FT_ERR_TOO_LARGE, "the table's rows are too long for one launch");
   FT_CUDA_OK(launch_early(ft::beam_reorder_kernel, dim3((unsigned)chunks, (unsigned)a->batch), ft::BEAM_THREADS, 0, static_cast<cudaStream_t>(a->stream), p));
   count_launch();
