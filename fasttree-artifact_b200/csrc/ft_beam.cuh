@@ -16,7 +16,9 @@
 namespace ft {
 
 constexpr int BEAM_THREADS = 256, BEAM_WARPS = BEAM_THREADS / 32;
-constexpr int BEAM_KEYS = 1024;  // candidates that a CTA lists; beyond that, which takes many equal logits, it picks one at a time
+constexpr int BEAM_LIST = 512;   // logits that a slice lists, and pieces with one that it sets aside behind its first chunk; where more
+constexpr int BEAM_ASIDE = 96;   // reach its bound, it goes over the slice again with the list cut on the way
+constexpr int BEAM_KEYS = 1024;  // candidates that the merge lists; beyond that, which takes many equal scores, it picks one at a time
 
 struct BeamParams {
   const void* logits;
@@ -27,32 +29,29 @@ struct BeamParams {
   unsigned long long* keys;  // [rows][slices][best] {ordered logit, ~token}, 0: none
   float2* sums;              // [rows][slices] {c, sum of 2^(logit log2(e) - c)}
   int64_t logits_s0, logits_s1, scores_s0, scores_s1, out_scores_s0, out_beams_s0, out_tokens_s0;
-  int32_t batch, beams, vocab, best, slices, slice_len, beams_64, tokens_64;  // slice_len: a multiple of 16 bytes
+  int32_t batch, beams, vocab, best, beams_64, tokens_64;
+  int32_t slices, chunks, per_cta;  // most slices of a row, its chunks, chunks of a CTA
 };
 
-// A lower bound of the n-th largest of a block's values that n of them reach, from each thread's largest: the least of the
-// largest of `groups` groups of threads, groups >= n a power of two up to BEAM_THREADS.  `largest`: of all.  A whole block; between
-// calls with the same shared memory there has to be a barrier.
-__device__ __forceinline__ float group_bound(float mine, int groups, float (&low)[BEAM_WARPS], float (&high)[BEAM_WARPS], float& largest) {
+// The scan's BEAM_THREADS threads that read logits; one more warp sends for them.
+__device__ __forceinline__ void beam_sync() { asm volatile("bar.sync 1, %0;\n" ::"n"(BEAM_THREADS) : "memory"); }
+
+// A lower bound of the n-th largest of those threads' values that n of them reach, from each thread's largest: the least of the
+// largest of `groups` groups of threads, groups >= n a power of two up to BEAM_THREADS.  By all of them; between calls with the same
+// shared memory there has to be a barrier.
+__device__ __forceinline__ float group_bound(float mine, int groups, float (&low)[BEAM_WARPS]) {
   const int lanes = BEAM_THREADS / groups;  // of a group, if that is less than a warp
-  float top = mine, bound = mine;
+  float bound = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float other = __shfl_xor_sync(0xffffffffu, bound, o);
     bound = o < lanes ? fmaxf(bound, other) : fminf(bound, other);
   }
-  if ((threadIdx.x & 31) == 0) {
-    low[threadIdx.x >> 5] = bound;
-    high[threadIdx.x >> 5] = top;
-  }
-  __syncthreads();
-  bound = low[0], largest = high[0];
+  if ((threadIdx.x & 31) == 0) low[threadIdx.x >> 5] = bound;
+  beam_sync();
+  bound = low[0];
 #pragma unroll
-  for (int w = 1; w < BEAM_WARPS; ++w) {
-    bound = fminf(bound, low[w]);
-    largest = fmaxf(largest, high[w]);
-  }
+  for (int w = 1; w < BEAM_WARPS; ++w) bound = fminf(bound, low[w]);
   return bound;
 }
 
@@ -66,15 +65,15 @@ __device__ __forceinline__ unsigned long long warp_max_key(unsigned long long k)
 constexpr float BEAM_LOG2E = 1.4426950408889634f;
 
 // The best of a list of n keys into out[0 .. best), 0 where the list ends: ranked by counting, or one at a time, whichever
-// takes fewer instructions.  A whole block, behind a barrier.
-__device__ __forceinline__ void best_of_list(const unsigned long long* keys, int n, unsigned long long* __restrict__ out, int best,
+// takes fewer instructions.  By all threads of the scan, behind a barrier.
+__device__ __forceinline__ void best_of_list(const unsigned long long* keys, int n, unsigned long long* out, int best,
                                              unsigned long long (&from_warp)[BEAM_WARPS]) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (n <= 128 + 16 * best) {
     for (int i = threadIdx.x; i < n; i += BEAM_THREADS) {
       const unsigned long long key = keys[i];
       int rank = 0;
-#pragma unroll 4
+#pragma unroll 8
       for (int k = 0; k < n; ++k) rank += keys[k] > key;
       if (rank < best) out[rank] = key;
     }
@@ -88,10 +87,10 @@ __device__ __forceinline__ void best_of_list(const unsigned long long* keys, int
       if (keys[i] < last) key = max(key, keys[i]);
     key = warp_max_key(key);
     if (lane == 0) from_warp[warp] = key;
-    __syncthreads();
+    beam_sync();
     last = warp_max_key(from_warp[lane & (BEAM_WARPS - 1)]);
     if (threadIdx.x == 0) out[r] = last;
-    __syncthreads();
+    beam_sync();
   }
 }
 
@@ -107,226 +106,337 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
-// One slice of one row, in chunks of NV x 16 bytes a thread that come by bulk copies, three chunks ahead.
+// Chunks of NV x 16 bytes a thread, that one warp sends for, three ahead of the eight that read them.  The call's rows are cut into
+// p.chunks chunks each, and a CTA takes p.per_cta of them as they follow one another: the end of a row, rows, the start of one.  What it
+// has of a row is a slice: slice number s of a row is that of the s-th CTA that has some of it.
 //
 // VEC: rows start on 16 bytes, and a thread reads 16 bytes at a time; else it reads words of 4 (a rule of the call, not of the row, so
-// that equal rows have equal sums).  Copies are of whole 16-byte pieces inside the row; what stands at its ends is filled in.
+// that equal rows cut alike have equal sums).  Copies are of whole 16-byte pieces inside the row; what stands at its ends is filled in.
 //
-// The sum: each thread has its own running maximum and adds 2^(x log2(e) - c), c = maximum x log2(e).
-// The `best` largest: in the first chunk each group of threads (a warp for up to 8 results) has a largest logit, and the least of them
-// bounds the `best`-th from below; what reaches it, 22 of 8192 logits on average for 8 groups, is listed, and what of the other chunks
-// does.  Where equal logits overflow the list, the best of the list and the chunk are picked one at a time.
+// The sum: each thread adds 2^(x log2(e) - c), c = its maximum x log2(e), which may lag by 8 (then by 2^11.5 a term).
+// The `best` largest: in a slice's first chunk each group of threads (a warp for up to 8 results) has a largest logit, and the least of
+// them bounds the `best`-th from below; what reaches it, 22 of 8192 logits on average for 8 groups, is listed, the list cut to the best,
+// and the last of those is the new bound; so again when four times as many chunks have passed (twice as many for more than 16 results),
+// so that about three times (once) `best` logits reach it in between, when the warps do not wait for each other.  A thread whose piece reaches the bound notes the piece, and the logits that do
+// are found by all threads together: done on the spot it takes the whole warp for one thread's.
 template <typename T, int NV, bool VEC>
-__global__ void __launch_bounds__(BEAM_THREADS, 3) beam_scan_kernel(const BeamParams p, const int groups) {
+__global__ void __launch_bounds__(BEAM_THREADS + 32, 3) beam_scan_kernel(const BeamParams p, const int groups) {
   using C = BeamScan<NV>;
-  constexpr int S = (int)sizeof(T), N = 16 / S, CHUNK = BEAM_THREADS * NV * N;
+  constexpr int S = (int)sizeof(T), N = 16 / S, CHUNK = BEAM_THREADS * NV * N, PAIR = NV > 1 ? 2 : 1;
+  constexpr int PIECES = BEAM_THREADS * NV / PAIR, E = PAIR * N;  // pieces (of one or two vectors) of a chunk, their elements
   constexpr uint32_t NONE = S == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;  // -inf
+  constexpr float LEAST = -3.4028234e38f, LAG = 8.f;
   extern __shared__ __align__(128) uint8_t stages[];
-  __shared__ unsigned long long keys[BEAM_KEYS];
-  __shared__ float low[BEAM_WARPS], high[BEAM_WARPS];
+  __shared__ unsigned long long keys[BEAM_LIST];
+  __shared__ float low[BEAM_WARPS];
   __shared__ float2 sums[BEAM_WARPS];
   __shared__ unsigned long long from_warp[BEAM_WARPS], picked[FT_MAX_BEAMS];
-  __shared__ __align__(8) unsigned long long barrier[C::STAGES];
-  __shared__ int more[3];  // listed by a chunk, by turns: the next chunk's is cleared before a chunk's last barrier
+  __shared__ __align__(8) unsigned long long barrier[2 * C::STAGES];  // full, empty
+  __shared__ __align__(16) uint4 aside[BEAM_ASIDE][PAIR];
+  __shared__ uint32_t aside_at[BEAM_ASIDE];              // chunk of the row x PIECES + piece
+  __shared__ uint16_t pieces[BEAM_THREADS * NV / PAIR];  // of the first chunk
+  __shared__ int listed, noted, more[3];
+  __shared__ volatile int dead;  // a wait has run out
   allow_dependent_launch();
   wait_for_prior_grid();
-  const int row = (int)(blockIdx.x / (unsigned)p.slices), slice = (int)(blockIdx.x - (unsigned)row * p.slices);
-  const int req = row / p.beams, beam = row - req * p.beams, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  unsigned long long* __restrict__ out = p.keys + (int64_t)blockIdx.x * p.best;
-  const int begin = slice * p.slice_len, end = min(p.vocab, begin + p.slice_len);
-  const float score = __ldg(p.scores + req * p.scores_s0 + beam * p.scores_s1);
-  if (!(fabsf(score) < INFINITY) || begin >= end) {  // nothing comes from this beam
-    for (int i = tid; i < p.best; i += BEAM_THREADS) out[i] = 0;
-    if (tid == 0) p.sums[blockIdx.x] = make_float2(-INFINITY, 0.f);
-    return;
-  }
-  const T* __restrict__ base = static_cast<const T*>(p.logits) + req * p.logits_s0 + beam * p.logits_s1;
-  const uintptr_t row_at = reinterpret_cast<uintptr_t>(base), row_end = row_at + (int64_t)p.vocab * S;
-  const uint32_t bars = (uint32_t)__cvta_generic_to_shared(barrier), ring = (uint32_t)__cvta_generic_to_shared(stages);
-  // a chunk's bytes: from `at` (its stage begins at the 16-byte border below), of which [from, to) are copied
-  struct Span {
-    uintptr_t at, from, to;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t all_chunks = (int64_t)p.batch * p.beams * p.chunks, chunk0 = (int64_t)blockIdx.x * p.per_cta;
+  const int todo = (int)(all_chunks - chunk0 < p.per_cta ? all_chunks - chunk0 : p.per_cta);
+  const uint32_t full0 = (uint32_t)__cvta_generic_to_shared(barrier), empty0 = full0 + 8 * C::STAGES;
+  struct Row {
+    uintptr_t at;
+    bool live;  // else nothing comes from this beam
   };
-  auto span_of = [&](int first) {
-    const uintptr_t a = row_at + (int64_t)first * S, b = row_at + (int64_t)min(end, first + CHUNK) * S;
-    Span s = {a, a & ~(uintptr_t)15, (b + 15) & ~(uintptr_t)15};
-    if (s.from < row_at) s.from += 16;
-    if (s.to > row_end) s.to -= 16;
-    if (s.to < s.from) s.to = s.from;
-    return s;
+  auto row_of = [&](int row) {
+    const int req = row / p.beams, beam = row - req * p.beams;
+    const float score = __ldg(p.scores + req * p.scores_s0 + beam * p.scores_s1);
+    return Row{reinterpret_cast<uintptr_t>(static_cast<const T*>(p.logits) + req * p.logits_s0 + beam * p.logits_s1), fabsf(score) < INFINITY};
   };
-  auto issue = [&](int chunk) {
-    const int first = begin + chunk * CHUNK;
-    if (first >= end) return;
-    const Span s = span_of(first);
-    const uint32_t bytes = (uint32_t)(s.to - s.from), bar = bars + 8 * (chunk % C::STAGES);
-    mbar_arrive_expect_tx(bar, bytes);
-    if (bytes > 0)
-      bulk_load(ring + (chunk % C::STAGES) * C::STAGE_BYTES + (uint32_t)(s.from - (s.at & ~(uintptr_t)15)), reinterpret_cast<const void*>(s.from), bytes, bar);
+  int row = (int)(chunk0 / p.chunks), k = (int)(chunk0 - (int64_t)row * p.chunks), stage = 0;
+  uint32_t phase = 0;
+  Row here = {0, false};
+  bool fresh = true;  // a slice begins
+  auto await = [&](uint32_t bar, uint32_t parity) {
+    if (dead == 0 && !mbar_wait_warp(bar, parity, C::WAIT_LIMIT)) dead = 1;
+  };
+  auto advance = [&]() {
+    if (++stage == C::STAGES) {
+      stage = 0;
+      phase ^= 1u;
+    }
+    if (++k == p.chunks) {
+      k = 0;
+      ++row;
+    }
   };
   if (tid == 0) {
-    for (int i = 0; i < C::STAGES; ++i) mbar_init(bars + 8 * i, 1);
+    for (int i = 0; i < C::STAGES; ++i) {
+      mbar_init(full0 + 8 * i, 1);
+      mbar_init(empty0 + 8 * i, BEAM_WARPS);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     proxy_fence();
-    for (int i = 0; i < C::STAGES; ++i) issue(i);
+    listed = noted = 0;
+    dead = 0;
   }
   if (tid < 3) more[tid] = 0;
   __syncthreads();
-  float top = -INFINITY, off = 0.f, sum = 0.f, least = -3.4028234e38f;
-  int listed = 0, turn = 0, chunk = 0;
-  uint32_t phase = 0;
-  bool late = false;
-#pragma unroll 1
-  for (int first = begin; first < end; first += CHUNK, ++chunk) {
-    const int stage = chunk % C::STAGES;
-    const int len = min(end - first, CHUNK);
-    const Span s = span_of(first);
-    uint8_t* const bytes = stages + stage * C::STAGE_BYTES;
-    const uint32_t shift = (uint32_t)(s.at & 15);
-    late |= !mbar_wait_warp(bars + 8 * stage, phase, C::WAIT_LIMIT);
-    if (stage == C::STAGES - 1) phase ^= 1u;
-    const uintptr_t stop = s.at + (int64_t)len * S, whole = (stop + 15) & ~(uintptr_t)15;
-    if (s.from > s.at || s.to < whole) {  // the row's ends, and -inf up to the next 16 bytes
-      if (tid < 2 * N) {
-        const uintptr_t at = tid < N ? s.at + tid * S : s.to + (tid - N) * S;
-        if (tid < N ? at < s.from && at < stop : at < whole && at >= s.at && at >= s.from)
-          *reinterpret_cast<T*>(bytes + (at - (s.at & ~(uintptr_t)15))) = at < stop ? *reinterpret_cast<const T*>(at) : from_float<T>(-INFINITY);
+  if (warp == BEAM_WARPS) {
+    // ---- a chunk's bytes: from `at`, whose stage begins at the 16-byte border below; [from, to) are copied, the rest, at the row's ends,
+    // is filled in, with -inf up to the next border
+    for (int n = 0; n < todo; ++n) {
+      if (n == 0 || k == 0) here = row_of(row);
+      const uint32_t full = full0 + 8 * stage;
+      await(empty0 + 8 * stage, phase ^ 1u);
+      uint32_t bytes = 0, to_stage = 0;
+      uintptr_t from = 0;
+      if (here.live) {
+        const int first = k * CHUNK;
+        const uintptr_t at = here.at + (int64_t)first * S, stop = here.at + (int64_t)min(p.vocab, first + CHUNK) * S;
+        const uintptr_t border = at & ~(uintptr_t)15, whole = (stop + 15) & ~(uintptr_t)15;
+        uintptr_t to = whole;
+        from = border < here.at ? border + 16 : border;
+        if (to > here.at + (int64_t)p.vocab * S) to -= 16;
+        if (to < from) to = from;
+        bytes = (uint32_t)(to - from);
+        uint8_t* const mine = stages + stage * C::STAGE_BYTES;
+        to_stage = (uint32_t)__cvta_generic_to_shared(mine + (from - border));
+        if (lane < 2 * N) {
+          const uintptr_t x = lane < N ? at + lane * S : to + (lane - N) * S;
+          if (lane < N ? x < from && x < stop : x < whole && x >= at && x >= from)
+            *reinterpret_cast<T*>(mine + (x - border)) = x < stop ? *reinterpret_cast<const T*>(x) : from_float<T>(-INFINITY);
+        }
+        proxy_fence();
       }
-      proxy_fence();
-      __syncthreads();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive_expect_tx(full, bytes);
+        if (bytes > 0) bulk_load(to_stage, reinterpret_cast<const void*>(from), bytes, full);
+      }
+      __syncwarp();
+      advance();
     }
-    // word w of piece j; number of its first element in the chunk
-    auto number = [&](int j, int e) {
-      if constexpr (VEC) return (j * BEAM_THREADS + tid) * N + e;
-      if constexpr (S == 4) return (4 * j + e) * BEAM_THREADS + tid;
-      return 2 * ((4 * j + (e >> 1)) * BEAM_THREADS + tid) + (e & 1);
+  } else {
+    // number in the chunk of element e of thread t's vector j
+    auto number_of = [&](int t, int j, int e) {
+      if constexpr (VEC) return (j * BEAM_THREADS + t) * N + e;
+      if constexpr (S == 4) return (4 * j + e) * BEAM_THREADS + t;
+      return 2 * ((4 * j + (e >> 1)) * BEAM_THREADS + t) + (e & 1);
     };
-    uint4 x[NV];
+    auto number = [&](int j, int e) { return number_of(tid, j, e); };
+    auto list = [&](float y, int at) {
+      const int to = atomicAdd(&listed, 1);
+      if (to < BEAM_LIST) keys[to] = ((unsigned long long)ordered(y) << 32) | (0xffffffffu - (uint32_t)at);
+    };
+    float top = -INFINITY, off = 0.f, least = LEAST;
+    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    int from_k = 0;     // the slice's first chunk
+    bool lost = false;  // more reached the bound than there was room for
+#pragma unroll 1
+    for (int n = 0; n < todo; ++n) {
+      if (fresh) {
+        here = row_of(row);
+        from_k = k;
+      }
+      const int first = k * CHUNK, len = p.vocab - first;
+      const uint32_t shift = VEC ? 0u : (uint32_t)(here.at & 15);
+      const uint8_t* const bytes = stages + stage * C::STAGE_BYTES + shift;
+      auto load = [&](auto full, int j) {
+        constexpr bool FULL = decltype(full)::value;
+        if constexpr (VEC) {
+          return FULL || number(j, 0) < len ? *reinterpret_cast<const uint4*>(bytes + number(j, 0) * S) : make_uint4(NONE, NONE, NONE, NONE);
+        } else {
+          uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if constexpr (VEC) {
-        x[j] = number(j, 0) < len ? *reinterpret_cast<const uint4*>(bytes + number(j, 0) * S) : make_uint4(NONE, NONE, NONE, NONE);
-      } else {
-        uint32_t w[4];
+          for (int e = 0; e < 4; ++e) {
+            const int i = number(j, e * (4 / S));
+            if constexpr (S == 4) {
+              w[e] = FULL || i < len ? *reinterpret_cast<const uint32_t*>(bytes + i * S) : NONE;
+            } else if (FULL && (shift & 2) == 0) {
+              w[e] = *reinterpret_cast<const uint32_t*>(bytes + i * S);
+            } else {
+              const uint32_t a = FULL || i < len ? *reinterpret_cast<const uint16_t*>(bytes + i * S) : NONE & 0xffffu;
+              w[e] = a | (FULL || i + 1 < len ? (uint32_t)*reinterpret_cast<const uint16_t*>(bytes + i * S + 2) << 16 : NONE & 0xffff0000u);
+            }
+          }
+          return make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      };
+      auto pass = [&](auto full) {
+        if (fresh) {
+          float mine = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = number(j, e * (4 / S));
-          const uint8_t* const from = bytes + shift + i * S;
-          if constexpr (S == 4) {
-            w[e] = i < len ? *reinterpret_cast<const uint32_t*>(from) : NONE;
-          } else {
-            const uint32_t a = i < len ? *reinterpret_cast<const uint16_t*>(from) : NONE & 0xffffu;
-            w[e] = a | (i + 1 < len ? (uint32_t)*reinterpret_cast<const uint16_t*>(from + 2) << 16 : NONE & 0xffff0000u);
+          for (int j = 0; j < NV; ++j) mine = fmaxf(mine, vec_max<T>(load(full, j)));
+          least = fmaxf(LEAST, group_bound(mine, groups, low));
+          top = mine;
+          off = top == -INFINITY ? 0.f : top * BEAM_LOG2E;
+        }
+        float2 off2 = make_float2(-off, -off);
+        float gate = top == -INFINITY ? LEAST : fminf(least, top + LAG);  // below it a piece needs nothing but its sum
+#pragma unroll
+        for (int j = 0; j < NV; j += PAIR) {
+          uint4 x[PAIR];
+          float most = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < PAIR; ++u) x[u] = load(full, j + u);
+          if constexpr (PAIR == 2 && S == 2)
+            most = vec_max<T>(make_uint4(max2(x[0].x, x[1].x, T()), max2(x[0].y, x[1].y, T()), max2(x[0].z, x[1].z, T()), max2(x[0].w, x[1].w, T())));
+          else
+#pragma unroll
+            for (int u = 0; u < PAIR; ++u) most = fmaxf(most, vec_max<T>(x[u]));
+          if (most >= gate) {
+            if (most > top + LAG || top == -INFINITY) {  // (with +inf, c is it too and the sum NaN, as with NaN)
+              const float c = most * BEAM_LOG2E, f = top == -INFINITY ? 1.f : fast_exp2(off - c);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) sum[i] = __fmul2_rn(sum[i], make_float2(f, f));
+              top = most;
+              off = c;
+              off2 = make_float2(-off, -off);
+              gate = fminf(least, top + LAG);
+            }
+            if (most >= least) {
+              const int to = atomicAdd(&noted, 1), piece = (j / PAIR) * BEAM_THREADS + tid;
+              if (fresh) {
+                pieces[to] = (uint16_t)piece;
+              } else if (to < BEAM_ASIDE) {
+#pragma unroll
+                for (int u = 0; u < PAIR; ++u) aside[to][u] = x[u];
+                aside_at[to] = (uint32_t)k * PIECES + piece;
+              }
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < PAIR; ++u) {
+            const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+#pragma unroll
+            for (int e = 0; e < N / 2; ++e) {
+              float2 y;
+              if constexpr (S == 4)
+                y = make_float2(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
+              else
+                y = unpack2<T>(w[e]);
+              y = __ffma2_rn(y, make_float2(BEAM_LOG2E, BEAM_LOG2E), off2);
+              sum[e & 1] = __fadd2_rn(sum[e & 1], make_float2(fast_exp2(y.x), fast_exp2(y.y)));
+            }
           }
         }
-        x[j] = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-    }
-    float piece[NV], mine = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      piece[j] = vec_max<T>(x[j]);
-      mine = fmaxf(mine, piece[j]);
-    }
-    if (mine > top) {  // (with +inf, c is it too and the sum NaN, as with NaN)
-      const float c = mine * BEAM_LOG2E;
-      sum = top == -INFINITY ? sum : sum * fast_exp2(off - c);
-      top = mine;
-      off = c;
-    }
-    float2 sum2[2] = {make_float2(sum, 0.f), make_float2(0.f, 0.f)};
-    const float2 scale2 = make_float2(BEAM_LOG2E, BEAM_LOG2E), off2 = make_float2(-off, -off);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
-#pragma unroll
-      for (int e = 0; e < N / 2; ++e) {
-        float2 y;
-        if constexpr (S == 4)
-          y = make_float2(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
+      };
+      await(full0 + 8 * stage, phase);
+      if (here.live) {
+        if (len >= CHUNK)
+          pass(std::true_type{});
         else
-          y = unpack2<T>(w[e]);
-        y = __ffma2_rn(y, scale2, off2);
-        sum2[e & 1] = __fadd2_rn(sum2[e & 1], make_float2(fast_exp2(y.x), fast_exp2(y.y)));
+          pass(std::false_type{});
       }
-    }
-    sum = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
-    if (first == begin) {
-      float all;
-      least = fmaxf(least, group_bound(mine, groups, low, high, all));
-    }
-    // what reaches the bound (the pieces are unpacked anew: kept since the sum they would take 100 registers)
-    if (__any_sync(0xffffffffu, mine >= least)) {
-      uint32_t hits = 0;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        if (!__any_sync(0xffffffffu, piece[j] >= least)) continue;
-        asm volatile("" : "+r"(x[j].x), "+r"(x[j].y), "+r"(x[j].z), "+r"(x[j].w));
-#pragma unroll
-        for (int e = 0; e < N; ++e) hits |= vec_at<T>(x[j], e) >= least ? 1u << (j * N + e) : 0u;
-      }
-      if (hits != 0) {
-        int to = listed + atomicAdd(&more[turn], __popc(hits));
-        for (; hits != 0; hits &= hits - 1, ++to) {
-          const int bit = __ffs(hits) - 1, i = number(bit / N, bit % N);
-          const float y = to_float<T>(*reinterpret_cast<const T*>(bytes + shift + i * S));
-          if (to < BEAM_KEYS) keys[to] = ((unsigned long long)ordered(y) << 32) | (0xffffffffu - (uint32_t)(first + i));
+      __syncwarp();
+      if (!fresh && lane == 0) mbar_arrive(empty0 + 8 * stage);
+      const bool ends = k == p.chunks - 1 || n == todo - 1;
+      const int passed = k - from_k + 1;
+      int count = 0;
+      if (((passed & (passed - 1)) == 0 && (p.best > 16 || (passed & 0x2aaaaaaa) == 0)) || ends) {
+        // the logits of the noted pieces, of the first chunk in its stage
+        beam_sync();
+        const int n_pieces = noted;
+        if (fresh) {
+          for (int i0 = tid; i0 < n_pieces * E; i0 += BEAM_THREADS) {
+            const int piece = pieces[i0 / E], e = i0 % E, i = number_of(piece % BEAM_THREADS, piece / BEAM_THREADS * PAIR + e / N, e % N);
+            const float y = i < len ? to_float<T>(*reinterpret_cast<const T*>(bytes + i * S)) : -INFINITY;
+            if (y >= least) list(y, first + i);
+          }
+        } else {
+          for (int i0 = tid; i0 < min(n_pieces, BEAM_ASIDE) * E; i0 += BEAM_THREADS) {
+            const int q = i0 / E, e = i0 % E, piece = (int)(aside_at[q] % PIECES);
+            const float y = to_float<T>(reinterpret_cast<const T*>(aside[q])[e]);
+            if (y >= least)
+              list(y, (int)(aside_at[q] / PIECES) * CHUNK + number_of(piece % BEAM_THREADS, piece / BEAM_THREADS * PAIR + e / N, e % N));
+          }
+          lost |= n_pieces > BEAM_ASIDE;
+        }
+        beam_sync();
+        if (fresh && lane == 0) mbar_arrive(empty0 + 8 * stage);
+        count = listed;
+        lost |= count > BEAM_LIST;
+        if (!ends) {
+          const bool cut = !lost && count > p.best;
+          if (cut) {
+            best_of_list(keys, count, picked, p.best, from_warp);
+            beam_sync();
+            if (tid < p.best) keys[tid] = picked[tid];
+            least = from_ordered((uint32_t)(picked[p.best - 1] >> 32));
+          } else if (lost) {
+            least = INFINITY;  // the list is made anew in any case
+            beam_sync();
+          }
+          if (tid == 0) {
+            noted = 0;
+            listed = cut ? p.best : count;
+          }
+          beam_sync();
         }
       }
-    }
-    const int next = turn == 2 ? 0 : turn + 1;
-    if (tid == 0) more[next] = 0;
-    __syncthreads();
-    const int now = listed + more[turn];
-    turn = next;
-    if (tid == 0) issue(chunk + C::STAGES);
-    if (now <= BEAM_KEYS) {
-      listed = now;
-      continue;
-    }
-    unsigned long long last = ~0ull;
-#pragma unroll 1
-    for (int r = 0; r < p.best; ++r) {
-      unsigned long long key = 0;
-      for (int i = tid; i < listed; i += BEAM_THREADS)
-        if (keys[i] < last) key = max(key, keys[i]);
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        asm volatile("" : "+r"(x[j].x), "+r"(x[j].y), "+r"(x[j].z), "+r"(x[j].w));
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float y = vec_at<T>(x[j], e);
-          const unsigned long long k = ((unsigned long long)ordered(y) << 32) | (0xffffffffu - (uint32_t)(first + number(j, e)));
-          if (y >= least && k < last) key = max(key, k);
+      fresh = ends;
+      if (ends) {
+        // ---- the slice's list, and the threads' sums over the largest offset
+        const int64_t slice = (int64_t)blockIdx.x - (int64_t)row * p.chunks / p.per_cta, at = (int64_t)row * p.slices + slice;
+        const float mine = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        const float mine_off = top == -INFINITY ? -INFINITY : off;
+        const float warp_off = warp_max(mine_off), from = warp_off == -INFINITY ? 0.f : warp_off;
+        const float total = warp_sum(mine == 0.f ? 0.f : mine * fast_exp2(mine_off - from));
+        if (lane == 0) sums[warp] = make_float2(warp_off, total);
+        if (lost) {
+          // more than the list holds, equal ones for the most part: a logit a thread at a time, cutting the list when it may overflow
+          const T* const logits = reinterpret_cast<const T*>(here.at);
+          const int stop = min(p.vocab, first + CHUNK);
+          unsigned long long bound = 0;
+          int turn = 0;
+          count = 0;
+          for (int i0 = from_k * CHUNK; i0 < stop; i0 += BEAM_THREADS) {
+            const int i = i0 + tid, next = turn == 2 ? 0 : turn + 1;
+            const float y = i < stop ? to_float<T>(logits[i]) : -INFINITY;
+            const unsigned long long key = ((unsigned long long)ordered(y) << 32) | (0xffffffffu - (uint32_t)i);
+            if (y > -INFINITY && key > bound) keys[count + atomicAdd(&more[turn], 1)] = key;
+            if (tid == 0) more[next] = 0;
+            beam_sync();
+            count += more[turn];
+            turn = next;
+            if (count > BEAM_LIST - BEAM_THREADS) {
+              best_of_list(keys, count, picked, p.best, from_warp);
+              beam_sync();
+              if (tid < p.best) keys[tid] = picked[tid];
+              bound = picked[p.best - 1];
+              count = p.best;
+              beam_sync();
+            }
+          }
+          beam_sync();
+          if (tid < 3) more[tid] = 0;
         }
+        best_of_list(keys, count, p.keys + at * p.best, p.best, from_warp);
+        beam_sync();
+        if (tid == 0) listed = noted = 0;
+        if (warp == 0) {
+          const float2 x = lane < BEAM_WARPS ? sums[lane] : make_float2(-INFINITY, 0.f);
+          const float most = warp_max(x.x), from_all = most == -INFINITY ? 0.f : most;
+          const float all = warp_sum(x.y == 0.f ? 0.f : x.y * fast_exp2(x.x - from_all));
+          if (lane == 0) p.sums[at] = make_float2(most, all);
+        }
+        if (k == p.chunks - 1)  // the row's other places stay empty
+          for (int s = (int)slice + 1; s < p.slices; ++s) {
+            if (tid < p.best) p.keys[(at + s - slice) * p.best + tid] = 0;
+            if (tid == 0) p.sums[at + s - slice] = make_float2(-INFINITY, 0.f);
+          }
+        beam_sync();
+        lost = false;
+        top = -INFINITY, off = 0.f, least = LEAST;
+        sum[0] = sum[1] = make_float2(0.f, 0.f);
       }
-      key = warp_max_key(key);
-      if (lane == 0) from_warp[warp] = key;
-      __syncthreads();
-      last = warp_max_key(from_warp[lane & (BEAM_WARPS - 1)]);
-      if (tid == 0) picked[r] = last;
-      __syncthreads();
+      advance();
     }
-    for (int i = tid; i < p.best; i += BEAM_THREADS) keys[i] = picked[i];
-    listed = p.best;
-    least = from_ordered((uint32_t)(last >> 32));  // (more than `best` were there, so none is missing)
-    __syncthreads();
   }
-  // the threads' sums, over the largest offset
-  if (top == -INFINITY) off = -INFINITY;
-  const float warp_off = warp_max(off), from = warp_off == -INFINITY ? 0.f : warp_off;
-  const float total = warp_sum(sum == 0.f ? 0.f : sum * fast_exp2(off - from));
-  if (lane == 0) sums[warp] = make_float2(warp_off, total);
-  best_of_list(keys, listed, out, p.best, from_warp);
-  if (__syncthreads_or(late)) {  // a copy that did not come: its bytes may not land in another CTA's memory
+  __syncthreads();
+  if (dead != 0) {  // a copy that did not come: its bytes may not land in another CTA's memory
     if (tid == 0) flag_error(FT_DEV_WAIT_TIMEOUT);
     for (int i = 0; i < 2000; ++i) __nanosleep(1000);
-  }
-  if (warp == 0) {
-    const float2 x = lane < BEAM_WARPS ? sums[lane] : make_float2(-INFINITY, 0.f);
-    const float most = warp_max(x.x), from_all = most == -INFINITY ? 0.f : most;
-    const float all = warp_sum(x.y == 0.f ? 0.f : x.y * fast_exp2(x.x - from_all));
-    if (lane == 0) p.sums[blockIdx.x] = make_float2(most, all);
   }
 }
 

@@ -50,8 +50,8 @@ int launch_accept(const ft::AcceptParams& p, int requests, int64_t row_bytes, bo
 }
 
 struct BeamShape {
-  int pieces, slices, slice_len;
-  int64_t keys, bytes;  // of the workspace: keys, then sums
+  int pieces, slices, chunks, per_cta;
+  int64_t ctas, keys, bytes;  // of the workspace: keys, then sums
 };
 
 int dtype_size(int dtype) { return dtype == FT_F32 ? 4 : 2; }
@@ -66,28 +66,21 @@ int check_beam_select(const ft_beam_select_args* a) {
   return FT_OK;
 }
 
-// Slices of a row, of whole chunks but for the last: of those sizes the one whose rounds of CTAs, three to an SM, end first.  A CTA takes
-// 1.1 us per chunk of 16 KB with the others' share of memory and 2 us beside, with fewer on its SM less by as much; chunks are
-// smaller where the call would leave SMs without any.  (148 SMs whatever the device: the workspace's size goes by this.)
+// Chunks of a call and how many a CTA takes: three CTAs to an SM, all at once.  Chunks of 16 KB, smaller ones where the call would leave SMs
+// without any.  (148 SMs whatever the device: the workspace's size goes by this.)
 BeamShape beam_shape(const ft_beam_select_args* a) {
   BeamShape s;
   const int n = 16 / dtype_size(a->dtype);
-  const int64_t rows = (int64_t)a->batch * a->beams;
-  for (s.pieces = 4; s.pieces > 1; s.pieces /= 2) {
-    const int64_t chunk = (int64_t)ft::BEAM_THREADS * n * s.pieces;
-    if (rows * ((a->vocab + chunk - 1) / chunk) >= 2 * 148) break;
+  const int64_t rows = (int64_t)a->batch * a->beams, ctas = 3 * 148;
+  int64_t chunk = 0;
+  for (s.pieces = 4;; s.pieces /= 2) {
+    chunk = (int64_t)ft::BEAM_THREADS * n * s.pieces;
+    s.chunks = (int)((a->vocab + chunk - 1) / chunk);
+    if (s.pieces == 1 || rows * s.chunks >= 2 * 148) break;
   }
-  const int64_t chunk = (int64_t)ft::BEAM_THREADS * n * s.pieces, chunks = (a->vocab + chunk - 1) / chunk;
-  double best = -1;
-  for (int m = 1; m <= 16 && m <= chunks; ++m) {
-    const int64_t slices = (chunks + m - 1) / m, ctas = rows * slices, rounds = (ctas + 3 * 148 - 1) / (3 * 148);
-    const double t = rounds * (2.0 + 1.1 * m);
-    if (best < 0 || t < best) {
-      best = t;
-      s.slices = (int)slices;
-      s.slice_len = (int)(m * chunk);
-    }
-  }
+  s.per_cta = (int)std::max<int64_t>(1, (rows * s.chunks + ctas - 1) / ctas);
+  s.ctas = (rows * s.chunks + s.per_cta - 1) / s.per_cta;
+  s.slices = std::min((s.chunks - 1) / s.per_cta + 2, s.chunks);
   s.keys = rows * s.slices * a->best;
   s.bytes = s.keys * 8 + rows * s.slices * 8;
   return s;
@@ -99,22 +92,21 @@ int pow2_at_least(int n, int low) {
 }
 
 template <typename T, int NV, bool VEC>
-int launch_scan_as(const ft::BeamParams& p, int groups, cudaStream_t st) {
+int launch_scan_as(const ft::BeamParams& p, const BeamShape& s, cudaStream_t st) {
   auto kernel = ft::beam_scan_kernel<T, NV, VEC>;
   static OncePerDevice once;
   FT_CUDA_OK(raise_smem_limit(once, kernel, ft::BeamScan<NV>::SMEM_BYTES));
-  kernel<<<(unsigned)((int64_t)p.batch * p.beams * p.slices), ft::BEAM_THREADS, ft::BeamScan<NV>::SMEM_BYTES, st>>>(p, groups);
+  kernel<<<(unsigned)s.ctas, ft::BEAM_THREADS + 32, ft::BeamScan<NV>::SMEM_BYTES, st>>>(p, pow2_at_least(p.best, ft::BEAM_WARPS));
   FT_CUDA_OK(cudaGetLastError());
   count_launch();
   return FT_OK;
 }
 
 template <typename T>
-int launch_beam_select(const ft::BeamParams& p, int pieces, bool vec, cudaStream_t st) {
-  const int groups = pow2_at_least(p.best, ft::BEAM_WARPS);
-  const int rc = pieces == 1   ? (vec ? launch_scan_as<T, 1, true>(p, groups, st) : launch_scan_as<T, 1, false>(p, groups, st))
-                 : pieces == 2 ? (vec ? launch_scan_as<T, 2, true>(p, groups, st) : launch_scan_as<T, 2, false>(p, groups, st))
-                               : (vec ? launch_scan_as<T, 4, true>(p, groups, st) : launch_scan_as<T, 4, false>(p, groups, st));
+int launch_beam_select(const ft::BeamParams& p, const BeamShape& s, bool vec, cudaStream_t st) {
+  const int rc = s.pieces == 1   ? (vec ? launch_scan_as<T, 1, true>(p, s, st) : launch_scan_as<T, 1, false>(p, s, st))
+                 : s.pieces == 2 ? (vec ? launch_scan_as<T, 2, true>(p, s, st) : launch_scan_as<T, 2, false>(p, s, st))
+                                 : (vec ? launch_scan_as<T, 4, true>(p, s, st) : launch_scan_as<T, 4, false>(p, s, st));
   if (rc != FT_OK) return rc;
   const int total = p.beams * p.slices * p.best;
   if (total <= 2 * ft::BEAM_THREADS)
@@ -208,7 +200,7 @@ int ft_beam_select(const ft_beam_select_args* a) {
     return fail(FT_ERR_INVALID_ARGUMENT, "logits / scores / out_scores / out_beams / out_tokens is NULL");
   if (a->workspace == nullptr || !aligned16(a->workspace)) return fail(FT_ERR_INVALID_ARGUMENT, "workspace is NULL or not 16-byte aligned");
   const BeamShape s = beam_shape(a);
-  if ((int64_t)a->batch * a->beams * s.slices > 0x7fffffffLL || (int64_t)a->beams * s.slices * a->best > 0x7fffffffLL / 2)
+  if ((int64_t)a->batch * a->beams > 0x7fffffffLL / 64 || s.ctas > 0x7fffffffLL || (int64_t)a->beams * s.slices * a->best > 0x7fffffffLL / 2)
     return fail(FT_ERR_TOO_LARGE, "more slices of logits than one launch takes");
   ft::BeamParams p;
   memset(&p, 0, sizeof(p));
@@ -217,14 +209,14 @@ int ft_beam_select(const ft_beam_select_args* a) {
   p.sums = reinterpret_cast<float2*>(p.keys + s.keys);
   p.logits_s0 = a->logits_stride0, p.logits_s1 = a->logits_stride1, p.scores_s0 = a->scores_stride0, p.scores_s1 = a->scores_stride1;
   p.out_scores_s0 = a->out_scores_stride0, p.out_beams_s0 = a->out_beams_stride0, p.out_tokens_s0 = a->out_tokens_stride0;
-  p.batch = a->batch, p.beams = a->beams, p.vocab = a->vocab, p.best = a->best, p.slices = s.slices, p.slice_len = s.slice_len;
+  p.batch = a->batch, p.beams = a->beams, p.vocab = a->vocab, p.best = a->best, p.slices = s.slices, p.chunks = s.chunks, p.per_cta = s.per_cta;
   p.beams_64 = a->beams_64, p.tokens_64 = a->tokens_64;
   const int n = 16 / dtype_size(a->dtype);
   const bool vec = aligned16(a->logits) && (a->batch == 1 || a->logits_stride0 % n == 0) && (a->beams == 1 || a->logits_stride1 % n == 0);
   cudaStream_t st = static_cast<cudaStream_t>(a->stream);
-  if (a->dtype == FT_F16) return launch_beam_select<__half>(p, s.pieces, vec, st);
-  if (a->dtype == FT_BF16) return launch_beam_select<__nv_bfloat16>(p, s.pieces, vec, st);
-  return launch_beam_select<float>(p, s.pieces, vec, st);
+  if (a->dtype == FT_F16) return launch_beam_select<__half>(p, s, vec, st);
+  if (a->dtype == FT_BF16) return launch_beam_select<__nv_bfloat16>(p, s, vec, st);
+  return launch_beam_select<float>(p, s, vec, st);
 }
 
 int ft_beam_reorder(const ft_beam_reorder_args* a) {

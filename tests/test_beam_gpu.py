@@ -282,3 +282,30 @@ def test_refusals_of_the_c_abi():
         b = lib.BeamReorderArgs.from_buffer_copy(r)
         setattr(b, field, bad)
         assert handle.ft_beam_reorder(ctypes.byref(b)) == -1
+
+
+@gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+def test_logits_in_rising_order_and_lists_that_overflow(dtype):
+    # every chunk holds larger logits than the ones before it, so each reaches the bound as a whole; then thousands of equal ones
+    vocab = 90001
+    rising = torch.linspace(-20, 20, vocab).to(DTYPES[dtype])
+    plateau = torch.where(torch.arange(vocab) % 3 == 0, torch.tensor(4.0), torch.tensor(-3.0)).to(DTYPES[dtype])
+    late = torch.full((vocab,), -math.inf)
+    late[60000:] = torch.randn(vocab - 60000, generator=torch.Generator().manual_seed(1))
+    rows = torch.stack([rising, plateau, late.to(DTYPES[dtype]), rising.flip(0)])
+    logits = rows.repeat(60, 1).view(60, 4, vocab).cuda()
+    scores = torch.linspace(-3, 0, 240).view(60, 4).cuda()
+    for best in (1, 8, 64):
+        out, ob, ot = select(logits, scores, best)
+        _, wb, wt = want(logits[:2], scores[:2], best)
+        assert torch.equal(ob[:2].cpu().long(), wb) and torch.equal(ot[:2].cpu().long(), wt)
+        assert bool((ot == ot[:1]).all())          # the same logits for every request
+
+
+@gpu
+def test_many_short_rows_in_a_cta():
+    for batch, beams, vocab in ((900, 3, 300), (2000, 1, 77), (300, 64, 40)):
+        logits, scores = inputs(batch, beams, vocab, torch.bfloat16, seed=vocab)
+        scores[::7, 0] = -math.inf
+        check(logits, scores, 5)
