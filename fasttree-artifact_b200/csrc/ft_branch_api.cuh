@@ -29,10 +29,10 @@ int current_sms() {
 }
 
 template <typename T>
-int launch_accept(const ft::AcceptParams& p, int requests, int64_t row_bytes, bool vec, cudaStream_t st) {
-  // CTAs per request: as many as the SMs hold two of, as long as each has 8 KB of a row to read (fewer bytes come no sooner)
+int launch_accept(const ft::AcceptParams& p, int requests, int64_t row_bytes, cudaStream_t st) {
+  // CTAs per request: as many as the SMs hold four of, as long as each has 8 KB of a row to read (fewer bytes come no sooner)
   int ranks = 1;
-  const int room = 2 * current_sms();
+  const int room = 4 * current_sms();
   while (p.targets == nullptr && ranks < 8 && (int64_t)requests * ranks * 2 <= room && row_bytes / (2 * ranks) >= 8192) ranks *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(requests * ranks));
@@ -44,7 +44,7 @@ int launch_accept(const ft::AcceptParams& p, int requests, int64_t row_bytes, bo
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  FT_CUDA_OK(cudaLaunchKernelEx(&cfg, ft::draft_accept_kernel<T>, p, (int)vec));
+  FT_CUDA_OK(cudaLaunchKernelEx(&cfg, ft::draft_accept_kernel<T>, p));
   count_launch();
   return FT_OK;
 }
@@ -178,13 +178,11 @@ int ft_draft_accept(const ft_draft_accept_args* a) {
   p.logits_s0 = a->logits_stride0, p.accepted_s0 = a->accepted_stride0, p.kv_entries_len = a->kv_entries_len;
   p.vocab = a->vocab, p.width = a->accepted_width;
   p.targets_64 = a->targets_64, p.tokens_64 = a->tokens_64, p.parents_64 = a->parents_64, p.next_64 = a->next_64, p.slots_64 = a->slots_64;
-  const int size = dtype_size(a->dtype), n = 16 / size;
-  const bool vec = aligned16(a->logits) && a->logits_stride0 % n == 0;
-  const int64_t row_bytes = (int64_t)a->vocab * size;
+  const int64_t row_bytes = (int64_t)a->vocab * dtype_size(a->dtype);
   cudaStream_t st = static_cast<cudaStream_t>(a->stream);
-  if (a->dtype == FT_F16) return launch_accept<__half>(p, pl.num_drafts, row_bytes, vec, st);
-  if (a->dtype == FT_BF16) return launch_accept<__nv_bfloat16>(p, pl.num_drafts, row_bytes, vec, st);
-  return launch_accept<float>(p, pl.num_drafts, row_bytes, vec, st);
+  if (a->dtype == FT_F16) return launch_accept<__half>(p, pl.num_drafts, row_bytes, st);
+  if (a->dtype == FT_BF16) return launch_accept<__nv_bfloat16>(p, pl.num_drafts, row_bytes, st);
+  return launch_accept<float>(p, pl.num_drafts, row_bytes, st);
 }
 
 int64_t ft_beam_select_workspace(const ft_beam_select_args* a) {

@@ -35,7 +35,7 @@ __device__ __forceinline__ int64_t load_index(const void* p, int is_64, int64_t 
 }
 
 // The tree of a request into shared memory: parent[i] is -1 (a root), -2 (padding) or an earlier token; what is none of these, and
-// what hangs on padding, becomes padding.  depth: filled if not NULL.  A whole block; ends with a barrier.
+// what hangs on padding, becomes padding.  A whole block; ends with a barrier.
 __device__ __forceinline__ void load_tree(const void* parents, int is_64, const Draft& d, int16_t* parent, int16_t* depth) {
   bool bad = false;
   for (int i = threadIdx.x; i < d.n; i += blockDim.x) {
@@ -57,7 +57,7 @@ __device__ __forceinline__ void load_tree(const void* parents, int is_64, const 
       lost |= 1u << k;
       steps = 0;
     }
-    if (depth != nullptr) depth[i] = (int16_t)steps;
+    depth[i] = (int16_t)steps;
   }
   __syncthreads();
   for (int i = threadIdx.x, k = 0; i < d.n; i += blockDim.x, ++k)
@@ -176,11 +176,14 @@ __device__ __forceinline__ float vec_at(const uint4& v, int e) {
 
 constexpr int ACCEPT_THREADS = 512;
 
-// Largest logit of one rank's share of a row, as {ordered value, ~index}: a thread's candidates come in rising
-// order, so a larger one only replaces the first of equals.
+// Largest logit of one rank's share of a row, as {ordered value, ~index}: a thread's candidates come in rising order, so a larger one
+// only replaces the first of equals.  Vectors from the row's first 16-byte border on; what stands before it and behind the last
+// vector goes to the first and the last rank.
 template <typename T>
-__device__ __forceinline__ unsigned long long row_argmax(const T* __restrict__ row, int vocab, bool vec, int rank, int ranks) {
+__device__ __forceinline__ unsigned long long row_argmax(const T* __restrict__ row, int vocab, int rank, int ranks) {
   constexpr int N = Vec<T>::N, U = 4;
+  const int head = min(vocab, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T)), nv = (vocab - head) / N, tail = head + nv * N;
+  const int lo = (int)((int64_t)nv * rank / ranks), hi = (int)((int64_t)nv * (rank + 1) / ranks), tid = threadIdx.x;
   float best = -INFINITY;
   uint32_t at = 0xffffffffu;
   auto take = [&](float x, int i) {
@@ -189,32 +192,19 @@ __device__ __forceinline__ unsigned long long row_argmax(const T* __restrict__ r
       at = (uint32_t)i;
     }
   };
-  if (vec) {
-    const int nv = vocab / N, lo = (int)((int64_t)nv * rank / ranks), hi = (int)((int64_t)nv * (rank + 1) / ranks);
-    for (int v0 = lo + (int)threadIdx.x; v0 < hi; v0 += U * ACCEPT_THREADS) {
-      uint4 x[U];
+  if (rank == 0 && tid < head) take(to_float<T>(row[tid]), tid);
+  for (int v0 = lo + tid; v0 < hi; v0 += U * ACCEPT_THREADS) {
+    uint4 x[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) x[u] = load_stream(row + (int64_t)min(v0 + u * ACCEPT_THREADS, hi - 1) * N);
+    for (int u = 0; u < U; ++u) x[u] = load_stream(row + head + (int64_t)min(v0 + u * ACCEPT_THREADS, hi - 1) * N);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (v0 + u * ACCEPT_THREADS < hi && vec_max<T>(x[u]) > best)
+    for (int u = 0; u < U; ++u) {
+      if (v0 + u * ACCEPT_THREADS < hi && vec_max<T>(x[u]) > best)
 #pragma unroll
-          for (int e = 0; e < N; ++e) take(vec_at<T>(x[u], e), (v0 + u * ACCEPT_THREADS) * N + e);
-      }
-    }
-    if (rank == ranks - 1 && nv * N + (int)threadIdx.x < vocab) take(to_float<T>(row[nv * N + threadIdx.x]), nv * N + (int)threadIdx.x);
-  } else {
-    constexpr int E = 8;
-    const int lo = (int)((int64_t)vocab * rank / ranks), hi = (int)((int64_t)vocab * (rank + 1) / ranks);
-    for (int i0 = lo + (int)threadIdx.x; i0 < hi; i0 += E * ACCEPT_THREADS) {
-      float x[E];
-#pragma unroll
-      for (int u = 0; u < E; ++u) x[u] = to_float<T>(row[min(i0 + u * ACCEPT_THREADS, hi - 1)]);
-#pragma unroll
-      for (int u = 0; u < E; ++u)
-        if (i0 + u * ACCEPT_THREADS < hi) take(x[u], i0 + u * ACCEPT_THREADS);
+        for (int e = 0; e < N; ++e) take(vec_at<T>(x[u], e), head + (v0 + u * ACCEPT_THREADS) * N + e);
     }
   }
+  if (rank == ranks - 1 && tail + tid < vocab) take(to_float<T>(row[tail + tid]), tail + tid);
   // (nothing above -inf: the row's first element will do)
   return at == 0xffffffffu ? 0xffffffffull - (rank == 0 ? 0u : 1u) : ((unsigned long long)ordered(best) << 32) | (0xffffffffu - at);
 }
@@ -228,7 +218,7 @@ __device__ __forceinline__ void cluster_arrive_wait() {
 // go on to the same child.  So only the rows along the path are read: one to a handful of, say, 32.  Each step costs a row's
 // way from memory and the exchange.
 template <typename T>
-__global__ void __launch_bounds__(ACCEPT_THREADS) draft_accept_kernel(const AcceptParams p, const int vec) {
+__global__ void __launch_bounds__(ACCEPT_THREADS) draft_accept_kernel(const AcceptParams p) {
   __shared__ int16_t parent[FT_MAX_DRAFT];
   __shared__ int32_t token[FT_MAX_DRAFT];
   __shared__ int16_t path[FT_MAX_DRAFT];
@@ -239,12 +229,20 @@ __global__ void __launch_bounds__(ACCEPT_THREADS) draft_accept_kernel(const Acce
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
   const Draft d = load_draft(p.drafts, blockIdx.x / ranks);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (p.logits != nullptr && d.n > 0) {  // the first row is on its way while the tree is read
+    const char* row = reinterpret_cast<const char*>(static_cast<const T*>(p.logits) + (int64_t)d.row * p.logits_s0);
+    const int64_t bytes = (int64_t)p.vocab * (int)sizeof(T);
+    for (int64_t i = 128 * ((int64_t)rank * ACCEPT_THREADS + threadIdx.x); i < bytes; i += 128LL * ranks * ACCEPT_THREADS)
+      asm volatile("prefetch.global.L2 [%0];\n" ::"l"(row + i));
+  }
+  // (a token that hangs on padding, or has no valid parent, is not reached)
   for (int i = threadIdx.x; i < d.n; i += ACCEPT_THREADS) {
-    const int64_t t = load_index(p.tokens, p.tokens_64, (int64_t)d.row + i);
+    const int64_t t = load_index(p.tokens, p.tokens_64, (int64_t)d.row + i), up = load_index(p.parents, p.parents_64, (int64_t)d.row + i);
     token[i] = t >= 0 && t <= 0x7fffffff ? (int)t : -1;
+    parent[i] = (int16_t)(up >= -1 && up < i ? (int)up : -2);
   }
   if (threadIdx.x < 3) child_at[threadIdx.x] = FT_MAX_DRAFT;
-  load_tree(p.parents, p.parents_64, d, parent, nullptr);
+  __syncthreads();
   if (ranks > 1) cluster_arrive_wait();  // all of them run before any writes to another
   int count = 0;
   int64_t next = -1;
@@ -255,7 +253,7 @@ __global__ void __launch_bounds__(ACCEPT_THREADS) draft_accept_kernel(const Acce
       if (p.targets != nullptr) {
         next = load_index(p.targets, p.targets_64, (int64_t)d.row + cur);
       } else {
-        unsigned long long key = row_argmax(static_cast<const T*>(p.logits) + ((int64_t)d.row + cur) * p.logits_s0, p.vocab, vec != 0, (int)rank, (int)ranks);
+        unsigned long long key = row_argmax(static_cast<const T*>(p.logits) + ((int64_t)d.row + cur) * p.logits_s0, p.vocab, (int)rank, (int)ranks);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
         if (lane == 0) from_warp[warp] = key;

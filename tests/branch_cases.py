@@ -18,7 +18,7 @@ def paths(parents):
     """Per token the numbers that it sees among its request's, and its depth; children of padding are padding."""
     sees, depth, pad = [], [], []
     for i, p in enumerate(parents):
-        bad = p < -1 or p >= i or (p >= 0 and pad[p])
+        bad = p < -1 or p >= i or (p >= 0 and pad[p])        # -2, what is no earlier token, what hangs on padding
         pad.append(bad)
         sees.append([] if bad else [i] if p == -1 else sees[p] + [i])
         depth.append(depth[p] + 1 if p >= 0 and not bad else 0)
