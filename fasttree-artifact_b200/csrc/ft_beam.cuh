@@ -55,12 +55,6 @@ __device__ __forceinline__ float group_bound(float mine, int groups, float (&low
   return bound;
 }
 
-__device__ __forceinline__ unsigned long long warp_max_key(unsigned long long k) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
-  return k;
-}
-
 // log2(e) as the kernels multiply by it: what a sum's offset is divided by to give a logarithm, in 64 bits.
 constexpr float BEAM_LOG2E = 1.4426950408889634f;
 
@@ -85,10 +79,10 @@ __device__ __forceinline__ void best_of_list(const unsigned long long* keys, int
     unsigned long long key = 0;
     for (int i = threadIdx.x; i < n; i += BEAM_THREADS)
       if (keys[i] < last) key = max(key, keys[i]);
-    key = warp_max_key(key);
+    key = warp_largest(key);
     if (lane == 0) from_warp[warp] = key;
     beam_sync();
-    last = warp_max_key(from_warp[lane & (BEAM_WARPS - 1)]);
+    last = warp_largest(from_warp[lane & (BEAM_WARPS - 1)]);
     if (threadIdx.x == 0) out[r] = last;
     beam_sync();
   }

@@ -30,10 +30,11 @@ int current_sms() {
 
 template <typename T>
 int launch_accept(const ft::AcceptParams& p, int requests, int64_t row_bytes, cudaStream_t st) {
-  // CTAs per request: as many as the SMs hold four of, as long as each has 8 KB of a row to read (fewer bytes come no sooner)
+  // CTAs per request: as many as the SMs hold two of, so that all are there at once, as long as each has 16 KB of a row to read (64
+  // requests, 131072 bf16 logits, 1 to 6 rows a path: 80, 53, 33, 43 us with 1, 2, 4, 8)
   int ranks = 1;
-  const int room = 4 * current_sms();
-  while (p.targets == nullptr && ranks < 8 && (int64_t)requests * ranks * 2 <= room && row_bytes / (2 * ranks) >= 8192) ranks *= 2;
+  const int room = 2 * current_sms();
+  while (p.targets == nullptr && ranks < 8 && (int64_t)requests * ranks * 2 <= room && row_bytes / (2 * ranks) >= 16384) ranks *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(requests * ranks));
   cfg.blockDim = dim3(ft::ACCEPT_THREADS);

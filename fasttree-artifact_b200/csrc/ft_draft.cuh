@@ -1,6 +1,6 @@
 // Drafted tokens: their trees into a plan's masks, and which of them the model agrees with.
 //
-// Kernels here and in ft_beam.cuh that write tables let no later launch start early: others read their tables before they wait.
+// Kernels here and in ft_beam.cuh that write row tables let no later launch start early: others read theirs before they wait.
 //
 // A request's drafted tokens are numbered so that a parent comes before its children.  The attention itself is ft_extend's: its
 // kernels read what a row sees from bits of the plan, and ft_draft_tree sets the few words of them that trees decide.
@@ -74,8 +74,17 @@ static_assert(FT_MAX_DRAFT <= 32 * DRAFT_THREADS, "a bit per token that a thread
 // atomic, and their order does not matter.
 __global__ void __launch_bounds__(DRAFT_THREADS) draft_tree_kernel(const DraftParams p) {
   __shared__ int16_t parent[FT_MAX_DRAFT], depth[FT_MAX_DRAFT];
+  allow_dependent_launch();
   const Draft d = load_draft(p.drafts, blockIdx.x);
   if (d.n == 0) return;
+  const int warp = threadIdx.x >> 5;
+  int4 a = make_int4(0, 0, 0, 0), b = a;  // the warp's next span
+  auto fetch = [&](int s) {
+    const int4* raw = reinterpret_cast<const int4*>(p.spans + d.span0 + s);
+    a = __ldg(raw);
+    b = __ldg(raw + 1);
+  };
+  if (warp < d.spans) fetch(warp);
   load_tree(p.parents, p.parents_64, d, parent, depth);
   if (p.positions != nullptr)
     for (int i = threadIdx.x; i < d.n; i += DRAFT_THREADS) {
@@ -85,9 +94,7 @@ __global__ void __launch_bounds__(DRAFT_THREADS) draft_tree_kernel(const DraftPa
       else
         static_cast<int*>(p.positions)[at] = d.cached + depth[i];
     }
-  for (int s = threadIdx.x >> 5; s < d.spans; s += DRAFT_THREADS / 32) {
-    const int4* raw = reinterpret_cast<const int4*>(p.spans + d.span0 + s);
-    const int4 a = __ldg(raw), b = __ldg(raw + 1);
+  for (int s = warp; s < d.spans; s += DRAFT_THREADS / 32) {
     const DraftSpan span = {a.x, a.y, a.z, a.w, b.x, b.y, 0, 0};
     for (int k = threadIdx.x & 31; k < span.tokens; k += 32)
       draft_span_words(span, k, p.window, parent, depth, [&](int word, uint32_t mask, uint32_t bits) {
@@ -99,6 +106,7 @@ __global__ void __launch_bounds__(DRAFT_THREADS) draft_tree_kernel(const DraftPa
           atomicOr(at, (int32_t)bits);
         }
       });
+    if (s + DRAFT_THREADS / 32 < d.spans) fetch(s + DRAFT_THREADS / 32);
   }
 }
 
@@ -174,6 +182,12 @@ __device__ __forceinline__ float vec_at(const uint4& v, int e) {
   }
 }
 
+// The largest of a warp's keys, by its halves.
+__device__ __forceinline__ unsigned long long warp_largest(unsigned long long key) {
+  const uint32_t high = __reduce_max_sync(0xffffffffu, (uint32_t)(key >> 32));
+  return ((unsigned long long)high << 32) | __reduce_max_sync(0xffffffffu, (uint32_t)(key >> 32) == high ? (uint32_t)key : 0u);
+}
+
 constexpr int ACCEPT_THREADS = 512;
 
 // Largest logit of one rank's share of a row, as {ordered value, ~index}: a thread's candidates come in rising order, so a larger one
@@ -186,25 +200,35 @@ __device__ __forceinline__ unsigned long long row_argmax(const T* __restrict__ r
   const int lo = (int)((int64_t)nv * rank / ranks), hi = (int)((int64_t)nv * (rank + 1) / ranks), tid = threadIdx.x;
   float best = -INFINITY;
   uint32_t at = 0xffffffffu;
-  auto take = [&](float x, int i) {
-    if (x > best) {
-      best = x;
-      at = (uint32_t)i;
-    }
-  };
-  if (rank == 0 && tid < head) take(to_float<T>(row[tid]), tid);
+  if (rank == 0 && tid < head) {
+    const float x = to_float<T>(row[tid]);
+    if (x > best) best = x, at = (uint32_t)tid;
+  }
+  uint4 held = make_uint4(0, 0, 0, 0);  // the first vector with the largest so far; which element it is is asked once
+  int held_at = -1;
   for (int v0 = lo + tid; v0 < hi; v0 += U * ACCEPT_THREADS) {
     uint4 x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) x[u] = load_stream(row + head + (int64_t)min(v0 + u * ACCEPT_THREADS, hi - 1) * N);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (v0 + u * ACCEPT_THREADS < hi && vec_max<T>(x[u]) > best)
-#pragma unroll
-        for (int e = 0; e < N; ++e) take(vec_at<T>(x[u], e), head + (v0 + u * ACCEPT_THREADS) * N + e);
+    for (int u = 0; u < U; ++u) {  // (the last vector once more changes nothing)
+      const float m = vec_max<T>(x[u]);
+      const bool more = m > best;
+      best = more ? m : best;
+      held_at = more ? v0 + u * ACCEPT_THREADS : held_at;
+      held.x = more ? x[u].x : held.x, held.y = more ? x[u].y : held.y, held.z = more ? x[u].z : held.z, held.w = more ? x[u].w : held.w;
     }
   }
-  if (rank == ranks - 1 && tail + tid < vocab) take(to_float<T>(row[tail + tid]), tail + tid);
+  if (held_at >= 0) {
+    int first = 0;
+#pragma unroll
+    for (int e = N - 1; e >= 0; --e) first = vec_at<T>(held, e) == best ? e : first;
+    at = (uint32_t)(head + min(held_at, hi - 1) * N + first);
+  }
+  if (rank == ranks - 1 && tail + tid < vocab) {
+    const float x = to_float<T>(row[tail + tid]);
+    if (x > best) best = x, at = (uint32_t)(tail + tid);
+  }
   // (nothing above -inf: the row's first element will do)
   return at == 0xffffffffu ? 0xffffffffull - (rank == 0 ? 0u : 1u) : ((unsigned long long)ordered(best) << 32) | (0xffffffffu - at);
 }
@@ -218,7 +242,7 @@ __device__ __forceinline__ void cluster_arrive_wait() {
 // go on to the same child.  So only the rows along the path are read: one to a handful of, say, 32.  Each step costs a row's
 // way from memory and the exchange.
 template <typename T>
-__global__ void __launch_bounds__(ACCEPT_THREADS) draft_accept_kernel(const AcceptParams p) {
+__global__ void __launch_bounds__(ACCEPT_THREADS, 2) draft_accept_kernel(const AcceptParams p) {
   __shared__ int16_t parent[FT_MAX_DRAFT];
   __shared__ int32_t token[FT_MAX_DRAFT];
   __shared__ int16_t path[FT_MAX_DRAFT];
@@ -229,12 +253,6 @@ __global__ void __launch_bounds__(ACCEPT_THREADS) draft_accept_kernel(const Acce
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
   const Draft d = load_draft(p.drafts, blockIdx.x / ranks);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (p.logits != nullptr && d.n > 0) {  // the first row is on its way while the tree is read
-    const char* row = reinterpret_cast<const char*>(static_cast<const T*>(p.logits) + (int64_t)d.row * p.logits_s0);
-    const int64_t bytes = (int64_t)p.vocab * (int)sizeof(T);
-    for (int64_t i = 128 * ((int64_t)rank * ACCEPT_THREADS + threadIdx.x); i < bytes; i += 128LL * ranks * ACCEPT_THREADS)
-      asm volatile("prefetch.global.L2 [%0];\n" ::"l"(row + i));
-  }
   // (a token that hangs on padding, or has no valid parent, is not reached)
   for (int i = threadIdx.x; i < d.n; i += ACCEPT_THREADS) {
     const int64_t t = load_index(p.tokens, p.tokens_64, (int64_t)d.row + i), up = load_index(p.parents, p.parents_64, (int64_t)d.row + i);
@@ -254,14 +272,11 @@ __global__ void __launch_bounds__(ACCEPT_THREADS) draft_accept_kernel(const Acce
         next = load_index(p.targets, p.targets_64, (int64_t)d.row + cur);
       } else {
         unsigned long long key = row_argmax(static_cast<const T*>(p.logits) + ((int64_t)d.row + cur) * p.logits_s0, p.vocab, (int)rank, (int)ranks);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
+        key = warp_largest(key);
         if (lane == 0) from_warp[warp] = key;
         __syncthreads();
         const int set = count & 1;
-        key = from_warp[lane & (ACCEPT_THREADS / 32 - 1)];
-#pragma unroll
-        for (int o = ACCEPT_THREADS / 64; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
+        key = warp_largest(from_warp[lane & (ACCEPT_THREADS / 32 - 1)]);
         if (ranks > 1) {
           if (threadIdx.x < ranks) {
             uint32_t there;

@@ -132,8 +132,7 @@ int launch_extend_tc(const ft::ExtendTcParams& tp, int ctas, cudaStream_t st) {
     }();
     if (regs != C::REGS_LAUNCH) return fail(FT_ERR_UNSUPPORTED, "the kernel was built with %d registers a thread, not %d", regs, C::REGS_LAUNCH);
   }
-  kernel<<<(unsigned)ctas, C::THREADS, C::SMEM_BYTES, st>>>(tp);
-  FT_CUDA_OK(cudaGetLastError());
+  FT_CUDA_OK(launch_early(kernel, (unsigned)ctas, C::THREADS, C::SMEM_BYTES, st, tp));
   count_launch();
   return FT_OK;
 }
@@ -163,8 +162,7 @@ int launch_extend_f32_as(const ft::ExtendParams& p, int ctas, cudaStream_t st) {
   auto kernel = ft::extend_f32_kernel<D, RPT>;
   static OncePerDevice once;
   FT_CUDA_OK(raise_smem_limit(once, kernel, ft::ExtF32Cfg<D, RPT>::SMEM_BYTES));
-  kernel<<<(unsigned)ctas, 256, ft::ExtF32Cfg<D, RPT>::SMEM_BYTES, st>>>(p);
-  FT_CUDA_OK(cudaGetLastError());
+  FT_CUDA_OK(launch_early(kernel, (unsigned)ctas, 256, ft::ExtF32Cfg<D, RPT>::SMEM_BYTES, st, p));
   count_launch();
   return FT_OK;
 }

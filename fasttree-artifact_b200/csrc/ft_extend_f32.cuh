@@ -47,6 +47,7 @@ __global__ void __launch_bounds__(256, ExtF32Cfg<D, RPT>::CTAS) extend_f32_kerne
   int* ids = reinterpret_cast<int*>(smem + C::IDS_OFF);
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   allow_dependent_launch();
+  wait_for_prior_grid();
   const int4 share = __ldg(reinterpret_cast<const int4*>(p.sms) + 4 * blockIdx.x);
   const float* qb = reinterpret_cast<const float*>(p.q);
   auto at4 = [&](uint32_t off) { return *reinterpret_cast<const float4*>(smem + off); };
