@@ -17,7 +17,7 @@ namespace ft {
 
 constexpr int BEAM_THREADS = 256, BEAM_WARPS = BEAM_THREADS / 32;
 constexpr int BEAM_LIST = 512;   // logits that a slice lists, and pieces with one that it sets aside behind its first chunk; where more
-constexpr int BEAM_ASIDE = 96;   // reach its bound, it goes over the slice again with the list cut on the way
+constexpr int BEAM_ASIDE = 256;  // reach its bound, it goes over the slice again with the list cut on the way
 constexpr int BEAM_KEYS = 1024;  // candidates that the merge lists; beyond that, which takes many equal scores, it picks one at a time
 
 struct BeamParams {
@@ -39,7 +39,7 @@ __device__ __forceinline__ void beam_sync() { asm volatile("bar.sync 1, %0;\n" :
 // A lower bound of the n-th largest of those threads' values that n of them reach, from each thread's largest: the least of the
 // largest of `groups` groups of threads, groups >= n a power of two up to BEAM_THREADS.  By all of them; between calls with the same
 // shared memory there has to be a barrier.
-__device__ __forceinline__ float group_bound(float mine, int groups, float (&low)[BEAM_WARPS]) {
+__device__ __forceinline__ float group_bound(float mine, int groups, float (&low)[32]) {
   const int lanes = BEAM_THREADS / groups;  // of a group, if that is less than a warp
   float bound = mine;
 #pragma unroll
@@ -53,6 +53,25 @@ __device__ __forceinline__ float group_bound(float mine, int groups, float (&low
 #pragma unroll
   for (int w = 1; w < BEAM_WARPS; ++w) bound = fminf(bound, low[w]);
   return bound;
+}
+
+// A closer one, for n <= 32: the n-th largest of the largest of 32 groups of eight threads, sorted by every warp for itself.
+__device__ __forceinline__ float sorted_bound(float mine, int n, float (&low)[32]) {
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+  const int lane = threadIdx.x & 31;
+  if ((lane & 7) == 0) low[threadIdx.x >> 3] = mine;
+  beam_sync();
+  mine = low[lane];
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int o = size >> 1; o > 0; o >>= 1) {
+      const float other = __shfl_xor_sync(0xffffffffu, mine, o);
+      // falling within blocks of `size` where the lane's bit of it is clear, rising where it is set
+      mine = ((lane & size) == 0) == ((lane & o) == 0) ? fmaxf(mine, other) : fminf(mine, other);
+    }
+  return __shfl_sync(0xffffffffu, mine, n - 1);
 }
 
 // log2(e) as the kernels multiply by it: what a sum's offset is divided by to give a logarithm, in 64 bits.
@@ -108,11 +127,13 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 // that equal rows cut alike have equal sums).  Copies are of whole 16-byte pieces inside the row; what stands at its ends is filled in.
 //
 // The sum: each thread adds 2^(x log2(e) - c), c = its maximum x log2(e), which may lag by 8 (then by 2^11.5 a term).
-// The `best` largest: in a slice's first chunk each group of threads (a warp for up to 8 results) has a largest logit, and the least of
-// them bounds the `best`-th from below; what reaches it, 22 of 8192 logits on average for 8 groups, is listed, the list cut to the best,
-// and the last of those is the new bound; so again when four times as many chunks have passed (twice as many for more than 16 results),
-// so that about three times (once) `best` logits reach it in between, when the warps do not wait for each other.  A thread whose piece reaches the bound notes the piece, and the logits that do
-// are found by all threads together: done on the spot it takes the whole warp for one thread's.
+// The `best` largest: the largest of groups of threads in a slice's first chunk bound the `best`-th from below.  Up to 16 results: the
+// `best`-th of 32 of them, which little more than `best` logits reach; else the least of as many as there are results, which 130 of
+// 4096 logits reach for 32, and those are listed, the list is cut to the best and the last one is the new bound.  It is cut (again) when four
+// times as many chunks have passed (twice for more than 32 results), so that about three times `best` logits reach the bound in between,
+// when the warps do not wait for each other: a cut takes a CTA 1 us, the sum of a chunk 0.6.  A thread whose piece reaches the
+// bound notes the piece, and the logits that do are found by all threads
+// together: done on the spot it takes the whole warp for one thread's.
 template <typename T, int NV, bool VEC>
 __global__ void __launch_bounds__(BEAM_THREADS + 32, 3) beam_scan_kernel(const BeamParams p, const int groups) {
   using C = BeamScan<NV>;
@@ -122,7 +143,7 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, 3) beam_scan_kernel(const B
   constexpr float LEAST = -3.4028234e38f, LAG = 8.f;
   extern __shared__ __align__(128) uint8_t stages[];
   __shared__ unsigned long long keys[BEAM_LIST];
-  __shared__ float low[BEAM_WARPS];
+  __shared__ float low[32];
   __shared__ float2 sums[BEAM_WARPS];
   __shared__ unsigned long long from_warp[BEAM_WARPS], picked[FT_MAX_BEAMS];
   __shared__ __align__(8) unsigned long long barrier[2 * C::STAGES];  // full, empty
@@ -178,8 +199,15 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, 3) beam_scan_kernel(const B
   if (warp == BEAM_WARPS) {
     // ---- a chunk's bytes: from `at`, whose stage begins at the 16-byte border below; [from, to) are copied, the rest, at the row's ends,
     // is filled in, with -inf up to the next border
+    // (a row's score is asked for a row ahead; the first row is copied without asking)
+    const int rows = p.batch * p.beams;
+    Row ahead = row_of(row);
+    ahead.live = true;
     for (int n = 0; n < todo; ++n) {
-      if (n == 0 || k == 0) here = row_of(row);
+      if (n == 0 || k == 0) {
+        here = ahead;
+        if (row + 1 < rows) ahead = row_of(row + 1);
+      }
       const uint32_t full = full0 + 8 * stage;
       await(empty0 + 8 * stage, phase ^ 1u);
       uint32_t bytes = 0, to_stage = 0;
@@ -225,6 +253,7 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, 3) beam_scan_kernel(const B
     float top = -INFINITY, off = 0.f, least = LEAST;
     float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     int from_k = 0;     // the slice's first chunk
+    const bool few = p.best <= 16;
     bool lost = false;  // more reached the bound than there was room for
 #pragma unroll 1
     for (int n = 0; n < todo; ++n) {
@@ -261,7 +290,7 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, 3) beam_scan_kernel(const B
           float mine = -INFINITY;
 #pragma unroll
           for (int j = 0; j < NV; ++j) mine = fmaxf(mine, vec_max<T>(load(full, j)));
-          least = fmaxf(LEAST, group_bound(mine, groups, low));
+          least = fmaxf(LEAST, few ? sorted_bound(mine, p.best, low) : group_bound(mine, groups, low));
           top = mine;
           off = top == -INFINITY ? 0.f : top * BEAM_LOG2E;
         }
@@ -290,7 +319,7 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, 3) beam_scan_kernel(const B
             }
             if (most >= least) {
               const int to = atomicAdd(&noted, 1), piece = (j / PAIR) * BEAM_THREADS + tid;
-              if (fresh) {
+              if (fresh && !few) {
                 pieces[to] = (uint16_t)piece;
               } else if (to < BEAM_ASIDE) {
 #pragma unroll
@@ -323,15 +352,15 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, 3) beam_scan_kernel(const B
           pass(std::false_type{});
       }
       __syncwarp();
-      if (!fresh && lane == 0) mbar_arrive(empty0 + 8 * stage);
+      if (!(fresh && !few) && lane == 0) mbar_arrive(empty0 + 8 * stage);
       const bool ends = k == p.chunks - 1 || n == todo - 1;
       const int passed = k - from_k + 1;
       int count = 0;
-      if (((passed & (passed - 1)) == 0 && (p.best > 16 || (passed & 0x2aaaaaaa) == 0)) || ends) {
-        // the logits of the noted pieces, of the first chunk in its stage
+      if (((passed & (passed - 1)) == 0 && (p.best > 32 || (passed & 0x2aaaaaaa) == 0) && !(few && passed == 1)) || ends) {
+        // the logits of the noted pieces, of many results' first chunk in its stage
         beam_sync();
         const int n_pieces = noted;
-        if (fresh) {
+        if (fresh && !few) {
           for (int i0 = tid; i0 < n_pieces * E; i0 += BEAM_THREADS) {
             const int piece = pieces[i0 / E], e = i0 % E, i = number_of(piece % BEAM_THREADS, piece / BEAM_THREADS * PAIR + e / N, e % N);
             const float y = i < len ? to_float<T>(*reinterpret_cast<const T*>(bytes + i * S)) : -INFINITY;
@@ -347,7 +376,7 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, 3) beam_scan_kernel(const B
           lost |= n_pieces > BEAM_ASIDE;
         }
         beam_sync();
-        if (fresh && lane == 0) mbar_arrive(empty0 + 8 * stage);
+        if (fresh && !few && lane == 0) mbar_arrive(empty0 + 8 * stage);
         count = listed;
         lost |= count > BEAM_LIST;
         if (!ends) {
@@ -378,29 +407,58 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, 3) beam_scan_kernel(const B
         const float total = warp_sum(mine == 0.f ? 0.f : mine * fast_exp2(mine_off - from));
         if (lane == 0) sums[warp] = make_float2(warp_off, total);
         if (lost) {
-          // more than the list holds, equal ones for the most part: a logit a thread at a time, cutting the list when it may overflow
+          // more than there was room for, equal ones for the most part: all of the slice's logits again, the list cut when it may overflow
+          constexpr int AT_ONCE = 8;
           const T* const logits = reinterpret_cast<const T*>(here.at);
           const int stop = min(p.vocab, first + CHUNK);
           unsigned long long bound = 0;
           int turn = 0;
           count = 0;
-          for (int i0 = from_k * CHUNK; i0 < stop; i0 += BEAM_THREADS) {
-            const int i = i0 + tid, next = turn == 2 ? 0 : turn + 1;
-            const float y = i < stop ? to_float<T>(logits[i]) : -INFINITY;
-            const unsigned long long key = ((unsigned long long)ordered(y) << 32) | (0xffffffffu - (uint32_t)i);
-            if (y > -INFINITY && key > bound) keys[count + atomicAdd(&more[turn], 1)] = key;
-            if (tid == 0) more[next] = 0;
+          auto cut_list = [&](int most) {
+            if (count <= most) return;
+            best_of_list(keys, count, picked, p.best, from_warp);
             beam_sync();
-            count += more[turn];
-            turn = next;
-            if (count > BEAM_LIST - BEAM_THREADS) {
-              best_of_list(keys, count, picked, p.best, from_warp);
-              beam_sync();
-              if (tid < p.best) keys[tid] = picked[tid];
-              bound = picked[p.best - 1];
-              count = p.best;
-              beam_sync();
+            if (tid < p.best) keys[tid] = picked[tid];
+            bound = picked[p.best - 1];
+            count = p.best;
+            beam_sync();
+          };
+          for (int i0 = from_k * CHUNK; i0 < stop; i0 += AT_ONCE * BEAM_THREADS) {
+            unsigned long long key[AT_ONCE];
+            int mine = 0;
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+              const int i = i0 + u * BEAM_THREADS + tid;
+              const float y = i < stop ? to_float<T>(logits[i]) : -INFINITY;
+              key[u] = y > -INFINITY ? ((unsigned long long)ordered(y) << 32) | (0xffffffffu - (uint32_t)i) : 0ull;
+              mine += key[u] > bound;
             }
+            // all of them if they are few, else one of each thread at a time
+            const int next = turn == 2 ? 0 : turn + 1;
+            if (mine > 0) atomicAdd(&more[turn], mine);
+            if (tid == 0) {
+              more[next] = 0;
+              listed = count;
+            }
+            beam_sync();
+            const bool fits = count + more[turn] <= BEAM_LIST;
+            turn = next;
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+              if (key[u] > bound) keys[atomicAdd(&listed, 1)] = key[u];
+              if (!fits) {
+                beam_sync();
+                count = listed;
+                beam_sync();
+                cut_list(BEAM_LIST - BEAM_THREADS);
+                if (tid == 0) listed = count;
+                beam_sync();
+              }
+            }
+            beam_sync();
+            count = listed;
+            beam_sync();
+            cut_list(BEAM_LIST - BEAM_THREADS);
           }
           beam_sync();
           if (tid < 3) more[tid] = 0;
