@@ -36,42 +36,41 @@ struct BeamParams {
 // The scan's BEAM_THREADS threads that read logits; one more warp sends for them.
 __device__ __forceinline__ void beam_sync() { asm volatile("bar.sync 1, %0;\n" ::"n"(BEAM_THREADS) : "memory"); }
 
-// A lower bound of the n-th largest of those threads' values that n of them reach, from each thread's largest: the least of the
-// largest of `groups` groups of threads, groups >= n a power of two up to BEAM_THREADS.  By all of them; between calls with the same
-// shared memory there has to be a barrier.
-__device__ __forceinline__ float group_bound(float mine, int groups, float (&low)[32]) {
-  const int lanes = BEAM_THREADS / groups;  // of a group, if that is less than a warp
-  float bound = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const float other = __shfl_xor_sync(0xffffffffu, bound, o);
-    bound = o < lanes ? fmaxf(bound, other) : fminf(bound, other);
-  }
-  if ((threadIdx.x & 31) == 0) low[threadIdx.x >> 5] = bound;
-  beam_sync();
-  bound = low[0];
-#pragma unroll
-  for (int w = 1; w < BEAM_WARPS; ++w) bound = fminf(bound, low[w]);
-  return bound;
-}
-
-// A closer one, for n <= 32: the n-th largest of the largest of 32 groups of eight threads, sorted by every warp for itself.
-__device__ __forceinline__ float sorted_bound(float mine, int n, float (&low)[32]) {
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+// A warp's values sorted, the largest in lane 0.
+__device__ __forceinline__ float warp_sorted(float x) {
   const int lane = threadIdx.x & 31;
-  if ((lane & 7) == 0) low[threadIdx.x >> 3] = mine;
-  beam_sync();
-  mine = low[lane];
 #pragma unroll
   for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
     for (int o = size >> 1; o > 0; o >>= 1) {
-      const float other = __shfl_xor_sync(0xffffffffu, mine, o);
+      const float other = __shfl_xor_sync(0xffffffffu, x, o);
       // falling within blocks of `size` where the lane's bit of it is clear, rising where it is set
-      mine = ((lane & size) == 0) == ((lane & o) == 0) ? fmaxf(mine, other) : fminf(mine, other);
+      x = ((lane & size) == 0) == ((lane & o) == 0) ? fmaxf(x, other) : fminf(x, other);
     }
-  return __shfl_sync(0xffffffffu, mine, n - 1);
+  return x;
+}
+
+// A lower bound of the n-th largest of those threads' logits, which n of them reach, from each thread's largest; `holders`: the
+// threads, from the first, that hold any.  Up to 16: the n-th of the largest of 32 groups of eight threads.  More: each full warp's
+// r-th, r of them in every warp being enough, and the least of those.  -inf: none.  Between calls with the same shared
+// memory there has to be a barrier.
+__device__ __forceinline__ float logit_bound(float mine, int n, int holders, float (&low)[32]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (n <= 16) {
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+    if ((lane & 7) == 0) low[threadIdx.x >> 3] = mine;
+    beam_sync();
+    return __shfl_sync(0xffffffffu, warp_sorted(low[lane]), n - 1);
+  }
+  const int full = min(holders >> 5, BEAM_WARPS), r = full > 0 ? (n + full - 1) / full : 33;
+  mine = __shfl_sync(0xffffffffu, warp_sorted(mine), min(r, 32) - 1);
+  if (lane == 0) low[warp] = r > 32 ? -INFINITY : warp < full ? mine : INFINITY;
+  beam_sync();
+  float bound = low[0];
+#pragma unroll
+  for (int w = 1; w < BEAM_WARPS; ++w) bound = fminf(bound, low[w]);
+  return bound;
 }
 
 // log2(e) as the kernels multiply by it: what a sum's offset is divided by to give a logarithm, in 64 bits.
@@ -128,14 +127,14 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 //
 // The sum: each thread adds 2^(x log2(e) - c), c = its maximum x log2(e), which may lag by 8 (then by 2^11.5 a term).
 // The `best` largest: the largest of groups of threads in a slice's first chunk bound the `best`-th from below.  Up to 16 results: the
-// `best`-th of 32 of them, which little more than `best` logits reach; else the least of as many as there are results, which 130 of
-// 4096 logits reach for 32, and those are listed, the list is cut to the best and the last one is the new bound.  It is cut (again) when four
+// `best`-th of 32 of them, which little more than `best` logits reach; else something looser (logit_bound), and what reaches it
+// is listed, the list is cut to the best and the last one is the new bound.  It is cut (again) when four
 // times as many chunks have passed (twice for more than 32 results), so that about three times `best` logits reach the bound in between,
 // when the warps do not wait for each other: a cut takes a CTA 1 us, the sum of a chunk 0.6.  A thread whose piece reaches the
 // bound notes the piece, and the logits that do are found by all threads
 // together: done on the spot it takes the whole warp for one thread's.
 template <typename T, int NV, bool VEC>
-__global__ void __launch_bounds__(BEAM_THREADS + 32, 3) beam_scan_kernel(const BeamParams p, const int groups) {
+__global__ void __launch_bounds__(BEAM_THREADS + 32, 3) beam_scan_kernel(const BeamParams p) {
   using C = BeamScan<NV>;
   constexpr int S = (int)sizeof(T), N = 16 / S, CHUNK = BEAM_THREADS * NV * N, PAIR = NV > 1 ? 2 : 1;
   constexpr int PIECES = BEAM_THREADS * NV / PAIR, E = PAIR * N;  // pieces (of one or two vectors) of a chunk, their elements
@@ -290,7 +289,7 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, 3) beam_scan_kernel(const B
           float mine = -INFINITY;
 #pragma unroll
           for (int j = 0; j < NV; ++j) mine = fmaxf(mine, vec_max<T>(load(full, j)));
-          least = fmaxf(LEAST, few ? sorted_bound(mine, p.best, low) : group_bound(mine, groups, low));
+          least = fmaxf(LEAST, logit_bound(mine, p.best, len >= CHUNK ? BEAM_THREADS : VEC ? (len + N - 1) / N : S == 4 ? len : (len + 1) / 2, low));
           top = mine;
           off = top == -INFINITY ? 0.f : top * BEAM_LOG2E;
         }
@@ -699,6 +698,12 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_reorder_kernel(const Reorde
   wait_for_prior_grid();
   const int req = blockIdx.y;
   const int64_t whole = p.width / p.words;
+  // (what does not depend on one another is asked for at once: the call's length is this chain, the rows' numbers, the rows)
+  int64_t beam = -1, t = -1;
+  if ((int)threadIdx.x < p.to) {
+    beam = load_index(p.beams, p.beams_64, req * p.beams_s0 + threadIdx.x);
+    t = load_index(p.out_rows, p.out_rows_64, req * p.out_rows_s0 + threadIdx.x);
+  }
   int64_t lo = p.starts != nullptr ? load_index(p.starts, p.starts_64, req) : 0, hi = p.ends != nullptr ? load_index(p.ends, p.ends_64, req) : whole;
   bool bad = lo < 0 || lo > whole || hi < 0 || hi > whole;
   lo = (lo < 0 ? 0 : lo > whole ? whole : lo) * p.words;
@@ -706,18 +711,16 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_reorder_kernel(const Reorde
   const int64_t first = lo + ((int64_t)blockIdx.x << p.shift);
   if (first >= hi && blockIdx.x > 0) return;
   if ((int)threadIdx.x < p.to) {
-    int64_t s = -1, t = -1;
-    const int64_t beam = load_index(p.beams, p.beams_64, req * p.beams_s0 + threadIdx.x);
+    int64_t s = -1;
     if (beam != -1) {
-      t = load_index(p.out_rows, p.out_rows_64, req * p.out_rows_s0 + threadIdx.x);
       s = beam >= 0 && beam < p.from ? load_index(p.rows, p.rows_64, req * p.rows_s0 + beam) : -1;
       if (s < 0 || s >= p.table_rows || t < 0 || t >= p.table_rows) {
         bad = true;
-        t = -1;
+        s = t = -1;
       }
     }
-    source[threadIdx.x] = s == t ? -1 : s;
-    target[threadIdx.x] = s == t ? -1 : t;
+    source[threadIdx.x] = s;
+    target[threadIdx.x] = beam == -1 || s == t ? -1 : t;
   }
   if (bad) flag_error(FT_DEV_BAD_ROW_INDEX);
   __syncthreads();

@@ -68,7 +68,7 @@ int check_beam_select(const ft_beam_select_args* a) {
 }
 
 // Chunks of a call and how many a CTA takes: three CTAs to an SM, all at once.  Chunks of 16 KB, smaller ones where the call would leave SMs
-// without any.  (148 SMs whatever the device: the workspace's size goes by this.)
+// without any or rows are shorter.  (148 SMs whatever the device: the workspace's size goes by this.)
 BeamShape beam_shape(const ft_beam_select_args* a) {
   BeamShape s;
   const int n = 16 / dtype_size(a->dtype);
@@ -77,7 +77,7 @@ BeamShape beam_shape(const ft_beam_select_args* a) {
   for (s.pieces = 4;; s.pieces /= 2) {
     chunk = (int64_t)ft::BEAM_THREADS * n * s.pieces;
     s.chunks = (int)((a->vocab + chunk - 1) / chunk);
-    if (s.pieces == 1 || rows * s.chunks >= 2 * 148) break;
+    if (s.pieces == 1 || (rows * s.chunks >= 2 * 148 && chunk <= a->vocab)) break;
   }
   s.per_cta = (int)std::max<int64_t>(1, (rows * s.chunks + ctas - 1) / ctas);
   s.ctas = (rows * s.chunks + s.per_cta - 1) / s.per_cta;
@@ -97,7 +97,7 @@ int launch_scan_as(const ft::BeamParams& p, const BeamShape& s, cudaStream_t st)
   auto kernel = ft::beam_scan_kernel<T, NV, VEC>;
   static OncePerDevice once;
   FT_CUDA_OK(raise_smem_limit(once, kernel, ft::BeamScan<NV>::SMEM_BYTES));
-  kernel<<<(unsigned)s.ctas, ft::BEAM_THREADS + 32, ft::BeamScan<NV>::SMEM_BYTES, st>>>(p, pow2_at_least(p.best, ft::BEAM_WARPS));
+  kernel<<<(unsigned)s.ctas, ft::BEAM_THREADS + 32, ft::BeamScan<NV>::SMEM_BYTES, st>>>(p);
   FT_CUDA_OK(cudaGetLastError());
   count_launch();
   return FT_OK;
