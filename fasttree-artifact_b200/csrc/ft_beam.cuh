@@ -491,25 +491,30 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, 3) beam_scan_kernel(const B
   }
 }
 
-// A candidate of the merge: its score, and in their order its beam, logit and token.
+// A candidate of the merge: its score as a whole number in the same order, and in their order its beam, logit and token.
 struct BeamCandidate {
-  double score;
-  unsigned long long key;
+  unsigned long long score, key;
   int beam;
 };
 __device__ __forceinline__ bool before(const BeamCandidate& a, const BeamCandidate& b) {
   return a.score != b.score ? a.score > b.score : a.beam != b.beam ? a.beam < b.beam : a.key > b.key;
 }
+__device__ __forceinline__ unsigned long long ordered64(double x) {
+  const long long b = __double_as_longlong(x + 0.0);
+  return b < 0 ? ~(unsigned long long)b : (unsigned long long)b | (1ull << 63);
+}
+__device__ __forceinline__ double from_ordered64(unsigned long long k) { return __longlong_as_double((long long)((k >> 63) != 0 ? k & ~(1ull << 63) : ~k)); }
 
-// A CTA per request: each beam's sum from its slices (64 bits), each listed logit's score, and a threshold between the best
-// and the rest, found by halving, that leaves few to be ranked.  REGS scores a thread stay in registers, in fp32 rounded down, which
-// keeps their order; more are made anew each time.
-template <int REGS>
+// A CTA per request: each beam's sum from its slices (64 bits) and its listed logits' scores, by a warp; then a threshold between
+// the best and the rest, found by halving, that leaves few to be ranked.  It goes by the scores in fp32 rounded down, which keep their order.
+// Bound by its chain of steps.
 __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamParams p) {
+  extern __shared__ float scores[];       // of all listed logits, -inf where there is none
   __shared__ double shift[FT_MAX_BEAMS];  // a beam's score less its logarithm; NaN: nothing comes from it
-  __shared__ BeamCandidate list[BEAM_KEYS];
+  __shared__ unsigned long long list_score[BEAM_KEYS], list_key[BEAM_KEYS];
+  __shared__ uint8_t list_beam[BEAM_KEYS];
   __shared__ float high[BEAM_WARPS];
-  __shared__ int counts[3][BEAM_WARPS], place[BEAM_KEYS];
+  __shared__ int counts[3][BEAM_WARPS];
   __shared__ BeamCandidate from_warp[BEAM_WARPS];
   __shared__ int listed;
   const int req = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -519,61 +524,72 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamPara
   const float2* __restrict__ sums = p.sums + (int64_t)req * p.beams * p.slices;
   const int per_beam = p.slices * p.best, total = p.beams * per_beam;
   const unsigned long long* __restrict__ keys = p.keys + (int64_t)req * total;
-  unsigned long long mine[REGS];
+  auto put_score = [&](int i, unsigned long long key) {
+    const double x = (double)from_ordered((uint32_t)(key >> 32)) + shift[i / per_beam];
+    return scores[i] = key != 0 && x == x ? __double2float_rd(x) : -INFINITY;
+  };
+  constexpr int EARLY = 4;  // keys a thread asks for before it needs them
+  unsigned long long early[EARLY];
 #pragma unroll
-  for (int k = 0; k < REGS; ++k) mine[k] = tid + k * BEAM_THREADS < total ? __ldcg(keys + tid + k * BEAM_THREADS) : 0;
-  for (int b = warp; b < p.beams; b += BEAM_WARPS) {
-    const float score = p.scores[req * p.scores_s0 + b * p.scores_s1];
-    float top = -INFINITY;
-    for (int s = lane; s < p.slices; s += 32) top = fmaxf(top, __ldcg(&sums[b * p.slices + s]).x);
-    top = warp_max(top);
+  for (int k = 0; k < EARLY; ++k) early[k] = tid + k * BEAM_THREADS < total ? __ldcg(keys + tid + k * BEAM_THREADS) : 0;
+  // 2^wide lanes to a beam, at least its slices if they are no more than 32
+  int wide = 2;
+  while (wide < 5 && (1 << wide) < p.slices) ++wide;
+  const int lanes = 1 << wide;
+  for (int b0 = warp << (5 - wide); b0 < p.beams; b0 += BEAM_WARPS << (5 - wide)) {
+    const int b = b0 + (lane >> wide);
+    const bool there = b < p.beams;
+    const float score = there ? p.scores[req * p.scores_s0 + b * p.scores_s1] : -INFINITY;
+    float2 x = make_float2(-INFINITY, 0.f);  // of the lane's slices
     double sum = 0;
-    for (int s = lane; s < p.slices; s += 32) {
-      const float2 x = __ldcg(&sums[b * p.slices + s]);
-      if (x.y != 0.f) sum += (double)x.y * exp2((double)x.x - (double)top);
+    for (int s = lane & (lanes - 1); there && s < p.slices; s += lanes) {
+      const float2 y = __ldcg(&sums[b * p.slices + s]);
+      if (s < lanes) {
+        x = y;
+        sum = (double)x.y;
+      } else {
+        const float most = fmaxf(x.x, y.x);
+        sum = (sum != 0 ? sum * exp2((double)x.x - (double)most) : 0.0) + (y.y != 0.f ? (double)y.y * exp2((double)y.x - (double)most) : 0.0);
+        x.x = most;
+      }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) {
-      // (the terms' exponents were taken x BEAM_LOG2E, which is not log2(e): by it the offset is a logit again, and what is left of
-      // the difference, 1.3e-8 of the distance from the largest logit to the mean, is below fp32's half step)
-      const double lse = (double)top / (double)BEAM_LOG2E + log(sum);
+    float most = x.x;
+    for (int o = 1; o < lanes; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    sum = sum != 0 ? sum * exp2((double)x.x - (double)most) : 0.0;
+    for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    // (the terms' exponents were taken x BEAM_LOG2E, which is not log2(e): by it the offset is a logit again, and what is left of the
+    // difference, 1.3e-8 of the distance from the largest logit to the mean, is below fp32's half step)
+    const double lse = (double)most * (1.0 / (double)BEAM_LOG2E) + log(sum);
+    if (there && (lane & (lanes - 1)) == 0)
       shift[b] = fabsf(score) < INFINITY && fabs(lse) < (double)INFINITY ? (double)score - lse : (double)NAN;
-    }
   }
   __syncthreads();
-  // candidate i with this key; false: there is none
-  auto candidate = [&](int i, unsigned long long key, BeamCandidate& c) {
-    c.key = key;
-    c.beam = i / per_beam;
-    c.score = (double)from_ordered((uint32_t)(key >> 32)) + shift[c.beam];
-    return key != 0 && c.score == c.score;
-  };
-  BeamCandidate c;
-  float score[REGS], top = -INFINITY;
+  float top = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < REGS; ++k) {
+  for (int k = 0; k < EARLY; ++k) {
     const int i = tid + k * BEAM_THREADS;
-    score[k] = i < total && candidate(i, mine[k], c) ? __double2float_rd(c.score) : -INFINITY;
-    top = fmaxf(top, score[k]);
+    if (i < total) top = fmaxf(top, put_score(i, early[k]));
   }
-  auto beyond = [&](auto fn) {  // those that no register holds
-    for (int i = tid + REGS * BEAM_THREADS; i < total; i += BEAM_THREADS)
-      if (candidate(i, __ldcg(keys + i), c)) fn(__double2float_rd(c.score));
-  };
-  beyond([&](float x) { top = fmaxf(top, x); });
+  for (int i = tid + EARLY * BEAM_THREADS; i < total; i += BEAM_THREADS) top = fmaxf(top, put_score(i, __ldcg(keys + i)));
   top = warp_max(top);
   if (lane == 0) high[warp] = top;
   __syncthreads();
   top = high[0];
 #pragma unroll
   for (int w = 1; w < BEAM_WARPS; ++w) top = fmaxf(top, high[w]);
+  // candidate i, which has a score
+  auto candidate = [&](int i) {
+    BeamCandidate c;
+    c.key = __ldcg(keys + i);
+    c.beam = i / per_beam;
+    c.score = ordered64((double)from_ordered((uint32_t)(c.key >> 32)) + shift[c.beam]);
+    return c;
+  };
   int turn = 0;
   auto reach = [&](float least) {  // how many do
     int n = 0;
-#pragma unroll
-    for (int k = 0; k < REGS; ++k) n += score[k] >= least;
-    beyond([&](float x) { n += x >= least; });
+#pragma unroll 4
+    for (int i = tid; i < total; i += BEAM_THREADS) n += scores[i] >= least;
     n = __reduce_add_sync(0xffffffffu, n);
     if (lane == 0) counts[turn][warp] = n;
     __syncthreads();
@@ -583,11 +599,11 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamPara
     turn = turn == 2 ? 0 : turn + 1;
     return n;
   };
-  // the threshold: steps that double away from the best until enough reach it, then halves between the last two
+  // the threshold: steps that grow away from the best until enough reach it, then halves between the last two
   const int enough = 2 * p.best + 32;
   float least = -3.4028234e38f;
-  int n = 0;
-  if (top > -INFINITY) {
+  int n = total;
+  if (top > -INFINITY && total > enough) {
     float above = top, step = 1.f;
     for (; step < 1e6f; step *= 4.f) {
       n = reach(top - step);
@@ -609,17 +625,16 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamPara
         }
       }
   }
-  auto put = [&](int i, unsigned long long key) {
-    if (candidate(i, key, c) && __double2float_rd(c.score) >= least) {
+  for (int i = tid; i < total; i += BEAM_THREADS)
+    if (scores[i] >= least) {
       const int to = atomicAdd(&listed, 1);
-      if (to < BEAM_KEYS) list[to] = c;
+      if (to < BEAM_KEYS) {
+        const BeamCandidate c = candidate(i);
+        list_score[to] = c.score;
+        list_key[to] = c.key;
+        list_beam[to] = (uint8_t)c.beam;
+      }
     }
-  };
-#pragma unroll
-  for (int k = 0; k < REGS; ++k)
-    if (score[k] >= least) put(tid + k * BEAM_THREADS, mine[k]);
-  for (int i = tid + REGS * BEAM_THREADS; i < total; i += BEAM_THREADS) put(i, __ldcg(keys + i));
-  for (int i = tid; i < BEAM_KEYS; i += BEAM_THREADS) place[i] = 0;
   __syncthreads();
   auto store = [&](int at, float score, int64_t beam, int64_t token) {
     p.out_scores[req * p.out_scores_s0 + at] = score;
@@ -632,30 +647,46 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamPara
     else
       static_cast<int*>(p.out_tokens)[req * p.out_tokens_s0 + at] = (int)token;
   };
-  auto store_candidate = [&](int at, const BeamCandidate& x) { store(at, (float)x.score, x.beam, 0xffffffffu - (uint32_t)x.key); };
+  auto store_candidate = [&](int at, const BeamCandidate& x) { store(at, (float)from_ordered64(x.score), x.beam, 0xffffffffu - (uint32_t)x.key); };
+  auto listed_candidate = [&](int i) { return BeamCandidate{list_score[i], list_key[i], list_beam[i]}; };
   n = listed;
   if (n <= BEAM_KEYS) {
-    // ranked by counting; where they are few, several threads share one's count
-    int parts = 1;
-    while (parts < 8 && n * parts * 2 <= BEAM_THREADS) parts *= 2;
-    for (int i = tid / parts; i < n; i += BEAM_THREADS / parts) {
-      c = list[i];
-      int rank = 0;
-      for (int k = tid & (parts - 1); k < n; k += parts) rank += before(list[k], c);
-      if (rank != 0) atomicAdd(&place[i], rank);
+    // ranked by counting, four threads to a candidate; the order among equal scores is asked for where there are any
+    for (int i0 = 0; i0 < n; i0 += BEAM_THREADS / 4) {
+      const int i = i0 + (tid >> 2);
+      const unsigned long long score = i < n ? list_score[i] : 0;
+      int rank = 0, equal = 0;
+#pragma unroll 4
+      for (int k = tid & 3; k < n; k += 4) {
+        const unsigned long long other = list_score[k];
+        rank += other > score;
+        equal += other == score;
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        rank += __shfl_xor_sync(0xffffffffu, rank, o);
+        equal += __shfl_xor_sync(0xffffffffu, equal, o);
+      }
+      if (i < n && (tid & 3) == 0) {
+        const BeamCandidate c = listed_candidate(i);
+        if (equal > 1)
+          for (int k = 0; k < n; ++k)
+            if (list_score[k] == score) rank += before(listed_candidate(k), c);
+        if (rank < p.best) store_candidate(rank, c);
+      }
     }
-    __syncthreads();
-    for (int i = tid; i < n; i += BEAM_THREADS)
-      if (place[i] < p.best) store_candidate(place[i], list[i]);
     for (int i = n + tid; i < p.best; i += BEAM_THREADS) store(i, -INFINITY, -1, -1);
     return;
   }
   // equal scores without end: one at a time, the best of what comes behind the last one
-  BeamCandidate last = {(double)INFINITY, 0, -1};
+  BeamCandidate last = {~0ull, 0, -1};
   for (int r = 0; r < p.best; ++r) {
-    BeamCandidate most = {-(double)INFINITY, 0, 0x7fffffff};
+    BeamCandidate most = {0, 0, 0x7fffffff};
     for (int i = tid; i < total; i += BEAM_THREADS)
-      if (candidate(i, __ldcg(keys + i), c) && before(last, c) && before(c, most)) most = c;
+      if (scores[i] > -INFINITY) {
+        const BeamCandidate c = candidate(i);
+        if (before(last, c) && before(c, most)) most = c;
+      }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       BeamCandidate other;

@@ -87,6 +87,8 @@ BeamShape beam_shape(const ft_beam_select_args* a) {
   return s;
 }
 
+constexpr int BEAM_MERGE_SMEM = 160 << 10;
+
 int pow2_at_least(int n, int low) {
   while (low < n) low *= 2;
   return low;
@@ -109,11 +111,11 @@ int launch_beam_select(const ft::BeamParams& p, const BeamShape& s, bool vec, cu
                  : s.pieces == 2 ? (vec ? launch_scan_as<T, 2, true>(p, s, st) : launch_scan_as<T, 2, false>(p, s, st))
                                  : (vec ? launch_scan_as<T, 4, true>(p, s, st) : launch_scan_as<T, 4, false>(p, s, st));
   if (rc != FT_OK) return rc;
-  const int total = p.beams * p.slices * p.best;
-  if (total <= 2 * ft::BEAM_THREADS)
-    FT_CUDA_OK(launch_early(ft::beam_merge_kernel<2>, dim3((unsigned)p.batch), ft::BEAM_THREADS, 0, st, p));
-  else
-    FT_CUDA_OK(launch_early(ft::beam_merge_kernel<16>, dim3((unsigned)p.batch), ft::BEAM_THREADS, 0, st, p));
+  const int64_t smem = 4LL * p.beams * p.slices * p.best;  // at most 64 results of 444 + 64 slices
+  static OncePerDevice once;
+  FT_CUDA_OK(raise_smem_limit(once, ft::beam_merge_kernel, BEAM_MERGE_SMEM));
+  if (smem > BEAM_MERGE_SMEM) return fail(FT_ERR_TOO_LARGE, "more slices of logits than a request's merge holds");
+  FT_CUDA_OK(launch_early(ft::beam_merge_kernel, dim3((unsigned)p.batch), ft::BEAM_THREADS, (size_t)smem, st, p));
   count_launch();
   return FT_OK;
 }
