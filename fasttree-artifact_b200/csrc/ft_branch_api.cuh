@@ -23,6 +23,11 @@ int check_draft_plan(const ft_extend_plan_info& pl, const int32_t* table, int64_
   return FT_OK;
 }
 
+// A row of `n` elements, or `rows` of them, as a place in memory.
+Place rows_at(const void* p, int64_t rows, int64_t n, int64_t s0, int size) { return Place(p, n > 0 ? rows : 0, 1, (int)n, s0, 0, size); }
+Place row_at(const void* p, int64_t n, int size) { return rows_at(p, p != nullptr ? n : 0, 1, 1, size); }
+int index_size(int is_64) { return is_64 ? 8 : 4; }
+
 int current_sms() {
   int dev = 0;
   return cudaGetDevice(&dev) == cudaSuccess ? sm_count(dev) : 148;
@@ -63,7 +68,7 @@ int check_beam_select(const ft_beam_select_args* a) {
     return fail(FT_ERR_INVALID_ARGUMENT, "dtype %d is not one of FT_F16/FT_BF16/FT_F32", a->dtype);
   if (a->batch < 0 || a->beams <= 0 || a->beams > FT_MAX_BEAMS || a->best <= 0 || a->best > FT_MAX_BEAMS)
     return fail(FT_ERR_INVALID_ARGUMENT, "beams %d and best %d must be 1 to %d", a->beams, a->best, FT_MAX_BEAMS);
-  if (a->vocab <= 0) return fail(FT_ERR_INVALID_ARGUMENT, "vocab must be positive");
+  if (a->vocab <= 0 || a->vocab > FT_MAX_VOCAB) return fail(FT_ERR_INVALID_ARGUMENT, "vocab must be 1 to 2^30");
   return FT_OK;
 }
 
@@ -135,6 +140,8 @@ int ft_draft_tree(const ft_draft_tree_args* a) {
   if (rc != FT_OK) return rc;
   if (a->plan.num_tokens == 0) return FT_OK;
   if (a->parents == nullptr) return fail(FT_ERR_INVALID_ARGUMENT, "parents is NULL");
+  if (may_overlap(row_at(a->positions, a->plan.q_rows, index_size(a->positions_64)), row_at(a->parents, a->plan.q_rows, index_size(a->parents_64))))
+    return fail(FT_ERR_INVALID_ARGUMENT, "positions overlaps parents");
   ft::DraftParams p;
   memset(&p, 0, sizeof(p));
   p.drafts = a->plan_table + a->plan.drafts_off;
@@ -158,7 +165,7 @@ int ft_draft_accept(const ft_draft_accept_args* a) {
     return fail(FT_ERR_INVALID_ARGUMENT, "one of logits and targets must be given");
   if (a->dtype != FT_F16 && a->dtype != FT_BF16 && a->dtype != FT_F32)
     return fail(FT_ERR_INVALID_ARGUMENT, "dtype %d is not one of FT_F16/FT_BF16/FT_F32", a->dtype);
-  if (a->logits != nullptr && a->vocab <= 0) return fail(FT_ERR_INVALID_ARGUMENT, "vocab must be positive");
+  if (a->logits != nullptr && (a->vocab <= 0 || a->vocab > FT_MAX_VOCAB)) return fail(FT_ERR_INVALID_ARGUMENT, "vocab must be 1 to 2^30");
   if (a->num_requests < pl.num_drafts) return fail(FT_ERR_INVALID_ARGUMENT, "the plan has %d requests, the results %d", pl.num_drafts, a->num_requests);
   if (a->accepted_width < pl.longest_draft)
     return fail(FT_ERR_INVALID_ARGUMENT, "accepted has %d entries a request, the longest draft %d tokens", a->accepted_width, pl.longest_draft);
@@ -172,6 +179,23 @@ int ft_draft_accept(const ft_draft_accept_args* a) {
   if (a->slots != nullptr && pl.kv_entries_len > a->kv_entries_len)
     return fail(FT_ERR_INVALID_ARGUMENT, "the plan names %lld entries of kv_entries, which has %lld", (long long)pl.kv_entries_len,
                 (long long)a->kv_entries_len);
+  // a request's tokens are read while another's results are written
+  const Place results[] = {rows_at(a->accepted, a->num_requests, a->accepted_width, a->accepted_stride0, 4), row_at(a->counts, a->num_requests, 4),
+                           row_at(a->next_tokens, a->num_requests, index_size(a->next_64)), row_at(a->slots != nullptr ? a->kv_entries : nullptr, a->kv_entries_len, 4)};
+  const char* const result_names[] = {"accepted", "counts", "next_tokens", "kv_entries"};
+  const Place inputs[] = {row_at(a->tokens, pl.q_rows, index_size(a->tokens_64)), row_at(a->parents, pl.q_rows, index_size(a->parents_64)),
+                          row_at(a->targets, pl.q_rows, index_size(a->targets_64)),
+                          rows_at(a->logits, a->logits != nullptr ? pl.q_rows : 0, a->vocab, a->logits_stride0, dtype_size(a->dtype)),
+                          row_at(a->slots, pl.q_rows, index_size(a->slots_64))};
+  const char* const input_names[] = {"tokens", "parents", "targets", "logits", "slots"};
+  for (int r = 0; r < 4; ++r) {
+    for (int i = 0; i < 5; ++i) {
+      if (r == 3 && i == 4 && pl.num_drafts == 1) continue;  // one request's rows may stand at their entries: they are read first
+      if (may_overlap(results[r], inputs[i])) return fail(FT_ERR_INVALID_ARGUMENT, "%s overlaps %s", result_names[r], input_names[i]);
+    }
+    for (int i = 0; i < r; ++i)
+      if (may_overlap(results[r], results[i])) return fail(FT_ERR_INVALID_ARGUMENT, "%s overlaps %s", result_names[r], result_names[i]);
+  }
   ft::AcceptParams p;
   memset(&p, 0, sizeof(p));
   p.drafts = a->plan_table + pl.drafts_off;
@@ -200,6 +224,20 @@ int ft_beam_select(const ft_beam_select_args* a) {
   if (a->logits == nullptr || a->scores == nullptr || a->out_scores == nullptr || a->out_beams == nullptr || a->out_tokens == nullptr)
     return fail(FT_ERR_INVALID_ARGUMENT, "logits / scores / out_scores / out_beams / out_tokens is NULL");
   if (a->workspace == nullptr || !aligned16(a->workspace)) return fail(FT_ERR_INVALID_ARGUMENT, "workspace is NULL or not 16-byte aligned");
+  // scores may be the results' rows, or the start of each: a request's are read before its results are written
+  const Place scores(a->scores, a->batch, a->beams, 1, a->scores_stride0, a->scores_stride1, 4);
+  const Place results[] = {rows_at(a->out_scores, a->batch, a->best, a->out_scores_stride0, 4),
+                           rows_at(a->out_beams, a->batch, a->best, a->out_beams_stride0, index_size(a->beams_64)),
+                           rows_at(a->out_tokens, a->batch, a->best, a->out_tokens_stride0, index_size(a->tokens_64))};
+  const bool in_place = static_cast<const void*>(a->scores) == a->out_scores && (a->batch == 1 || a->scores_stride0 == a->out_scores_stride0) &&
+                        (a->beams == 1 || a->scores_stride1 == 1) && (a->batch == 1 || a->beams <= a->scores_stride0);
+  const Place logits[] = {Place(a->logits, a->batch, a->beams, a->vocab, a->logits_stride0, a->logits_stride1, dtype_size(a->dtype))};
+  for (int r = 0; r < 3; ++r) {
+    if (may_overlap(results[r], logits[0])) return fail(FT_ERR_INVALID_ARGUMENT, "a result overlaps logits");
+    if (!(r == 0 && in_place) && may_overlap(results[r], scores)) return fail(FT_ERR_INVALID_ARGUMENT, "a result overlaps scores, whose rows are not its own");
+    for (int i = 0; i < r; ++i)
+      if (may_overlap(results[r], results[i])) return fail(FT_ERR_INVALID_ARGUMENT, "two results overlap");
+  }
   const BeamShape s = beam_shape(a);
   if ((int64_t)a->batch * a->beams > 0x7fffffffLL / 64 || s.ctas > 0x7fffffffLL || (int64_t)a->beams * s.slices * a->best > 0x7fffffffLL / 2)
     return fail(FT_ERR_TOO_LARGE, "more slices of logits than one launch takes");
@@ -230,6 +268,14 @@ int ft_beam_reorder(const ft_beam_reorder_args* a) {
   if (a->table == nullptr || a->rows == nullptr || a->beams == nullptr || a->out_rows == nullptr)
     return fail(FT_ERR_INVALID_ARGUMENT, "table / rows / beams / out_rows is NULL");
   if (a->batch > 65535) return fail(FT_ERR_TOO_LARGE, "more than 65535 requests");
+  if (a->width > 0x7fffffffLL / 8) return fail(FT_ERR_TOO_LARGE, "the table's rows are too long for one launch");
+  const Place table = rows_at(a->table, a->table_rows, a->width, a->table_stride0, a->elem_bytes);
+  const Place numbers[] = {rows_at(a->rows, a->batch, a->from, a->rows_stride0, index_size(a->rows_64)),
+                           rows_at(a->beams, a->batch, a->to, a->beams_stride0, index_size(a->beams_64)),
+                           rows_at(a->out_rows, a->batch, a->to, a->out_rows_stride0, index_size(a->out_rows_64)),
+                           row_at(a->starts, a->batch, index_size(a->starts_64)), row_at(a->ends, a->batch, index_size(a->ends_64))};
+  for (const Place& n : numbers)
+    if (may_overlap(table, n)) return fail(FT_ERR_INVALID_ARGUMENT, "the table overlaps the rows' or beams' numbers");
   ft::ReorderParams p;
   memset(&p, 0, sizeof(p));
   p.words = a->elem_bytes / 4;
@@ -241,7 +287,6 @@ int ft_beam_reorder(const ft_beam_reorder_args* a) {
   p.rows_64 = a->rows_64, p.beams_64 = a->beams_64, p.out_rows_64 = a->out_rows_64, p.starts_64 = a->starts_64, p.ends_64 = a->ends_64;
   for (p.shift = 12; pow2_at_least(a->to, 1) << p.shift > ft::REORDER_WORDS * ft::BEAM_THREADS;) --p.shift;
   const int64_t chunks = (p.width + (1 << p.shift) - 1) >> p.shift;
-  if (chunks > 0x7fffffffLL) return fail(FT_ERR_TOO_LARGE, "the table's rows are too long for one launch");
   FT_CUDA_OK(launch_early(ft::beam_reorder_kernel, dim3((unsigned)chunks, (unsigned)a->batch), ft::BEAM_THREADS, 0, static_cast<cudaStream_t>(a->stream), p));
   count_launch();
   return FT_OK;

@@ -512,7 +512,6 @@ PyObject* py_draft_tree(PyObject*, PyObject* const* x, Py_ssize_t n) {
     a.parents = parents.data_ptr(), a.parents_64 = is_long(parents), a.rows = parents.size(0);
     if (x[3] != Py_None) {
       const at::Tensor& pos = index_row("positions", x[3], parents, parents.size(0));
-      if (pos.numel() > 0 && pos.data_ptr() == parents.data_ptr()) refuse("%s", "positions must not be parents");
       a.positions = pos.data_ptr(), a.positions_64 = is_long(pos);
     }
     return launch_on(parents, a, g_draft_tree);
@@ -535,7 +534,7 @@ PyObject* py_draft_accept(PyObject*, PyObject* const* x, Py_ssize_t n) {
       const at::Tensor& logits = on_device_of("logits", tensor("logits", x[0]), tokens);
       a.dtype = dtype_code(logits.scalar_type());
       if (logits.dim() != 2 || logits.size(0) != rows) refuse("%s", "logits must be [tokens, vocabulary]");
-      if (logits.size(1) < 1 || logits.size(1) > INT32_MAX) refuse("%s", "the vocabulary must have 1 to 2^31 - 1 entries");
+      if (logits.size(1) < 1 || logits.size(1) > FT_MAX_VOCAB) refuse("%s", "the vocabulary must have 1 to 2^30 entries");
       if (logits.size(1) > 1 && logits.stride(1) != 1) refuse("%s", "logits must be contiguous along the vocabulary");
       a.logits = logits.data_ptr(), a.vocab = (int32_t)logits.size(1);
       a.logits_stride0 = rows > 1 ? logits.stride(0) : 0;

@@ -34,6 +34,11 @@ __device__ __forceinline__ int64_t load_index(const void* p, int is_64, int64_t 
   return is_64 ? __ldg(static_cast<const long long*>(p) + i) : (int64_t)__ldg(static_cast<const int*>(p) + i);
 }
 
+// (by plain loads: slots may be written by the same kernel)
+__device__ __forceinline__ int64_t load_slot(const void* p, int is_64, int64_t i) {
+  return is_64 ? static_cast<const volatile long long*>(p)[i] : (int64_t)static_cast<const volatile int*>(p)[i];
+}
+
 // The tree of a request into shared memory: parent[i] is -1 (a root), -2 (padding) or an earlier token; what is none of these, and
 // what hangs on padding, becomes padding.  A whole block; ends with a barrier.
 __device__ __forceinline__ void load_tree(const void* parents, int is_64, const Draft& d, int16_t* parent, int16_t* depth) {
@@ -314,13 +319,16 @@ __global__ void __launch_bounds__(ACCEPT_THREADS, 2) draft_accept_kernel(const A
   }
   for (int i = threadIdx.x; i < p.width; i += ACCEPT_THREADS) p.accepted[out * p.accepted_s0 + i] = i < count ? path[i] : -1;
   if (p.slots == nullptr) return;
-  // the path's rows first, then the others', each in order: the path rises
+  // the path's rows first, then the others', each in order: the path rises.  All are read before any is written: they may stand at
+  // these entries.
+  for (int i = threadIdx.x; i < d.n; i += ACCEPT_THREADS) token[i] = (int32_t)load_slot(p.slots, p.slots_64, (int64_t)d.row + i);
+  __syncthreads();
   for (int i = threadIdx.x; i < d.n; i += ACCEPT_THREADS) {
     int before = 0;
     while (before < count && path[before] < i) ++before;
     const int to = before < count && path[before] == i ? before : count + i - before;
     const int64_t entry = d.entries + d.cached + to;
-    if (entry < p.kv_entries_len) p.kv_entries[entry] = (int32_t)load_index(p.slots, p.slots_64, (int64_t)d.row + i);
+    if (entry < p.kv_entries_len) p.kv_entries[entry] = token[i];
   }
 }
 

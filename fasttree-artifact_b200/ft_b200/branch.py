@@ -38,7 +38,8 @@ def draft_accept(logits, tokens, parents, plan, accepted, counts, next_tokens, s
     (int32 ``[requests]``): how many.  ``next_tokens`` (int32 or int64 ``[requests]``); a request without tokens, or whose first is no
     root, has count 0 and -1.  With ``slots`` (the tokens' pool rows, as :func:`ft_b200.extend.append` took them) the request's entries
     of ``kv_entries`` behind its cached ones become the accepted tokens' rows, in path order, and then the others', which the caller
-    may free: the request goes on with cached + count tokens in the cache."""
+    may free: the request goes on with cached + count tokens in the cache.  No result may overlap what is read, except that one
+    request's ``slots`` may be its entries themselves."""
     rc = _lib.call_module().draft_accept(logits, targets, tokens, parents, *_draft_plan(plan), accepted, counts, next_tokens, slots, kv_entries)
     if rc != 0:
         _lib.check(rc)
@@ -51,7 +52,8 @@ def beam_select(logits, scores, out_scores, out_beams, out_tokens):
     ``[batch, beams]``.  Results ``[batch, n]``, best first: ``out_scores`` fp32, ``out_beams`` and ``out_tokens`` int32 or int64; at most 64
     beams and results.  Of equal scores the lowest beam's comes first, then the larger logit, then the lowest token.  Logits of -inf are
     never chosen (banned tokens), nor is anything from a beam whose score is not finite (-inf: a beam that ended, or has not begun) or whose
-    logits hold NaN or +inf; where too little is left the last results are score -inf, beam -1, token -1.  Two launches."""
+    logits hold NaN or +inf; where too little is left the last results are score -inf, beam -1, token -1.  ``out_scores`` may be ``scores``, or start with it
+    in every row; otherwise no result may overlap what is read.  Two launches."""
     rc = _lib.call_module().beam_select(logits, scores, out_scores, out_beams, out_tokens)
     if rc != 0:
         _lib.check(rc)
@@ -65,7 +67,7 @@ def beam_reorder(table, rows, beams, starts=None, ends=None, out_rows=None):
 
     ``table`` ``[rows, width]`` of 4- or 8-byte elements; ``rows`` ``[batch, beams]``, ``beams`` and ``out_rows`` ``[batch, n]`` (int32 or
     int64, at most 64 each); beam -1 leaves its row alone.  A row that is written belongs to one request and stands once among its
-    ``out_rows``.  One launch."""
+    ``out_rows``.  The table must not overlap the numbers.  One launch."""
     rc = _lib.call_module().beam_reorder(table, rows, beams, out_rows, starts, ends)
     if rc != 0:
         _lib.check(rc)

@@ -488,6 +488,7 @@ const char* ft_extend_path_name(const ft_extend_args* args);
 /* ---- branching continuations: drafted trees, beams -------------------------------------------------------- */
 
 #define FT_MAX_DRAFT 1024 /* drafted tokens of a request */
+#define FT_MAX_VOCAB (1 << 30)
 
 /* ft_extend_plan_build for drafted tokens: the new tokens of request i are draft_lens[i] (at most FT_MAX_DRAFT) nodes of a tree,
  * and a token sees the cached tokens, its ancestors and itself.  The plan is made for the sizes alone; the trees are given to
@@ -527,7 +528,8 @@ typedef struct ft_draft_accept_args {
   int32_t* counts;      /* [num requests] accepted tokens */
   void* next_tokens;    /* [num requests] the model's token behind the last accepted one; -1 without any */
   const void* slots;    /* NULL, or [rows] the tokens' pool rows: with kv_entries, the request's entries behind its cached ones */
-  int32_t* kv_entries;  /*   become the accepted tokens' rows, in path order, then the others' */
+  int32_t* kv_entries;  /*   become the accepted tokens' rows, in path order, then the others'.  Of a plan with one request slots may lie
+                             in kv_entries (be those very entries); otherwise no result may overlap what is read */
   int32_t dtype;        /* enum ft_dtype, of logits */
   int32_t vocab;
   int32_t targets_64, tokens_64, parents_64, next_64, slots_64, num_requests;
@@ -551,7 +553,7 @@ int ft_draft_accept(const ft_draft_accept_args* args);
 typedef struct ft_beam_select_args {
   const void* logits;   /* [batch, beams, vocab] */
   const float* scores;  /* [batch, beams] */
-  float* out_scores;    /* [batch, best] */
+  float* out_scores;    /* [batch, best]; may be scores (its rows the same or longer), else no result may overlap what is read */
   void* out_beams;      /* [batch, best] int32 or int64, as out_tokens */
   void* out_tokens;
   void* workspace;      /* ft_beam_select_workspace(args) bytes, 16-byte aligned; the call's own */

@@ -263,6 +263,41 @@ def test_refusals():
         fasttree.fasttree_beam_reorder(table, many, many)
 
 
+@gpu
+def test_scores_in_place():
+    logits, scores = inputs(30, 4, 7000, torch.bfloat16, seed=9)
+    out, ob, ot = select(logits, scores, 4)
+    again = scores.clone()
+    fasttree.fasttree_beam_select(logits, again, again, ob.clone(), ot.clone())
+    wide = torch.zeros(30, 9, device="cuda")
+    wide[:, :4] = scores
+    fasttree.fasttree_beam_select(logits, wide[:, :4], wide[:, :4], ob.clone(), ot.clone())
+    assert torch.equal(again, out) and torch.equal(wide[:, :4], out) and bool((wide[:, 4:] == 0).all())
+    out, ob, ot = select(logits, scores, 9)
+    wide[:, :4] = scores
+    fasttree.fasttree_beam_select(logits, wide[:, :4], wide, ob.clone(), ot.clone())
+    assert torch.equal(wide, out)
+
+
+@gpu
+def test_results_that_overlap_what_is_read_are_refused():
+    logits, scores = inputs(3, 4, 100, torch.float32, seed=9)
+    big = torch.zeros(100, device="cuda")
+    ints = torch.zeros(100, dtype=torch.int32, device="cuda")
+    out, ob, ot = big[50:62].view(3, 4), ints[:12].view(3, 4), ints[12:24].view(3, 4)
+    for args in ((logits, scores, logits[:, :, :4][:, 0], ob, ot), (logits, big[:12].view(3, 4), big[4:16].view(3, 4), ob, ot),
+                 (logits, big[:24].view(3, 8)[:, ::2], big[:24].view(3, 8)[:, :4], ob, ot),
+                 (logits, scores, out, ob, ints[4:16].view(3, 4)), (logits, scores, ints.view(torch.float32)[:12].view(3, 4), ob, ot)):
+        with pytest.raises(lib.FastTreeError, match="overlap"):
+            fasttree.fasttree_beam_select(*args)
+    table = torch.zeros(6, 10, dtype=torch.int32, device="cuda")
+    rows = torch.arange(4, dtype=torch.int32, device="cuda").view(2, 2)
+    for args, kw in (((table, table[:2, :2], rows), {}), ((table, rows, table[2:4, 3:5]), {}), ((table, rows, rows), {"starts": table[0, :2]}),
+                     ((table, rows, rows), {"ends": table[5, 8:]}), ((table, rows, rows), {"out_rows": table[:2, :2]})):
+        with pytest.raises(lib.FastTreeError, match="overlap"):
+            fasttree.fasttree_beam_reorder(*args, **kw)
+
+
 def test_refusals_of_the_c_abi():
     handle = lib.load()
     a = lib.BeamSelectArgs()

@@ -217,6 +217,34 @@ def test_refusals():
             fasttree.fasttree_draft_accept(**{**good, **change})
 
 
+@gpu
+def test_the_rows_may_stand_at_their_entries():
+    for seed in range(3):
+        s = Step([40], 900, torch.float16, seed=seed)
+        expect = s.run()
+        table = torch.full((1, s.width), -5, dtype=torch.int32, device="cuda")
+        entries = table[0, s.cached[0]:s.cached[0] + 40]
+        entries.copy_(s.slots)
+        accepted, counts = torch.empty(1, 40, dtype=torch.int32, device="cuda"), torch.empty(1, dtype=torch.int32, device="cuda")
+        fasttree.fasttree_draft_accept(s.logits.cuda(), s.tokens.cuda(), torch.tensor(s.trees[0], device="cuda"), s.plan, accepted, counts,
+                                       torch.empty(1, dtype=torch.int64, device="cuda"), slots=entries, kv_entries=table)
+        assert torch.equal(table.cpu(), expect[3])
+
+
+@gpu
+def test_results_that_overlap_what_is_read_are_refused():
+    s = Step([3, 4], 50, torch.float16)
+    lg, pr = s.logits.cuda(), torch.zeros(7, dtype=torch.int32, device="cuda") - 1
+    big = torch.zeros(40, dtype=torch.int32, device="cuda")
+    tk, acc, cnt, nxt, table = big[:7], big[8:16].view(2, 4), big[16:18], big[18:20], torch.zeros(2 * s.width, dtype=torch.int32, device="cuda")
+    good = dict(logits=lg, tokens=tk, parents=pr, plan=s.plan, accepted=acc, counts=cnt, next_tokens=nxt, slots=big[20:27], kv_entries=table)
+    fasttree.fasttree_draft_accept(**good)
+    for change in ({"next_tokens": big[5:7]}, {"counts": big[0:2]}, {"accepted": big[4:12].view(2, 4)}, {"counts": big[12:14]}, {"next_tokens": big[17:19]},
+                   {"slots": table[3:10]}, {"slots": big[14:21]}, {"parents": big[10:17]}):
+        with pytest.raises(lib.FastTreeError, match="overlaps"):
+            fasttree.fasttree_draft_accept(**{**good, **change})
+
+
 def test_refusals_of_the_c_abi():
     handle = lib.load()
     a = lib.DraftAcceptArgs()
