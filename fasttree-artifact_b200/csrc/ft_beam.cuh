@@ -15,6 +15,7 @@
 
 namespace ft {
 
+constexpr int BEAM_CTAS = 4;  // of the scan on an SM
 constexpr int BEAM_THREADS = 256, BEAM_WARPS = BEAM_THREADS / 32;
 constexpr int BEAM_LIST = 512;   // logits that a slice lists, and pieces with one that it sets aside behind its first chunk; where more
 constexpr int BEAM_ASIDE = 256;  // reach its bound, it goes over the slice again with the list cut on the way
@@ -31,6 +32,7 @@ struct BeamParams {
   int64_t logits_s0, logits_s1, scores_s0, scores_s1, out_scores_s0, out_beams_s0, out_tokens_s0;
   int32_t batch, beams, vocab, best, beams_64, tokens_64;
   int32_t slices, chunks, per_cta;  // most slices of a row, its chunks, chunks of a CTA
+  int32_t pitch;                    // places for a row's chunks: as many as it has, or what its own CTAs have together
 };
 
 // The scan's BEAM_THREADS threads that read logits; one more warp sends for them.
@@ -109,7 +111,7 @@ __device__ __forceinline__ void best_of_list(const unsigned long long* keys, int
 // Shared memory of beam_scan_kernel: stages of a chunk each, as its bytes stand in memory from the 16-byte border below on.
 template <int NV>
 struct BeamScan {
-  static constexpr int STAGES = 3, CHUNK_BYTES = BEAM_THREADS * NV * 16, STAGE_BYTES = CHUNK_BYTES + 32, SMEM_BYTES = STAGES * STAGE_BYTES;
+  static constexpr int STAGES = 2, CHUNK_BYTES = BEAM_THREADS * NV * 16, STAGE_BYTES = CHUNK_BYTES + 32, SMEM_BYTES = STAGES * STAGE_BYTES;
   static constexpr int WAIT_LIMIT = 1 << 16;
 };
 
@@ -118,9 +120,10 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
-// Chunks of NV x 16 bytes a thread, that one warp sends for, three ahead of the eight that read them.  The call's rows are cut into
-// p.chunks chunks each, and a CTA takes p.per_cta of them as they follow one another: the end of a row, rows, the start of one.  What it
-// has of a row is a slice: slice number s of a row is that of the s-th CTA that has some of it.
+// Chunks of NV x 16 bytes a thread, that one warp sends for, two ahead of the eight that read them.  A row has p.chunks chunks in
+// p.pitch places, and a CTA takes p.per_cta of the places as they follow one another.  What it has of a row is a slice: slice
+// number s of a row is that of the s-th CTA that has some of it.  A slice costs about as much as seven chunks beside its own, so
+// rows are cut into slices of CTAs of their own (whole rows if they are many) where that leaves few CTAs idle.
 //
 // VEC: rows start on 16 bytes, and a thread reads 16 bytes at a time; else it reads words of 4 (a rule of the call, not of the row, so
 // that equal rows cut alike have equal sums).  Copies are of whole 16-byte pieces inside the row; what stands at its ends is filled in.
@@ -134,7 +137,7 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 // bound notes the piece, and the logits that do are found by all threads
 // together: done on the spot it takes the whole warp for one thread's.
 template <typename T, int NV, bool VEC>
-__global__ void __launch_bounds__(BEAM_THREADS + 32, 3) beam_scan_kernel(const BeamParams p) {
+__global__ void __launch_bounds__(BEAM_THREADS + 32, BEAM_CTAS) beam_scan_kernel(const BeamParams p) {
   using C = BeamScan<NV>;
   constexpr int S = (int)sizeof(T), N = 16 / S, CHUNK = BEAM_THREADS * NV * N, PAIR = NV > 1 ? 2 : 1;
   constexpr int PIECES = BEAM_THREADS * NV / PAIR, E = PAIR * N;  // pieces (of one or two vectors) of a chunk, their elements
@@ -154,8 +157,8 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, 3) beam_scan_kernel(const B
   allow_dependent_launch();
   wait_for_prior_grid();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t all_chunks = (int64_t)p.batch * p.beams * p.chunks, chunk0 = (int64_t)blockIdx.x * p.per_cta;
-  const int todo = (int)(all_chunks - chunk0 < p.per_cta ? all_chunks - chunk0 : p.per_cta);
+  const int64_t all_places = (int64_t)p.batch * p.beams * p.pitch, place0 = (int64_t)blockIdx.x * p.per_cta;
+  int todo = (int)(all_places - place0 < p.per_cta ? all_places - place0 : p.per_cta);
   const uint32_t full0 = (uint32_t)__cvta_generic_to_shared(barrier), empty0 = full0 + 8 * C::STAGES;
   struct Row {
     uintptr_t at;
@@ -166,7 +169,8 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, 3) beam_scan_kernel(const B
     const float score = __ldg(p.scores + req * p.scores_s0 + beam * p.scores_s1);
     return Row{reinterpret_cast<uintptr_t>(static_cast<const T*>(p.logits) + req * p.logits_s0 + beam * p.logits_s1), fabsf(score) < INFINITY};
   };
-  int row = (int)(chunk0 / p.chunks), k = (int)(chunk0 - (int64_t)row * p.chunks), stage = 0;
+  int row = (int)(place0 / p.pitch), k = (int)(place0 - (int64_t)row * p.pitch), stage = 0;
+  if (p.pitch > p.chunks) todo = min(todo, p.chunks - k);  // (a row's CTAs are its own: the last one's last places are empty)
   uint32_t phase = 0;
   Row here = {0, false};
   bool fresh = true;  // a slice begins
@@ -399,7 +403,7 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, 3) beam_scan_kernel(const B
       fresh = ends;
       if (ends) {
         // ---- the slice's list, and the threads' sums over the largest offset
-        const int64_t slice = (int64_t)blockIdx.x - (int64_t)row * p.chunks / p.per_cta, at = (int64_t)row * p.slices + slice;
+        const int64_t slice = (int64_t)blockIdx.x - (int64_t)row * p.pitch / p.per_cta, at = (int64_t)row * p.slices + slice;
         const float mine = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         const float mine_off = top == -INFINITY ? -INFINITY : off;
         const float warp_off = warp_max(mine_off), from = warp_off == -INFINITY ? 0.f : warp_off;

@@ -56,7 +56,7 @@ int launch_accept(const ft::AcceptParams& p, int requests, int64_t row_bytes, cu
 }
 
 struct BeamShape {
-  int pieces, slices, chunks, per_cta;
+  int pieces, slices, chunks, per_cta, pitch;
   int64_t ctas, keys, bytes;  // of the workspace: keys, then sums
 };
 
@@ -72,27 +72,41 @@ int check_beam_select(const ft_beam_select_args* a) {
   return FT_OK;
 }
 
-// Chunks of a call and how many a CTA takes: three CTAs to an SM, all at once.  Chunks of 16 KB, smaller ones where the call would leave SMs
-// without any or rows are shorter.  (148 SMs whatever the device: the workspace's size goes by this.)
+// Chunks of a call and how many a CTA takes, all CTAs at once.  Chunks of 16 KB, smaller ones where the call would leave SMs without any or
+// rows are shorter.  In chunks, a slice costs seven beside its own: dealt evenly, a CTA has the ends of two rows or more; with CTAs
+// of their own, or whole rows to a CTA, rows have no more slices than they need (64 x 4 rows of 16 chunks, two CTAs to a row: 29 us,
+// seven chunks to a CTA 31).  (148 SMs whatever the device: the workspace's size goes by this.)
 BeamShape beam_shape(const ft_beam_select_args* a) {
   BeamShape s;
   const int n = 16 / dtype_size(a->dtype);
-  const int64_t rows = (int64_t)a->batch * a->beams, ctas = 3 * 148;
+  const int64_t rows = std::max<int64_t>(1, (int64_t)a->batch * a->beams), ctas = ft::BEAM_CTAS * 148;
   int64_t chunk = 0;
   for (s.pieces = 4;; s.pieces /= 2) {
     chunk = (int64_t)ft::BEAM_THREADS * n * s.pieces;
     s.chunks = (int)((a->vocab + chunk - 1) / chunk);
     if (s.pieces == 1 || (rows * s.chunks >= 2 * 148 && chunk <= a->vocab)) break;
   }
-  s.per_cta = (int)std::max<int64_t>(1, (rows * s.chunks + ctas - 1) / ctas);
-  s.ctas = (rows * s.chunks + s.per_cta - 1) / s.per_cta;
-  s.slices = std::min((s.chunks - 1) / s.per_cta + 2, s.chunks);
+  const int64_t even = (rows * s.chunks + ctas - 1) / ctas;
+  s.per_cta = (int)even;
+  s.pitch = s.chunks;
+  if (rows <= ctas) {
+    const int64_t own = (s.chunks + ctas / rows - 1) / (ctas / rows);  // chunks of a CTA, with ctas / rows of them to a row
+    if (own <= even + 7) {
+      s.per_cta = (int)own;
+      s.pitch = (int)((s.chunks + own - 1) / own * own);
+    }
+  } else {
+    const int64_t each = (rows + ctas - 1) / ctas;  // rows of a CTA; dealt evenly it has one more slice
+    if (each * s.chunks <= even + 7) s.per_cta = (int)(each * s.chunks);
+  }
+  s.ctas = (rows * s.pitch + s.per_cta - 1) / s.per_cta;
+  s.slices = s.pitch > s.chunks ? s.pitch / s.per_cta : s.chunks % s.per_cta == 0 ? s.chunks / s.per_cta : s.per_cta % s.chunks == 0 ? 1 : std::min((s.chunks - 1) / s.per_cta + 2, s.chunks);
   s.keys = rows * s.slices * a->best;
   s.bytes = s.keys * 8 + rows * s.slices * 8;
   return s;
 }
 
-constexpr int BEAM_MERGE_SMEM = 160 << 10;
+constexpr int BEAM_MERGE_SMEM = 176 << 10;
 
 int pow2_at_least(int n, int low) {
   while (low < n) low *= 2;
@@ -116,7 +130,7 @@ int launch_beam_select(const ft::BeamParams& p, const BeamShape& s, bool vec, cu
                  : s.pieces == 2 ? (vec ? launch_scan_as<T, 2, true>(p, s, st) : launch_scan_as<T, 2, false>(p, s, st))
                                  : (vec ? launch_scan_as<T, 4, true>(p, s, st) : launch_scan_as<T, 4, false>(p, s, st));
   if (rc != FT_OK) return rc;
-  const int64_t smem = 4LL * p.beams * p.slices * p.best;  // at most 64 results of 444 + 64 slices
+  const int64_t smem = 4LL * p.beams * p.slices * p.best;  // at most 64 results of 592 + 64 slices
   static OncePerDevice once;
   FT_CUDA_OK(raise_smem_limit(once, ft::beam_merge_kernel, BEAM_MERGE_SMEM));
   if (smem > BEAM_MERGE_SMEM) return fail(FT_ERR_TOO_LARGE, "more slices of logits than a request's merge holds");
@@ -248,7 +262,7 @@ int ft_beam_select(const ft_beam_select_args* a) {
   p.sums = reinterpret_cast<float2*>(p.keys + s.keys);
   p.logits_s0 = a->logits_stride0, p.logits_s1 = a->logits_stride1, p.scores_s0 = a->scores_stride0, p.scores_s1 = a->scores_stride1;
   p.out_scores_s0 = a->out_scores_stride0, p.out_beams_s0 = a->out_beams_stride0, p.out_tokens_s0 = a->out_tokens_stride0;
-  p.batch = a->batch, p.beams = a->beams, p.vocab = a->vocab, p.best = a->best, p.slices = s.slices, p.chunks = s.chunks, p.per_cta = s.per_cta;
+  p.batch = a->batch, p.beams = a->beams, p.vocab = a->vocab, p.best = a->best, p.slices = s.slices, p.chunks = s.chunks, p.per_cta = s.per_cta, p.pitch = s.pitch;
   p.beams_64 = a->beams_64, p.tokens_64 = a->tokens_64;
   const int n = 16 / dtype_size(a->dtype);
   const bool vec = aligned16(a->logits) && (a->batch == 1 || a->logits_stride0 % n == 0) && (a->beams == 1 || a->logits_stride1 % n == 0);
