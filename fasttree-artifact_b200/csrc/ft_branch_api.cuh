@@ -164,7 +164,9 @@ int ft_draft_tree(const ft_draft_tree_args* a) {
   p.parents = a->parents, p.positions = a->positions;
   p.parents_64 = a->parents_64, p.positions_64 = a->positions_64;
   p.window = a->plan.window, p.words = a->plan.tile_tokens / 32;
-  ft::draft_tree_kernel<<<(unsigned)a->plan.num_drafts, ft::DRAFT_THREADS, 0, static_cast<cudaStream_t>(a->stream)>>>(p);
+  // (a token of a long chain climbs through all of its spans: a CTA for every 128 tokens of the longest draft)
+  const dim3 grid((unsigned)a->plan.num_drafts, (unsigned)((a->plan.longest_draft + 127) / 128));
+  ft::draft_tree_kernel<<<grid, ft::DRAFT_THREADS, 0, static_cast<cudaStream_t>(a->stream)>>>(p);
   FT_CUDA_OK(cudaGetLastError());
   count_launch();
   return FT_OK;

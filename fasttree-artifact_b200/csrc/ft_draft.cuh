@@ -39,50 +39,74 @@ __device__ __forceinline__ int64_t load_slot(const void* p, int is_64, int64_t i
   return is_64 ? static_cast<const volatile long long*>(p)[i] : (int64_t)static_cast<const volatile int*>(p)[i];
 }
 
+constexpr int DRAFT_THREADS = 128, DRAFT_OWN = FT_MAX_DRAFT / DRAFT_THREADS;  // tokens that a thread looks after
+static_assert(DRAFT_OWN * DRAFT_THREADS == FT_MAX_DRAFT, "every token has a thread");
+
 // The tree of a request into shared memory: parent[i] is -1 (a root), -2 (padding) or an earlier token; what is none of these, and
-// what hangs on padding, becomes padding.  A whole block; ends with a barrier.
-__device__ __forceinline__ void load_tree(const void* parents, int is_64, const Draft& d, int16_t* parent, int16_t* depth) {
+// what hangs on padding, becomes padding.  Depths by doubling: jump[i] is i's 2^n-th ancestor, or what its climb ends on (below 0),
+// depth[i] the steps to it, so ten rounds do for the longest chain.  A whole block; ends with a barrier.
+__device__ __forceinline__ void load_tree(const void* parents, int is_64, const Draft& d, int16_t* parent, int16_t* depth, int16_t* jump) {
+  const int own = (d.n + DRAFT_THREADS - 1) / DRAFT_THREADS;
   bool bad = false;
-  for (int i = threadIdx.x; i < d.n; i += blockDim.x) {
-    const int64_t p = load_index(parents, is_64, (int64_t)d.row + i);
-    const bool ok = p >= -2 && p < i;
-    bad |= !ok;
-    parent[i] = (int16_t)(ok ? (int)p : -2);
+  int to[DRAFT_OWN], steps[DRAFT_OWN];
+#pragma unroll
+  for (int k = 0; k < DRAFT_OWN; ++k) {
+    const int i = threadIdx.x + k * DRAFT_THREADS;
+    to[k] = -2, steps[k] = 0;
+    if (k >= own) continue;
+    if (i < d.n) {
+      const int64_t p = load_index(parents, is_64, (int64_t)d.row + i);
+      const bool ok = p >= -2 && p < i;
+      bad |= !ok;
+      to[k] = ok ? (int)p : -2;
+      steps[k] = to[k] >= 0;
+      parent[i] = jump[i] = (int16_t)to[k];
+      depth[i] = (int16_t)steps[k];
+    }
   }
   __syncthreads();
-  // climbs see the parents as they were given, so what hangs on padding is marked afterwards
-  uint32_t lost = 0;
-  for (int i = threadIdx.x, k = 0; i < d.n; i += blockDim.x, ++k) {
-    int at = i, steps = 0;
-    for (int up = parent[at]; up >= 0; up = parent[at]) {
-      at = up;
-      ++steps;
+  while (true) {
+    bool more = false;
+#pragma unroll
+    for (int k = 0; k < DRAFT_OWN; ++k)
+      if (k < own && to[k] >= 0) {
+        steps[k] += depth[to[k]];
+        to[k] = jump[to[k]];
+        more |= to[k] >= 0;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < DRAFT_OWN; ++k) {
+      const int i = threadIdx.x + k * DRAFT_THREADS;
+      if (k < own && i < d.n) {
+        jump[i] = (int16_t)to[k];
+        depth[i] = (int16_t)steps[k];
+      }
     }
-    if (at != i && parent[at] == -2) {
-      lost |= 1u << k;
-      steps = 0;
-    }
-    depth[i] = (int16_t)steps;
+    if (!__syncthreads_or(more)) break;
   }
-  __syncthreads();
-  for (int i = threadIdx.x, k = 0; i < d.n; i += blockDim.x, ++k)
-    if ((lost >> k & 1u) != 0) parent[i] = -2;
-  if (bad || lost != 0) flag_error(FT_DEV_BAD_PARENT);
+#pragma unroll
+  for (int k = 0; k < DRAFT_OWN; ++k) {
+    const int i = threadIdx.x + k * DRAFT_THREADS;
+    if (k < own && i < d.n && to[k] == -2 && steps[k] > 0) {  // it hangs on padding
+      bad = true;
+      parent[i] = -2;
+      depth[i] = 0;
+    }
+  }
+  if (bad) flag_error(FT_DEV_BAD_PARENT);
   __syncthreads();
 }
 
-constexpr int DRAFT_THREADS = 128;
-static_assert(FT_MAX_DRAFT <= 32 * DRAFT_THREADS, "a bit per token that a thread looks at");
-
-// A CTA per request: positions of its tokens, and the words that its tree decides.  Bound by a chain of three reads (request, parents
-// and spans, words) and a climb.  Two stretches of a tile may share a word, in different bits: clearing and setting are
+// A CTA per request (several, with the spans shared out, where drafts are long): positions of its tokens, and the words that its tree
+// decides.  Bound by a chain of three reads (request, parents and spans, words) and a climb.  Two stretches of a tile may share a word, in different bits: clearing and setting are
 // atomic, and their order does not matter.
 __global__ void __launch_bounds__(DRAFT_THREADS) draft_tree_kernel(const DraftParams p) {
-  __shared__ int16_t parent[FT_MAX_DRAFT], depth[FT_MAX_DRAFT];
+  __shared__ int16_t parent[FT_MAX_DRAFT], depth[FT_MAX_DRAFT], jump[FT_MAX_DRAFT];
   allow_dependent_launch();
   const Draft d = load_draft(p.drafts, blockIdx.x);
   if (d.n == 0) return;
-  const int warp = threadIdx.x >> 5;
+  const int warp = (threadIdx.x >> 5) + blockIdx.y * (DRAFT_THREADS / 32), warps = gridDim.y * (DRAFT_THREADS / 32);
   int4 a = make_int4(0, 0, 0, 0), b = a;  // the warp's next span
   auto fetch = [&](int s) {
     const int4* raw = reinterpret_cast<const int4*>(p.spans + d.span0 + s);
@@ -90,8 +114,8 @@ __global__ void __launch_bounds__(DRAFT_THREADS) draft_tree_kernel(const DraftPa
     b = __ldg(raw + 1);
   };
   if (warp < d.spans) fetch(warp);
-  load_tree(p.parents, p.parents_64, d, parent, depth);
-  if (p.positions != nullptr)
+  load_tree(p.parents, p.parents_64, d, parent, depth, jump);
+  if (p.positions != nullptr && blockIdx.y == 0)
     for (int i = threadIdx.x; i < d.n; i += DRAFT_THREADS) {
       const int64_t at = (int64_t)d.row + i;
       if (p.positions_64)
@@ -99,7 +123,7 @@ __global__ void __launch_bounds__(DRAFT_THREADS) draft_tree_kernel(const DraftPa
       else
         static_cast<int*>(p.positions)[at] = d.cached + depth[i];
     }
-  for (int s = warp; s < d.spans; s += DRAFT_THREADS / 32) {
+  for (int s = warp; s < d.spans; s += warps) {
     const DraftSpan span = {a.x, a.y, a.z, a.w, b.x, b.y, 0, 0};
     for (int k = threadIdx.x & 31; k < span.tokens; k += 32)
       draft_span_words(span, k, p.window, parent, depth, [&](int word, uint32_t mask, uint32_t bits) {
@@ -111,7 +135,7 @@ __global__ void __launch_bounds__(DRAFT_THREADS) draft_tree_kernel(const DraftPa
           atomicOr(at, (int32_t)bits);
         }
       });
-    if (s + DRAFT_THREADS / 32 < d.spans) fetch(s + DRAFT_THREADS / 32);
+    if (s + warps < d.spans) fetch(s + warps);
   }
 }
 

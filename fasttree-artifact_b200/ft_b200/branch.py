@@ -52,7 +52,8 @@ def beam_select(logits, scores, out_scores, out_beams, out_tokens):
     ``[batch, beams]``.  Results ``[batch, n]``, best first: ``out_scores`` fp32, ``out_beams`` and ``out_tokens`` int32 or int64; at most 64
     beams and results.  Of equal scores the lowest beam's comes first, then the larger logit, then the lowest token.  Logits of -inf are
     never chosen (banned tokens), nor is anything from a beam whose score is not finite (-inf: a beam that ended, or has not begun) or whose
-    logits hold NaN or +inf; where too little is left the last results are score -inf, beam -1, token -1.  ``out_scores`` may be ``scores``, or start with it
+    logits hold NaN or +inf; where too little is left the last results are score -inf, beam -1, token -1.  The logarithms are good to about
+    1e-7: scores of different beams that are closer may come in either order.  ``out_scores`` may be ``scores``, or start with it
     in every row; otherwise no result may overlap what is read.  Two launches."""
     rc = _lib.call_module().beam_select(logits, scores, out_scores, out_beams, out_tokens)
     if rc != 0:

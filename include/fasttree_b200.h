@@ -549,7 +549,8 @@ int ft_draft_accept(const ft_draft_accept_args* args);
 /* The `best` best continuations of each request's beams: score = scores[beam] + logits[beam][token] - log sum exp(logits[beam]),
  * best first; of equal scores the lowest beam's first, then the larger logit, then the lowest token.  Logits of -inf are never chosen, nor is anything from a
  * beam whose score is not finite (one that ended, say) or whose logits hold NaN or +inf; where too little is left the last
- * results are score -inf, beam -1, token -1. */
+ * results are score -inf, beam -1, token -1.  Scores are compared in 64 bits; the logarithms are good to about 1e-7, so closer scores
+ * of different beams may come in either order. */
 typedef struct ft_beam_select_args {
   const void* logits;   /* [batch, beams, vocab] */
   const float* scores;  /* [batch, beams] */

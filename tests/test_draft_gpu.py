@@ -167,6 +167,30 @@ def test_captured_step_with_new_trees():
 
 
 @gpu
+def test_captured_behind_copies():
+    # launches that may start early, with a copy instead of a kernel before them
+    s = Step([150, 90], [20, 33], [], 32, 8, 128, torch.float16, seed=6)
+    s.grow()
+    want, _ = s.run()
+    q, o = torch.zeros_like(s.gq), torch.empty_like(s.gq)
+    rows = torch.arange(6, device="cuda").view(2, 3)
+    beams, source = torch.tensor([[2, 0, 1], [1, 1, 0]], device="cuda"), torch.arange(600, device="cuda").view(6, 100)
+    table, graph = torch.zeros_like(source), torch.cuda.CUDAGraph()
+    extend.extend(s.gq, s.gk, s.gv, o, s.gt, s.plan, s.scale)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        q.copy_(s.gq)
+        fasttree.fasttree_extend(q, s.gk, s.gv, o, s.gt, s.plan, s.scale)
+        table.copy_(source)
+        fasttree.fasttree_beam_reorder(table, rows, beams)
+    for _ in range(3):
+        o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o[:53], want[:53]) and torch.equal(table, source[torch.gather(rows, 1, beams).flatten()])
+
+
+@gpu
 def test_refusals():
     s = Step([3], [4], [], 8, 2, 128, torch.float16, pad_rows=0)
     good = s.parents()
