@@ -39,70 +39,63 @@ __device__ __forceinline__ int64_t load_slot(const void* p, int is_64, int64_t i
   return is_64 ? static_cast<const volatile long long*>(p)[i] : (int64_t)static_cast<const volatile int*>(p)[i];
 }
 
-constexpr int DRAFT_THREADS = 128, DRAFT_OWN = FT_MAX_DRAFT / DRAFT_THREADS;  // tokens that a thread looks after
-static_assert(DRAFT_OWN * DRAFT_THREADS == FT_MAX_DRAFT, "every token has a thread");
+constexpr int DRAFT_THREADS = 128;
 
-// The tree of a request into shared memory: parent[i] is -1 (a root), -2 (padding) or an earlier token; what is none of these, and
-// what hangs on padding, becomes padding.  Depths by doubling: jump[i] is i's 2^n-th ancestor, or what its climb ends on (below 0),
-// depth[i] the steps to it, so ten rounds do for the longest chain.  A whole block; ends with a barrier.
-__device__ __forceinline__ void load_tree(const void* parents, int is_64, const Draft& d, int16_t* parent, int16_t* depth, int16_t* jump) {
-  const int own = (d.n + DRAFT_THREADS - 1) / DRAFT_THREADS;
+// A request's tree in shared memory.
+struct Tree {
+  int16_t parent[FT_MAX_DRAFT];                      // -1: a root, -2: padding, else an earlier token
+  int16_t jump[2][FT_MAX_DRAFT], depth[2][FT_MAX_DRAFT];  // by turns, see load_tree
+};
+
+// Reads the tree; a parent that is none, and what hangs on padding, makes a token padding.  Depths by doubling: jump is a token's
+// 2^n-th ancestor, or what its climb ends on (below 0), depth the steps to it, so ten rounds do for the longest chain.  Returns
+// the depths.  A whole block; ends with a barrier.  (Loops are not unrolled: the kernel is as long as its way from memory.)
+__device__ __forceinline__ const int16_t* load_tree(const void* parents, int is_64, const Draft& d, Tree& t) {
   bool bad = false;
-  int to[DRAFT_OWN], steps[DRAFT_OWN];
-#pragma unroll
-  for (int k = 0; k < DRAFT_OWN; ++k) {
-    const int i = threadIdx.x + k * DRAFT_THREADS;
-    to[k] = -2, steps[k] = 0;
-    if (k >= own) continue;
-    if (i < d.n) {
-      const int64_t p = load_index(parents, is_64, (int64_t)d.row + i);
-      const bool ok = p >= -2 && p < i;
-      bad |= !ok;
-      to[k] = ok ? (int)p : -2;
-      steps[k] = to[k] >= 0;
-      parent[i] = jump[i] = (int16_t)to[k];
-      depth[i] = (int16_t)steps[k];
-    }
+#pragma unroll 1
+  for (int i = threadIdx.x; i < d.n; i += DRAFT_THREADS) {
+    const int64_t p = load_index(parents, is_64, (int64_t)d.row + i);
+    const bool ok = p >= -2 && p < i;
+    bad |= !ok;
+    t.parent[i] = t.jump[0][i] = (int16_t)(ok ? (int)p : -2);
+    t.depth[0][i] = ok && p >= 0;
   }
   __syncthreads();
-  while (true) {
-    bool more = false;
-#pragma unroll
-    for (int k = 0; k < DRAFT_OWN; ++k)
-      if (k < own && to[k] >= 0) {
-        steps[k] += depth[to[k]];
-        to[k] = jump[to[k]];
-        more |= to[k] >= 0;
+  int now = 0;
+  bool more;
+#pragma unroll 1
+  do {
+    more = false;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < d.n; i += DRAFT_THREADS) {
+      int to = t.jump[now][i], steps = t.depth[now][i];
+      if (to >= 0) {
+        steps += t.depth[now][to];
+        to = t.jump[now][to];
+        more |= to >= 0;
       }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < DRAFT_OWN; ++k) {
-      const int i = threadIdx.x + k * DRAFT_THREADS;
-      if (k < own && i < d.n) {
-        jump[i] = (int16_t)to[k];
-        depth[i] = (int16_t)steps[k];
-      }
+      t.jump[now ^ 1][i] = (int16_t)to;
+      t.depth[now ^ 1][i] = (int16_t)steps;
     }
-    if (!__syncthreads_or(more)) break;
-  }
-#pragma unroll
-  for (int k = 0; k < DRAFT_OWN; ++k) {
-    const int i = threadIdx.x + k * DRAFT_THREADS;
-    if (k < own && i < d.n && to[k] == -2 && steps[k] > 0) {  // it hangs on padding
+    now ^= 1;
+  } while (__syncthreads_or(more));
+#pragma unroll 1
+  for (int i = threadIdx.x; i < d.n; i += DRAFT_THREADS)
+    if (t.jump[now][i] == -2 && t.depth[now][i] > 0) {  // it hangs on padding
       bad = true;
-      parent[i] = -2;
-      depth[i] = 0;
+      t.parent[i] = -2;
+      t.depth[now][i] = 0;
     }
-  }
   if (bad) flag_error(FT_DEV_BAD_PARENT);
   __syncthreads();
+  return t.depth[now];
 }
 
 // A CTA per request (several, with the spans shared out, where drafts are long): positions of its tokens, and the words that its tree
 // decides.  Bound by a chain of three reads (request, parents and spans, words) and a climb.  Two stretches of a tile may share a word, in different bits: clearing and setting are
 // atomic, and their order does not matter.
 __global__ void __launch_bounds__(DRAFT_THREADS) draft_tree_kernel(const DraftParams p) {
-  __shared__ int16_t parent[FT_MAX_DRAFT], depth[FT_MAX_DRAFT], jump[FT_MAX_DRAFT];
+  __shared__ Tree tree;
   allow_dependent_launch();
   const Draft d = load_draft(p.drafts, blockIdx.x);
   if (d.n == 0) return;
@@ -114,7 +107,7 @@ __global__ void __launch_bounds__(DRAFT_THREADS) draft_tree_kernel(const DraftPa
     b = __ldg(raw + 1);
   };
   if (warp < d.spans) fetch(warp);
-  load_tree(p.parents, p.parents_64, d, parent, depth, jump);
+  const int16_t* const depth = load_tree(p.parents, p.parents_64, d, tree);
   if (p.positions != nullptr && blockIdx.y == 0)
     for (int i = threadIdx.x; i < d.n; i += DRAFT_THREADS) {
       const int64_t at = (int64_t)d.row + i;
@@ -126,7 +119,7 @@ __global__ void __launch_bounds__(DRAFT_THREADS) draft_tree_kernel(const DraftPa
   for (int s = warp; s < d.spans; s += warps) {
     const DraftSpan span = {a.x, a.y, a.z, a.w, b.x, b.y, 0, 0};
     for (int k = threadIdx.x & 31; k < span.tokens; k += 32)
-      draft_span_words(span, k, p.window, parent, depth, [&](int word, uint32_t mask, uint32_t bits) {
+      draft_span_words(span, k, p.window, tree.parent, depth, [&](int word, uint32_t mask, uint32_t bits) {
         int32_t* at = p.extra + span.bits + k * p.words + word;
         if (mask == 0xffffffffu) {
           *at = (int32_t)bits;

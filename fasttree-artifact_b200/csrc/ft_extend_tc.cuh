@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
   auto bar = [&](int i) { return bars + 8u * i; };
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   allow_dependent_launch();
-  wait_for_prior_grid();
+  // (before the wait for the kernel ahead: set-up, and of memory the plan's schedule alone, which no kernel writes)
   const int4* my_share = reinterpret_cast<const int4*>(p.sms) + 4 * blockIdx.x;
   const int4 share = __ldg(my_share);
   const int task_lo = share.x, task_hi = share.y;
@@ -298,6 +298,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
   }
   // the end of the set-up, which every role passes once, before it waits for or touches anything that was set up
   auto set_up = [&]() {
+    wait_for_prior_grid();
     tc_fence_before();
     asm volatile("bar.sync 0;\n" ::: "memory");
     tc_fence_after();
@@ -873,17 +874,17 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
           ids_phase ^= 1u;
         }
       };
+      const int4 head = __ldg(my_share + 1), first_rec = __ldg(my_share + 2);
       set_up();
       for (int n = task_lo; n < task_hi && !dead; ++n, ++items) {
         int kvh, t0, t1, tile0;
         int4 rec;
         const int32_t* item = item_of(n, kvh);
         if (n == task_lo) {
-          const int4 head = __ldg(my_share + 1);
           t0 = head.x;
           t1 = head.y;
           tile0 = head.z;
-          rec = __ldg(my_share + 2);
+          rec = first_rec;
         } else {
           t0 = __ldg(item);
           t1 = __ldg(item + 1);
