@@ -537,10 +537,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamPara
     const double x = (double)from_ordered((uint32_t)(key >> 32)) + shift[i / per_beam];
     return scores[i] = key != 0 && x == x ? __double2float_rd(x) : -INFINITY;
   };
-  constexpr int EARLY = 4;  // keys a thread asks for before it needs them
-  unsigned long long early[EARLY];
-#pragma unroll
-  for (int k = 0; k < EARLY; ++k) early[k] = tid + k * BEAM_THREADS < total ? __ldcg(keys + tid + k * BEAM_THREADS) : 0;
+  const unsigned long long early = tid < total ? __ldcg(keys + tid) : 0;  // asked for before it is needed
   // 2^wide lanes to a beam, at least its slices if they are no more than 32
   int wide = 2;
   while (wide < 5 && (1 << wide) < p.slices) ++wide;
@@ -574,12 +571,8 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamPara
   }
   __syncthreads();
   float top = -INFINITY;
-#pragma unroll
-  for (int k = 0; k < EARLY; ++k) {
-    const int i = tid + k * BEAM_THREADS;
-    if (i < total) top = fmaxf(top, put_score(i, early[k]));
-  }
-  for (int i = tid + EARLY * BEAM_THREADS; i < total; i += BEAM_THREADS) top = fmaxf(top, put_score(i, __ldcg(keys + i)));
+#pragma unroll 1
+  for (int i = tid; i < total; i += BEAM_THREADS) top = fmaxf(top, put_score(i, i == tid ? early : __ldcg(keys + i)));
   top = warp_max(top);
   if (lane == 0) high[warp] = top;
   __syncthreads();
@@ -597,7 +590,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamPara
   int turn = 0;
   auto reach = [&](float least) {  // how many do
     int n = 0;
-#pragma unroll 4
+#pragma unroll 2
     for (int i = tid; i < total; i += BEAM_THREADS) n += scores[i] >= least;
     n = __reduce_add_sync(0xffffffffu, n);
     if (lane == 0) counts[turn][warp] = n;

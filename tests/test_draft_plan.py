@@ -9,7 +9,6 @@ import branch_cases
 import extend_cases
 import fasttree
 from ft_b200 import extend, lib
-from test_extend_plan import shown
 
 
 def plan_of(cached, nodes, shared, hq, hkv, d, dtype=torch.float16, window=0, sms=148):
@@ -46,7 +45,7 @@ def grow(info, plan, trees):
 
 def check_sight(info, plan, table, cached, trees, window):
     entries = table.reshape(-1).numpy()
-    seen, writers, _, _ = shown_with_empty(info, plan, entries)
+    seen, writers = shown(info, plan, entries)
     row = 0
     for r, (c, parents) in enumerate(zip(cached, trees)):
         sight, _ = branch_cases.in_sight(c, parents, window)
@@ -57,12 +56,9 @@ def check_sight(info, plan, table, cached, trees, window):
     assert not [x for x in seen if x >= row]
 
 
-def shown_with_empty(info, plan, entries):
-    """test_extend_plan.shown, which holds that a token with a partial row sees something there: a tree may take that away."""
-    try:
-        return shown(info, plan, entries)
-    except AssertionError:
-        pass
+def shown(info, plan, entries):
+    """Per q row the pool rows it is shown and its writers.  (test_extend_plan.shown holds that a token with a partial row sees something
+    there: a tree may take that away.)"""
     t = plan.tolist()
     words = info.tile_tokens // 32
     seen, writers = {}, {}
@@ -92,7 +88,7 @@ def shown_with_empty(info, plan, entries):
     for i in range(info.num_merged):
         q_row = t[info.merge_off + 4 * i]
         writers[q_row] = writers.get(q_row, 0) + 1
-    return seen, writers, None, None
+    return seen, writers
 
 
 HEADS = [(32, 8, 128, torch.float16), (16, 16, 64, torch.bfloat16), (16, 8, 256, torch.float16), (8, 2, 128, torch.float32),
