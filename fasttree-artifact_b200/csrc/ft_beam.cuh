@@ -415,11 +415,21 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, BEAM_CTAS) beam_scan_kernel
         const float total = warp_sum(mine == 0.f ? 0.f : mine * fast_exp2(mine_off - from));
         if (lane == 0) sums[warp] = make_float2(warp_off, total);
         if (lost) {
-          // more than there was room for, equal ones for the most part: all of the slice's logits again, the list cut when it may overflow
+          // more than there was room for (the largest logits late in the slice, or many equal ones): all of the slice's logits twice
+          // again, for a bound by the threads' largest of all and for the list, which is cut when it may overflow
           constexpr int AT_ONCE = 8;
           const T* const logits = reinterpret_cast<const T*>(here.at);
           const int stop = min(p.vocab, first + CHUNK);
-          unsigned long long bound = 0;
+          float largest = -INFINITY;
+          for (int i0 = from_k * CHUNK; i0 < stop; i0 += AT_ONCE * BEAM_THREADS) {
+            float y[AT_ONCE];
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) y[u] = i0 + u * BEAM_THREADS + tid < stop ? to_float<T>(logits[i0 + u * BEAM_THREADS + tid]) : -INFINITY;
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) largest = fmaxf(largest, y[u]);
+          }
+          const float low_bound = logit_bound(largest, p.best, min(stop - from_k * CHUNK, BEAM_THREADS), low);
+          unsigned long long bound = (unsigned long long)ordered(fmaxf(low_bound, LEAST)) << 32;  // (below every key of that value)
           int turn = 0;
           count = 0;
           auto cut_list = [&](int most) {
