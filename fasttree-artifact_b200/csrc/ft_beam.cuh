@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamPara
     }
     if (step < 1e6f)
       for (int i = 0; i < 24 && n > enough; ++i) {
-        const float middle = 0.5f * (above + least);
+        const float middle = 0.5f * above + 0.5f * least;  // (their sum may be beyond fp32)
         const int m = reach(middle);
         if (m >= p.best) {
           least = middle;
