@@ -543,9 +543,11 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamPara
   const float2* __restrict__ sums = p.sums + (int64_t)req * p.beams * p.slices;
   const int per_beam = p.slices * p.best, total = p.beams * per_beam;
   const unsigned long long* __restrict__ keys = p.keys + (int64_t)req * total;
+  constexpr float LEAST = -3.4028234e38f;
   auto put_score = [&](int i, unsigned long long key) {
     const double x = (double)from_ordered((uint32_t)(key >> 32)) + shift[i / per_beam];
-    return scores[i] = key != 0 && x == x ? __double2float_rd(x) : -INFINITY;
+    // (one that is lower than all of fp32 is a candidate still)
+    return scores[i] = key != 0 && x == x ? fmaxf(__double2float_rd(x), LEAST) : -INFINITY;
   };
   const unsigned long long early = tid < total ? __ldcg(keys + tid) : 0;  // asked for before it is needed
   // 2^wide lanes to a beam, at least its slices if they are no more than 32
@@ -613,7 +615,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamPara
   };
   // the threshold: steps that grow away from the best until enough reach it, then halves between the last two
   const int enough = 2 * p.best + 32;
-  float least = -3.4028234e38f;
+  float least = LEAST;
   int n = total;
   if (top > -INFINITY && total > enough) {
     float above = top, step = 1.f;

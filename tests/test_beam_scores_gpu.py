@@ -38,3 +38,15 @@ def test_scores_far_from_one_another(far):
     scores[3] = torch.linspace(-far, far, 6)
     for best in (3, 40):
         check(logits, scores, best)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sums_below_all_of_fp32(dtype):
+    # logit and score are fp32's own, their sum is not: such a token comes last, and its score rounds to -inf
+    logits, scores, _ = inputs(2, 3, 8, dtype, seed=7)
+    logits[:, :, 1::4] = -2e38
+    scores[0, 0] = -2e38
+    scores[1] = -2e38
+    for best in (20, 64):
+        check(logits, scores, best)
