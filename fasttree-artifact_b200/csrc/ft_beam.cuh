@@ -29,7 +29,7 @@ struct BeamParams {
   void* out_beams;
   void* out_tokens;
   unsigned long long* keys;  // [rows][slices][best] {ordered logit, ~token}, 0: none
-  float2* sums;              // [rows][slices] {c, sum of 2^(logit log2(e) - c)}
+  float2* sums;              // [rows][slices] {top, sum of e^(logit - top)}, as the scan's threads add it
   int64_t logits_s0, logits_s1, scores_s0, scores_s1, out_scores_s0, out_beams_s0, out_tokens_s0;
   int32_t batch, beams, vocab, best, beams_64, tokens_64;
   int32_t slices, chunks, per_cta;  // most slices of a row, its chunks, chunks of a CTA
@@ -76,8 +76,21 @@ __device__ __forceinline__ float logit_bound(float mine, int n, int holders, flo
   return bound;
 }
 
-// log2(e) as the kernels multiply by it: what a sum's offset is divided by to give a logarithm, in 64 bits.
-constexpr float BEAM_LOG2E = 1.4426950408889634f;
+// A sum of exponentials around the logit `top` adds 2^(a x - a top): a is log2(e), by one fma with the product a top rounded
+// before.  Beyond 2^30 a is 1: that rounding is then more than 2^6 and at last beyond fp32, while x - top is exact, and any logit but top
+// itself is 64 or more away, so that its term is 0 in either form.
+constexpr float BEAM_LOG2E = 1.4426950408889634f, BEAM_FAR = 1073741824.f;
+__device__ __forceinline__ bool beam_near(float top) { return fabsf(top) < BEAM_FAR; }
+__device__ __forceinline__ float beam_offset(float top) { return beam_near(top) ? __fmul_rn(top, BEAM_LOG2E) : top; }
+// What a sum around `from` is multiplied by to be one around `to`, which is no less; -inf: an empty sum's.
+__device__ __forceinline__ float beam_rescale(float from, float to) {
+  if (beam_near(from) && beam_near(to)) return fast_exp2(__fsub_rn(__fmul_rn(from, BEAM_LOG2E), __fmul_rn(to, BEAM_LOG2E)));
+  return from == to ? 1.f : 0.f;
+}
+__device__ __forceinline__ double beam_rescale64(float from, float to) {
+  if (beam_near(from) && beam_near(to)) return exp2((double)beam_offset(from) - (double)beam_offset(to));
+  return from == to ? 1.0 : 0.0;
+}
 
 // The best of a list of n keys into out[0 .. best), 0 where the list ends: ranked by counting, or one at a time, whichever
 // takes fewer instructions.  By all threads of the scan, behind a barrier.
@@ -129,7 +142,7 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 // VEC: rows start on 16 bytes, and a thread reads 16 bytes at a time; else it reads words of 4 (a rule of the call, not of the row, so
 // that equal rows cut alike have equal sums).  Copies are of whole 16-byte pieces inside the row; what stands at its ends is filled in.
 //
-// The sum: each thread adds 2^(x log2(e) - c), c = its maximum x log2(e), which may lag by 8 (then by 2^11.5 a term).
+// The sum: each thread adds its terms around its largest logit (beam_offset), which may lag by 8 (then by 2^11.5 a term).
 // The `best` largest: the largest of groups of threads in a slice's first chunk bound the `best`-th from below.  Up to 16 results: the
 // `best`-th of 32 of them, which little more than `best` logits reach; else something looser (logit_bound), and what reaches it is
 // listed, the list is cut to the best and the last one is the new bound.  It is cut (again) when four times as many chunks have passed
@@ -258,7 +271,7 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, BEAM_CTAS) beam_scan_kernel
       const int to = atomicAdd(&listed, 1);
       if (to < BEAM_LIST) keys[to] = ((unsigned long long)ordered(y) << 32) | (0xffffffffu - (uint32_t)at);
     };
-    float top = -INFINITY, off = 0.f, least = LEAST;
+    float top = -INFINITY, least = LEAST;
     float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     int from_k = 0;     // the slice's first chunk
     const bool few = p.best <= 16;
@@ -300,9 +313,14 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, BEAM_CTAS) beam_scan_kernel
           for (int j = 0; j < NV; ++j) mine = fmaxf(mine, vec_max<T>(load(full, j)));
           least = fmaxf(LEAST, logit_bound(mine, p.best, len >= CHUNK ? BEAM_THREADS : VEC ? (len + N - 1) / N : S == 4 ? len : (len + 1) / 2, low));
           top = mine;
-          off = top == -INFINITY ? 0.f : top * BEAM_LOG2E;
         }
-        float2 off2 = make_float2(-off, -off);
+        float2 off2, mul2;
+        auto around_top = [&]() {
+          const float off = top == -INFINITY ? 0.f : beam_offset(top), mul = top == -INFINITY || beam_near(top) ? BEAM_LOG2E : 1.f;
+          off2 = make_float2(-off, -off);
+          mul2 = make_float2(mul, mul);
+        };
+        around_top();
         float gate = top == -INFINITY ? LEAST : fminf(least, top + LAG);  // below it a piece needs nothing but its sum
 #pragma unroll
         for (int j = 0; j < NV; j += PAIR) {
@@ -316,13 +334,12 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, BEAM_CTAS) beam_scan_kernel
 #pragma unroll
             for (int u = 0; u < PAIR; ++u) most = fmaxf(most, vec_max<T>(x[u]));
           if (most >= gate) {
-            if (most > top + LAG || top == -INFINITY) {  // (with +inf, c is it too and the sum NaN, as with NaN)
-              const float c = most * BEAM_LOG2E, f = top == -INFINITY ? 1.f : fast_exp2(off - c);
+            if (most > top + LAG || top == -INFINITY) {  // (around +inf the sum is NaN, as with NaN)
+              const float f = beam_rescale(top, most);
 #pragma unroll
               for (int i = 0; i < 2; ++i) sum[i] = __fmul2_rn(sum[i], make_float2(f, f));
               top = most;
-              off = c;
-              off2 = make_float2(-off, -off);
+              around_top();
               gate = fminf(least, top + LAG);
             }
             if (most >= least) {
@@ -346,7 +363,7 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, BEAM_CTAS) beam_scan_kernel
                 y = make_float2(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
               else
                 y = unpack2<T>(w[e]);
-              y = __ffma2_rn(y, make_float2(BEAM_LOG2E, BEAM_LOG2E), off2);
+              y = __ffma2_rn(y, mul2, off2);
               sum[e & 1] = __fadd2_rn(sum[e & 1], make_float2(fast_exp2(y.x), fast_exp2(y.y)));
             }
           }
@@ -407,13 +424,11 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, BEAM_CTAS) beam_scan_kernel
       }
       fresh = ends;
       if (ends) {
-        // ---- the slice's list, and the threads' sums over the largest offset
+        // ---- the slice's list, and the threads' sums around the largest of their logits
         const int64_t slice = (int64_t)blockIdx.x - (int64_t)row * p.pitch / p.per_cta, at = (int64_t)row * p.slices + slice;
         const float mine = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-        const float mine_off = top == -INFINITY ? -INFINITY : off;
-        const float warp_off = warp_max(mine_off), from = warp_off == -INFINITY ? 0.f : warp_off;
-        const float total = warp_sum(mine == 0.f ? 0.f : mine * fast_exp2(mine_off - from));
-        if (lane == 0) sums[warp] = make_float2(warp_off, total);
+        const float warp_top = warp_max(top), total = warp_sum(mine * beam_rescale(top, warp_top));
+        if (lane == 0) sums[warp] = make_float2(warp_top, total);
         if (lost) {
           // more than there was room for (the largest logits late in the slice, or many equal ones): all of the slice's logits twice
           // again, for a bound by the threads' largest of all and for the list, which is cut when it may overflow
@@ -486,8 +501,7 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, BEAM_CTAS) beam_scan_kernel
         if (tid == 0) listed = noted = 0;
         if (warp == 0) {
           const float2 x = lane < BEAM_WARPS ? sums[lane] : make_float2(-INFINITY, 0.f);
-          const float most = warp_max(x.x), from_all = most == -INFINITY ? 0.f : most;
-          const float all = warp_sum(x.y == 0.f ? 0.f : x.y * fast_exp2(x.x - from_all));
+          const float most = warp_max(x.x), all = warp_sum(x.y * beam_rescale(x.x, most));
           if (lane == 0) p.sums[at] = make_float2(most, all);
         }
         if (k == p.chunks - 1)  // the row's other places stay empty
@@ -497,7 +511,7 @@ __global__ void __launch_bounds__(BEAM_THREADS + 32, BEAM_CTAS) beam_scan_kernel
           }
         beam_sync();
         lost = false;
-        top = -INFINITY, off = 0.f, least = LEAST;
+        top = -INFINITY, least = LEAST;
         sum[0] = sum[1] = make_float2(0.f, 0.f);
       }
       advance();
@@ -529,7 +543,9 @@ __device__ __forceinline__ double from_ordered64(unsigned long long k) { return 
 // Bound by its chain of steps.
 __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamParams p) {
   extern __shared__ float scores[];       // of all listed logits, -inf where there is none
-  __shared__ double shift[FT_MAX_BEAMS];  // a beam's score less its logarithm; NaN: nothing comes from it
+  // of a beam the logit that its sum is around, and its score less the sum's logarithm (not one number: the logit may dwarf the
+  // others); NaN: nothing comes from it
+  __shared__ double around[FT_MAX_BEAMS], shift[FT_MAX_BEAMS];
   __shared__ unsigned long long list_score[BEAM_KEYS], list_key[BEAM_KEYS];
   __shared__ uint8_t list_beam[BEAM_KEYS];
   __shared__ float high[BEAM_WARPS];
@@ -544,8 +560,9 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamPara
   const int per_beam = p.slices * p.best, total = p.beams * per_beam;
   const unsigned long long* __restrict__ keys = p.keys + (int64_t)req * total;
   constexpr float LEAST = -3.4028234e38f;
+  auto score_of = [&](unsigned long long key, int beam) { return ((double)from_ordered((uint32_t)(key >> 32)) - around[beam]) + shift[beam]; };
   auto put_score = [&](int i, unsigned long long key) {
-    const double x = (double)from_ordered((uint32_t)(key >> 32)) + shift[i / per_beam];
+    const double x = score_of(key, i / per_beam);
     // (one that is lower than all of fp32 is a candidate still)
     return scores[i] = key != 0 && x == x ? fmaxf(__double2float_rd(x), LEAST) : -INFINITY;
   };
@@ -567,19 +584,21 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamPara
         sum = (double)x.y;
       } else {
         const float most = fmaxf(x.x, y.x);
-        sum = (sum != 0 ? sum * exp2((double)x.x - (double)most) : 0.0) + (y.y != 0.f ? (double)y.y * exp2((double)y.x - (double)most) : 0.0);
+        sum = sum * beam_rescale64(x.x, most) + (double)y.y * beam_rescale64(y.x, most);
         x.x = most;
       }
     }
     float most = x.x;
     for (int o = 1; o < lanes; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    sum = sum != 0 ? sum * exp2((double)x.x - (double)most) : 0.0;
+    sum *= beam_rescale64(x.x, most);
     for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     // (the terms' exponents were taken x BEAM_LOG2E, which is not log2(e): by it the offset is a logit again, and what is left of the
     // difference, 1.3e-8 of the distance from the largest logit to the mean, is below fp32's half step)
-    const double lse = (double)most * (1.0 / (double)BEAM_LOG2E) + log(sum);
-    if (there && (lane & (lanes - 1)) == 0)
-      shift[b] = fabsf(score) < INFINITY && fabs(lse) < (double)INFINITY ? (double)score - lse : (double)NAN;
+    const double logit = beam_near(most) ? (double)beam_offset(most) * (1.0 / (double)BEAM_LOG2E) : (double)most, lse = log(sum);
+    if (there && (lane & (lanes - 1)) == 0) {
+      around[b] = logit;
+      shift[b] = fabsf(score) < INFINITY && fabs(logit + lse) < (double)INFINITY ? (double)score - lse : (double)NAN;
+    }
   }
   __syncthreads();
   float top = -INFINITY;
@@ -596,7 +615,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamPara
     BeamCandidate c;
     c.key = __ldcg(keys + i);
     c.beam = i / per_beam;
-    c.score = ordered64((double)from_ordered((uint32_t)(c.key >> 32)) + shift[c.beam]);
+    c.score = ordered64(score_of(c.key, c.beam));
     return c;
   };
   int turn = 0;
