@@ -72,10 +72,15 @@ int check_beam_select(const ft_beam_select_args* a) {
   return FT_OK;
 }
 
+// Shared memory for the listed logits of a request, 4 bytes each: 64 results of 592 slices (rows with CTAs of their own, all CTAs at once)
+// take 148 KB of it.
+constexpr int BEAM_MERGE_SMEM = 176 << 10;
+
 // Chunks of a call and how many a CTA takes, all CTAs at once.  Chunks of 16 KB, smaller ones where the call would leave SMs without any or
 // rows are shorter.  In chunks, a slice costs seven beside its own: dealt evenly, a CTA has the ends of two rows or more; with CTAs
 // of their own, or whole rows to a CTA, rows have no more slices than they need (64 x 4 rows of 16 chunks, two CTAs to a row: 29 us,
-// seven chunks to a CTA 31).  (148 SMs whatever the device: the workspace's size goes by this.)
+// seven chunks to a CTA 31).  Few long rows dealt evenly can have more slices than the merge holds (1 x 59 rows: 708): they get CTAs of their own
+// too.  (148 SMs whatever the device: the workspace's size goes by this.)
 BeamShape beam_shape(const ft_beam_select_args* a) {
   BeamShape s;
   const int n = 16 / dtype_size(a->dtype);
@@ -89,9 +94,12 @@ BeamShape beam_shape(const ft_beam_select_args* a) {
   const int64_t even = (rows * s.chunks + ctas - 1) / ctas;
   s.per_cta = (int)even;
   s.pitch = s.chunks;
+  auto dealt_slices = [&]() {
+    return s.chunks % s.per_cta == 0 ? s.chunks / s.per_cta : s.per_cta % s.chunks == 0 ? 1 : std::min((s.chunks - 1) / s.per_cta + 2, s.chunks);
+  };
   if (rows <= ctas) {
     const int64_t own = (s.chunks + ctas / rows - 1) / (ctas / rows);  // chunks of a CTA, with ctas / rows of them to a row
-    if (own <= even + 7) {
+    if (own <= even + 7 || 4LL * a->beams * dealt_slices() * a->best > BEAM_MERGE_SMEM) {
       s.per_cta = (int)own;
       s.pitch = (int)((s.chunks + own - 1) / own * own);
     }
@@ -100,13 +108,11 @@ BeamShape beam_shape(const ft_beam_select_args* a) {
     if (each * s.chunks <= even + 7) s.per_cta = (int)(each * s.chunks);
   }
   s.ctas = (rows * s.pitch + s.per_cta - 1) / s.per_cta;
-  s.slices = s.pitch > s.chunks ? s.pitch / s.per_cta : s.chunks % s.per_cta == 0 ? s.chunks / s.per_cta : s.per_cta % s.chunks == 0 ? 1 : std::min((s.chunks - 1) / s.per_cta + 2, s.chunks);
+  s.slices = s.pitch > s.chunks ? s.pitch / s.per_cta : dealt_slices();
   s.keys = rows * s.slices * a->best;
   s.bytes = s.keys * 8 + rows * s.slices * 8;
   return s;
 }
-
-constexpr int BEAM_MERGE_SMEM = 176 << 10;
 
 int pow2_at_least(int n, int low) {
   while (low < n) low *= 2;
@@ -130,10 +136,9 @@ int launch_beam_select(const ft::BeamParams& p, const BeamShape& s, bool vec, cu
                  : s.pieces == 2 ? (vec ? launch_scan_as<T, 2, true>(p, s, st) : launch_scan_as<T, 2, false>(p, s, st))
                                  : (vec ? launch_scan_as<T, 4, true>(p, s, st) : launch_scan_as<T, 4, false>(p, s, st));
   if (rc != FT_OK) return rc;
-  const int64_t smem = 4LL * p.beams * p.slices * p.best;  // at most 64 results of 592 + 64 slices
+  const int64_t smem = 4LL * p.beams * p.slices * p.best;
   static OncePerDevice once;
   FT_CUDA_OK(raise_smem_limit(once, ft::beam_merge_kernel, BEAM_MERGE_SMEM));
-  if (smem > BEAM_MERGE_SMEM) return fail(FT_ERR_TOO_LARGE, "more slices of logits than a request's merge holds");
   FT_CUDA_OK(launch_early(ft::beam_merge_kernel, dim3((unsigned)p.batch), ft::BEAM_THREADS, (size_t)smem, st, p));
   count_launch();
   return FT_OK;
