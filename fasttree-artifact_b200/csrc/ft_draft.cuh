@@ -312,11 +312,11 @@ __global__ void __launch_bounds__(ACCEPT_THREADS, 2) draft_accept_kernel(const A
         }
         next = (int64_t)(0xffffffffu - (uint32_t)key);
       }
-      // the first child that holds it
+      // the first child that holds it (-1 stands for a token that is none, which no target is)
       const int turn = count % 3;
       int found = FT_MAX_DRAFT;
       for (int i = cur + 1 + (int)threadIdx.x; i < d.n; i += ACCEPT_THREADS)
-        if (parent[i] == cur && (int64_t)token[i] == next) found = min(found, i);
+        if (parent[i] == cur && next >= 0 && (int64_t)token[i] == next) found = min(found, i);
       found = __reduce_min_sync(0xffffffffu, found);
       if (lane == 0 && found < FT_MAX_DRAFT) atomicMin(&child_at[turn], found);
       if (threadIdx.x == 0) child_at[(count + 1) % 3] = FT_MAX_DRAFT;
