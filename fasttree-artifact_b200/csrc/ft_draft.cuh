@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(ACCEPT_THREADS, 2) draft_accept_kernel(const A
     if (p.next_64)
       static_cast<long long*>(p.next_tokens)[out] = next;
     else
-      static_cast<int*>(p.next_tokens)[out] = (int)next;
+      static_cast<int*>(p.next_tokens)[out] = next == (int64_t)(int)next ? (int)next : -1;
   }
   for (int i = threadIdx.x; i < p.width; i += ACCEPT_THREADS) p.accepted[out * p.accepted_s0 + i] = i < count ? path[i] : -1;
   if (p.slots == nullptr) return;

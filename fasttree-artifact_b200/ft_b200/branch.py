@@ -35,8 +35,8 @@ def draft_accept(logits, tokens, parents, plan, accepted, counts, next_tokens, s
     the request's next one.  ``logits`` ``[tokens, vocabulary]``, fp16, bf16 or fp32: row t is the model's after token t; or None, with
     ``targets`` ``[tokens]`` the model's token behind each (sampled ones, say).  ``tokens``, ``parents``: one entry per row of ``q``.
     ``accepted`` (int32 ``[requests, at least the longest draft]``): the accepted tokens' numbers, from 0 on, then -1.  ``counts``
-    (int32 ``[requests]``): how many.  ``next_tokens`` (int32 or int64 ``[requests]``); a request without tokens, or whose first is no
-    root, has count 0 and -1.  With ``slots`` (the tokens' pool rows, as :func:`ft_b200.extend.append` took them) the request's entries
+    (int32 ``[requests]``): how many.  ``next_tokens`` (int32 or int64 ``[requests]``; int32 has -1 where it does not hold a target); a
+    request without tokens, or whose first is no root, has count 0 and -1.  With ``slots`` (the tokens' pool rows, as :func:`ft_b200.extend.append` took them) the request's entries
     of ``kv_entries`` behind its cached ones become the accepted tokens' rows, in path order, and then the others', which the caller
     may free: the request goes on with cached + count tokens in the cache.  No result may overlap what is read, except that one
     request's ``slots`` may be its entries themselves."""

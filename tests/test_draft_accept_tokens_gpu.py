@@ -34,3 +34,11 @@ def test_a_target_that_is_no_token_accepts_nothing(token, target):
 def test_a_drafted_token_that_is_none_is_passed_over():
     path, following, _ = accept([3, -1, 1 << 33, 7, 9], [7, 5, 5, 9, 4], [-1, 0, 0, 0, 3])
     assert path == [0, 3, 4] and following == 4
+
+
+@gpu
+def test_a_next_token_that_int32_does_not_hold():
+    assert accept([3, 4], [4, (1 << 33) + 5], [-1, 0], out=torch.int32)[:2] == ([0, 1], -1)
+    assert accept([3, 4], [-(1 << 40), 5], [-1, 0], out=torch.int32)[:2] == ([0], -1)
+    assert accept([3, 4], [-7, 5], [-1, 0], out=torch.int32)[:2] == ([0], -7)
+    assert accept([3, 4], [(1 << 31) - 1, 5], [-1, 0], out=torch.int32)[:2] == ([0], (1 << 31) - 1)
