@@ -338,7 +338,14 @@ __global__ void __launch_bounds__(ACCEPT_THREADS, 2) draft_accept_kernel(const A
   if (p.slots == nullptr) return;
   // the path's rows first, then the others', each in order: the path rises.  All are read before any is written: they may stand at
   // these entries.
-  for (int i = threadIdx.x; i < d.n; i += ACCEPT_THREADS) token[i] = (int32_t)load_slot(p.slots, p.slots_64, (int64_t)d.row + i);
+  bool bad = false;
+  for (int i = threadIdx.x; i < d.n; i += ACCEPT_THREADS) {
+    const int64_t slot = load_slot(p.slots, p.slots_64, (int64_t)d.row + i);
+    const bool ok = slot == (int64_t)(int32_t)slot;
+    bad |= !ok;
+    token[i] = ok ? (int32_t)slot : -1;
+  }
+  if (bad) flag_error(FT_DEV_BAD_KV_INDEX);
   __syncthreads();
   for (int i = threadIdx.x; i < d.n; i += ACCEPT_THREADS) {
     int before = 0;

@@ -38,7 +38,7 @@ def draft_accept(logits, tokens, parents, plan, accepted, counts, next_tokens, s
     (int32 ``[requests]``): how many.  ``next_tokens`` (int32 or int64 ``[requests]``; int32 has -1 where it does not hold a target); a
     request without tokens, or whose first is no root, has count 0 and -1.  With ``slots`` (the tokens' pool rows, as :func:`ft_b200.extend.append` took them) the request's entries
     of ``kv_entries`` behind its cached ones become the accepted tokens' rows, in path order, and then the others', which the caller
-    may free: the request goes on with cached + count tokens in the cache.  No result may overlap what is read, except that one
+    may free (a row that int32 does not hold becomes -1 and is flagged): the request goes on with cached + count tokens in the cache.  No result may overlap what is read, except that one
     request's ``slots`` may be its entries themselves."""
     rc = _lib.call_module().draft_accept(logits, targets, tokens, parents, *_draft_plan(plan), accepted, counts, next_tokens, slots, kv_entries)
     if rc != 0:

@@ -528,7 +528,8 @@ typedef struct ft_draft_accept_args {
   int32_t* counts;      /* [num requests] accepted tokens */
   void* next_tokens;    /* [num requests] the model's token behind the last accepted one; -1 without any, or where int32 does not hold it */
   const void* slots;    /* NULL, or [rows] the tokens' pool rows: with kv_entries, the request's entries behind its cached ones */
-  int32_t* kv_entries;  /*   become the accepted tokens' rows, in path order, then the others'.  Of a plan with one request slots may lie
+  int32_t* kv_entries;  /*   become the accepted tokens' rows, in path order, then the others' (-1 for one that int32 does not hold,
+                             flagged FT_DEV_BAD_KV_INDEX).  Of a plan with one request slots may lie
                              in kv_entries (be those very entries); otherwise no result may overlap what is read */
   int32_t dtype;        /* enum ft_dtype, of logits */
   int32_t vocab;

@@ -42,3 +42,14 @@ def test_a_next_token_that_int32_does_not_hold():
     assert accept([3, 4], [-(1 << 40), 5], [-1, 0], out=torch.int32)[:2] == ([0], -1)
     assert accept([3, 4], [-7, 5], [-1, 0], out=torch.int32)[:2] == ([0], -7)
     assert accept([3, 4], [(1 << 31) - 1, 5], [-1, 0], out=torch.int32)[:2] == ([0], (1 << 31) - 1)
+
+
+@gpu
+def test_rows_that_int32_does_not_hold():
+    lib.read_device_status()
+    path, _, table = accept([3, 4, 5], [5, 0, 9], [-1, 0, 0], slots=[11, 12, 13])
+    assert path == [0, 2] and table[4:] == [11, 13, 12] and lib.read_device_status() == 0
+    path, _, table = accept([3, 4, 5], [5, 0, 9], [-1, 0, 0], slots=[(1 << 32) + 11, -1, 13])
+    assert path == [0, 2] and table[4:] == [-1, 13, -1] and lib.read_device_status() == lib.FT_DEV_BAD_KV_INDEX
+    path, _, table = accept([3, 4, 5], [5, 0, 9], [-1, 0, 0], slots=[11, 12, -(1 << 40)])
+    assert path == [0, 2] and table[4:] == [11, -1, 12] and lib.read_device_status() == lib.FT_DEV_BAD_KV_INDEX
