@@ -659,6 +659,9 @@ void pack(const Problem& p, const Builder& b, ft_extend_plan* out) {
   t.insert(t.end(), tiles.begin(), tiles.end());
   info.extra_off = (int64_t)t.size();
   t.insert(t.end(), extra.begin(), extra.end());
+  // ft_extend's kernels read sms before the kernel ahead of them, which may be ft_draft_tree's, has ended: a cache line of 128 bytes,
+  // wherever the table starts, lies between those ints and the words that it writes
+  if (p.draft) t.insert(t.end(), 32, 0);
   align();
   info.sms_off = (int64_t)t.size();
   for (int c = 0; c < p.slots; ++c) {
