@@ -50,6 +50,14 @@ __device__ __forceinline__ ExtendStream extend_stream(const int32_t* item, int w
   return {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 }
 
+// A word of what a token sees.  ft_draft_tree's kernel may write it while a kernel that was launched early waits for that one, so it
+// is no data for ld.global.nc, which is for what nobody writes as long as the kernel runs.
+__device__ __forceinline__ uint32_t extend_bits(const int32_t* p) {
+  uint32_t x;
+  asm volatile("ld.global.b32 %0, [%1];\n" : "=r"(x) : "l"(p));
+  return x;
+}
+
 // Where the rows of token `tok` of a stream go: to o (-1), to a partial row, or nowhere (-2: the token sees nothing there).
 __device__ __forceinline__ int extend_part(const ExtendParams& p, const ExtendStream& st, int tok) {
   return st.part < 0 ? -1 : __ldg(p.extra + st.part + tok);
@@ -109,7 +117,7 @@ __device__ __noinline__ void extend_row(const ExtendParams& p, const int32_t* it
     const int bits_at = __ldg(tile + 4 + st.block_tile);
     if (steps != 0 && lane == 0) asm volatile("red.shared.add.u32 [%0], 1;\n" ::"r"(steps) : "memory");
     for (int k = 0; k < words; ++k) {
-      uint32_t todo = bits_at < 0 ? 0xffffffffu : (uint32_t)__ldg(p.extra + bits_at + (st.first + tok) * words + k);
+      uint32_t todo = bits_at < 0 ? 0xffffffffu : extend_bits(p.extra + bits_at + (st.first + tok) * words + k);
       while (todo != 0) {
         int64_t row[TB];
         float s[TB];
@@ -200,7 +208,7 @@ __device__ __noinline__ int extend_bad_in_sight(const ExtendParams& p, const int
     for (int k = 0; k < words; ++k) {
       const int i = 32 * k + lane, id = i < rec.z ? __ldg(p.kv_entries + extend_entry(p, rec, i)) : 0;
       const uint32_t out = __ballot_sync(0xffffffffu, i < rec.z && (id < 0 || id >= p.kv_rows));
-      if (out != 0) n += __popc(out & (bits_at < 0 ? 0xffffffffu : (uint32_t)__ldg(p.extra + bits_at + (st.first + tok) * words + k)));
+      if (out != 0) n += __popc(out & (bits_at < 0 ? 0xffffffffu : extend_bits(p.extra + bits_at + (st.first + tok) * words + k)));
     }
   }
   return n;

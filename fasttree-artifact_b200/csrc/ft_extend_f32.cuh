@@ -148,8 +148,8 @@ __global__ void __launch_bounds__(256, ExtF32Cfg<D, RPT>::CTAS) extend_f32_kerne
           float mx = -INFINITY;
           uint32_t in[2] = {0xffffffffu, 0xffffffffu};
           if (mask >= 0) {
-            in[0] = (uint32_t)__ldg(bits[i] + mask);
-            in[1] = (uint32_t)__ldg(bits[i] + mask + 1);
+            in[0] = extend_bits(bits[i] + mask);
+            in[1] = extend_bits(bits[i] + mask + 1);
             hidden[i] |= (in[0] & in[1]) != 0xffffffffu;
           }
 #pragma unroll

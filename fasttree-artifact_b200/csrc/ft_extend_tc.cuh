@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
         uint32_t some = 0, every = 0xffffffffu;
 #pragma unroll
         for (int k = 0; k < TILE / 32; ++k) {
-          see[k] = row < rows ? (uint32_t)__ldg(bits + mask + k) : 0u;
+          see[k] = row < rows ? extend_bits(bits + mask + k) : 0u;
           some |= see[k];
           every &= see[k];
         }
