@@ -755,6 +755,18 @@ struct ReorderParams {
   int32_t shift;  // a CTA has 2^shift columns, in words
 };
 
+// (not by ld.global.nc: the selection's merge may write them while this kernel, launched early, waits for it)
+__device__ __forceinline__ int64_t load_number(const void* p, int is_64, int64_t i) {
+  long long x;
+  int y;
+  if (is_64) {
+    asm volatile("ld.global.b64 %0, [%1];\n" : "=l"(x) : "l"(static_cast<const long long*>(p) + i));
+    return x;
+  }
+  asm volatile("ld.global.b32 %0, [%1];\n" : "=r"(y) : "l"(static_cast<const int*>(p) + i));
+  return y;
+}
+
 // A CTA has some columns of all of a request's rows: it reads every word that it moves before it writes any, so that rows may
 // change places.
 __global__ void __launch_bounds__(BEAM_THREADS) beam_reorder_kernel(const ReorderParams p) {
@@ -765,10 +777,10 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_reorder_kernel(const Reorde
   // (what does not depend on one another is asked for at once: the call's length is this chain, the rows' numbers, the rows)
   int64_t beam = -1, t = -1;
   if ((int)threadIdx.x < p.to) {
-    beam = load_index(p.beams, p.beams_64, req * p.beams_s0 + threadIdx.x);
-    t = load_index(p.out_rows, p.out_rows_64, req * p.out_rows_s0 + threadIdx.x);
+    beam = load_number(p.beams, p.beams_64, req * p.beams_s0 + threadIdx.x);
+    t = load_number(p.out_rows, p.out_rows_64, req * p.out_rows_s0 + threadIdx.x);
   }
-  int64_t lo = p.starts != nullptr ? load_index(p.starts, p.starts_64, req) : 0, hi = p.ends != nullptr ? load_index(p.ends, p.ends_64, req) : whole;
+  int64_t lo = p.starts != nullptr ? load_number(p.starts, p.starts_64, req) : 0, hi = p.ends != nullptr ? load_number(p.ends, p.ends_64, req) : whole;
   bool bad = lo < 0 || lo > whole || hi < 0 || hi > whole;
   lo = (lo < 0 ? 0 : lo > whole ? whole : lo) * p.words;
   hi = (hi < 0 ? 0 : hi > whole ? whole : hi) * p.words;
@@ -777,7 +789,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_reorder_kernel(const Reorde
   if ((int)threadIdx.x < p.to) {
     int64_t s = -1;
     if (beam != -1) {
-      s = beam >= 0 && beam < p.from ? load_index(p.rows, p.rows_64, req * p.rows_s0 + beam) : -1;
+      s = beam >= 0 && beam < p.from ? load_number(p.rows, p.rows_64, req * p.rows_s0 + beam) : -1;
       if (s < 0 || s >= p.table_rows || t < 0 || t >= p.table_rows) {
         bad = true;
         s = t = -1;
