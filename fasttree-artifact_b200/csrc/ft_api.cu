@@ -204,9 +204,10 @@ ft::Stage1Params stage1_params(const ft_decode_args* a) {
 }
 
 // Every stage-1 kernel is launched with permission to be scheduled before the preceding kernel of the stream has
-// drained (programmatic dependent launch).  The kernels do nothing but on-chip set-up before their
-// griddepcontrol.wait, which returns once the preceding kernel has completed and its writes are visible, so the
-// permission is safe after any kernel; it pays after kernels that release their dependents early, as both stages of
+// drained (programmatic dependent launch).  Before their griddepcontrol.wait, which returns once the preceding kernel has
+// completed and its writes are visible, the kernels do nothing but on-chip set-up and reads of plan tables that no kernel of
+// this library writes (the merges their lists, the tensor-core extend kernel its schedule, which lies a cache line away from the
+// words that ft_draft_tree writes), so the permission is safe after any kernel but one that writes a plan's table; it pays after kernels that release their dependents early, as both stages of
 // this library do: back-to-back decode calls overlap each launch and set-up with the previous kernel's tail.
 template <typename... KArgs, typename... Args>
 cudaError_t launch_early(void (*kernel)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, Args&&... args) {

@@ -35,8 +35,8 @@ int current_sms() {
 
 template <typename T>
 int launch_accept(const ft::AcceptParams& p, int requests, int64_t row_bytes, cudaStream_t st) {
-  // CTAs per request: as many as the SMs hold two of, so that all are there at once, as long as each has 16 KB of a row to read (64
-  // requests, 131072 bf16 logits, 1 to 6 rows a path: 80, 53, 33, 43 us with 1, 2, 4, 8)
+  // CTAs per request: as many as the SMs hold two of, so that all are there at once, as long as each has 16 KB of a row to read (with
+  // 1, 2, 4, 8: 64 requests, 131072 bf16 logits, 1 to 6 rows a path 45, 35, 29, 41 us; 33 requests, 100003 fp32, 1 to 5 rows 53, 38, 29, 24)
   int ranks = 1;
   const int room = 2 * current_sms();
   while (p.targets == nullptr && ranks < 8 && (int64_t)requests * ranks * 2 <= room && row_bytes / (2 * ranks) >= 16384) ranks *= 2;

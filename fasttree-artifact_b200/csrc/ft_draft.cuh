@@ -1,6 +1,7 @@
 // Drafted tokens: their trees into a plan's masks, and which of them the model agrees with.
 //
-// Kernels here and in ft_beam.cuh that write row tables let no later launch start early: others read theirs before they wait.
+// Kernels here and in ft_beam.cuh that write row tables let no later launch start early.  That of a tree does: no kernel reads what it
+// writes before its own wait.
 //
 // A request's drafted tokens are numbered so that a parent comes before its children.  The attention itself is ft_extend's: its
 // kernels read what a row sees from bits of the plan, and ft_draft_tree sets the few words of them that trees decide.
@@ -92,8 +93,9 @@ __device__ __forceinline__ const int16_t* load_tree(const void* parents, int is_
 }
 
 // A CTA per request (several, with the spans shared out, where drafts are long): positions of its tokens, and the words that its tree
-// decides.  Bound by a chain of three reads (request, parents and spans, words) and a climb.  Two stretches of a tile may share a word, in different bits: clearing and setting are
-// atomic, and their order does not matter.
+// decides.  Bound by a chain of three reads (request, parents and spans, words), the rounds of the depths and a span's climb: 3.1 to
+// 5.6 us for drafts of 5 to 64 tokens.  Two stretches of a tile may share a word, in different bits: clearing and setting are atomic, and
+// their order does not matter.
 __global__ void __launch_bounds__(DRAFT_THREADS) draft_tree_kernel(const DraftParams p) {
   __shared__ Tree tree;
   allow_dependent_launch();

@@ -16,7 +16,7 @@ struct DraftSpan {
   int32_t token0;    // the first token's number among the request's drafted ones
   int32_t bit0, bit1;
   int32_t pos0;      // position of bit0 less the request's cached tokens: below 0 are cached ones, the rest are drafted
-  int32_t zero0, zero1;
+  int32_t zero0, zero1;  // to eight ints, which are read as two times four
 };
 
 // Token k of the span, word by word from the last: emit(word, mask of the span's bits in it, those that the token sees).

@@ -254,7 +254,8 @@ __global__ void __launch_bounds__(ExtCfg<D>::THREADS, 1) extend_tc_kernel(const 
   // CTAs would be placed one by one as this one's end, in another order than onto idle SMs (8 prompts of 700 to 2500 tokens, 28/4
   // heads, capped, one call behind the other: 424 us, with the order kept 409; small calls 0.5 us more).
   if (p.num_merged > 0) allow_dependent_launch();
-  // (before the wait for the kernel ahead: set-up, and of memory the plan's schedule alone, which no kernel writes)
+  // (before the wait for the kernel ahead: set-up, and of memory the plan's schedule alone, which no kernel writes, nor
+  // anything within a cache line of it)
   const int4* my_share = reinterpret_cast<const int4*>(p.sms) + 4 * blockIdx.x;
   const int4 share = __ldg(my_share);
   const int task_lo = share.x, task_hi = share.y;

@@ -32,14 +32,17 @@ def draft_accept(logits, tokens, parents, plan, accepted, counts, next_tokens, s
 
     A request's token 0 is certain (the newest one that was chosen, a root).  From it on, the first child that holds the token of the
     largest logit (of equal ones the lowest; NaN is passed over) is accepted, as long as there is one; the token that no child held is
-    the request's next one.  ``logits`` ``[tokens, vocabulary]``, fp16, bf16 or fp32: row t is the model's after token t; or None, with
-    ``targets`` ``[tokens]`` the model's token behind each (sampled ones, say).  ``tokens``, ``parents``: one entry per row of ``q``.
+    the request's next one.  ``logits`` ``[tokens, vocabulary]``, fp16, bf16 or fp32: row t is the model's after token t (a
+    row with nothing above -inf gives token 0); or None, with ``targets`` ``[tokens]`` the model's token behind each (sampled ones, say).
+    Tokens are whole numbers from 0 that int32 holds: nothing else is accepted, nor matches a target.  ``tokens``, ``parents``: one entry
+    per row of ``q``.
     ``accepted`` (int32 ``[requests, at least the longest draft]``): the accepted tokens' numbers, from 0 on, then -1.  ``counts``
     (int32 ``[requests]``): how many.  ``next_tokens`` (int32 or int64 ``[requests]``; int32 has -1 where it does not hold a target); a
-    request without tokens, or whose first is no root, has count 0 and -1.  With ``slots`` (the tokens' pool rows, as :func:`ft_b200.extend.append` took them) the request's entries
-    of ``kv_entries`` behind its cached ones become the accepted tokens' rows, in path order, and then the others', which the caller
-    may free (a row that int32 does not hold becomes -1 and is flagged): the request goes on with cached + count tokens in the cache.  No result may overlap what is read, except that one
-    request's ``slots`` may be its entries themselves."""
+    request without tokens, or whose first is no root, has count 0 and -1.  With ``slots`` (the tokens' pool rows, as
+    :func:`ft_b200.extend.append` took them) the request's entries of ``kv_entries`` behind its cached ones become the accepted tokens'
+    rows, in path order, and then the others', which the caller may free (a row that int32 does not hold becomes -1 and is flagged): the
+    request goes on with cached + count tokens in the cache.  No result may overlap what is read, except that one request's ``slots`` may
+    be its entries themselves."""
     rc = _lib.call_module().draft_accept(logits, targets, tokens, parents, *_draft_plan(plan), accepted, counts, next_tokens, slots, kv_entries)
     if rc != 0:
         _lib.check(rc)
@@ -52,8 +55,10 @@ def beam_select(logits, scores, out_scores, out_beams, out_tokens):
     ``[batch, beams]``.  Results ``[batch, n]``, best first: ``out_scores`` fp32, ``out_beams`` and ``out_tokens`` int32 or int64; at most 64
     beams and results.  Of equal scores the lowest beam's comes first, then the larger logit, then the lowest token.  Logits of -inf are
     never chosen (banned tokens), nor is anything from a beam whose score is not finite (-inf: a beam that ended, or has not begun) or whose
-    logits hold NaN or +inf; where too little is left the last results are score -inf, beam -1, token -1.  The logarithms are good to about
-    1e-7: scores of different beams that are closer may come in either order.  ``out_scores`` may be ``scores``, or start with it
+    logits hold NaN or +inf; where too little is left the last results are score -inf, beam -1, token -1.  Logits and scores may be of any
+    finite size: tokens masked with the type's lowest value come last, and a score that fp32 does not hold rounds to -inf.  The logarithms
+    come from fp32 sums, within 2^-17 up to 131072 logits a row (3e-7 as measured): scores of different beams that are closer may come in
+    either order.  ``out_scores`` may be ``scores``, or start with it
     in every row; otherwise no result may overlap what is read.  Two launches."""
     rc = _lib.call_module().beam_select(logits, scores, out_scores, out_beams, out_tokens)
     if rc != 0:

@@ -467,7 +467,8 @@ typedef struct ft_extend_args {
   int64_t o_stride0, o_stride1;
   const int32_t* kv_entries; /* pool rows, the table that the plan's kv_starts index */
   int64_t kv_entries_len;
-  const int32_t* plan_table; /* device copy of the table of ft_extend_plan_copy, 16-byte aligned */
+  const int32_t* plan_table; /* device copy of the table of ft_extend_plan_copy, 16-byte aligned.  Its schedule is read before the kernel
+                                ahead on the stream has ended: that one may not write the table, ft_draft_tree's apart */
   ft_extend_plan_info plan;
   float* mid_o;          /* [partial_rows, num_qo_heads, head_dim] and [partial_rows, num_qo_heads], packed; the call's */
   float* mid_lse;        /* own scratch, may be NULL if the plan has no partial rows.  Calls that may overlap need their own */
@@ -550,8 +551,9 @@ int ft_draft_accept(const ft_draft_accept_args* args);
 /* The `best` best continuations of each request's beams: score = scores[beam] + logits[beam][token] - log sum exp(logits[beam]),
  * best first; of equal scores the lowest beam's first, then the larger logit, then the lowest token.  Logits of -inf are never chosen, nor is anything from a
  * beam whose score is not finite (one that ended, say) or whose logits hold NaN or +inf; where too little is left the last
- * results are score -inf, beam -1, token -1.  Scores are compared in 64 bits; the logarithms are good to about 1e-7, so closer scores
- * of different beams may come in either order. */
+ * results are score -inf, beam -1, token -1.  Scores are compared in 64 bits; the logarithms come from fp32 sums, within 2^-17 up
+ * to 131072 logits a row (3e-7 as measured), so closer scores of different beams may come in either order.  Logits may be of any finite
+ * size (masks of a type's lowest value are ordinary, if unlikely, tokens); a score that fp32 does not hold rounds to -inf. */
 typedef struct ft_beam_select_args {
   const void* logits;   /* [batch, beams, vocab] */
   const float* scores;  /* [batch, beams] */
