@@ -519,7 +519,8 @@ int ft_draft_tree(const ft_draft_tree_args* args);
 
 /* Which drafted tokens the model agrees with: from a request's token 0 (its newest certain token, a root) on, the child that holds
  * the token of the largest logit (of equal ones the lowest; NaN is passed over), the first such child, as long as there is one.
- * Only the rows of logits along that path are read.  parents as in ft_draft_tree (what they take for padding is never accepted). */
+ * Only the rows of logits along that path are read.  parents as in ft_draft_tree (what they take for padding is never accepted).
+ * Tokens are 0 to 2^31 - 1: no other drafted token is accepted, and no other target matches one. */
 typedef struct ft_draft_accept_args {
   const void* logits;   /* [rows, vocab], row t: the model's after token t; NULL if targets is given */
   const void* targets;  /* [rows] the model's next token behind each token, in place of logits (sampled, say), or NULL */
