@@ -14,8 +14,7 @@ def accept(tokens, targets, parents, out=torch.int64, slots=None):
     accepted = torch.full((1, n), -9, dtype=torch.int32, device="cuda")
     counts, following = torch.full((1,), -9, dtype=torch.int32, device="cuda"), torch.full((1,), -9, dtype=out, device="cuda")
     table = torch.full((n + 4,), -5, dtype=torch.int32, device="cuda")
-    wide = torch.tensor([0, 1 << 40]).cuda()                   # (one index type for all)
-    tokens, targets, parents = (torch.tensor(x, dtype=wide.dtype, device="cuda") for x in (tokens, targets, parents))
+    tokens, targets, parents = (torch.tensor(x, dtype=torch.int64, device="cuda") for x in (tokens, targets, parents))
     rows = {} if slots is None else {"slots": torch.tensor(slots, device="cuda"), "kv_entries": table}
     fasttree.fasttree_draft_accept(None, tokens, parents, plan, accepted, counts, following, targets=targets, **rows)
     torch.cuda.synchronize()

@@ -30,7 +30,7 @@ def test_replays_with_new_trees(cached, nodes, heads, dtype):
         steps.append((parents, o))
     parents, o, graph = steps[0][0].clone(), torch.empty_like(s.gq), torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        for _ in range(3):                      # three layers of a step
+        for _ in range(3):                      # trees and attention in turn
             fasttree.fasttree_draft_tree(parents, s.plan)
             fasttree.fasttree_extend(s.gq, s.gk, s.gv, o, s.gt, s.plan, s.scale)
     wrong = torch.zeros((), dtype=torch.int64, device="cuda")
